@@ -285,6 +285,57 @@ int nwc_argmax(void *stream, const uint16_t *logits, uint32_t V, int64_t *cur, i
 int nwc_argmax_tp(void *stream, const uint16_t *logits, uint32_t V, int64_t *cur, int64_t *log, int32_t *pos,
                   int32_t *step, uint32_t log_len, uint32_t max_pos, void *const *buffers, int rank, int world);
 
+/* ---- a cache for long sessions and for several tokens at once (no counterpart in the reference, which leaves the cache to
+   Transformers) -------------------------------------------------------------------------------------------------------
+
+   Per layer and key/value head `capacity` slots of head_dim numbers (64, 128 or 256) for K and for V: bf16, or e4m3 codes
+   with one byte b per row: value = code * 2^(b - 127), the smallest exponent that keeps the row's largest magnitude within
+   448 * 2^(b - 127).
+   window == 0: position p lives in slot p and a token sees every position up to its own; sessions end at `capacity`.
+   window > 0: a token sees the last `window` positions, its own among them, and the first `sinks` positions of the session.
+   Positions below `sinks` keep their slots, the others take the remaining capacity - sinks slots in turn, so a session may
+   run to 2^31 - 1 positions; a call of T tokens needs capacity - sinks >= window + T - 1.
+   k, v, qkv, q and out are 16-byte aligned; every call is asynchronous on its stream, allocates nothing and can be captured.
+   *pos (device) is the position of a call's first token.  *status (device) collects bits, 0 = fine: 1 a position outside the
+   cache or the rotary tables (the call, or with `depth` that token, wrote nothing), 2 a key or value that was not finite (0
+   was stored in its place), 4 a path that is not one (nothing was moved). */
+#define NWC_KV_MAX_TOKENS 65535
+#define NWC_KV_MAX_TREE 1024
+typedef struct {
+    void *k, *v;                 /* [layers][n_kv][capacity][head_dim] */
+    uint8_t *k_exp, *v_exp;      /* e4m3: [layers][n_kv][capacity]; bf16: NULL */
+    uint32_t layers, n_kv, head_dim, capacity, window, sinks;
+    int elem;                    /* 0 bf16, 1 e4m3 */
+} nwc_kv_cache;
+
+/* T tokens of a fused q/k/v projection enter layer `layer`: qkv[t] = [n_q | n_kv | n_kv] heads x head_dim, rows ldqkv apart
+   (a multiple of 8).  q and k take their per-head RMSNorm (q_norm and k_norm, or both NULL) and the rotary embedding with row
+   pos + depth[t] (depth NULL: pos + t) of the bf16 tables [max_pos][head_dim], in fp32 throughout; q_out (bf16 [T][n_q][head_dim]),
+   k and v are rounded once, to what is stored.  Token t is stored at position *pos + t. */
+int nwc_kv_append(void *stream, const nwc_kv_cache *cache, uint32_t layer, const uint16_t *qkv, uint64_t ldqkv, uint32_t T,
+                  uint32_t n_q, const uint16_t *q_norm, const uint16_t *k_norm, const uint16_t *cos_t, const uint16_t *sin_t,
+                  uint32_t max_pos, const int32_t *pos, const int32_t *depth, float eps, uint16_t *q_out, int *status);
+
+/* Positions first .. first + count - 1 of a layer as bf16 [n_kv][count][head_dim].  Of a ring's positions the caller asks for
+   ones that it still holds. */
+int nwc_kv_read(void *stream, const nwc_kv_cache *cache, uint32_t layer, uint32_t first, uint32_t count, uint16_t *k_out,
+                uint16_t *v_out);
+
+/* T tokens at positions *pos .. *pos + T - 1, already stored, attend: out[t] = sum_p softmax_p(scale q[t] . k_p) v_p (bf16
+   [T][n_q * head_dim]) over the positions that token t sees; a token that sees none gets zeros.  q rows are ldq apart (a multiple
+   of 8).  visible != NULL: the tokens are drafts of a tree (T <= NWC_KV_MAX_TREE); token t stands at position *pos + depth[t],
+   sees what is cached below *pos as above, and of the drafts those whose bit is set: bit j of word visible[t][j / 32]
+   ([T][(T + 31) / 32]), its own included or not. */
+int nwc_kv_attention(void *stream, const nwc_kv_cache *cache, uint32_t layer, const uint16_t *q, uint64_t ldq, uint32_t T,
+                     uint32_t n_q, const int32_t *pos, const uint32_t *visible, const int32_t *depth, float scale,
+                     uint16_t *out, int *status);
+
+/* The accepted path of a draft tree of T tokens at *pos: row path[i] of the drafts becomes row i for i < *count (<= most <= T),
+   in all layers; path (device, `most` entries) rises strictly.  The caller then advances *pos by *count; the drafts behind
+   the path count as never stored. */
+int nwc_kv_commit(void *stream, const nwc_kv_cache *cache, uint32_t T, const int32_t *pos, const int32_t *path,
+                  const int32_t *count, uint32_t most, int *status);
+
 #ifdef __cplusplus
 }
 #endif

@@ -13,6 +13,7 @@ __version__ = "0.1.0"
 from .weight import NWCWeight, fits, choose_block, quantize_fp8, ref_fp8_matvec                    # noqa: F401
 from .modules import NWCLinear, NWCEmbedding, convert, fuse, RefFP8Linear, convert_ref_fp8          # noqa: F401
 from .checkpoint import save_pretrained, load_pretrained, export_bf16                                # noqa: F401
+from .kvcache import KVCache, draft_tree                                                             # noqa: F401
 
 __all__ = ["NWCWeight", "NWCLinear", "NWCEmbedding", "convert", "fuse", "fits", "choose_block", "quantize_fp8",
-           "save_pretrained", "load_pretrained", "export_bf16", "__version__"]
+           "save_pretrained", "load_pretrained", "export_bf16", "KVCache", "draft_tree", "__version__"]

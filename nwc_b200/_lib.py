@@ -69,6 +69,10 @@ _SIGNATURES = {
     "nwc_comm_import": (I, [P, P]),
     "nwc_comm_release": (I, [P]),
     "nwc_comm_slot": (P, [P, U32, I]),
+    "nwc_kv_append": (I, [P, P, U32, P, U64, U32, U32, P, P, P, P, U32, P, P, ctypes.c_float, P, P]),
+    "nwc_kv_read": (I, [P, P, U32, U32, U32, P, P]),
+    "nwc_kv_attention": (I, [P, P, U32, P, U64, U32, U32, P, P, P, ctypes.c_float, P, P]),
+    "nwc_kv_commit": (I, [P, P, U32, P, P, P, U32, P]),
     "nwc_allreduce_add_rmsnorm": (I, [P, P, I, I, I, P, P, P, ctypes.c_float, U32, P]),
 }
 for _name, (_res, _args) in _SIGNATURES.items():
@@ -84,6 +88,12 @@ class FusedOptions(ctypes.Structure):
                 ("out_slot", ctypes.c_int), ("H", ctypes.c_uint32), ("side", ctypes.c_void_p),
                 ("next_low", ctypes.c_void_p), ("next_n", ctypes.c_uint64), ("next_K", ctypes.c_uint32), ("next_elem", ctypes.c_int),
                 ("next_mode", ctypes.c_int)]
+
+
+class KvCache(ctypes.Structure):
+    """nwc_kv_cache of include/nwc_ops.h."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_exp", ctypes.c_void_p), ("v_exp", ctypes.c_void_p), ("layers", U32), ("n_kv", U32),
+                ("head_dim", U32), ("capacity", U32), ("window", U32), ("sinks", U32), ("elem", ctypes.c_int)]
 
 
 VERSION = lib.nwc_info(0)

@@ -1,0 +1,267 @@
+/* The cache that is quantised as it is written: store (per-head RMSNorm, rotary positions, rounding to the cache's type),
+ * read back, and the move of an accepted draft path.  Formats and slot rules: nwc_kv.h.
+ *
+ * All three move bytes: their floor is the bytes in and out at the memory's rate, and for one token a launch.
+ */
+#include <cuda_fp8.h>
+#include "nwc_kv.h"
+#include "nwc_launch.h"
+
+#define NWC_EXPORT extern "C" __attribute__((visibility("default")))
+
+namespace {
+
+using namespace nwc;
+
+__device__ __forceinline__ void dependency_sync() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ float lo16(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float hi16(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) { uint32_t d; asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(b), "f"(a)); return d; }
+__device__ __forceinline__ uint16_t pack_e4m3(float a, float b) { return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3); }
+
+__device__ __forceinline__ uint4 pack8(const float (&y)[8]) { return make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7])); }
+constexpr float kLargestBf16 = 3.3895313892515355e38f;
+
+struct StoreArgs {
+    KvLayer c;
+    const uint16_t *qkv; uint64_t ldqkv;
+    uint32_t T, n_q;
+    const uint16_t *q_norm, *k_norm, *cos_t, *sin_t;
+    uint32_t max_pos;
+    const int32_t *pos, *depth;
+    float eps;
+    uint16_t *q_out;
+    int *status;
+};
+
+/* HD / 8 lanes hold one row, eight numbers each, so a row is one 16-byte load per lane; the rotary partner of a number lives
+   in the lane HD / 16 away.  A warp takes kRows rows of one token at a time (their loads are in flight together and share the
+   token's cos / sin).  Everything between the loaded bf16 numbers and what is stored is fp32, rounded once. */
+template <int HD, int ELEM>
+__global__ void __launch_bounds__(256) kv_store_kernel(const StoreArgs a) {
+    constexpr uint32_t kLanesPerRow = HD / 8, kSide = 32 / kLanesPerRow, kPasses = 4, kRows = kSide * kPasses;
+    const uint32_t lane = threadIdx.x & 31u, sub = lane % kLanesPerRow, side = lane / kLanesPerRow, d0 = sub * 8u;
+    const uint32_t heads = a.n_q + 2u * a.c.n_kv, groups = (heads + kRows - 1u) / kRows;
+    const uint64_t unit = (uint64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    dependency_sync();
+    if (unit >= (uint64_t)groups * a.T) return;
+    const uint32_t t = (uint32_t)(unit / groups), row0 = (uint32_t)(unit % groups) * kRows;
+    const int32_t pos = *a.pos, depth = a.depth ? a.depth[t] : (int32_t)t;
+    const uint32_t limit = a.c.window ? 0x7FFFFFFFu : a.c.capacity;
+    const bool ok = pos >= 0 && (uint64_t)pos + a.T <= limit && depth >= 0 && (uint32_t)depth < a.T && (uint64_t)pos + (a.depth ? (uint32_t)depth + 1u : a.T) <= a.max_pos;
+    if (!ok) { if (lane == 0) atomicOr(a.status, kKvStatusPosition); return; }
+    const uint32_t slot = kv_slot((uint32_t)pos + t, a.c.capacity, a.c.window, a.c.sinks);
+    uint4 raw[kPasses];
+#pragma unroll
+    for (uint32_t i = 0; i < kPasses; i++) {
+        const uint32_t row = row0 + i * kSide + side;
+        raw[i] = row < heads ? *reinterpret_cast<const uint4 *>(a.qkv + (uint64_t)t * a.ldqkv + (uint64_t)row * HD + d0) : make_uint4(0u, 0u, 0u, 0u);
+    }
+    const uint64_t at = ((uint64_t)pos + (uint32_t)depth) * HD + d0;
+    const uint4 cw = *reinterpret_cast<const uint4 *>(a.cos_t + at), sw = *reinterpret_cast<const uint4 *>(a.sin_t + at);
+    const uint32_t cu[4] = {cw.x, cw.y, cw.z, cw.w}, su[4] = {sw.x, sw.y, sw.z, sw.w};
+#pragma unroll
+    for (uint32_t i = 0; i < kPasses; i++) {
+        const uint32_t row = row0 + i * kSide + side;
+        const bool live = row < heads, is_q = row < a.n_q, is_v = row >= a.n_q + a.c.n_kv;
+        const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 4; j++) { x[2 * j] = lo16(u[j]); x[2 * j + 1] = hi16(u[j]); }
+        const uint16_t *weight = is_q ? a.q_norm : a.k_norm;
+        if (a.q_norm) {                                               /* (the sum of a V row is not used) */
+            float ss = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; j++) ss = fmaf(x[j], x[j], ss);
+#pragma unroll
+            for (uint32_t o = kLanesPerRow / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            const float inv = rsqrtf(ss * (1.f / HD) + a.eps);
+            if (!is_v) {
+                const uint4 ww = *reinterpret_cast<const uint4 *>(weight + d0);
+                const uint32_t wu[4] = {ww.x, ww.y, ww.z, ww.w};
+#pragma unroll
+                for (int j = 0; j < 4; j++) { x[2 * j] *= inv * lo16(wu[j]); x[2 * j + 1] *= inv * hi16(wu[j]); }
+            }
+        }
+        const float sign = sub < kLanesPerRow / 2 ? -1.f : 1.f;
+        float y[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float other = __shfl_xor_sync(0xffffffffu, x[j], kLanesPerRow / 2);
+            const float c = j & 1 ? hi16(cu[j >> 1]) : lo16(cu[j >> 1]), s = j & 1 ? hi16(su[j >> 1]) : lo16(su[j >> 1]);
+            y[j] = is_v ? x[j] : fmaf(x[j], c, sign * other * s);
+        }
+        if (is_q) *reinterpret_cast<uint4 *>(a.q_out + ((uint64_t)t * a.n_q + row) * HD + d0) = pack8(y);
+        /* a key or value that is not finite would reach every query through the cache: it is kept out (0) and reported */
+        bool fine = true;
+        float top = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            if (!(fabsf(y[j]) <= kLargestBf16)) { fine = false; y[j] = 0.f; }
+            /* (1.875 * 2^127: the largest value of three mantissa bits in range; rounding a larger one up would reach 2^128) */
+            if (ELEM == kKvE4m3) y[j] = fminf(fmaxf(y[j], -3.1901471898837980e38f), 3.1901471898837980e38f);
+            top = fmaxf(top, fabsf(y[j]));
+        }
+        const uint32_t kvh = is_v ? row - a.n_q - a.c.n_kv : row - a.n_q;
+        const uint64_t cell = (uint64_t)kvh * a.c.capacity + slot;
+        if (ELEM == kKvE4m3) {
+#pragma unroll
+            for (uint32_t o = kLanesPerRow / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            /* smallest e with top <= 1.75 * 2^(8 + e): from top's exponent field, one more where its mantissa is above 0.75 */
+            const uint32_t bits = __float_as_uint(top);
+            const int32_t b = max(0, (int32_t)(bits >> 23) - 8 + ((bits & 0x7FFFFFu) > 0x600000u ? 1 : 0));
+            const float inv = __uint_as_float((uint32_t)(254 - b) << 23);         /* 2^(127 - b): exact */
+            if (live && !is_q) {
+                uint2 codes;
+                codes.x = pack_e4m3(y[0] * inv, y[1] * inv) | ((uint32_t)pack_e4m3(y[2] * inv, y[3] * inv) << 16);
+                codes.y = pack_e4m3(y[4] * inv, y[5] * inv) | ((uint32_t)pack_e4m3(y[6] * inv, y[7] * inv) << 16);
+                *reinterpret_cast<uint2 *>((is_v ? a.c.v : a.c.k) + cell * HD + d0) = codes;
+                if (sub == 0) (is_v ? a.c.v_exp : a.c.k_exp)[cell] = (uint8_t)b;
+            }
+        } else if (live && !is_q) {
+            *reinterpret_cast<uint4 *>((is_v ? a.c.v : a.c.k) + (cell * HD + d0) * 2u) = pack8(y);
+        }
+        if (live && !is_q && !fine) atomicOr(a.status, kKvStatusNotFinite);
+    }
+}
+
+struct ReadArgs {
+    KvLayer c;
+    uint32_t first, count, head_dim;
+    uint16_t *k_out, *v_out;     /* bf16 [n_kv][count][head_dim] */
+};
+
+/* One thread reads back 16 numbers; K (blockIdx.z = 0) and V (1) of one head per blockIdx.y. */
+template <int ELEM>
+__global__ void __launch_bounds__(256) kv_read_kernel(const ReadArgs a) {
+    const uint32_t per_row = a.head_dim >> 4;
+    const uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    dependency_sync();
+    if (i >= (uint64_t)a.count * per_row) return;
+    const uint32_t r = (uint32_t)(i / per_row), d0 = (uint32_t)(i % per_row) * 16u;
+    const uint64_t cell = (uint64_t)blockIdx.y * a.c.capacity + kv_slot(a.first + r, a.c.capacity, a.c.window, a.c.sinks);
+    const uint8_t *from = blockIdx.z ? a.c.v : a.c.k;
+    uint4 *to = reinterpret_cast<uint4 *>((blockIdx.z ? a.v_out : a.k_out) + ((uint64_t)blockIdx.y * a.count + r) * a.head_dim + d0);
+    if (ELEM == kKvE4m3) {
+        const uint4 w = *reinterpret_cast<const uint4 *>(from + cell * a.head_dim + d0);
+        const uint32_t unit2 = kv_unit2((blockIdx.z ? a.c.v_exp : a.c.k_exp)[cell]);
+        uint4 lo, hi;
+        kv_values4(w.x, unit2, lo.x, lo.y); kv_values4(w.y, unit2, lo.z, lo.w);
+        kv_values4(w.z, unit2, hi.x, hi.y); kv_values4(w.w, unit2, hi.z, hi.w);
+        to[0] = lo; to[1] = hi;
+    } else {
+        const uint4 *src = reinterpret_cast<const uint4 *>(from + (cell * a.head_dim + d0) * 2u);
+        const uint4 lo = src[0], hi = src[1];
+        to[0] = lo; to[1] = hi;
+    }
+}
+
+/* The accepted path of a draft tree, moved together: row pos + path[i] -> row pos + i for i < count, in every layer and
+   head.  path rises strictly, so path[i] >= i and a row is read before anything overwrites it when the moves run in order;
+   each thread owns one 16-byte column (or the exponent bytes) of all rows and therefore needs no synchronisation. */
+__global__ void __launch_bounds__(64) kv_commit_kernel(KvLayer c, uint32_t row_bytes, uint32_t T, const int32_t *pos_ptr, const int32_t *path, const int32_t *count_ptr, uint32_t most, int *status) {
+    dependency_sync();
+    const int32_t pos = *pos_ptr, count = *count_ptr;
+    bool ok = pos >= 0 && count >= 0 && (uint32_t)count <= most && (uint64_t)pos + T <= (c.window ? 0x7FFFFFFFu : c.capacity);
+    for (int32_t i = 0, last = -1; ok && i < count; i++) { const int32_t p = path[i]; ok = p > last && (uint32_t)p < T; last = p; }
+    if (!ok) { if (threadIdx.x == 0) atomicOr(status, kKvStatusPath); return; }
+    const uint64_t head = blockIdx.x, cell0 = head * c.capacity;
+    const uint32_t columns = row_bytes >> 4;
+    for (uint32_t j = threadIdx.x; j < 2u * columns + (c.k_exp ? 2u : 0u); j += blockDim.x) {
+        if (j < 2u * columns) {
+            uint8_t *base = (j < columns ? c.k : c.v) + cell0 * row_bytes + (j % columns) * 16u;
+            for (int32_t i = 0; i < count; i++) {
+                const int32_t p = path[i];
+                if (p != i) *reinterpret_cast<uint4 *>(base + (uint64_t)kv_slot(pos + i, c.capacity, c.window, c.sinks) * row_bytes) = *reinterpret_cast<const uint4 *>(base + (uint64_t)kv_slot(pos + p, c.capacity, c.window, c.sinks) * row_bytes);
+            }
+        } else {
+            uint8_t *base = (j == 2u * columns ? c.k_exp : c.v_exp) + cell0;
+            for (int32_t i = 0; i < count; i++) { const int32_t p = path[i]; if (p != i) base[kv_slot(pos + i, c.capacity, c.window, c.sinks)] = base[kv_slot(pos + p, c.capacity, c.window, c.sinks)]; }
+        }
+    }
+}
+
+template <class... Params, class... Args>
+cudaError_t launch(void (*kernel)(Params...), dim3 grid, dim3 block, void *stream, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid; cfg.blockDim = block; cfg.stream = (cudaStream_t)stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr; cfg.numAttrs = nwc::dependent_launch() ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
+
+bool aligned16(const void *p) { return !(reinterpret_cast<uintptr_t>(p) & 15u); }
+
+/* the cache is one the kernels can address, and T tokens at once fit beside what its window still has to see */
+bool cache_ok(const nwc_kv_cache *c, uint32_t layer, uint32_t T) {
+    if (!c || !c->layers || layer >= c->layers || !c->n_kv || !c->capacity || c->capacity > 0x7FFFFF00u || (c->elem != kKvBf16 && c->elem != kKvE4m3)) return false;
+    if (c->head_dim != 64u && c->head_dim != 128u && c->head_dim != 256u) return false;
+    if (!c->k || !c->v || !aligned16(c->k) || !aligned16(c->v) || (c->elem == kKvE4m3 && (!c->k_exp || !c->v_exp))) return false;
+    if ((uint64_t)c->layers * c->n_kv > 0x7FFFFFFFull) return false;
+    if (c->window) return c->sinks < c->capacity && (uint64_t)c->window + (T ? T - 1u : 0u) <= c->capacity - c->sinks;
+    return T <= c->capacity;
+}
+KvLayer layer_of(const nwc_kv_cache *c, uint32_t layer) {
+    const uint64_t cells = (uint64_t)layer * c->n_kv * c->capacity, bytes = cells * c->head_dim * (c->elem == kKvBf16 ? 2u : 1u);
+    const bool q = c->elem == kKvE4m3;
+    return KvLayer{static_cast<uint8_t *>(c->k) + bytes, static_cast<uint8_t *>(c->v) + bytes, q ? c->k_exp + cells : nullptr, q ? c->v_exp + cells : nullptr,
+                   c->n_kv, c->capacity, c->window, c->window ? c->sinks : 0u};
+}
+
+template <int HD>
+cudaError_t launch_store(int elem, const StoreArgs &a, void *stream) {
+    constexpr uint32_t rows = 4u * 32u / (HD / 8u);
+    const uint64_t units = (uint64_t)((a.n_q + 2u * a.c.n_kv + rows - 1u) / rows) * a.T, blocks = (units + 7u) / 8u;
+    if (blocks > 0x7FFFFFFFull) return cudaErrorInvalidValue;
+    const uint32_t threads = units >= 8u ? 256u : (uint32_t)units * 32u;
+    return elem == kKvE4m3 ? launch(kv_store_kernel<HD, kKvE4m3>, dim3((uint32_t)blocks), dim3(threads), stream, a)
+                           : launch(kv_store_kernel<HD, kKvBf16>, dim3((uint32_t)blocks), dim3(threads), stream, a);
+}
+
+}  // namespace
+
+NWC_EXPORT int nwc_kv_append(void *stream, const nwc_kv_cache *cache, uint32_t layer, const uint16_t *qkv, uint64_t ldqkv, uint32_t T, uint32_t n_q,
+                             const uint16_t *q_norm, const uint16_t *k_norm, const uint16_t *cos_t, const uint16_t *sin_t, uint32_t max_pos,
+                             const int32_t *pos, const int32_t *depth, float eps, uint16_t *q_out, int *status) {
+    if (!cache_ok(cache, layer, T) || !T || T > NWC_KV_MAX_TOKENS || !n_q || n_q % cache->n_kv || n_q > 65535u) return -1;
+    if (!qkv || !cos_t || !sin_t || !pos || !q_out || !status || !q_norm != !k_norm) return -1;
+    const uint64_t width = (uint64_t)(n_q + 2u * cache->n_kv) * cache->head_dim;
+    if (ldqkv < width || ldqkv % 8u) return -1;
+    if (!aligned16(qkv) || !aligned16(cos_t) || !aligned16(sin_t) || !aligned16(q_out) || !aligned16(q_norm) || !aligned16(k_norm)) return -1;
+    const StoreArgs a{layer_of(cache, layer), qkv, ldqkv, T, n_q, q_norm, k_norm, cos_t, sin_t, max_pos, pos, depth, eps, q_out, status};
+    return (int)(cache->head_dim == 64u ? launch_store<64>(cache->elem, a, stream) : cache->head_dim == 128u ? launch_store<128>(cache->elem, a, stream) : launch_store<256>(cache->elem, a, stream));
+}
+
+NWC_EXPORT int nwc_kv_read(void *stream, const nwc_kv_cache *cache, uint32_t layer, uint32_t first, uint32_t count, uint16_t *k_out, uint16_t *v_out) {
+    if (!cache_ok(cache, layer, 0u) || !count || !k_out || !v_out || !aligned16(k_out) || !aligned16(v_out) || cache->n_kv > 65535u) return -1;
+    const uint64_t end = (uint64_t)first + count;
+    if (end > (cache->window ? 0x7FFFFFFFull : cache->capacity)) return -1;
+    /* rows of the ring that one call asks for must be there at the same time */
+    if (cache->window && end > cache->sinks && end - (first > cache->sinks ? first : cache->sinks) > cache->capacity - cache->sinks) return -1;
+    const ReadArgs a{layer_of(cache, layer), first, count, cache->head_dim, k_out, v_out};
+    const uint64_t threads = (uint64_t)count * (cache->head_dim >> 4);
+    const dim3 grid((uint32_t)((threads + 255u) / 256u), cache->n_kv, 2u);
+    return (int)(cache->elem == kKvE4m3 ? launch(kv_read_kernel<kKvE4m3>, grid, dim3(256), stream, a) : launch(kv_read_kernel<kKvBf16>, grid, dim3(256), stream, a));
+}
+
+NWC_EXPORT int nwc_kv_commit(void *stream, const nwc_kv_cache *cache, uint32_t T, const int32_t *pos, const int32_t *path, const int32_t *count, uint32_t most, int *status) {
+    if (!cache_ok(cache, 0u, T) || !T || T > NWC_KV_MAX_TREE || most > T || !pos || !path || !count || !status) return -1;
+    if (!most) return 0;
+    const uint32_t row_bytes = cache->head_dim * (cache->elem == kKvBf16 ? 2u : 1u);
+    return (int)launch(kv_commit_kernel, dim3(cache->layers * cache->n_kv), dim3(64), stream, layer_of(cache, 0u), row_bytes, T, pos, path, count, most, status);
+}
+
+NWC_EXPORT int nwc_kv_attention(void *stream, const nwc_kv_cache *cache, uint32_t layer, const uint16_t *q, uint64_t ldq, uint32_t T, uint32_t n_q,
+                                const int32_t *pos, const uint32_t *visible, const int32_t *depth, float scale, uint16_t *out, int *status) {
+    if (!cache_ok(cache, layer, T) || !T || T > NWC_KV_MAX_TOKENS || !n_q || n_q % cache->n_kv || n_q > 65535u) return -1;
+    if (!q || !pos || !out || !status || !aligned16(q) || !aligned16(out) || ldq < (uint64_t)n_q * cache->head_dim || ldq % 8u) return -1;
+    if (visible ? T > NWC_KV_MAX_TREE || !depth : depth != nullptr) return -1;
+    if (!(scale > 0.f) || scale > 3e38f) return -1;
+    const KvAttention a{layer_of(cache, layer), q, ldq, T, n_q, pos, visible, depth, scale * 1.4426950408889634f, out, status};
+    return (int)launch_kv_attention((cudaStream_t)stream, cache->elem, cache->head_dim, a);
+}

@@ -1,0 +1,188 @@
+"""Key/value cache for long sessions and for several tokens at once: bf16 or quantised as it is written (e4m3 codes with one
+power-of-two scale per row), plain or a ring under a sliding window whose first tokens ("sinks") stay visible, read by one
+token, by a chunk of a prompt or by a tree of drafted tokens.  One call = one or two kernels of this library on the current
+stream; positions live in device memory, so every call can be captured in a CUDA graph.
+
+    cache = KVCache(n_kv=8, head_dim=128, capacity=8192, elem="fp8", layers=36)
+    q = cache.append(qkv, pos, cos, sin, q_norm, k_norm, layer=i)        # T tokens at positions pos .. pos + T - 1
+    out = cache.attend(q, pos, layer=i)                                  # [T, n_q * head_dim]
+
+A draft tree is verified with the same two calls and the masks of `draft_tree`, then `commit` moves the accepted path together.
+"""
+import ctypes
+import math
+
+import torch
+
+from . import _lib as L
+
+ELEMS = {"bf16": (0, torch.bfloat16), "fp8": (1, torch.float8_e4m3fn)}
+STATUS_TEXT = ((1, "a position outside the cache or the rotary tables"), (2, "a key or value that is not finite"), (4, "an accepted path that is not one"))
+
+
+def draft_tree(parents, device="cuda"):
+    """Masks of a draft tree: parents[i] < i is the draft that token i continues, -1 where it continues the cached text.
+    Returns (visible int32 [T, ceil(T / 32)], depth int32 [T]): every token sees its ancestors and itself."""
+    T = len(parents)
+    if not T: raise ValueError("a draft tree has at least one token")
+    if T > 1024: raise ValueError(f"a draft tree has at most 1024 tokens, not {T}")
+    masks, depth = [], []
+    for i, p in enumerate(parents):
+        p = int(p)
+        if not -1 <= p < i: raise ValueError(f"draft {i} hangs below draft {p}: a parent comes before its children (-1 = none)")
+        masks.append((masks[p] if p >= 0 else 0) | 1 << i)
+        depth.append(depth[p] + 1 if p >= 0 else 0)
+    words = [[(m >> 32 * w) & 0xFFFFFFFF for w in range((T + 31) // 32)] for m in masks]
+    signed = [[w - (1 << 32) if w >> 31 else w for w in row] for row in words]
+    return torch.tensor(signed, dtype=torch.int32, device=device), torch.tensor(depth, dtype=torch.int32, device=device)
+
+
+class KVCache:
+    """`layers` x `n_kv` heads x `capacity` slots of head_dim (64, 128 or 256) numbers for K and for V.
+
+    window = 0: position p lives in slot p, a token sees every position up to its own.
+    window > 0: a token sees the last `window` positions (its own among them) and the first `sinks`; slots beyond the sinks are
+    taken in turn, so positions run on without end.  T tokens at once need capacity - sinks >= window + T - 1.
+
+    Position tensors are int32 [1] on the cache's device.  Values that are not finite are stored as 0 and reported by check(),
+    as are positions outside the cache."""
+
+    def __init__(self, n_kv, head_dim, capacity, elem="bf16", layers=1, window=0, sinks=0, device="cuda"):
+        L.require_cuda()
+        _, dtype = _elem(elem)
+        if min(layers, n_kv, head_dim, capacity) < 1: raise ValueError("layers, n_kv, head_dim and capacity are at least 1")
+        shape = (layers, n_kv, capacity, head_dim)
+        # zeros, not empty: a slot that no token has reached holds numbers
+        zeros = lambda: torch.zeros(shape, dtype=torch.uint8 if elem == "fp8" else dtype, device=device).view(dtype)
+        exps = (lambda: torch.zeros(shape[:3], dtype=torch.uint8, device=device)) if elem == "fp8" else (lambda: None)
+        self._bind(zeros(), zeros(), exps(), exps(), window, sinks)
+
+    @classmethod
+    def over(cls, k, v, k_exp=None, v_exp=None, window=0, sinks=0):
+        """A cache over tensors that the caller holds: k, v [layers, n_kv, capacity, head_dim] bf16, or float8_e4m3fn with the
+        rows' exponent bytes k_exp, v_exp uint8 [layers, n_kv, capacity]."""
+        self = cls.__new__(cls)
+        self._bind(k, v, k_exp, v_exp, window, sinks)
+        return self
+
+    def _bind(self, k, v, k_exp, v_exp, window, sinks):
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device: raise ValueError("k and v are [layers, n_kv, capacity, head_dim] of one type on one device")
+        if k.dtype not in (torch.bfloat16, torch.float8_e4m3fn): raise ValueError(f"a cache holds bfloat16 or float8_e4m3fn, not {k.dtype}")
+        quantised = k.dtype == torch.float8_e4m3fn
+        if not (k.is_contiguous() and v.is_contiguous()): raise ValueError("k and v are contiguous")
+        for t in (k_exp, v_exp):
+            if quantised != (t is not None): raise ValueError("fp8 caches come with exponent bytes, bf16 caches without")
+            if quantised and (t.dtype != torch.uint8 or t.shape != k.shape[:3] or not t.is_contiguous() or t.device != k.device): raise ValueError("exponent bytes are contiguous uint8 [layers, n_kv, capacity] beside the codes")
+        self.layers, self.n_kv, self.capacity, self.head_dim = k.shape
+        if self.head_dim not in (64, 128, 256): raise ValueError(f"head_dim is 64, 128 or 256, not {self.head_dim}")
+        window, sinks = int(window), int(sinks)
+        if window < 0 or sinks < 0: raise ValueError("window and sinks are not negative")
+        if not window and sinks: raise ValueError("sinks need a window")
+        if window and self.capacity - sinks < window: raise ValueError(f"a window of {window} behind {sinks} sinks needs a capacity of {window + sinks} at least, not {self.capacity}")
+        if self.capacity > 0x7FFFFF00: raise ValueError("capacity is below 2^31 - 256")
+        if not k.is_cuda: raise ValueError("a cache lives on a CUDA device")
+        if k.data_ptr() % 16 or v.data_ptr() % 16: raise ValueError("k and v are 16-byte aligned")
+        self.window, self.sinks, self.elem = window, sinks, "fp8" if quantised else "bf16"
+        self.k, self.v, self.k_exp, self.v_exp, self.device = k, v, k_exp, v_exp, k.device
+        self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
+        at = lambda t: None if t is None else t.data_ptr()
+        self._c = L.KvCache(at(k), at(v), at(k_exp), at(v_exp), self.layers, self.n_kv, self.head_dim, self.capacity, window, sinks, 1 if quantised else 0)
+        self._ref, self._status = ctypes.byref(self._c), self.status.data_ptr()
+
+    # ---- calls ----
+    def append(self, qkv, pos, cos, sin, q_norm=None, k_norm=None, eps=1e-6, depth=None, layer=0):
+        """Store T tokens of a fused projection qkv [T, (n_q + 2 n_kv) head_dim] (bf16; a vector is one token) at positions
+        pos .. pos + T - 1: per-head RMSNorm of q and k (with both weights), rotary embedding with rows of the bf16 tables cos /
+        sin [positions, head_dim] - row pos + depth[t] for drafts, pos + t otherwise - and one rounding to the cache's type.
+        Returns the queries, bf16 [T, n_q, head_dim]."""
+        if qkv.dim() == 1: qkv = qkv[None]
+        T, width = self._tokens(qkv, 2, "qkv")
+        heads, hd = width // self.head_dim, self.head_dim
+        n_q = heads - 2 * self.n_kv
+        if width % hd or n_q <= 0 or n_q % self.n_kv: raise ValueError(f"qkv rows of {width} are not (n_q + 2 * {self.n_kv}) heads of {hd}, n_q a multiple of {self.n_kv}")
+        if (q_norm is None) != (k_norm is None): raise ValueError("q_norm and k_norm come together")
+        for t, shape in ((cos, None), (sin, cos.shape), (q_norm, (hd,)), (k_norm, (hd,))):
+            if t is not None and (t.dtype != torch.bfloat16 or t.device != self.device or not t.is_contiguous() or t.shape[-1] != hd or shape is not None and tuple(t.shape) != tuple(shape)):
+                raise ValueError(f"cos and sin are bf16 [positions, {hd}], q_norm and k_norm bf16 [{hd}], on the cache's device")
+        if depth is not None: self._int32(depth, T, "depth")
+        self._int32(pos, 1, "pos")
+        self._layer(layer)
+        out = qkv.new_empty((T, n_q, hd))
+        self._call("nwc_kv_append", L.lib.nwc_kv_append, layer, qkv.data_ptr(), qkv.stride(0), T, n_q, None if q_norm is None else q_norm.data_ptr(),
+                   None if k_norm is None else k_norm.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0], pos.data_ptr(), None if depth is None else depth.data_ptr(),
+                   eps, out.data_ptr(), self._status)
+        return out
+
+    def attend(self, q, pos, visible=None, depth=None, layer=0, scale=None):
+        """Attention of T stored tokens at positions pos .. pos + T - 1 (q [T, n_q, head_dim], bf16) over what each of them
+        sees; with the masks of draft_tree the tokens are drafts (at most 1024).  Returns bf16 [T, n_q * head_dim]; a token that
+        sees nothing gets zeros.  scale: of the scores, 1 / sqrt(head_dim) by default."""
+        T, n_q, hd = self._tokens(q, 3, "q")
+        if hd != self.head_dim or n_q % self.n_kv or q.stride(1) != hd: raise ValueError(f"q is [T, n_q, {self.head_dim}] with n_q a multiple of {self.n_kv} and a token's heads side by side")
+        if (visible is None) != (depth is None): raise ValueError("visible and depth come together (draft_tree makes them)")
+        if visible is not None:
+            if T > 1024: raise ValueError(f"a draft tree has at most 1024 tokens, not {T}")
+            self._int32(visible, T * ((T + 31) // 32), "visible"); self._int32(depth, T, "depth")
+        self._int32(pos, 1, "pos")
+        self._layer(layer)
+        out = q.new_empty((T, n_q * hd))
+        self._call("nwc_kv_attention", L.lib.nwc_kv_attention, layer, q.data_ptr(), q.stride(0), T, n_q, pos.data_ptr(), None if visible is None else visible.data_ptr(),
+                   None if depth is None else depth.data_ptr(), 1.0 / math.sqrt(hd) if scale is None else float(scale), out.data_ptr(), self._status)
+        return out
+
+    def read(self, first, count, layer=0):
+        """Positions first .. first + count - 1 of a layer as bf16 (K, V), each [n_kv, count, head_dim].  Of a ring, positions
+        that it still holds."""
+        first, count = int(first), int(count)
+        if first < 0 or count < 1: raise ValueError("positions from 0 on, at least one")
+        if not self.window and first + count > self.capacity: raise ValueError(f"positions {first} .. {first + count - 1} are outside a cache of {self.capacity}")
+        if self.window and first + count - max(first, self.sinks) > self.capacity - self.sinks: raise ValueError(f"{count} positions do not lie in a ring of {self.capacity - self.sinks} at the same time")
+        self._layer(layer)
+        k = torch.empty((self.n_kv, count, self.head_dim), dtype=torch.bfloat16, device=self.device)
+        v = torch.empty_like(k)
+        self._call("nwc_kv_read", L.lib.nwc_kv_read, layer, first, count, k.data_ptr(), v.data_ptr())
+        return k, v
+
+    def commit(self, pos, path, count, tokens=None):
+        """The accepted path of the draft tree stored at pos, in all layers: row path[i] of the drafts becomes row i for i <
+        count (int32 [1]; path int32, strictly rising).  `tokens`: size of the tree (default: as many as the cache allows to be
+        told apart from a wrong path).  The caller then advances pos by count."""
+        if path.dim() != 1: raise ValueError("path is a vector of draft numbers")
+        self._int32(path, path.numel(), "path"); self._int32(count, 1, "count"); self._int32(pos, 1, "pos")
+        if tokens is None: tokens = min(1024, self.capacity - self.sinks - self.window + 1 if self.window else self.capacity)
+        self._call("nwc_kv_commit", L.lib.nwc_kv_commit, None, tokens, pos.data_ptr(), path.data_ptr(), count.data_ptr(), min(path.numel(), tokens), self._status)
+
+    def check(self):
+        """Waits for the device; raises when a call since the last check met one of STATUS_TEXT."""
+        bits = int(self.status.item())
+        if bits:
+            self.status.zero_()
+            raise RuntimeError("key/value cache: " + "; ".join(text for bit, text in STATUS_TEXT if bits & bit))
+
+    # ---- helpers ----
+    def _tokens(self, t, dims, name):
+        if t.dim() != dims or t.dtype != torch.bfloat16 or t.device != self.device or t.stride(-1) != 1 or t.stride(0) % 8 or t.data_ptr() % 16:
+            raise ValueError(f"{name} is a {dims}-dimensional bf16 tensor on {self.device}, rows contiguous and 16-byte aligned")
+        if not 0 < t.shape[0] <= 65535: raise ValueError(f"a call takes 1 to 65535 tokens, not {t.shape[0]}")
+        return t.shape
+
+    def _int32(self, t, n, name):
+        if t.dtype != torch.int32 or t.device != self.device or t.numel() != n or not t.is_contiguous(): raise ValueError(f"{name} is int32 with {n} elements on {self.device}")
+
+    def _layer(self, layer):
+        if not 0 <= layer < self.layers: raise IndexError(f"layer {layer} of a cache of {self.layers}")
+
+    def _call(self, name, fn, layer, *args):
+        """One library call on the current stream of the cache's device."""
+        head = (self._ref,) if layer is None else (self._ref, layer)
+        index = self.device.index
+        if torch._C._cuda_getDevice() == index: err = fn(torch._C._cuda_getCurrentRawStream(index), *head, *args)
+        else:
+            with torch.cuda.device(index): err = fn(torch._C._cuda_getCurrentRawStream(index), *head, *args)
+        if err == -1: raise ValueError(f"{name}: the cache ({self.capacity} slots, window {self.window}, {self.sinks} sinks) does not take this call")
+        if err: raise RuntimeError(f"{name} error {err}")
+
+
+def _elem(elem):
+    if elem not in ELEMS: raise ValueError(f"elem is 'bf16' or 'fp8', not {elem!r}")
+    return ELEMS[elem]

@@ -1,0 +1,111 @@
+"""Key/value cache: what its entry points refuse before anything touches the GPU, the masks of a draft tree, and the 64-bit
+restatement that the GPU tests rely on, checked against elementary cases."""
+import ctypes
+
+import pytest
+import torch
+
+import kv_reference as R
+
+A = 1 << 20                                                            # an aligned address that nothing reads
+
+
+@pytest.fixture(scope="module")
+def L():
+    from nwc_b200 import _lib
+    return _lib
+
+
+def cache(L, **kw):
+    f = dict(k=A, v=A, k_exp=None, v_exp=None, layers=2, n_kv=2, head_dim=128, capacity=64, window=0, sinks=0, elem=0)
+    f.update(kw)
+    return ctypes.byref(L.KvCache(*[f[n] for n, _ in L.KvCache._fields_]))
+
+
+BAD_CACHES = [dict(head_dim=96), dict(head_dim=0), dict(n_kv=0), dict(layers=0), dict(capacity=0), dict(elem=2), dict(k=None), dict(v=A + 8), dict(elem=1),
+              dict(elem=1, k_exp=A), dict(window=64, sinks=1), dict(window=64), dict(window=10, sinks=64), dict(capacity=0x7FFFFF01), dict(capacity=2)]
+
+
+@pytest.mark.parametrize("bad", BAD_CACHES, ids=lambda b: "-".join(f"{k}={v}" for k, v in b.items()))
+def test_caches_that_no_kernel_addresses(L, bad):
+    """(capacity 2 and a window of 64 of 64 slots: right for one token, refused for the three of the call)"""
+    c = cache(L, **bad)
+    assert L.lib.nwc_kv_append(None, c, 0, A, 1024, 3, 4, None, None, A, A, 99, A, None, 1e-6, A, A) == -1
+    assert L.lib.nwc_kv_attention(None, c, 0, A, 512, 3, 4, A, None, None, 0.1, A, A) == -1
+    if "capacity" not in bad or bad["capacity"] != 2:
+        assert L.lib.nwc_kv_commit(None, c, 3, A, A, A, 2, A) == -1
+
+
+def test_append_refusals(L):
+    good = dict(layer=0, qkv=A, ld=1024, T=3, n_q=4, qn=None, kn=None, cos=A, sin=A, rows=99, pos=A, depth=None, eps=1e-6, out=A, status=A)
+    for bad in (dict(layer=2), dict(qkv=None), dict(qkv=A + 2), dict(ld=1016), dict(ld=1028), dict(T=0), dict(T=65536), dict(n_q=0), dict(n_q=3), dict(qn=A), dict(kn=A),
+                dict(cos=None), dict(sin=None), dict(cos=A + 8), dict(pos=None), dict(out=None), dict(out=A + 4), dict(status=None), dict(T=65)):
+        a = {**good, **bad}
+        assert L.lib.nwc_kv_append(None, cache(L), *a.values()) == -1, bad
+
+
+def test_attention_refusals(L):
+    good = dict(layer=0, q=A, ld=512, T=3, n_q=4, pos=A, visible=None, depth=None, scale=0.1, out=A, status=A)
+    for bad in (dict(layer=2), dict(q=None), dict(q=A + 8), dict(ld=504), dict(ld=516), dict(T=0), dict(T=65), dict(n_q=0), dict(n_q=5), dict(pos=None), dict(visible=A), dict(depth=A),
+                dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(out=None), dict(out=A + 2), dict(status=None)):
+        a = {**good, **bad}
+        assert L.lib.nwc_kv_attention(None, cache(L), *a.values()) == -1, bad
+    a = {**good, "T": 1025, "visible": A, "depth": A}
+    assert L.lib.nwc_kv_attention(None, cache(L, capacity=4096), *a.values()) == -1
+
+
+def test_read_and_commit_refusals(L):
+    for first, count in ((0, 0), (0, 65), (64, 1), (0xFFFFFFFF, 2)):
+        assert L.lib.nwc_kv_read(None, cache(L), 0, first, count, A, A) == -1
+    ring = cache(L, window=20, sinks=4)
+    for first, count in ((4, 61), (100, 61), (0, 65), (0x7FFFFFFF, 1)):
+        assert L.lib.nwc_kv_read(None, ring, 0, first, count, A, A) == -1
+    assert L.lib.nwc_kv_read(None, cache(L), 0, 0, 4, A + 8, A) == -1 and L.lib.nwc_kv_read(None, cache(L), 0, 0, 4, A, None) == -1
+    for T, most, path in ((0, 0, A), (1025, 3, A), (3, 4, A), (3, 3, None), (65, 3, A)):
+        assert L.lib.nwc_kv_commit(None, cache(L), T, A, path, A, most, A) == -1
+    assert L.lib.nwc_kv_commit(None, cache(L), 3, A, A, A, 0, A) == 0                       # an empty path: nothing to launch
+
+
+def test_python_refusals():
+    from nwc_b200 import KVCache
+    bf = torch.zeros(1, 2, 8, 64, dtype=torch.bfloat16)
+    codes, byte = torch.zeros(1, 2, 8, 64, dtype=torch.uint8).view(torch.float8_e4m3fn), torch.zeros(1, 2, 8, dtype=torch.uint8)
+    for args, kw, text in (((bf, bf[:, :1]), {}, "one type"), ((bf.float(), bf.float()), {}, "bfloat16 or float8"), ((bf.transpose(1, 2), bf.transpose(1, 2)), {}, "contiguous"),
+                           ((codes, codes), {}, "exponent bytes"), ((bf, bf, byte, byte), {}, "exponent bytes"), ((codes, codes, byte, byte[:, :, :4]), {}, "exponent bytes are"),
+                           ((bf[..., :32].contiguous(), bf[..., :32].contiguous()), {}, "head_dim"), ((bf, bf), dict(window=-1), "negative"), ((bf, bf), dict(sinks=2), "need a window"),
+                           ((bf, bf), dict(window=8, sinks=1), "capacity of 9"), ((bf, bf), {}, "CUDA")):
+        with pytest.raises(ValueError, match=text): KVCache.over(*args, **kw)
+
+
+def test_draft_tree_masks():
+    from nwc_b200 import draft_tree
+    parents = [-1, 0, 0, 2, -1] + [4 + i for i in range(40)]
+    visible, depth = draft_tree(parents, "cpu")
+    assert visible.shape == (45, 2) and depth.tolist()[:6] == [0, 1, 1, 2, 0, 1] and int(depth[-1]) == 40
+    for t in range(45):
+        seen, at = set(), t
+        while at >= 0: seen.add(at); at = parents[at]
+        assert {j for j in range(45) if (int(visible[t, j // 32]) >> (j % 32)) & 1} == seen
+    for bad in ([], [0], [-1, 1], [-1, -2], list(range(-1, 1024))):
+        with pytest.raises(ValueError): draft_tree(bad, "cpu")
+
+
+def test_reference_rounding_is_that_of_the_type():
+    y = torch.cat([torch.arange(256, dtype=torch.uint8).view(torch.float8_e4m3fn).double(), torch.linspace(-448, 448, 20001, dtype=torch.float64),
+                   torch.linspace(-0.03, 0.03, 20001, dtype=torch.float64)])
+    y = y[torch.isfinite(y)].float().double()
+    assert torch.equal(R.rounded_e4m3(y), y.float().to(torch.float8_e4m3fn).double())
+    x = torch.tensor([[448.0], [449.0], [0.0], [447.0], [224.0], [225.0], [1e-45]])
+    assert R.unit_exponent(x).tolist() == [0, 1, -127, 0, -1, 0, -127]
+
+
+def test_reference_attention_in_a_case_done_by_hand():
+    k = torch.tensor([[[0.0], [0.0], [9.0], [0.0]]], dtype=torch.float64); v = torch.tensor([[[1.0], [3.0], [100.0], [8.0]]], dtype=torch.float64)
+    q = torch.tensor([[[1.0]], [[1.0]]], dtype=torch.float64)
+    out, weight = R.attend(q, k, v, pos=0)
+    assert out.flatten().tolist() == [1.0, 2.0] and weight.flatten().tolist() == [1.0, 2.0]
+    out, _ = R.attend(q, k, v, pos=0, visible=R.tree_bits(2, [[], [1]]), depth=torch.tensor([0, 0]))
+    assert out.flatten().tolist() == [0.0, 3.0]
+    # ring of three behind one sink: position 4 lives in slot 1, 5 in slot 2
+    out, _ = R.attend(q[:1], k, v, pos=4, window=1, sinks=1)
+    assert out.item() == 2.0
