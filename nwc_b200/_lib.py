@@ -71,7 +71,8 @@ _SIGNATURES = {
     "nwc_comm_slot": (P, [P, U32, I]),
     "nwc_kv_append": (I, [P, P, U32, P, U64, U32, U32, P, P, P, P, U32, P, P, ctypes.c_float, P, P]),
     "nwc_kv_read": (I, [P, P, U32, U32, U32, P, P]),
-    "nwc_kv_attention": (I, [P, P, U32, P, U64, U32, U32, P, P, P, ctypes.c_float, P, P]),
+    "nwc_kv_attention": (I, [P, P, U32, P, U64, U32, U32, P, P, P, ctypes.c_float, P, P, U64, P]),
+    "nwc_kv_attention_workspace": (U64, [P, U32, U32]),
     "nwc_kv_commit": (I, [P, P, U32, P, P, P, U32, P]),
     "nwc_allreduce_add_rmsnorm": (I, [P, P, I, I, I, P, P, P, ctypes.c_float, U32, P]),
 }

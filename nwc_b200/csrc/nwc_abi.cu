@@ -4,6 +4,7 @@
 #include "../../include/nwc_ops.h"
 #include "nwc_encode.h"
 #include "nwc_launch.h"
+#include "nwc_kv.h"
 
 #define NWC_EXPORT extern "C" __attribute__((visibility("default")))
 
@@ -26,6 +27,7 @@ int device_sms() {
     configure_segment_kernels();
     configure_model_kernels();
     configure_prefill_kernels();
+    configure_kv_kernels();
     prepare_static_scratch();
     g_sm_count[dev] = sms;
     return sms;
@@ -253,7 +255,7 @@ NWC_EXPORT int nwc_ref_fp8(void *stream, const uint8_t *w, const float *scale, c
 NWC_EXPORT int nwc_setup(void) { return device_sms(); }
 
 NWC_EXPORT int nwc_kernel_status(int clear) {
-    const int v[4] = {read_kernel_status(clear != 0), read_prefill_status(clear != 0), read_comm_status(clear != 0), read_model_status(clear != 0)};
+    const int v[5] = {read_kernel_status(clear != 0), read_prefill_status(clear != 0), read_comm_status(clear != 0), read_model_status(clear != 0), read_kv_status(clear != 0)};
     int worst = v[0];
     for (int i = 1; i < 4; i++) if (v[i] > worst) worst = v[i];
     return worst;

@@ -256,12 +256,31 @@ NWC_EXPORT int nwc_kv_commit(void *stream, const nwc_kv_cache *cache, uint32_t T
     return (int)launch(kv_commit_kernel, dim3(cache->layers * cache->n_kv), dim3(64), stream, layer_of(cache, 0u), row_bytes, T, pos, path, count, most, status);
 }
 
+/* fp32 sums and (maximum, sum) pairs of every split: 0 where the keys are not divided */
+static uint64_t workspace_bytes(uint32_t splits, uint32_t T, uint32_t n_q, uint32_t head_dim) {
+    return splits == 1u ? 0u : (uint64_t)splits * T * n_q * (head_dim + 2u) * sizeof(float);
+}
+
+NWC_EXPORT uint64_t nwc_kv_attention_workspace(const nwc_kv_cache *cache, uint32_t T, uint32_t n_q) {
+    if (!cache || !T || T > NWC_KV_MAX_TOKENS || !n_q || n_q > 65535u || !cache->n_kv || n_q % cache->n_kv) return 0;
+    const int sms = nwc_setup();
+    if (sms <= 0) return 0;
+    return workspace_bytes(kv_attention_splits(cache->head_dim, cache->n_kv, cache->capacity, cache->window, cache->sinks, T, n_q, sms), T, n_q, cache->head_dim);
+}
+
 NWC_EXPORT int nwc_kv_attention(void *stream, const nwc_kv_cache *cache, uint32_t layer, const uint16_t *q, uint64_t ldq, uint32_t T, uint32_t n_q,
-                                const int32_t *pos, const uint32_t *visible, const int32_t *depth, float scale, uint16_t *out, int *status) {
+                                const int32_t *pos, const uint32_t *visible, const int32_t *depth, float scale, uint16_t *out, void *workspace,
+                                uint64_t workspace_size, int *status) {
     if (!cache_ok(cache, layer, T) || !T || T > NWC_KV_MAX_TOKENS || !n_q || n_q % cache->n_kv || n_q > 65535u) return -1;
-    if (!q || !pos || !out || !status || !aligned16(q) || !aligned16(out) || ldq < (uint64_t)n_q * cache->head_dim || ldq % 8u) return -1;
+    if (!q || !pos || !out || !status || !aligned16(q) || !aligned16(out) || !aligned16(workspace) || ldq < (uint64_t)n_q * cache->head_dim || ldq % 8u) return -1;
     if (visible ? T > NWC_KV_MAX_TREE || !depth : depth != nullptr) return -1;
     if (!(scale > 0.f) || scale > 3e38f) return -1;
-    const KvAttention a{layer_of(cache, layer), q, ldq, T, n_q, pos, visible, depth, scale * 1.4426950408889634f, out, status};
-    return (int)launch_kv_attention((cudaStream_t)stream, cache->elem, cache->head_dim, a);
+    const int sms = nwc_setup();
+    if (sms <= 0) return (int)cudaErrorNoDevice;
+    const uint32_t splits = kv_attention_splits(cache->head_dim, cache->n_kv, cache->capacity, cache->window, cache->sinks, T, n_q, sms);
+    const uint64_t need = workspace_bytes(splits, T, n_q, cache->head_dim);
+    if (need && (!workspace || workspace_size < need)) return -1;
+    float *part_o = static_cast<float *>(workspace), *part_ml = need ? part_o + (uint64_t)splits * T * n_q * cache->head_dim : nullptr;
+    const KvAttention a{layer_of(cache, layer), q, ldq, T, n_q, pos, visible, depth, scale * 1.4426950408889634f, out, status, part_o, part_ml, splits};
+    return (int)launch_kv_attention((cudaStream_t)stream, cache->elem, cache->head_dim, a, sms);
 }

@@ -83,7 +83,14 @@ struct KvAttention {
     float scale;                 /* softmax scale times log2(e) */
     uint16_t *out;               /* bf16 [T][n_q * head_dim] */
     int *status;
+    /* where the keys are divided over `splits` CTAs, each leaves its share here (row = token * n_q + head):
+       part_o fp32 [splits][T * n_q][head_dim] unnormalised, part_ml fp32 [splits][T * n_q][2] = running maximum (log2), sum */
+    float *part_o, *part_ml;
+    uint32_t splits;
 };
-cudaError_t launch_kv_attention(cudaStream_t st, int elem, uint32_t head_dim, const KvAttention &a);
+uint32_t kv_attention_splits(uint32_t head_dim, uint32_t n_kv, uint32_t capacity, uint32_t window, uint32_t sinks, uint32_t T, uint32_t n_q, int sms);
+cudaError_t launch_kv_attention(cudaStream_t st, int elem, uint32_t head_dim, const KvAttention &a, int sms);
+void configure_kv_kernels();                 /* per-device shared-memory opt-ins */
+int read_kv_status(bool clear);              /* 0, or 2 when a bounded wait gave up */
 
 }  // namespace nwc

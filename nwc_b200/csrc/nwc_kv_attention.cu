@@ -1,99 +1,448 @@
-/* Attention of one or many tokens over a cache of nwc_kv.h: o_t = sum over the positions p that token t sees of
+/* Attention of a few query rows over a cache of nwc_kv.h: o_t = sum over the positions p that token t sees of
  * softmax_p(scale q_t . k_p) v_p, grouped heads; zeros where a token sees nothing.
  *
  * What token t (position own = pos + t, or pos + depth[t] with a draft tree) sees:
  *   p < pos + T with p <= own (no tree) or p < pos or bit p - pos of visible[t] (tree); and, with a window and for p that are
  *   not drafted, p < sinks or p > own - window.
+ *
+ * One token reads every visible row once and computes little: the bound is the memory's rate.  So the rows of a key/value
+ * head are read once for all of its query rows (T * group of them, 16 or 32 at a time: the M of mma.m16n8k16), the keys are
+ * divided over the CTAs of the whole GPU, and every warp streams its own tiles through a ring of bulk copies in shared memory,
+ * deep enough to keep the memory busy.  There is no barrier between the warps of a CTA until their shares are joined.
+ *
+ * Fragments.  A dot product may add its terms in any order, so the B fragment of K takes the 16-byte piece that a lane reads
+ * from a key's row as it lies, and Q is laid out once to match; likewise the columns of V: the n-th column of an MMA is the
+ * dimension that lane group n's piece holds at that place.  Neither K nor V is ever transposed or re-stored.  e4m3 codes become
+ * bf16 in registers (a code is exact in bf16); the unit 2^e of a K row multiplies its scores, that of a V row its weights.
+ * The weights are rounded to bf16 for the second product (2^-9 relative on average, averaged out over the keys): the sum of
+ * the weights, the running maximum, and all accumulators are fp32.
  */
 #include "nwc_kv.h"
+#include "nwc_async.cuh"
 #include "nwc_launch.h"
 
 namespace nwc {
+
+namespace {
 
 __device__ __forceinline__ void kv_dependency_sync() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
 }
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) { uint32_t d; asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(b), "f"(a)); return d; }
+__device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+/* codes (already in the high bytes of both halves of w; the low bytes may hold anything) -> bf16 pair */
+__device__ __forceinline__ uint32_t codes_to_bf16(uint32_t w) { return kv_mul2(((w >> 4) & 0x07F007F0u) | (w & 0x80008000u), kTwoTo120); }
 
-/* The plain kernel: one CTA per token and query head, its warps take the visible positions in turn, lanes own head_dim / 32
-   numbers each; online softmax in fp32. */
-template <int VPL, int ELEM>
-__global__ void __launch_bounds__(128) kv_attention_plain_kernel(const KvAttention a) {
-    constexpr uint32_t HD = 32u * VPL, kWarps = 4;
-    __shared__ float part_max[kWarps], part_den[kWarps], part_acc[kWarps][HD];
-    const uint32_t t = blockIdx.x, head = blockIdx.y, kvh = head / (a.n_q / a.c.n_kv), lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, d0 = lane * VPL;
+/* Shape of the few-rows kernel: tiles of kKeys keys per warp, kStages of them in flight. */
+template <int HD, int ELEM> struct Few {
+    static constexpr uint32_t kRowBytes = HD * (ELEM == kKvE4m3 ? 1u : 2u);
+    static constexpr uint32_t kKeys = ELEM == kKvE4m3 ? 32u : 16u;
+    static constexpr uint32_t kStageBytes = 2u * kKeys * kRowBytes;                     /* K and V */
+    static constexpr uint32_t kWarps = HD == 256 ? 4u : 8u, kStages = HD == 64 ? 4u : 3u;
+    static constexpr uint32_t kRing = kWarps * kStages * kStageBytes;
+};
+template <int HD, int ELEM, int MT> __host__ __device__ constexpr uint32_t few_smem() {
+    return Few<HD, ELEM>::kRing + MT * 16u * HD * 2u + Few<HD, ELEM>::kWarps * Few<HD, ELEM>::kStages * 8u + 2u * Few<HD, ELEM>::kWarps * MT * 16u * 4u;
+}
+
+}  // namespace
+
+template <int HD, int ELEM, int MT>
+__global__ void __launch_bounds__(32 * Few<HD, ELEM>::kWarps, 1) kv_attention_few_kernel(const KvAttention a) {
+    using F = Few<HD, ELEM>;
+    constexpr uint32_t kRows = 16u * MT, kNT = F::kKeys / 8u, kSteps = HD / 16u, kWarps = F::kWarps;
+    extern __shared__ __align__(128) uint8_t few_raw[];
+    const uint32_t ring = smem_addr(few_raw), tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, g = lane >> 2, c = lane & 3u;
+    uint8_t *qs = few_raw + F::kRing;                                                  /* Q in fragment order: [kSteps][MT][32 lanes] uint4 */
+    const uint32_t bars = smem_addr(qs + kRows * HD * 2u), mine = ring + warp * F::kStages * F::kStageBytes, my_bars = bars + warp * F::kStages * 8u;
+    float *part_m = reinterpret_cast<float *>(qs + kRows * HD * 2u + kWarps * F::kStages * 8u), *part_l = part_m + kWarps * kRows;
+    const uint32_t group = a.n_q / a.c.n_kv, rows = a.T * group, kvh = blockIdx.y % a.c.n_kv, row0 = (blockIdx.y / a.c.n_kv) * kRows, split = blockIdx.x;
+    if (lane == 0) {
+        for (uint32_t s = 0; s < F::kStages; s++) mbar_init(my_bars + s * 8u, 1u);
+        mbar_init_fence();
+    }
+    __syncwarp();
     kv_dependency_sync();
     const int32_t pos = *a.pos;
-    const uint32_t limit = a.c.window ? 0x7FFFFFFFu : a.c.capacity;
-    if (pos < 0 || (uint64_t)pos + a.T > limit) { if (threadIdx.x == 0) atomicOr(a.status, kKvStatusPosition); return; }
+    if (pos < 0 || (uint64_t)pos + a.T > (a.c.window ? 0x7FFFFFFFu : a.c.capacity)) { if (tid == 0) atomicOr(a.status, kKvStatusPosition); return; }
     const KvSpan span = kv_span(pos, a.T, a.c.window, a.c.sinks);
-    const uint32_t own = a.depth ? (uint32_t)(pos + a.depth[t]) : (uint32_t)pos + t, words = (a.T + 31u) / 32u;
-    float q[VPL], acc[VPL], m = -INFINITY, den = 0.f;
-    const uint16_t *qp = a.q + (uint64_t)t * a.ldq + (uint64_t)head * HD + d0;
-#pragma unroll
-    for (int j = 0; j < VPL; j++) { q[j] = __uint_as_float((uint32_t)qp[j] << 16) * a.scale; acc[j] = 0.f; }
-    for (uint32_t i = warp; i < span.count; i += kWarps) {
-        const uint32_t p = i < span.lead ? i : span.first + (i - span.lead);
-        bool sees = !a.c.window || p < a.c.sinks || p + a.c.window > own;
-        if (!a.visible) sees = sees && p <= own;
-        else if (p >= (uint32_t)pos) { const uint32_t j = p - (uint32_t)pos; sees = (a.visible[(uint64_t)t * words + (j >> 5)] >> (j & 31u)) & 1u; }
-        if (!sees) continue;
-        const uint64_t cell = (uint64_t)kvh * a.c.capacity + kv_slot(p, a.c.capacity, a.c.window, a.c.sinks);
-        float k[VPL], v[VPL];
-        if (ELEM == kKvBf16) {
-            const uint16_t *kp = reinterpret_cast<const uint16_t *>(a.c.k) + cell * HD + d0, *vp = reinterpret_cast<const uint16_t *>(a.c.v) + cell * HD + d0;
-#pragma unroll
-            for (int j = 0; j < VPL; j++) { k[j] = __uint_as_float((uint32_t)kp[j] << 16); v[j] = __uint_as_float((uint32_t)vp[j] << 16); }
-        } else {
-            const uint32_t ku = kv_unit2(a.c.k_exp[cell]), vu = kv_unit2(a.c.v_exp[cell]);
-            const uint8_t *kp = a.c.k + cell * HD + d0, *vp = a.c.v + cell * HD + d0;
-#pragma unroll
-            for (int j = 0; j < VPL; j += 2) {
-                uint32_t kw, vw, none;
-                kv_values4((uint32_t)kp[j] | ((uint32_t)kp[j + 1] << 8), ku, kw, none);
-                kv_values4((uint32_t)vp[j] | ((uint32_t)vp[j + 1] << 8), vu, vw, none);
-                k[j] = __uint_as_float(kw << 16); k[j + 1] = __uint_as_float(kw & 0xFFFF0000u);
-                v[j] = __uint_as_float(vw << 16); v[j + 1] = __uint_as_float(vw & 0xFFFF0000u);
+    /* this CTA's keys, in tiles of kKeys; tile i of a warp is the CTA's tile warp + i * kWarps */
+    const uint32_t all_tiles = (span.count + F::kKeys - 1u) / F::kKeys, first_tile = (uint32_t)((uint64_t)all_tiles * split / a.splits), last_tile = (uint32_t)((uint64_t)all_tiles * (split + 1u) / a.splits);
+    const uint32_t my_tiles = last_tile - first_tile > warp ? (last_tile - first_tile - warp + kWarps - 1u) / kWarps : 0u;
+    auto position = [&](uint32_t i) { return i < span.lead ? i : span.first + (i - span.lead); };
+    auto slot_of = [&](uint32_t i) { return kv_slot(position(i), a.c.capacity, a.c.window, a.c.sinks); };
+    auto issue = [&](uint32_t i) {
+        const uint32_t s = i % F::kStages, key0 = (first_tile + warp + i * kWarps) * F::kKeys, n = min(F::kKeys, span.count - key0);
+        const uint32_t dst = mine + s * F::kStageBytes, bar = my_bars + s * 8u;
+        const uint32_t a0 = slot_of(key0);
+        const bool straight = slot_of(key0 + n - 1u) == a0 + n - 1u;                    /* neither the end of the sinks nor of the ring inside */
+        const uint64_t cell = (uint64_t)kvh * a.c.capacity;
+        if (lane == 0) {
+            mbar_expect(bar, 2u * n * F::kRowBytes);
+            if (straight) {
+                bulk_load(dst, a.c.k + (cell + a0) * F::kRowBytes, n * F::kRowBytes, bar);
+                bulk_load(dst + F::kKeys * F::kRowBytes, a.c.v + (cell + a0) * F::kRowBytes, n * F::kRowBytes, bar);
             }
         }
-        float s = 0.f;
-#pragma unroll
-        for (int j = 0; j < VPL; j++) s = fmaf(q[j], k[j], s);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        const float m_new = fmaxf(m, s), corr = m_new == -INFINITY ? 1.f : exp2f(m - m_new), w = m_new == -INFINITY ? 0.f : exp2f(s - m_new);
-        den = den * corr + w;
-#pragma unroll
-        for (int j = 0; j < VPL; j++) acc[j] = fmaf(w, v[j], acc[j] * corr);
-        m = m_new;
-    }
-    if (lane == 0) { part_max[warp] = m; part_den[warp] = den; }
-#pragma unroll
-    for (int j = 0; j < VPL; j++) part_acc[warp][d0 + j] = acc[j];
-    __syncthreads();
-    float top = part_max[0];
-    for (uint32_t w = 1; w < kWarps; w++) top = fmaxf(top, part_max[w]);
-    for (uint32_t d = threadIdx.x; d < HD; d += blockDim.x) {
-        float total = 0.f, o = 0.f;
-        for (uint32_t w = 0; w < kWarps; w++) {
-            const float f = top == -INFINITY ? 0.f : exp2f(part_max[w] - top);
-            total = fmaf(part_den[w], f, total); o = fmaf(part_acc[w][d], f, o);
+        if (!straight) {
+            __syncwarp();
+            if (lane < n) {
+                const uint64_t row = cell + slot_of(key0 + lane);
+                bulk_load(dst + lane * F::kRowBytes, a.c.k + row * F::kRowBytes, F::kRowBytes, bar);
+                bulk_load(dst + (F::kKeys + lane) * F::kRowBytes, a.c.v + row * F::kRowBytes, F::kRowBytes, bar);
+            }
         }
-        const float r = total == 0.f ? 0.f : o / total;
-        a.out[((uint64_t)t * a.n_q + head) * HD + d] = __bfloat16_as_ushort(__float2bfloat16_rn(r));
+    };
+    /* the exponent bytes of the key that this lane stands for in tile i: K's in the low, V's in the high half */
+    auto units = [&](uint32_t i) -> uint32_t {
+        if (ELEM != kKvE4m3) return 0u;
+        const uint32_t key = (first_tile + warp + i * kWarps) * F::kKeys + lane;
+        if (i >= my_tiles || key >= span.count) return 0u;
+        const uint64_t cell = (uint64_t)kvh * a.c.capacity + slot_of(key);
+        return (uint32_t)a.c.k_exp[cell] | (uint32_t)a.c.v_exp[cell] << 16;
+    };
+    for (uint32_t i = 0; i < F::kStages && i < my_tiles; i++) issue(i);
+    uint32_t unit_now = units(0u);
+    /* Q: the 16-byte (e4m3: 2 x 16-byte) piece of a row that meets the K piece of lane c, in the order the codes unfold to */
+    for (uint32_t e = tid; e < kRows * HD / 8u; e += blockDim.x) {
+        const uint32_t r = e / (HD / 8u), d = (e % (HD / 8u)) * 8u, row = row0 + r;
+        uint4 w = make_uint4(0u, 0u, 0u, 0u);
+        if (row < rows) w = *reinterpret_cast<const uint4 *>(a.q + (uint64_t)(row / group) * a.ldq + (uint64_t)(kvh * group + row % group) * HD + d);
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (uint32_t j = 0; j < 4u; j++) {                                            /* dimensions d + 2j, d + 2j + 1 */
+            uint32_t step, cc, half;
+            if (ELEM == kKvE4m3) { const uint32_t dd = d + 2u * j, in = dd & 15u; cc = (dd >> 4) & 3u; step = (dd >> 6) * 4u + (in >> 2); half = (in >> 1) & 1u; }
+            else { const uint32_t dd = d + 2u * j, in = dd & 7u; cc = (dd >> 3) & 3u; step = (dd >> 5) * 2u + (in >> 2); half = (in >> 1) & 1u; }
+            const uint32_t at = ((step * MT + (r >> 4)) * 32u + (r & 7u) * 4u + cc) * 4u + half * 2u + ((r >> 3) & 1u);      /* a0 a1 a2 a3 = (g, lo) (g + 8, lo) (g, hi) (g + 8, hi) */
+            reinterpret_cast<uint32_t *>(qs)[at] = u[j];
+        }
+    }
+    __syncthreads();
+    /* this lane's rows: token and own position */
+    uint32_t token[2 * MT], own[2 * MT], own_min = 0xFFFFFFFFu, own_max = 0u;
+#pragma unroll
+    for (uint32_t i = 0; i < 2u * MT; i++) {
+        const uint32_t row = min(row0 + (i >> 1) * 16u + (i & 1u) * 8u + g, rows - 1u);
+        token[i] = row / group;
+        own[i] = (uint32_t)pos + (a.depth ? (uint32_t)a.depth[token[i]] : token[i]);
+        own_min = min(own_min, own[i]); own_max = max(own_max, own[i]);
+    }
+    own_max = __reduce_max_sync(0xffffffffu, own_max); own_min = __reduce_min_sync(0xffffffffu, own_min);
+    const uint32_t open_end = a.visible ? (uint32_t)pos : own_min + 1u;                 /* positions below it are seen by every row, window apart */
+    const uint32_t words = (a.T + 31u) / 32u;
+    float o[MT][HD / 8][4], m[2 * MT], l[2 * MT];
+#pragma unroll
+    for (uint32_t i = 0; i < MT; i++)
+#pragma unroll
+        for (uint32_t j = 0; j < HD / 8u; j++)
+#pragma unroll
+            for (uint32_t e = 0; e < 4u; e++) o[i][j][e] = 0.f;
+#pragma unroll
+    for (uint32_t i = 0; i < 2u * MT; i++) { m[i] = -INFINITY; l[i] = 0.f; }
+    bool alive = true;                                                                  /* a wait that gave up: no new copies, but those in flight are waited for */
+    uint32_t issued = min(F::kStages, my_tiles);
+    for (uint32_t it = 0; it < issued; it++) {
+        const uint32_t s = it % F::kStages, key0 = (first_tile + warp + it * kWarps) * F::kKeys, n = min(F::kKeys, span.count - key0);
+        const uint32_t kt = mine + s * F::kStageBytes, vt = kt + F::kKeys * F::kRowBytes;
+        const uint32_t unit = unit_now;
+        alive = mbar_wait(my_bars + s * 8u, (it / F::kStages) & 1u) && alive;
+        if (!alive) continue;
+        unit_now = units(it + 1u);
+        if (n < F::kKeys) {                                                             /* V rows behind the last key: weight 0 times whatever lies there must be 0 */
+            for (uint32_t e = lane; e < (F::kKeys - n) * (F::kRowBytes / 16u); e += 32u) asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vt + n * F::kRowBytes + e * 16u), "r"(0u) : "memory");
+            __syncwarp();
+        }
+        /* scores */
+        float sc[MT][kNT][4];
+#pragma unroll
+        for (uint32_t i = 0; i < MT; i++)
+#pragma unroll
+            for (uint32_t j = 0; j < kNT; j++)
+#pragma unroll
+                for (uint32_t e = 0; e < 4u; e++) sc[i][j][e] = 0.f;
+        constexpr uint32_t kPieces = F::kRowBytes / 64u, kStepsPerPiece = ELEM == kKvE4m3 ? 4u : 2u;
+#pragma unroll
+        for (uint32_t pc = 0; pc < kPieces; pc++) {
+            uint4 qf[kStepsPerPiece][MT];
+#pragma unroll
+            for (uint32_t st = 0; st < kStepsPerPiece; st++)
+#pragma unroll
+                for (uint32_t i = 0; i < MT; i++) qf[st][i] = reinterpret_cast<const uint4 *>(qs)[((pc * kStepsPerPiece + st) * MT + i) * 32u + lane];
+#pragma unroll
+            for (uint32_t j = 0; j < kNT; j++) {
+                const uint4 w = lds128(kt + (j * 8u + g) * F::kRowBytes + pc * 64u + c * 16u);
+                const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+                if (ELEM == kKvE4m3) {
+#pragma unroll
+                    for (uint32_t st = 0; st < 4u; st++) {
+                        const uint32_t b0 = codes_to_bf16(__byte_perm(u[st], 0u, 0x1404)), b1 = codes_to_bf16(__byte_perm(u[st], 0u, 0x3424));
+#pragma unroll
+                        for (uint32_t i = 0; i < MT; i++) mma16816(sc[i][j], qf[st][i], b0, b1);
+                    }
+                } else {
+#pragma unroll
+                    for (uint32_t st = 0; st < 2u; st++)
+#pragma unroll
+                        for (uint32_t i = 0; i < MT; i++) mma16816(sc[i][j], qf[st % kStepsPerPiece][i], u[2 * st], u[2 * st + 1]);
+                }
+            }
+        }
+        /* log2 scores, masked; a tile that every row sees whole needs no mask */
+        const uint32_t p_first = position(key0), p_last = position(key0 + n - 1u);
+        const bool open = n == F::kKeys && p_last < open_end && (!a.c.window || p_last < a.c.sinks || (p_first > own_max || own_max - p_first < a.c.window));
+#pragma unroll
+        for (uint32_t j = 0; j < kNT; j++) {
+#pragma unroll
+            for (uint32_t b = 0; b < 2u; b++) {
+                const uint32_t kk = j * 8u + 2u * c + b;
+                float f = a.scale;
+                if (ELEM == kKvE4m3) f *= kv_unit(__shfl_sync(0xffffffffu, unit, kk) & 0xFFFFu);
+#pragma unroll
+                for (uint32_t i = 0; i < MT; i++) { sc[i][j][b] *= f; sc[i][j][b + 2] *= f; }
+            }
+        }
+        if (!open) {
+#pragma unroll
+            for (uint32_t j = 0; j < kNT; j++)
+#pragma unroll
+                for (uint32_t b = 0; b < 2u; b++) {
+                    const uint32_t kk = j * 8u + 2u * c + b, p = position(key0 + kk);
+#pragma unroll
+                    for (uint32_t i = 0; i < 2u * MT; i++) {
+                        bool sees = kk < n && (!a.c.window || p < a.c.sinks || p + a.c.window > own[i]);
+                        if (!a.visible) sees = sees && p <= own[i];
+                        else if (p >= (uint32_t)pos && kk < n) { const uint32_t d = p - (uint32_t)pos; sees = (a.visible[(uint64_t)token[i] * words + (d >> 5)] >> (d & 31u)) & 1u; }
+                        if (!sees) sc[i >> 1][j][b + 2u * (i & 1u)] = -INFINITY;
+                    }
+                }
+        }
+        /* running maximum: raised (and the sums rescaled) only when some row's tile maximum passes it by more than 2^8, so
+           weights stay below 2^8 and the rescaling is rare */
+        bool raise = false;
+        float top[2 * MT];
+#pragma unroll
+        for (uint32_t i = 0; i < 2u * MT; i++) {
+            float t = -INFINITY;
+#pragma unroll
+            for (uint32_t j = 0; j < kNT; j++) t = fmaxf(t, fmaxf(sc[i >> 1][j][2u * (i & 1u)], sc[i >> 1][j][2u * (i & 1u) + 1u]));
+            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1)); t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+            top[i] = t; raise = raise || t > m[i] + 8.f;
+        }
+        if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+            for (uint32_t i = 0; i < 2u * MT; i++) {
+                const float up = fmaxf(m[i], top[i]), f = up == -INFINITY ? 1.f : exp2_fast(m[i] - up);
+                m[i] = up; l[i] *= f;
+#pragma unroll
+                for (uint32_t j = 0; j < HD / 8u; j++) { o[i >> 1][j][2u * (i & 1u)] *= f; o[i >> 1][j][2u * (i & 1u) + 1u] *= f; }
+            }
+        }
+        float base[2 * MT];
+#pragma unroll
+        for (uint32_t i = 0; i < 2u * MT; i++) base[i] = m[i] == -INFINITY ? 0.f : m[i];
+#pragma unroll
+        for (uint32_t j = 0; j < kNT; j++)
+#pragma unroll
+            for (uint32_t b = 0; b < 2u; b++) {
+                const float vu = ELEM == kKvE4m3 ? kv_unit(__shfl_sync(0xffffffffu, unit, j * 8u + 2u * c + b) >> 16) : 1.f;
+#pragma unroll
+                for (uint32_t i = 0; i < 2u * MT; i++) {
+                    float &x = sc[i >> 1][j][2u * (i & 1u) + b];
+                    x = exp2_fast(x - base[i]);
+                    l[i] += x;
+                    if (ELEM == kKvE4m3) x *= vu;
+                }
+            }
+        /* o += P V, 16 keys at a time; lane (g, c) holds keys 2c, 2c + 1, 2c + 8, 2c + 9 of the columns of piece g */
+#pragma unroll
+        for (uint32_t h = 0; h < kNT / 2u; h++) {
+            uint4 pf[MT];
+#pragma unroll
+            for (uint32_t i = 0; i < MT; i++)
+                pf[i] = make_uint4(pack_bf16(sc[i][2 * h][0], sc[i][2 * h][1]), pack_bf16(sc[i][2 * h][2], sc[i][2 * h][3]),
+                                   pack_bf16(sc[i][2 * h + 1][0], sc[i][2 * h + 1][1]), pack_bf16(sc[i][2 * h + 1][2], sc[i][2 * h + 1][3]));
+            const uint32_t v0 = vt + (h * 16u + 2u * c) * F::kRowBytes;
+            constexpr uint32_t kPieceDims = ELEM == kKvE4m3 ? (HD == 64 ? 8u : 16u) : 8u, kVPieces = HD / (8u * kPieceDims);
+#pragma unroll
+            for (uint32_t pc = 0; pc < kVPieces; pc++) {
+                uint32_t w[4][4];                                                       /* [key][word] */
+#pragma unroll
+                for (uint32_t e = 0; e < 4u; e++) {
+                    const uint32_t from = v0 + ((e & 1u) + (e >> 1) * 8u) * F::kRowBytes;
+                    if (ELEM == kKvE4m3 && HD == 64) { const uint2 x = lds64(from + g * 8u); w[e][0] = x.x; w[e][1] = x.y; }
+                    else { const uint4 x = lds128(from + pc * 128u + g * 16u); w[e][0] = x.x; w[e][1] = x.y; w[e][2] = x.z; w[e][3] = x.w; }
+                }
+                if (ELEM == kKvE4m3) {
+#pragma unroll
+                    for (uint32_t d = 0; d < kPieceDims; d++) {
+                        /* byte d % 4 of the two keys' words into the high bytes of the halves */
+                        const uint32_t sel = (d & 3u) << 4 | ((d & 3u) + 4u) << 12;
+                        const uint32_t b0 = codes_to_bf16(__byte_perm(w[0][d >> 2], w[1][d >> 2], sel)), b1 = codes_to_bf16(__byte_perm(w[2][d >> 2], w[3][d >> 2], sel));
+#pragma unroll
+                        for (uint32_t i = 0; i < MT; i++) mma16816(o[i][pc * kPieceDims + d], pf[i], b0, b1);
+                    }
+                } else {
+#pragma unroll
+                    for (uint32_t d = 0; d < 8u; d++) {
+                        const uint32_t sel = d & 1u ? 0x7632u : 0x5410u;
+                        const uint32_t b0 = __byte_perm(w[0][d >> 1], w[1][d >> 1], sel), b1 = __byte_perm(w[2][d >> 1], w[3][d >> 1], sel);
+#pragma unroll
+                        for (uint32_t i = 0; i < MT; i++) mma16816(o[i][pc * 8u + d], pf[i], b0, b1);
+                    }
+                }
+            }
+        }
+        async_proxy_fence();
+        __syncwarp();
+        if (issued < my_tiles) issue(issued++);
+    }
+    /* join the warps: common maximum, then sums and outputs rescaled to it, in warp order */
+#pragma unroll
+    for (uint32_t i = 0; i < 2u * MT; i++) { l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1); l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2); }
+    __syncthreads();                                                                    /* every warp has done with its ring: O goes there */
+    float *part = reinterpret_cast<float *>(few_raw);                                   /* [kWarps][kRows][HD] */
+    static_assert(kWarps * kRows * HD * 4u <= F::kRing, "the warps' outputs fit the ring");
+    if (c == 0) {
+#pragma unroll
+        for (uint32_t i = 0; i < 2u * MT; i++) { const uint32_t r = (i >> 1) * 16u + (i & 1u) * 8u + g; part_m[warp * kRows + r] = m[i]; part_l[warp * kRows + r] = l[i]; }
+    }
+    constexpr uint32_t kPieceDims = ELEM == kKvE4m3 ? (HD == 64 ? 8u : 16u) : 8u;
+#pragma unroll
+    for (uint32_t i = 0; i < 2u * MT; i++) {
+        float *to = part + (warp * kRows + (i >> 1) * 16u + (i & 1u) * 8u + g) * HD;
+        /* accumulator j, columns 2c and 2c + 1 = place j % kPieceDims of the pieces 2c, 2c + 1 */
+#pragma unroll
+        for (uint32_t j = 0; j < HD / 8u; j++) {
+            const uint32_t d = (j / kPieceDims) * 8u * kPieceDims + 2u * c * kPieceDims + j % kPieceDims;
+            to[d] = o[i >> 1][j][2u * (i & 1u)]; to[d + kPieceDims] = o[i >> 1][j][2u * (i & 1u) + 1u];
+        }
+    }
+    __syncthreads();
+    constexpr uint32_t kOut = kRows * HD / (32u * kWarps);                              /* outputs per thread */
+#pragma unroll
+    for (uint32_t e = 0; e < kOut; e++) {
+        const uint32_t at = e * 32u * kWarps + tid, r = at / HD, d = at % HD, row = row0 + r;
+        if (row >= rows) continue;
+        float top = -INFINITY, total = 0.f, sum = 0.f;
+#pragma unroll
+        for (uint32_t w = 0; w < kWarps; w++) top = fmaxf(top, part_m[w * kRows + r]);
+#pragma unroll
+        for (uint32_t w = 0; w < kWarps; w++) {
+            const float mw = part_m[w * kRows + r], f = mw == -INFINITY ? 0.f : exp2_fast(mw - top);
+            total = fmaf(part_l[w * kRows + r], f, total); sum = fmaf(part[w * kRows * HD + at], f, sum);
+        }
+        const uint64_t line = (uint64_t)(row / group) * a.n_q + kvh * group + row % group;
+        if (a.splits == 1u) a.out[line * HD + d] = __bfloat16_as_ushort(__float2bfloat16_rn(total == 0.f ? 0.f : sum / total));
+        else {
+            const uint64_t cell = (uint64_t)split * a.T * a.n_q + line;
+            a.part_o[cell * HD + d] = sum;
+            if (d == 0) { a.part_ml[cell * 2u] = top; a.part_ml[cell * 2u + 1u] = total; }
+        }
     }
 }
 
-template <int VPL>
-static cudaError_t launch_plain(cudaStream_t st, int elem, const KvAttention &a) {
-    const dim3 grid(a.T, a.n_q);
-    if (elem == kKvE4m3) kv_attention_plain_kernel<VPL, kKvE4m3><<<grid, 128, 0, st>>>(a);
-    else kv_attention_plain_kernel<VPL, kKvBf16><<<grid, 128, 0, st>>>(a);
-    return cudaGetLastError();
+/* The shares of the splits joined in split order: one warp per output row and 128 (64) of its dimensions. */
+template <int HD>
+__global__ void __launch_bounds__(128) kv_attention_join_kernel(const KvAttention a) {
+    constexpr uint32_t kPer = HD >= 128 ? 4u : 2u, kWarpsPerRow = HD / (32u * kPer);
+    const uint32_t lane = threadIdx.x & 31u;
+    const uint64_t unit = (uint64_t)blockIdx.x * 4u + (threadIdx.x >> 5), lines = (uint64_t)a.T * a.n_q;
+    kv_dependency_sync();
+    if (unit >= lines * kWarpsPerRow) return;
+    const uint64_t line = unit / kWarpsPerRow;
+    const uint32_t d = (uint32_t)(unit % kWarpsPerRow) * 32u * kPer + lane * kPer;
+    const int32_t pos = *a.pos;
+    if (pos < 0 || (uint64_t)pos + a.T > (a.c.window ? 0x7FFFFFFFu : a.c.capacity)) return;
+    float top = -INFINITY;
+    for (uint32_t s = lane; s < a.splits; s += 32u) top = fmaxf(top, __ldcg(a.part_ml + ((uint64_t)s * lines + line) * 2u));
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    float total = 0.f, sum[kPer];
+#pragma unroll
+    for (uint32_t j = 0; j < kPer; j++) sum[j] = 0.f;
+#pragma unroll 4
+    for (uint32_t s = 0; s < a.splits; s++) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(a.part_ml) + (uint64_t)s * lines + line);
+        const float *from = a.part_o + ((uint64_t)s * lines + line) * HD + d;
+        float x[kPer];
+        if (kPer == 4u) { const float4 v = __ldcg(reinterpret_cast<const float4 *>(from)); x[0] = v.x; x[1] = v.y; x[kPer - 2] = v.z; x[kPer - 1] = v.w; }
+        else { const float2 v = __ldcg(reinterpret_cast<const float2 *>(from)); x[0] = v.x; x[1] = v.y; }
+        if (ml.x == -INFINITY) continue;
+        const float f = exp2_fast(ml.x - top);
+        total = fmaf(ml.y, f, total);
+#pragma unroll
+        for (uint32_t j = 0; j < kPer; j++) sum[j] = fmaf(x[j], f, sum[j]);
+    }
+    const float r = total == 0.f ? 0.f : 1.f / total;
+    uint16_t *to = a.out + line * HD + d;
+#pragma unroll
+    for (uint32_t j = 0; j < kPer; j += 2u) *reinterpret_cast<uint32_t *>(to + j) = pack_bf16(sum[j] * r, sum[j + 1] * r);
 }
 
-cudaError_t launch_kv_attention(cudaStream_t st, int elem, uint32_t head_dim, const KvAttention &a) {
-    return head_dim == 64u ? launch_plain<2>(st, elem, a) : head_dim == 128u ? launch_plain<4>(st, elem, a) : launch_plain<8>(st, elem, a);
+namespace {
+
+template <class... Params, class... Args>
+cudaError_t launch(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, bool dependent, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid; cfg.blockDim = block; cfg.dynamicSmemBytes = smem; cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr; cfg.numAttrs = dependent ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
+
+template <int HD, int ELEM, int MT>
+cudaError_t launch_few(cudaStream_t st, const KvAttention &a) {
+    const uint32_t rows = a.T * (a.n_q / a.c.n_kv), tiles = (rows + 16u * MT - 1u) / (16u * MT);
+    return launch(kv_attention_few_kernel<HD, ELEM, MT>, dim3(a.splits, a.c.n_kv * tiles), dim3(32u * Few<HD, ELEM>::kWarps), few_smem<HD, ELEM, MT>(), st, dependent_launch(), a);
+}
+template <int HD, int ELEM>
+cudaError_t launch_all(cudaStream_t st, const KvAttention &a) {
+    const uint32_t rows = a.T * (a.n_q / a.c.n_kv);
+    cudaError_t err;
+    if constexpr (HD == 256) err = launch_few<HD, ELEM, 1>(st, a);
+    else err = rows > 16u ? launch_few<HD, ELEM, 2>(st, a) : launch_few<HD, ELEM, 1>(st, a);
+    if (err != cudaSuccess || a.splits == 1u) return err;
+    const uint64_t units = (uint64_t)a.T * a.n_q * (HD >= 128 ? HD / 128 : 1);
+    /* (an ordinary dependent launch: the join's set-up overlaps the last CTAs; it waits for the whole grid before it reads) */
+    return launch(kv_attention_join_kernel<HD>, dim3((uint32_t)((units + 3u) / 4u)), dim3(128), 0, st, true, a);
+}
+template <int HD, int ELEM, int MT> void configure_few() { cudaFuncSetAttribute(kv_attention_few_kernel<HD, ELEM, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)few_smem<HD, ELEM, MT>()); }
+
+}  // namespace
+
+uint32_t kv_attention_splits(uint32_t head_dim, uint32_t n_kv, uint32_t capacity, uint32_t window, uint32_t sinks, uint32_t T, uint32_t n_q, int sms) {
+    const uint32_t rows = T * (n_q / n_kv), per = head_dim == 256u ? 16u : (rows > 16u ? 32u : 16u);
+    const uint64_t ctas = (uint64_t)n_kv * ((rows + per - 1u) / per), keys = window ? (uint64_t)sinks + window + T - 1u : capacity;
+    if (ctas >= (uint64_t)sms) return 1u;
+    /* no CTA below a tile for each of its warps */
+    const uint64_t most = (keys + 127u) / 128u, want = (uint64_t)sms / ctas;
+    return (uint32_t)(want < most ? want : most);
+}
+
+cudaError_t launch_kv_attention(cudaStream_t st, int elem, uint32_t head_dim, const KvAttention &a, int) {
+    if (elem == kKvE4m3) return head_dim == 64u ? launch_all<64, kKvE4m3>(st, a) : head_dim == 128u ? launch_all<128, kKvE4m3>(st, a) : launch_all<256, kKvE4m3>(st, a);
+    return head_dim == 64u ? launch_all<64, kKvBf16>(st, a) : head_dim == 128u ? launch_all<128, kKvBf16>(st, a) : launch_all<256, kKvBf16>(st, a);
+}
+
+void configure_kv_kernels() {
+    configure_few<64, kKvBf16, 1>(); configure_few<64, kKvBf16, 2>(); configure_few<64, kKvE4m3, 1>(); configure_few<64, kKvE4m3, 2>();
+    configure_few<128, kKvBf16, 1>(); configure_few<128, kKvBf16, 2>(); configure_few<128, kKvE4m3, 1>(); configure_few<128, kKvE4m3, 2>();
+    configure_few<256, kKvBf16, 1>(); configure_few<256, kKvE4m3, 1>();
+}
+
+int read_kv_status(bool clear) {
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_kernel_status, sizeof(int)) != cudaSuccess) return -1;
+    if (clear && v) { const int z = 0; cudaMemcpyToSymbol(g_kernel_status, &z, sizeof(int)); }
+    return v;
 }
 
 }  // namespace nwc

@@ -87,6 +87,7 @@ class KVCache:
         self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
         at = lambda t: None if t is None else t.data_ptr()
         self._c = L.KvCache(at(k), at(v), at(k_exp), at(v_exp), self.layers, self.n_kv, self.head_dim, self.capacity, window, sinks, 1 if quantised else 0)
+        self._need = {}                                               # workspace bytes per (tokens, query heads)
         self._ref, self._status = ctypes.byref(self._c), self.status.data_ptr()
 
     # ---- calls ----
@@ -126,8 +127,13 @@ class KVCache:
         self._int32(pos, 1, "pos")
         self._layer(layer)
         out = q.new_empty((T, n_q * hd))
+        need = self._need.get((T, n_q))
+        if need is None:
+            with torch.cuda.device(self.device): need = self._need[T, n_q] = L.lib.nwc_kv_attention_workspace(self._ref, T, n_q)
+        # a workspace of the call's own: the allocator keeps it from calls on other streams, a graph keeps it in its pool
+        work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
         self._call("nwc_kv_attention", L.lib.nwc_kv_attention, layer, q.data_ptr(), q.stride(0), T, n_q, pos.data_ptr(), None if visible is None else visible.data_ptr(),
-                   None if depth is None else depth.data_ptr(), 1.0 / math.sqrt(hd) if scale is None else float(scale), out.data_ptr(), self._status)
+                   None if depth is None else depth.data_ptr(), 1.0 / math.sqrt(hd) if scale is None else float(scale), out.data_ptr(), None if work is None else work.data_ptr(), need, self._status)
         return out
 
     def read(self, first, count, layer=0):

@@ -31,7 +31,7 @@ def test_caches_that_no_kernel_addresses(L, bad):
     """(capacity 2 and a window of 64 of 64 slots: right for one token, refused for the three of the call)"""
     c = cache(L, **bad)
     assert L.lib.nwc_kv_append(None, c, 0, A, 1024, 3, 4, None, None, A, A, 99, A, None, 1e-6, A, A) == -1
-    assert L.lib.nwc_kv_attention(None, c, 0, A, 512, 3, 4, A, None, None, 0.1, A, A) == -1
+    assert L.lib.nwc_kv_attention(None, c, 0, A, 512, 3, 4, A, None, None, 0.1, A, None, 0, A) == -1
     if "capacity" not in bad or bad["capacity"] != 2:
         assert L.lib.nwc_kv_commit(None, c, 3, A, A, A, 2, A) == -1
 
@@ -45,8 +45,8 @@ def test_append_refusals(L):
 
 
 def test_attention_refusals(L):
-    good = dict(layer=0, q=A, ld=512, T=3, n_q=4, pos=A, visible=None, depth=None, scale=0.1, out=A, status=A)
-    for bad in (dict(layer=2), dict(q=None), dict(q=A + 8), dict(ld=504), dict(ld=516), dict(T=0), dict(T=65), dict(n_q=0), dict(n_q=5), dict(pos=None), dict(visible=A), dict(depth=A),
+    good = dict(layer=0, q=A, ld=512, T=3, n_q=4, pos=A, visible=None, depth=None, scale=0.1, out=A, work=None, size=0, status=A)
+    for bad in (dict(layer=2), dict(work=A + 8), dict(q=None), dict(q=A + 8), dict(ld=504), dict(ld=516), dict(T=0), dict(T=65), dict(n_q=0), dict(n_q=5), dict(pos=None), dict(visible=A), dict(depth=A),
                 dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(out=None), dict(out=A + 2), dict(status=None)):
         a = {**good, **bad}
         assert L.lib.nwc_kv_attention(None, cache(L), *a.values()) == -1, bad
