@@ -12,10 +12,13 @@
  *
  * Fragments.  A dot product may add its terms in any order, so the B fragment of K takes the 16-byte piece that a lane reads
  * from a key's row as it lies, and Q is laid out once to match; likewise the columns of V: the n-th column of an MMA is the
- * dimension that lane group n's piece holds at that place.  Neither K nor V is ever transposed or re-stored.  e4m3 codes become
- * bf16 in registers (a code is exact in bf16); the unit 2^e of a K row multiplies its scores, that of a V row its weights.
- * The weights are rounded to bf16 for the second product (2^-9 relative on average, averaged out over the keys): the sum of
- * the weights, the running maximum, and all accumulators are fp32.
+ * dimension that lane group n's piece holds at that place.  Neither K nor V is ever transposed or re-stored.
+ *
+ * bf16 caches take bf16 products.  e4m3 codes become f16 (exactly, one conversion for two codes; bf16 would take bit moves and a
+ * multiplication, 640 instead of 230 instructions of the 1150 per tile of 32 keys, and the kernel is bound by its issue rate),
+ * with a query row scaled by a power of two to fill f16's range; the unit 2^e of a K row multiplies its scores, that of a V
+ * row, relative to the largest met so far, its weights.  The weights are rounded for the second product to bf16 (2^-8) or f16
+ * (2^-11); their sum, the running maximum and all accumulators are fp32.
  */
 #include "nwc_kv.h"
 #include "nwc_async.cuh"
@@ -35,32 +38,39 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint4 &a, uint32_t
 }
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) { uint32_t d; asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(b), "f"(a)); return d; }
 __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-/* codes (already in the high bytes of both halves of w; the low bytes may hold anything) -> bf16 pair */
-__device__ __forceinline__ uint32_t codes_to_bf16(uint32_t w) { return kv_mul2(((w >> 4) & 0x07F007F0u) | (w & 0x80008000u), kTwoTo120); }
+__device__ __forceinline__ void mma16816_half(float (&c)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_half(float a, float b) { uint32_t d; asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(b), "f"(a)); return d; }
+/* four codes -> two f16 pairs (codes 0, 1 and 2, 3): exact */
+__device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+}
+/* 2^e for -126 <= e <= 127 */
+__device__ __forceinline__ float power_of_two(int32_t e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
 /* Shape of the few-rows kernel: tiles of kKeys keys per warp, kStages of them in flight. */
-template <int HD, int ELEM> struct Few {
+template <int HD, int ELEM, int MT> struct Few {
     static constexpr uint32_t kRowBytes = HD * (ELEM == kKvE4m3 ? 1u : 2u);
     static constexpr uint32_t kKeys = ELEM == kKvE4m3 ? 32u : 16u;
     static constexpr uint32_t kStageBytes = 2u * kKeys * kRowBytes;                     /* K and V */
-    static constexpr uint32_t kWarps = HD == 256 ? 4u : 8u, kStages = HD == 64 ? 4u : 3u;
-    static constexpr uint32_t kRing = kWarps * kStages * kStageBytes;
+    static constexpr uint32_t kWarps = HD == 256 ? 6u : MT == 2 ? 8u : 12u, kStages = HD == 64 ? 4u : MT == 2 ? 3u : 2u;
+    static constexpr uint32_t kRing = kWarps * kStages * kStageBytes, kRows = 16u * MT;
+    static constexpr uint32_t kQ = kRing, kBars = kQ + kRows * HD * 2u, kPart = kBars + kWarps * kStages * 8u, kQUnit = kPart + 2u * kWarps * kRows * 4u, kSmem = kQUnit + kRows * 4u;
 };
-template <int HD, int ELEM, int MT> __host__ __device__ constexpr uint32_t few_smem() {
-    return Few<HD, ELEM>::kRing + MT * 16u * HD * 2u + Few<HD, ELEM>::kWarps * Few<HD, ELEM>::kStages * 8u + 2u * Few<HD, ELEM>::kWarps * MT * 16u * 4u;
-}
 
 }  // namespace
 
 template <int HD, int ELEM, int MT>
-__global__ void __launch_bounds__(32 * Few<HD, ELEM>::kWarps, 1) kv_attention_few_kernel(const KvAttention a) {
-    using F = Few<HD, ELEM>;
-    constexpr uint32_t kRows = 16u * MT, kNT = F::kKeys / 8u, kSteps = HD / 16u, kWarps = F::kWarps;
+__global__ void __launch_bounds__(32 * Few<HD, ELEM, MT>::kWarps, 1) kv_attention_few_kernel(const KvAttention a) {
+    using F = Few<HD, ELEM, MT>;
+    constexpr uint32_t kRows = F::kRows, kNT = F::kKeys / 8u, kSteps = HD / 16u, kWarps = F::kWarps;
     extern __shared__ __align__(128) uint8_t few_raw[];
     const uint32_t ring = smem_addr(few_raw), tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, g = lane >> 2, c = lane & 3u;
-    uint8_t *qs = few_raw + F::kRing;                                                  /* Q in fragment order: [kSteps][MT][32 lanes] uint4 */
-    const uint32_t bars = smem_addr(qs + kRows * HD * 2u), mine = ring + warp * F::kStages * F::kStageBytes, my_bars = bars + warp * F::kStages * 8u;
-    float *part_m = reinterpret_cast<float *>(qs + kRows * HD * 2u + kWarps * F::kStages * 8u), *part_l = part_m + kWarps * kRows;
+    uint8_t *qs = few_raw + F::kQ;                                                  /* Q in fragment order: [kSteps][MT][32 lanes] uint4 */
+    const uint32_t bars = ring + F::kBars, mine = ring + warp * F::kStages * F::kStageBytes, my_bars = bars + warp * F::kStages * 8u;
+    float *part_m = reinterpret_cast<float *>(few_raw + F::kPart), *part_l = part_m + kWarps * kRows, *q_unit = reinterpret_cast<float *>(few_raw + F::kQUnit);
     const uint32_t group = a.n_q / a.c.n_kv, rows = a.T * group, kvh = blockIdx.y % a.c.n_kv, row0 = (blockIdx.y / a.c.n_kv) * kRows, split = blockIdx.x;
     if (lane == 0) {
         for (uint32_t s = 0; s < F::kStages; s++) mbar_init(my_bars + s * 8u, 1u);
@@ -98,40 +108,55 @@ __global__ void __launch_bounds__(32 * Few<HD, ELEM>::kWarps, 1) kv_attention_fe
             }
         }
     };
-    /* the exponent bytes of the key that this lane stands for in tile i: K's in the low, V's in the high half */
-    auto units = [&](uint32_t i) -> uint32_t {
-        if (ELEM != kKvE4m3) return 0u;
-        const uint32_t key = (first_tile + warp + i * kWarps) * F::kKeys + lane;
-        if (i >= my_tiles || key >= span.count) return 0u;
-        const uint64_t cell = (uint64_t)kvh * a.c.capacity + slot_of(key);
-        return (uint32_t)a.c.k_exp[cell] | (uint32_t)a.c.v_exp[cell] << 16;
+    /* the exponent bytes of the key that this lane stands for in tile i (a tile early; behind the last key, the last one's) */
+    uint8_t k_next = 0, v_next = 0;
+    auto units = [&](uint32_t i) {
+        if (ELEM != kKvE4m3) return;
+        const uint64_t cell = (uint64_t)kvh * a.c.capacity + slot_of(min((first_tile + warp + i * kWarps) * F::kKeys + lane, span.count - 1u));
+        k_next = a.c.k_exp[cell]; v_next = a.c.v_exp[cell];
     };
     for (uint32_t i = 0; i < F::kStages && i < my_tiles; i++) issue(i);
-    uint32_t unit_now = units(0u);
-    /* Q: the 16-byte (e4m3: 2 x 16-byte) piece of a row that meets the K piece of lane c, in the order the codes unfold to */
-    for (uint32_t e = tid; e < kRows * HD / 8u; e += blockDim.x) {
-        const uint32_t r = e / (HD / 8u), d = (e % (HD / 8u)) * 8u, row = row0 + r;
-        uint4 w = make_uint4(0u, 0u, 0u, 0u);
-        if (row < rows) w = *reinterpret_cast<const uint4 *>(a.q + (uint64_t)(row / group) * a.ldq + (uint64_t)(kvh * group + row % group) * HD + d);
-        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    units(0u);
+    /* Q: the 16-byte piece of a row that meets the K piece of lane c, in the order its words are used.  A row is one warp's. */
+    for (uint32_t r = warp; r < kRows; r += kWarps) {
+        const uint32_t row = row0 + r;
+        uint32_t w[HD / 64];
+        float top = 0.f;
 #pragma unroll
-        for (uint32_t j = 0; j < 4u; j++) {                                            /* dimensions d + 2j, d + 2j + 1 */
-            uint32_t step, cc, half;
-            if (ELEM == kKvE4m3) { const uint32_t dd = d + 2u * j, in = dd & 15u; cc = (dd >> 4) & 3u; step = (dd >> 6) * 4u + (in >> 2); half = (in >> 1) & 1u; }
-            else { const uint32_t dd = d + 2u * j, in = dd & 7u; cc = (dd >> 3) & 3u; step = (dd >> 5) * 2u + (in >> 2); half = (in >> 1) & 1u; }
-            const uint32_t at = ((step * MT + (r >> 4)) * 32u + (r & 7u) * 4u + cc) * 4u + half * 2u + ((r >> 3) & 1u);      /* a0 a1 a2 a3 = (g, lo) (g + 8, lo) (g, hi) (g + 8, hi) */
-            reinterpret_cast<uint32_t *>(qs)[at] = u[j];
+        for (uint32_t j = 0; j < HD / 64u; j++) {                                       /* dimensions 2 (32 j + lane), + 1 */
+            w[j] = row < rows ? *reinterpret_cast<const uint32_t *>(a.q + (uint64_t)(row / group) * a.ldq + (uint64_t)(kvh * group + row % group) * HD + 64u * j + 2u * lane) : 0u;
+            top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[j] << 16)), fabsf(__uint_as_float(w[j] & 0xFFFF0000u))));
+        }
+        if (ELEM == kKvE4m3) {
+            /* largest magnitude into [2^14, 2^15): a number 2^-29 of it is still held to bf16's precision */
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+            const int32_t e = max((int32_t)(__float_as_uint(top) >> 23) - 127, -100);
+            const float up = power_of_two(14 - e);
+            if (lane == 0) q_unit[r] = power_of_two(e - 14);
+#pragma unroll
+            for (uint32_t j = 0; j < HD / 64u; j++) w[j] = pack_half(__uint_as_float(w[j] << 16) * up, __uint_as_float(w[j] & 0xFFFF0000u) * up);
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < HD / 64u; j++) {
+            const uint32_t d = 64u * j + 2u * lane;
+            uint32_t step, cc;
+            if (ELEM == kKvE4m3) { step = (d >> 6) * 4u + ((d & 15u) >> 2); cc = (d >> 4) & 3u; } else { step = (d >> 5) * 2u + ((d & 7u) >> 2); cc = (d >> 3) & 3u; }
+            /* a0 a1 a2 a3 = (row g, first pair) (row g + 8, first) (g, second) (g + 8, second) */
+            reinterpret_cast<uint32_t *>(qs)[((step * MT + (r >> 4)) * 32u + (r & 7u) * 4u + cc) * 4u + ((d >> 1) & 1u) * 2u + ((r >> 3) & 1u)] = w[j];
         }
     }
     __syncthreads();
     /* this lane's rows: token and own position */
-    uint32_t token[2 * MT], own[2 * MT], own_min = 0xFFFFFFFFu, own_max = 0u;
+    float row_scale[2 * MT];
+    uint32_t token[2 * MT], own[2 * MT], top_byte = 0u, own_min = 0xFFFFFFFFu, own_max = 0u;
 #pragma unroll
     for (uint32_t i = 0; i < 2u * MT; i++) {
         const uint32_t row = min(row0 + (i >> 1) * 16u + (i & 1u) * 8u + g, rows - 1u);
         token[i] = row / group;
         own[i] = (uint32_t)pos + (a.depth ? (uint32_t)a.depth[token[i]] : token[i]);
         own_min = min(own_min, own[i]); own_max = max(own_max, own[i]);
+        row_scale[i] = ELEM == kKvE4m3 ? a.scale * q_unit[(i >> 1) * 16u + (i & 1u) * 8u + g] : a.scale;
     }
     own_max = __reduce_max_sync(0xffffffffu, own_max); own_min = __reduce_min_sync(0xffffffffu, own_min);
     const uint32_t open_end = a.visible ? (uint32_t)pos : own_min + 1u;                 /* positions below it are seen by every row, window apart */
@@ -150,10 +175,10 @@ __global__ void __launch_bounds__(32 * Few<HD, ELEM>::kWarps, 1) kv_attention_fe
     for (uint32_t it = 0; it < issued; it++) {
         const uint32_t s = it % F::kStages, key0 = (first_tile + warp + it * kWarps) * F::kKeys, n = min(F::kKeys, span.count - key0);
         const uint32_t kt = mine + s * F::kStageBytes, vt = kt + F::kKeys * F::kRowBytes;
-        const uint32_t unit = unit_now;
+        const uint32_t k_byte = k_next, v_byte = v_next;
         alive = mbar_wait(my_bars + s * 8u, (it / F::kStages) & 1u) && alive;
         if (!alive) continue;
-        unit_now = units(it + 1u);
+        units(it + 1u);
         if (n < F::kKeys) {                                                             /* V rows behind the last key: weight 0 times whatever lies there must be 0 */
             for (uint32_t e = lane; e < (F::kKeys - n) * (F::kRowBytes / 16u); e += 32u) asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vt + n * F::kRowBytes + e * 16u), "r"(0u) : "memory");
             __syncwarp();
@@ -180,33 +205,35 @@ __global__ void __launch_bounds__(32 * Few<HD, ELEM>::kWarps, 1) kv_attention_fe
                 const uint32_t u[4] = {w.x, w.y, w.z, w.w};
                 if (ELEM == kKvE4m3) {
 #pragma unroll
-                    for (uint32_t st = 0; st < 4u; st++) {
-                        const uint32_t b0 = codes_to_bf16(__byte_perm(u[st], 0u, 0x1404)), b1 = codes_to_bf16(__byte_perm(u[st], 0u, 0x3424));
+                    for (uint32_t st = 0; st < kStepsPerPiece; st++) {
+                        uint32_t b0, b1;
+                        codes_to_half(u[st], b0, b1);
 #pragma unroll
-                        for (uint32_t i = 0; i < MT; i++) mma16816(sc[i][j], qf[st][i], b0, b1);
+                        for (uint32_t i = 0; i < MT; i++) mma16816_half(sc[i][j], qf[st][i], b0, b1);
                     }
                 } else {
 #pragma unroll
                     for (uint32_t st = 0; st < 2u; st++)
 #pragma unroll
-                        for (uint32_t i = 0; i < MT; i++) mma16816(sc[i][j], qf[st % kStepsPerPiece][i], u[2 * st], u[2 * st + 1]);
+                        for (uint32_t i = 0; i < MT; i++) mma16816(sc[i][j], qf[st][i], u[2 * st], u[2 * st + 1]);
                 }
             }
         }
         /* log2 scores, masked; a tile that every row sees whole needs no mask */
         const uint32_t p_first = position(key0), p_last = position(key0 + n - 1u);
         const bool open = n == F::kKeys && p_last < open_end && (!a.c.window || p_last < a.c.sinks || (p_first > own_max || own_max - p_first < a.c.window));
+        const float k_unit = kv_unit(k_byte);
 #pragma unroll
-        for (uint32_t j = 0; j < kNT; j++) {
+        for (uint32_t j = 0; j < kNT; j++)
 #pragma unroll
             for (uint32_t b = 0; b < 2u; b++) {
-                const uint32_t kk = j * 8u + 2u * c + b;
-                float f = a.scale;
-                if (ELEM == kKvE4m3) f *= kv_unit(__shfl_sync(0xffffffffu, unit, kk) & 0xFFFFu);
+                const float f = ELEM == kKvE4m3 ? __shfl_sync(0xffffffffu, k_unit, j * 8u + 2u * c + b) : 1.f;
 #pragma unroll
-                for (uint32_t i = 0; i < MT; i++) { sc[i][j][b] *= f; sc[i][j][b + 2] *= f; }
+                for (uint32_t i = 0; i < 2u * MT; i++) {
+                    float &x = sc[i >> 1][j][2u * (i & 1u) + b];
+                    x *= ELEM == kKvE4m3 ? f * row_scale[i] : row_scale[i];
+                }
             }
-        }
         if (!open) {
 #pragma unroll
             for (uint32_t j = 0; j < kNT; j++)
@@ -234,23 +261,30 @@ __global__ void __launch_bounds__(32 * Few<HD, ELEM>::kWarps, 1) kv_attention_fe
             t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1)); t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
             top[i] = t; raise = raise || t > m[i] + 8.f;
         }
+        /* the same for the largest unit of the V rows: weights are multiplied by 2^(v_byte - top_byte) <= 1 */
+        uint32_t byte_up = top_byte;
+        if (ELEM == kKvE4m3) { byte_up = max(top_byte, __reduce_max_sync(0xffffffffu, v_byte)); raise = raise || byte_up != top_byte; }
         if (__any_sync(0xffffffffu, raise)) {
+            const float v_down = ELEM == kKvE4m3 ? power_of_two(max((int32_t)(top_byte - byte_up), -126)) : 1.f;
+            top_byte = byte_up;
 #pragma unroll
             for (uint32_t i = 0; i < 2u * MT; i++) {
                 const float up = fmaxf(m[i], top[i]), f = up == -INFINITY ? 1.f : exp2_fast(m[i] - up);
                 m[i] = up; l[i] *= f;
+                const float fo = f * v_down;
 #pragma unroll
-                for (uint32_t j = 0; j < HD / 8u; j++) { o[i >> 1][j][2u * (i & 1u)] *= f; o[i >> 1][j][2u * (i & 1u) + 1u] *= f; }
+                for (uint32_t j = 0; j < HD / 8u; j++) { o[i >> 1][j][2u * (i & 1u)] *= fo; o[i >> 1][j][2u * (i & 1u) + 1u] *= fo; }
             }
         }
         float base[2 * MT];
 #pragma unroll
         for (uint32_t i = 0; i < 2u * MT; i++) base[i] = m[i] == -INFINITY ? 0.f : m[i];
+        const float v_unit = power_of_two(max((int32_t)(v_byte - top_byte), -126));
 #pragma unroll
         for (uint32_t j = 0; j < kNT; j++)
 #pragma unroll
             for (uint32_t b = 0; b < 2u; b++) {
-                const float vu = ELEM == kKvE4m3 ? kv_unit(__shfl_sync(0xffffffffu, unit, j * 8u + 2u * c + b) >> 16) : 1.f;
+                const float vu = ELEM == kKvE4m3 ? __shfl_sync(0xffffffffu, v_unit, j * 8u + 2u * c + b) : 1.f;
 #pragma unroll
                 for (uint32_t i = 0; i < 2u * MT; i++) {
                     float &x = sc[i >> 1][j][2u * (i & 1u) + b];
@@ -264,9 +298,11 @@ __global__ void __launch_bounds__(32 * Few<HD, ELEM>::kWarps, 1) kv_attention_fe
         for (uint32_t h = 0; h < kNT / 2u; h++) {
             uint4 pf[MT];
 #pragma unroll
-            for (uint32_t i = 0; i < MT; i++)
-                pf[i] = make_uint4(pack_bf16(sc[i][2 * h][0], sc[i][2 * h][1]), pack_bf16(sc[i][2 * h][2], sc[i][2 * h][3]),
-                                   pack_bf16(sc[i][2 * h + 1][0], sc[i][2 * h + 1][1]), pack_bf16(sc[i][2 * h + 1][2], sc[i][2 * h + 1][3]));
+            for (uint32_t i = 0; i < MT; i++) {
+                auto pack = [](float x, float y) { return ELEM == kKvE4m3 ? pack_half(x, y) : pack_bf16(x, y); };
+                pf[i] = make_uint4(pack(sc[i][2 * h][0], sc[i][2 * h][1]), pack(sc[i][2 * h][2], sc[i][2 * h][3]),
+                                   pack(sc[i][2 * h + 1][0], sc[i][2 * h + 1][1]), pack(sc[i][2 * h + 1][2], sc[i][2 * h + 1][3]));
+            }
             const uint32_t v0 = vt + (h * 16u + 2u * c) * F::kRowBytes;
             constexpr uint32_t kPieceDims = ELEM == kKvE4m3 ? (HD == 64 ? 8u : 16u) : 8u, kVPieces = HD / (8u * kPieceDims);
 #pragma unroll
@@ -280,12 +316,16 @@ __global__ void __launch_bounds__(32 * Few<HD, ELEM>::kWarps, 1) kv_attention_fe
                 }
                 if (ELEM == kKvE4m3) {
 #pragma unroll
-                    for (uint32_t d = 0; d < kPieceDims; d++) {
-                        /* byte d % 4 of the two keys' words into the high bytes of the halves */
-                        const uint32_t sel = (d & 3u) << 4 | ((d & 3u) + 4u) << 12;
-                        const uint32_t b0 = codes_to_bf16(__byte_perm(w[0][d >> 2], w[1][d >> 2], sel)), b1 = codes_to_bf16(__byte_perm(w[2][d >> 2], w[3][d >> 2], sel));
+                    for (uint32_t d = 0; d < kPieceDims; d += 2u) {
+                        /* bytes d % 4 and d % 4 + 1 of the two keys' words, side by side */
+                        const uint32_t sel = d & 2u ? 0x7362u : 0x5140u;
+                        uint32_t b0[2], b1[2];
+                        codes_to_half(__byte_perm(w[0][d >> 2], w[1][d >> 2], sel), b0[0], b0[1]);
+                        codes_to_half(__byte_perm(w[2][d >> 2], w[3][d >> 2], sel), b1[0], b1[1]);
 #pragma unroll
-                        for (uint32_t i = 0; i < MT; i++) mma16816(o[i][pc * kPieceDims + d], pf[i], b0, b1);
+                        for (uint32_t x = 0; x < 2u; x++)
+#pragma unroll
+                            for (uint32_t i = 0; i < MT; i++) mma16816_half(o[i][pc * kPieceDims + d + x], pf[i], b0[x], b1[x]);
                     }
                 } else {
 #pragma unroll
@@ -313,6 +353,7 @@ __global__ void __launch_bounds__(32 * Few<HD, ELEM>::kWarps, 1) kv_attention_fe
         for (uint32_t i = 0; i < 2u * MT; i++) { const uint32_t r = (i >> 1) * 16u + (i & 1u) * 8u + g; part_m[warp * kRows + r] = m[i]; part_l[warp * kRows + r] = l[i]; }
     }
     constexpr uint32_t kPieceDims = ELEM == kKvE4m3 ? (HD == 64 ? 8u : 16u) : 8u;
+    const float o_unit = ELEM == kKvE4m3 ? kv_unit(top_byte) : 1.f;
 #pragma unroll
     for (uint32_t i = 0; i < 2u * MT; i++) {
         float *to = part + (warp * kRows + (i >> 1) * 16u + (i & 1u) * 8u + g) * HD;
@@ -320,14 +361,12 @@ __global__ void __launch_bounds__(32 * Few<HD, ELEM>::kWarps, 1) kv_attention_fe
 #pragma unroll
         for (uint32_t j = 0; j < HD / 8u; j++) {
             const uint32_t d = (j / kPieceDims) * 8u * kPieceDims + 2u * c * kPieceDims + j % kPieceDims;
-            to[d] = o[i >> 1][j][2u * (i & 1u)]; to[d + kPieceDims] = o[i >> 1][j][2u * (i & 1u) + 1u];
+            to[d] = o[i >> 1][j][2u * (i & 1u)] * o_unit; to[d + kPieceDims] = o[i >> 1][j][2u * (i & 1u) + 1u] * o_unit;
         }
     }
     __syncthreads();
-    constexpr uint32_t kOut = kRows * HD / (32u * kWarps);                              /* outputs per thread */
-#pragma unroll
-    for (uint32_t e = 0; e < kOut; e++) {
-        const uint32_t at = e * 32u * kWarps + tid, r = at / HD, d = at % HD, row = row0 + r;
+    for (uint32_t at = tid; at < kRows * HD; at += 32u * kWarps) {
+        const uint32_t r = at / HD, d = at % HD, row = row0 + r;
         if (row >= rows) continue;
         float top = -INFINITY, total = 0.f, sum = 0.f;
 #pragma unroll
@@ -401,7 +440,7 @@ cudaError_t launch(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem
 template <int HD, int ELEM, int MT>
 cudaError_t launch_few(cudaStream_t st, const KvAttention &a) {
     const uint32_t rows = a.T * (a.n_q / a.c.n_kv), tiles = (rows + 16u * MT - 1u) / (16u * MT);
-    return launch(kv_attention_few_kernel<HD, ELEM, MT>, dim3(a.splits, a.c.n_kv * tiles), dim3(32u * Few<HD, ELEM>::kWarps), few_smem<HD, ELEM, MT>(), st, dependent_launch(), a);
+    return launch(kv_attention_few_kernel<HD, ELEM, MT>, dim3(a.splits, a.c.n_kv * tiles), dim3(32u * Few<HD, ELEM, MT>::kWarps), Few<HD, ELEM, MT>::kSmem, st, dependent_launch(), a);
 }
 template <int HD, int ELEM>
 cudaError_t launch_all(cudaStream_t st, const KvAttention &a) {
@@ -414,7 +453,7 @@ cudaError_t launch_all(cudaStream_t st, const KvAttention &a) {
     /* (an ordinary dependent launch: the join's set-up overlaps the last CTAs; it waits for the whole grid before it reads) */
     return launch(kv_attention_join_kernel<HD>, dim3((uint32_t)((units + 3u) / 4u)), dim3(128), 0, st, true, a);
 }
-template <int HD, int ELEM, int MT> void configure_few() { cudaFuncSetAttribute(kv_attention_few_kernel<HD, ELEM, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)few_smem<HD, ELEM, MT>()); }
+template <int HD, int ELEM, int MT> void configure_few() { cudaFuncSetAttribute(kv_attention_few_kernel<HD, ELEM, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Few<HD, ELEM, MT>::kSmem); }
 
 }  // namespace
 
