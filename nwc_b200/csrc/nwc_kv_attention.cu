@@ -50,21 +50,41 @@ __device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t &lo, uint32_t
 /* 2^e for -126 <= e <= 127 */
 __device__ __forceinline__ float power_of_two(int32_t e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-/* Shape of the few-rows kernel: tiles of kKeys keys per warp, kStages of them in flight. */
-template <int HD, int ELEM, int MT> struct Few {
+__host__ __device__ constexpr uint32_t larger(uint32_t a, uint32_t b) { return a > b ? a : b; }
+
+/* Shape of the few-rows kernel: warps that take tiles of kKeys keys, kStages of them in flight per warp.
+   Long caches (SHORT = 0): one CTA per SM whose rings fill its shared memory; the CTAs' shares meet in a second kernel.
+   Short ones (SHORT = 1): small tiles, so that the dependent chain of one warp is short, four warps, and the CTAs that divide
+   one head's keys form a cluster that joins its shares through distributed shared memory: no second launch. */
+template <int HD, int ELEM, int MT, int SHORT> struct Few {
     static constexpr uint32_t kRowBytes = HD * (ELEM == kKvE4m3 ? 1u : 2u);
-    static constexpr uint32_t kKeys = ELEM == kKvE4m3 ? 32u : 16u;
+    static constexpr uint32_t kKeys = ELEM == kKvE4m3 && !SHORT ? 32u : 16u;
     static constexpr uint32_t kStageBytes = 2u * kKeys * kRowBytes;                     /* K and V */
-    static constexpr uint32_t kWarps = HD == 256 ? 6u : MT == 2 ? 8u : 12u, kStages = HD == 64 ? 4u : MT == 2 ? 3u : 2u;
-    static constexpr uint32_t kRing = kWarps * kStages * kStageBytes, kRows = 16u * MT;
-    static constexpr uint32_t kQ = kRing, kBars = kQ + kRows * HD * 2u, kPart = kBars + kWarps * kStages * 8u, kQUnit = kPart + 2u * kWarps * kRows * 4u, kSmem = kQUnit + kRows * 4u;
+    static constexpr uint32_t kWarps = SHORT ? 4u : HD == 256 ? 6u : MT == 2 ? 8u : 12u, kStages = SHORT ? (ELEM == kKvE4m3 ? 4u : 3u) : HD == 64 ? 4u : MT == 2 ? 3u : 2u;
+    static constexpr uint32_t kRows = 16u * MT;
+    /* a row of a warp's outputs: ten floats for the eight columns of an accumulator, eight (mod 32) between rows: both the
+       stores in fragment order and the loads in order of dimensions meet different banks */
+    static constexpr uint32_t kPitch = (HD / 8u * 10u + 23u) / 32u * 32u + 8u;
+    static constexpr uint32_t kRing = larger(kWarps * kStages * kStageBytes, kWarps * kRows * kPitch * 4u);
+    static constexpr uint32_t kQ = kRing, kBars = kQ + kRows * HD * 2u, kPart = kBars + kWarps * kStages * 8u, kQUnit = kPart + 2u * kWarps * kRows * 4u, kShare = (kQUnit + kRows * 4u + 15u) / 16u * 16u;
+    static constexpr uint32_t kSmem = kShare + (SHORT ? kRows * (HD + 2u) * 4u + 16u * kRows * 8u : kRows * 8u);
 };
+__device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
+    uint32_t there; float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
+    return v;
+}
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 
 }  // namespace
 
-template <int HD, int ELEM, int MT>
-__global__ void __launch_bounds__(32 * Few<HD, ELEM, MT>::kWarps, 1) kv_attention_few_kernel(const KvAttention a) {
-    using F = Few<HD, ELEM, MT>;
+template <int HD, int ELEM, int MT, int SHORT>
+__global__ void __launch_bounds__(32 * Few<HD, ELEM, MT, SHORT>::kWarps, 1) kv_attention_few_kernel(const KvAttention a) {
+    using F = Few<HD, ELEM, MT, SHORT>;
     constexpr uint32_t kRows = F::kRows, kNT = F::kKeys / 8u, kSteps = HD / 16u, kWarps = F::kWarps;
     extern __shared__ __align__(128) uint8_t few_raw[];
     const uint32_t ring = smem_addr(few_raw), tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, g = lane >> 2, c = lane & 3u;
@@ -345,44 +365,81 @@ __global__ void __launch_bounds__(32 * Few<HD, ELEM, MT>::kWarps, 1) kv_attentio
     /* join the warps: common maximum, then sums and outputs rescaled to it, in warp order */
 #pragma unroll
     for (uint32_t i = 0; i < 2u * MT; i++) { l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1); l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2); }
+    const uint32_t live = min(kRows, rows - row0);                                      /* rows of this tile that exist */
     __syncthreads();                                                                    /* every warp has done with its ring: O goes there */
-    float *part = reinterpret_cast<float *>(few_raw);                                   /* [kWarps][kRows][HD] */
-    static_assert(kWarps * kRows * HD * 4u <= F::kRing, "the warps' outputs fit the ring");
-    if (c == 0) {
-#pragma unroll
-        for (uint32_t i = 0; i < 2u * MT; i++) { const uint32_t r = (i >> 1) * 16u + (i & 1u) * 8u + g; part_m[warp * kRows + r] = m[i]; part_l[warp * kRows + r] = l[i]; }
-    }
+    float *part = reinterpret_cast<float *>(few_raw);                                   /* [kWarps][kRows][kPitch] */
     constexpr uint32_t kPieceDims = ELEM == kKvE4m3 ? (HD == 64 ? 8u : 16u) : 8u;
     const float o_unit = ELEM == kKvE4m3 ? kv_unit(top_byte) : 1.f;
 #pragma unroll
     for (uint32_t i = 0; i < 2u * MT; i++) {
-        float *to = part + (warp * kRows + (i >> 1) * 16u + (i & 1u) * 8u + g) * HD;
-        /* accumulator j, columns 2c and 2c + 1 = place j % kPieceDims of the pieces 2c, 2c + 1 */
+        const uint32_t r = (i >> 1) * 16u + (i & 1u) * 8u + g;
+        if (c == 0) { part_m[warp * kRows + r] = m[i]; part_l[warp * kRows + r] = l[i]; }
+        if (r < live && m[i] != -INFINITY) {
+            float *to = part + (warp * kRows + r) * F::kPitch + 2u * c;
 #pragma unroll
-        for (uint32_t j = 0; j < HD / 8u; j++) {
-            const uint32_t d = (j / kPieceDims) * 8u * kPieceDims + 2u * c * kPieceDims + j % kPieceDims;
-            to[d] = o[i >> 1][j][2u * (i & 1u)] * o_unit; to[d + kPieceDims] = o[i >> 1][j][2u * (i & 1u) + 1u] * o_unit;
+            for (uint32_t j = 0; j < HD / 8u; j++) *reinterpret_cast<float2 *>(to + j * 10u) = make_float2(o[i >> 1][j][2u * (i & 1u)] * o_unit, o[i >> 1][j][2u * (i & 1u) + 1u] * o_unit);
         }
     }
     __syncthreads();
-    for (uint32_t at = tid; at < kRows * HD; at += 32u * kWarps) {
-        const uint32_t r = at / HD, d = at % HD, row = row0 + r;
-        if (row >= rows) continue;
-        float top = -INFINITY, total = 0.f, sum = 0.f;
+    float *share = reinterpret_cast<float *>(few_raw + F::kShare), *share_ml = share + (SHORT ? kRows * HD : 0u);      /* [kRows][HD] (a cluster's only), [kRows][2] */
+    if (tid < kRows) {
+        float top = -INFINITY, total = 0.f;
 #pragma unroll
-        for (uint32_t w = 0; w < kWarps; w++) top = fmaxf(top, part_m[w * kRows + r]);
+        for (uint32_t w = 0; w < kWarps; w++) top = fmaxf(top, part_m[w * kRows + tid]);
 #pragma unroll
         for (uint32_t w = 0; w < kWarps; w++) {
-            const float mw = part_m[w * kRows + r], f = mw == -INFINITY ? 0.f : exp2_fast(mw - top);
-            total = fmaf(part_l[w * kRows + r], f, total); sum = fmaf(part[w * kRows * HD + at], f, sum);
+            const float mw = part_m[w * kRows + tid], f = mw == -INFINITY ? 0.f : exp2_fast(mw - top);
+            total = fmaf(part_l[w * kRows + tid], f, total);
+            part_m[w * kRows + tid] = f;                                                /* from here on the warp's factor */
+        }
+        share_ml[2u * tid] = top; share_ml[2u * tid + 1u] = total;
+    }
+    __syncthreads();
+    for (uint32_t at = tid; at < live * HD; at += 32u * kWarps) {
+        const uint32_t r = at / HD, d = at % HD, row = row0 + r;
+        /* dimension d = place d % kPieceDims of piece (d / kPieceDims) % 8: accumulator j, column d / kPieceDims % 8 */
+        const uint32_t j = d / (8u * kPieceDims) * kPieceDims + d % kPieceDims, x = j * 10u + (d / kPieceDims) % 8u;
+        float sum = 0.f;
+#pragma unroll
+        for (uint32_t w = 0; w < kWarps; w++) {
+            const float f = part_m[w * kRows + r];
+            if (f != 0.f) sum = fmaf(part[(w * kRows + r) * F::kPitch + x], f, sum);
         }
         const uint64_t line = (uint64_t)(row / group) * a.n_q + kvh * group + row % group;
-        if (a.splits == 1u) a.out[line * HD + d] = __bfloat16_as_ushort(__float2bfloat16_rn(total == 0.f ? 0.f : sum / total));
+        if (a.splits == 1u) {
+            const float total = share_ml[2u * r + 1u];
+            a.out[line * HD + d] = __bfloat16_as_ushort(__float2bfloat16_rn(total == 0.f ? 0.f : sum / total));
+        } else if (SHORT) share[at] = sum;
         else {
             const uint64_t cell = (uint64_t)split * a.T * a.n_q + line;
             a.part_o[cell * HD + d] = sum;
-            if (d == 0) { a.part_ml[cell * 2u] = top; a.part_ml[cell * 2u + 1u] = total; }
+            if (d == 0) *reinterpret_cast<float2 *>(a.part_ml + cell * 2u) = make_float2(share_ml[2u * r], share_ml[2u * r + 1u]);
         }
+    }
+    if (SHORT && a.splits > 1u) {
+        /* join the CTAs of the cluster: each takes its part of the outputs, reading the others' shares; rank order */
+        cluster_barrier();
+        float2 *ml = reinterpret_cast<float2 *>(share_ml + 2u * kRows);                /* [16][kRows] */
+        const uint32_t from = smem_addr(share), from_ml = smem_addr(share_ml);
+        for (uint32_t e = tid; e < a.splits * live; e += 32u * kWarps) {
+            const uint32_t y = e / live, r = e % live;
+            ml[y * kRows + r] = make_float2(ld_cluster(from_ml + r * 8u, y), ld_cluster(from_ml + r * 8u + 4u, y));
+        }
+        __syncthreads();
+        for (uint32_t at = split * 32u * kWarps + tid; at < live * HD; at += a.splits * 32u * kWarps) {
+            const uint32_t r = at / HD, d = at % HD, row = row0 + r;
+            float top = -INFINITY, total = 0.f, sum = 0.f;
+            for (uint32_t y = 0; y < a.splits; y++) top = fmaxf(top, ml[y * kRows + r].x);
+#pragma unroll 4
+            for (uint32_t y = 0; y < a.splits; y++) {
+                const float2 w = ml[y * kRows + r];
+                const float f = w.x == -INFINITY ? 0.f : exp2_fast(w.x - top);
+                total = fmaf(w.y, f, total); sum = fmaf(ld_cluster(from + at * 4u, y), f, sum);
+            }
+            const uint64_t line = (uint64_t)(row / group) * a.n_q + kvh * group + row % group;
+            a.out[line * HD + d] = __bfloat16_as_ushort(__float2bfloat16_rn(total == 0.f ? 0.f : sum / total));
+        }
+        cluster_barrier();                                                              /* nobody leaves while its share is being read */
     }
 }
 
@@ -427,55 +484,68 @@ __global__ void __launch_bounds__(128) kv_attention_join_kernel(const KvAttentio
 namespace {
 
 template <class... Params, class... Args>
-cudaError_t launch(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, bool dependent, Args... args) {
+cudaError_t launch(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, bool dependent, uint32_t cluster, Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid; cfg.blockDim = block; cfg.dynamicSmemBytes = smem; cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr; cfg.numAttrs = dependent ? 1 : 0;
+    cudaLaunchAttribute attr[2];
+    uint32_t n = 0;
+    if (dependent) { attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[n++].val.programmaticStreamSerializationAllowed = 1; }
+    if (cluster > 1u) { attr[n].id = cudaLaunchAttributeClusterDimension; attr[n].val.clusterDim.x = cluster; attr[n].val.clusterDim.y = 1; attr[n++].val.clusterDim.z = 1; }
+    cfg.attrs = attr; cfg.numAttrs = n;
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
 }
 
-template <int HD, int ELEM, int MT>
+template <int HD, int ELEM, int MT, int SHORT>
 cudaError_t launch_few(cudaStream_t st, const KvAttention &a) {
-    const uint32_t rows = a.T * (a.n_q / a.c.n_kv), tiles = (rows + 16u * MT - 1u) / (16u * MT);
-    return launch(kv_attention_few_kernel<HD, ELEM, MT>, dim3(a.splits, a.c.n_kv * tiles), dim3(32u * Few<HD, ELEM, MT>::kWarps), Few<HD, ELEM, MT>::kSmem, st, dependent_launch(), a);
+    using F = Few<HD, ELEM, MT, SHORT>;
+    const uint32_t rows = a.T * (a.n_q / a.c.n_kv), tiles = (rows + F::kRows - 1u) / F::kRows;
+    return launch(kv_attention_few_kernel<HD, ELEM, MT, SHORT>, dim3(a.splits, a.c.n_kv * tiles), dim3(32u * F::kWarps), F::kSmem, st, dependent_launch(), SHORT ? a.splits : 1u, a);
 }
 template <int HD, int ELEM>
-cudaError_t launch_all(cudaStream_t st, const KvAttention &a) {
+cudaError_t launch_all(cudaStream_t st, const KvAttention &a, bool in_clusters) {
     const uint32_t rows = a.T * (a.n_q / a.c.n_kv);
     cudaError_t err;
-    if constexpr (HD == 256) err = launch_few<HD, ELEM, 1>(st, a);
-    else err = rows > 16u ? launch_few<HD, ELEM, 2>(st, a) : launch_few<HD, ELEM, 1>(st, a);
-    if (err != cudaSuccess || a.splits == 1u) return err;
+    if constexpr (HD == 256) err = in_clusters ? launch_few<HD, ELEM, 1, 1>(st, a) : launch_few<HD, ELEM, 1, 0>(st, a);
+    else if (in_clusters) err = rows > 16u ? launch_few<HD, ELEM, 2, 1>(st, a) : launch_few<HD, ELEM, 1, 1>(st, a);
+    else err = rows > 16u ? launch_few<HD, ELEM, 2, 0>(st, a) : launch_few<HD, ELEM, 1, 0>(st, a);
+    if (err != cudaSuccess || a.splits == 1u || in_clusters) return err;
     const uint64_t units = (uint64_t)a.T * a.n_q * (HD >= 128 ? HD / 128 : 1);
     /* (an ordinary dependent launch: the join's set-up overlaps the last CTAs; it waits for the whole grid before it reads) */
-    return launch(kv_attention_join_kernel<HD>, dim3((uint32_t)((units + 3u) / 4u)), dim3(128), 0, st, true, a);
+    return launch(kv_attention_join_kernel<HD>, dim3((uint32_t)((units + 3u) / 4u)), dim3(128), 0, st, true, 1u, a);
 }
-template <int HD, int ELEM, int MT> void configure_few() { cudaFuncSetAttribute(kv_attention_few_kernel<HD, ELEM, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Few<HD, ELEM, MT>::kSmem); }
+template <int HD, int ELEM, int MT, int SHORT> void configure_one() {
+    cudaFuncSetAttribute(kv_attention_few_kernel<HD, ELEM, MT, SHORT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Few<HD, ELEM, MT, SHORT>::kSmem);
+    if (SHORT) cudaFuncSetAttribute(kv_attention_few_kernel<HD, ELEM, MT, SHORT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+}
+template <int HD, int MT> void configure_few() {
+    configure_one<HD, kKvBf16, MT, 0>(); configure_one<HD, kKvBf16, MT, 1>(); configure_one<HD, kKvE4m3, MT, 0>(); configure_one<HD, kKvE4m3, MT, 1>();
+}
 
 }  // namespace
 
-uint32_t kv_attention_splits(uint32_t head_dim, uint32_t n_kv, uint32_t capacity, uint32_t window, uint32_t sinks, uint32_t T, uint32_t n_q, int sms) {
+KvPlan kv_attention_plan(uint32_t head_dim, uint32_t n_kv, uint32_t capacity, uint32_t window, uint32_t sinks, uint32_t T, uint32_t n_q, int sms) {
     const uint32_t rows = T * (n_q / n_kv), per = head_dim == 256u ? 16u : (rows > 16u ? 32u : 16u);
     const uint64_t ctas = (uint64_t)n_kv * ((rows + per - 1u) / per), keys = window ? (uint64_t)sinks + window + T - 1u : capacity;
-    if (ctas >= (uint64_t)sms) return 1u;
+    KvPlan p{1u, false};
+    if (ctas >= (uint64_t)sms * 2u) return p;
+    if (keys <= kKvShortKeys) {
+        /* clusters of 2^k CTAs, a tile of 16 keys for each of their four warps, as long as the GPU has room for them */
+        p.in_clusters = true;
+        while (p.splits < 16u && (uint64_t)p.splits * 64u < keys && ctas * p.splits < (uint64_t)sms) p.splits *= 2u;
+        return p;
+    }
     /* no CTA below a tile for each of its warps */
-    const uint64_t most = (keys + 127u) / 128u, want = (uint64_t)sms / ctas;
-    return (uint32_t)(want < most ? want : most);
+    const uint64_t most = (keys + 383u) / 384u, want = (uint64_t)sms > ctas ? (uint64_t)sms / ctas : 1u;
+    p.splits = (uint32_t)(want < most ? want : most);
+    return p;
 }
 
-cudaError_t launch_kv_attention(cudaStream_t st, int elem, uint32_t head_dim, const KvAttention &a, int) {
-    if (elem == kKvE4m3) return head_dim == 64u ? launch_all<64, kKvE4m3>(st, a) : head_dim == 128u ? launch_all<128, kKvE4m3>(st, a) : launch_all<256, kKvE4m3>(st, a);
-    return head_dim == 64u ? launch_all<64, kKvBf16>(st, a) : head_dim == 128u ? launch_all<128, kKvBf16>(st, a) : launch_all<256, kKvBf16>(st, a);
+cudaError_t launch_kv_attention(cudaStream_t st, int elem, uint32_t head_dim, const KvAttention &a, const KvPlan &p) {
+    if (elem == kKvE4m3) return head_dim == 64u ? launch_all<64, kKvE4m3>(st, a, p.in_clusters) : head_dim == 128u ? launch_all<128, kKvE4m3>(st, a, p.in_clusters) : launch_all<256, kKvE4m3>(st, a, p.in_clusters);
+    return head_dim == 64u ? launch_all<64, kKvBf16>(st, a, p.in_clusters) : head_dim == 128u ? launch_all<128, kKvBf16>(st, a, p.in_clusters) : launch_all<256, kKvBf16>(st, a, p.in_clusters);
 }
 
-void configure_kv_kernels() {
-    configure_few<64, kKvBf16, 1>(); configure_few<64, kKvBf16, 2>(); configure_few<64, kKvE4m3, 1>(); configure_few<64, kKvE4m3, 2>();
-    configure_few<128, kKvBf16, 1>(); configure_few<128, kKvBf16, 2>(); configure_few<128, kKvE4m3, 1>(); configure_few<128, kKvE4m3, 2>();
-    configure_few<256, kKvBf16, 1>(); configure_few<256, kKvE4m3, 1>();
-}
+void configure_kv_kernels() { configure_few<64, 1>(); configure_few<64, 2>(); configure_few<128, 1>(); configure_few<128, 2>(); configure_few<256, 1>(); }
 
 int read_kv_status(bool clear) {
     int v = 0;
