@@ -502,9 +502,11 @@ cudaError_t launch_few(cudaStream_t st, const KvAttention &a) {
     return launch(kv_attention_few_kernel<HD, ELEM, MT, SHORT>, dim3(a.splits, a.c.n_kv * tiles), dim3(32u * F::kWarps), F::kSmem, st, dependent_launch(), SHORT ? a.splits : 1u, a);
 }
 template <int HD, int ELEM>
-cudaError_t launch_all(cudaStream_t st, const KvAttention &a, bool in_clusters) {
+cudaError_t launch_all(cudaStream_t st, const KvAttention &a, const KvPlan &p) {
     const uint32_t rows = a.T * (a.n_q / a.c.n_kv);
+    const bool in_clusters = p.in_clusters;
     cudaError_t err;
+    if (p.many) err = launch_kv_many(st, ELEM, HD, a); else
     if constexpr (HD == 256) err = in_clusters ? launch_few<HD, ELEM, 1, 1>(st, a) : launch_few<HD, ELEM, 1, 0>(st, a);
     else if (in_clusters) err = rows > 16u ? launch_few<HD, ELEM, 2, 1>(st, a) : launch_few<HD, ELEM, 1, 1>(st, a);
     else err = rows > 16u ? launch_few<HD, ELEM, 2, 0>(st, a) : launch_few<HD, ELEM, 1, 0>(st, a);
@@ -526,7 +528,14 @@ template <int HD, int MT> void configure_few() {
 KvPlan kv_attention_plan(uint32_t head_dim, uint32_t n_kv, uint32_t capacity, uint32_t window, uint32_t sinks, uint32_t T, uint32_t n_q, int sms) {
     const uint32_t rows = T * (n_q / n_kv), per = head_dim == 256u ? 16u : (rows > 16u ? 32u : 16u);
     const uint64_t ctas = (uint64_t)n_kv * ((rows + per - 1u) / per), keys = window ? (uint64_t)sinks + window + T - 1u : capacity;
-    KvPlan p{1u, false};
+    KvPlan p{1u, false, head_dim != 256u && rows > kKvFewRows};
+    if (p.many) {
+        /* a CTA per SM, each with at least two tiles of 128 keys */
+        const uint64_t ctas = (uint64_t)n_kv * ((rows + 255u) / 256u), keys = window ? (uint64_t)sinks + window + (T < 256u ? T : 256u) : capacity;
+        const uint64_t most = (keys + 255u) / 256u, want = ctas < (uint64_t)sms ? (uint64_t)sms / ctas : 1u;
+        p.splits = (uint32_t)(want < most ? want : most);
+        return p;
+    }
     if (ctas >= (uint64_t)sms * 2u) return p;
     if (keys <= kKvShortKeys) {
         /* clusters of 2^k CTAs, a tile of 16 keys for each of their four warps, as long as the GPU has room for them */
@@ -541,17 +550,18 @@ KvPlan kv_attention_plan(uint32_t head_dim, uint32_t n_kv, uint32_t capacity, ui
 }
 
 cudaError_t launch_kv_attention(cudaStream_t st, int elem, uint32_t head_dim, const KvAttention &a, const KvPlan &p) {
-    if (elem == kKvE4m3) return head_dim == 64u ? launch_all<64, kKvE4m3>(st, a, p.in_clusters) : head_dim == 128u ? launch_all<128, kKvE4m3>(st, a, p.in_clusters) : launch_all<256, kKvE4m3>(st, a, p.in_clusters);
-    return head_dim == 64u ? launch_all<64, kKvBf16>(st, a, p.in_clusters) : head_dim == 128u ? launch_all<128, kKvBf16>(st, a, p.in_clusters) : launch_all<256, kKvBf16>(st, a, p.in_clusters);
+    if (elem == kKvE4m3) return head_dim == 64u ? launch_all<64, kKvE4m3>(st, a, p) : head_dim == 128u ? launch_all<128, kKvE4m3>(st, a, p) : launch_all<256, kKvE4m3>(st, a, p);
+    return head_dim == 64u ? launch_all<64, kKvBf16>(st, a, p) : head_dim == 128u ? launch_all<128, kKvBf16>(st, a, p) : launch_all<256, kKvBf16>(st, a, p);
 }
 
-void configure_kv_kernels() { configure_few<64, 1>(); configure_few<64, 2>(); configure_few<128, 1>(); configure_few<128, 2>(); configure_few<256, 1>(); }
+void configure_kv_kernels() { configure_kv_many(); configure_few<64, 1>(); configure_few<64, 2>(); configure_few<128, 1>(); configure_few<128, 2>(); configure_few<256, 1>(); }
 
 int read_kv_status(bool clear) {
     int v = 0;
     if (cudaMemcpyFromSymbol(&v, g_kernel_status, sizeof(int)) != cudaSuccess) return -1;
     if (clear && v) { const int z = 0; cudaMemcpyToSymbol(g_kernel_status, &z, sizeof(int)); }
-    return v;
+    const int w = read_kv_many_status(clear);
+    return v ? v : w;
 }
 
 }  // namespace nwc

@@ -1,0 +1,473 @@
+/* Attention of many query rows (a prompt chunk, a large draft tree) over a cache of nwc_kv.h on the 5th-generation tensor
+ * cores.  What a token sees: see nwc_kv_attention.cu.
+ *
+ * All query heads of a key/value head are rows of one matrix (row = token * group + head), so K and V are read once for the
+ * group.  A CTA holds two tiles of 128 rows ("streams") and walks over tiles of 128 keys: S = Q K^T into tensor memory, 128
+ * threads per stream turn their row of S into weights P (one thread = one row: no shuffles), P goes back to tensor memory as
+ * the A operand of O += P V.  While one stream's weights are computed the tensor cores work for the other:
+ *
+ *   tensor:   S0(j+1)  PV1(j) S1(j+1)   PV0(j+1) S0(j+2) ...
+ *   stream 0:      weights of S0(j+1)
+ *   stream 1:                  weights of S1(j+1)
+ *
+ * With at most 128 rows in all, both streams hold the same rows and take the key tiles in turn; their shares meet at the end.
+ * Few rows over a long cache: the keys are divided over several CTAs and joined by kv_attention_join_kernel.
+ *
+ * Bound: 4 * 128 * 128 * head_dim multiply-adds per pair of tiles on the tensor cores (2048 clocks at head_dim 128), and as
+ * many clocks of the exponential unit (16 per SM and clock) for 2 * 128 * 128 weights.
+ *
+ * Roles: warps 0-3 and 4-7 weights of stream 0 and 1 (they also load Q, rescale and write out O), warps 8-11 bring K and V
+ * into shared memory, one thread of warp 12 issues the MMAs.  The copies are 16 bytes per thread, so a tile may begin, end and
+ * wrap anywhere in the ring and a row that is no key of the call is written as zeros (whatever its slot holds, weight 0 times
+ * it must be 0).  e4m3 rows become bf16 on the way, exactly: code and unit have fewer bits than a bf16 number.  All waits are
+ * bounded; a role that gives up records the status word and stops, the others run out, tensor memory is freed.
+ *
+ * O is rescaled in tensor memory only when a row's maximum passes the one it is scaled by by more than 2^8 (weights stay below
+ * 2^8, sums are fp32): after the first tiles hardly ever.  P is rounded to bf16 (2^-8 relative), the sum of the weights is not.
+ */
+#include "nwc_kv.h"
+#include "nwc_async.cuh"
+#include "nwc_launch.h"
+
+namespace nwc {
+
+namespace {
+
+constexpr uint32_t kManyRows = 128u, kManyKeys = 128u, kManyThreads = 13u * 32u;
+
+template <int HD, int ELEM> struct Many {
+    static constexpr uint32_t kHalves = HD / 64u, kTile = kManyKeys * HD * 2u, kHalfBytes = kManyKeys * 128u;      /* a bf16 tile: halves of 64 dimensions, 128-byte rows, swizzled */
+    static constexpr uint32_t kSlots = ELEM == kKvE4m3 ? (HD == 64 ? 6u : 3u) : (HD == 64 ? 8u : 5u);
+    static constexpr uint32_t kStaging = ELEM == kKvE4m3 ? 4u : 0u, kStagingBytes = kManyKeys * HD;              /* raw codes in flight */
+    static constexpr uint32_t kAhead = ELEM == kKvE4m3 ? 3u : 2u;                                                 /* tiles in flight beyond the one awaited */
+    static constexpr uint32_t kQ = 0u, kRing = 2u * kTile, kStage = kRing + kSlots * kTile, kBars = kStage + kStaging * kStagingBytes;
+    static constexpr uint32_t kSmem = 1024u + kBars + (2u * kSlots + 8u) * 8u + 16u;
+};
+
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr, uint32_t lead_bytes) {
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(lead_bytes >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) | ((uint64_t)1u << 46) | ((uint64_t)2u << 61);
+}
+__host__ __device__ constexpr uint32_t idesc_bf16(uint32_t M, uint32_t N, bool b_mn_major) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn_major ? 1u << 16 : 0u) | ((N >> 3) << 17) | ((M >> 4) << 24);
+}
+__device__ __forceinline__ uint32_t swizzled(uint32_t row, uint32_t chunk) { return row * 128u + ((chunk ^ (row & 7u)) << 4); }
+__device__ __forceinline__ void sts128u(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) { asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory"); }
+__device__ __forceinline__ void arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, uint32_t bytes) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory"); }
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void mma_commit(uint32_t bar) { asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tm_load32(uint32_t addr, uint32_t (&v)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+                   "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+                 : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tm_store32(uint32_t addr, const uint32_t (&v)[32]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+                 ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
+                   "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]) : "memory");
+}
+__device__ __forceinline__ void tm_store16(uint32_t addr, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
+}
+__device__ __forceinline__ void tm_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tm_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tm_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tm_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) { uint32_t d; asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(b), "f"(a)); return d; }
+__device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+/* bits [lo, hi) of a word whose bit 0 is number 0; lo and hi may lie anywhere */
+__device__ __forceinline__ uint32_t bit_range(int32_t lo, int32_t hi) {
+    lo = max(lo, 0); hi = min(hi, 32);
+    if (lo >= hi) return 0u;
+    return (0xFFFFFFFFu >> (32 - (hi - lo))) << lo;
+}
+
+}  // namespace
+
+template <int HD, int ELEM>
+__global__ void __launch_bounds__(kManyThreads, 1) kv_attention_many_kernel(const KvAttention a) {
+    using F = Many<HD, ELEM>;
+    constexpr uint32_t NS = F::kSlots;
+    extern __shared__ uint8_t many_raw[];
+    const uint32_t base = (smem_addr(many_raw) + 1023u) & ~1023u;
+    const uint32_t bars = base + F::kBars, full = bars, empty = bars + NS * 8u, q_full = bars + 2u * NS * 8u, s_full = q_full + 16u, p_full = s_full + 16u, o_full = p_full + 16u, tmem_slot = o_full + 16u;
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+    const uint32_t group = a.n_q / a.c.n_kv, rows = a.T * group, kvh = blockIdx.y % a.c.n_kv, row0 = (blockIdx.y / a.c.n_kv) * 2u * kManyRows, split = blockIdx.x;
+    const bool solo = rows - row0 <= kManyRows;
+    if (warp == 12u) {
+        if (lane == 0) {
+            for (uint32_t s = 0; s < NS; s++) { mbar_init(full + s * 8u, 128u); mbar_init(empty + s * 8u, 1u); }
+            for (uint32_t s = 0; s < 2u; s++) { mbar_init(q_full + s * 8u, 128u); mbar_init(s_full + s * 8u, 1u); mbar_init(p_full + s * 8u, 128u); mbar_init(o_full + s * 8u, 1u); }
+            mbar_init_fence();
+        }
+        __syncwarp();
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tmem_slot) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int32_t pos = *a.pos;
+    const bool pos_ok = pos >= 0 && (uint64_t)pos + a.T <= (a.c.window ? 0x7FFFFFFFu : a.c.capacity);
+    tm_fence_before();
+    __syncthreads();
+    tm_fence_after();
+    uint32_t tmem; asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
+    /* the keys that this CTA's tokens see: as kv_span, for their positions; list index = lead sinks, then positions from first */
+    const uint32_t t_first = row0 / group, t_last = min(a.T - 1u, (row0 + 2u * kManyRows - 1u) / group);
+    KvSpan span{0u, 0u, 0u};
+    if (pos_ok) span = a.visible ? kv_span(pos, a.T, a.c.window, a.c.sinks) : kv_span((uint32_t)pos + t_first, t_last - t_first + 1u, a.c.window, a.c.sinks);
+    const uint32_t slot_first = kv_slot(span.first, a.c.capacity, a.c.window, a.c.sinks), ring = a.c.capacity - a.c.sinks;
+    const uint32_t all = (span.count + kManyKeys - 1u) / kManyKeys, tile0 = (uint32_t)((uint64_t)all * split / a.splits), n = (uint32_t)((uint64_t)all * (split + 1u) / a.splits) - tile0;
+    /* items of the operand ring: K0 K1 V0 K2 V1 ... K(n-1) V(n-2) V(n-1) */
+    auto item_k = [](uint32_t t) { return t ? 2u * t - 1u : 0u; };
+    auto item_v = [n](uint32_t t) { return t + 1u < n ? 2u * t + 2u : 2u * n - 1u; };
+    bool alive = true;
+    if (warp < 8u) {
+        /* ---- weights ---- */
+        const uint32_t s = warp >> 2, wt = tid & 127u, q_tile = solo ? 0u : s, my_row0 = row0 + q_tile * kManyRows;
+        const uint32_t my_n = solo ? (s ? n / 2u : (n + 1u) / 2u) : n;                 /* tiles of this stream */
+        if (n && !(solo && s)) {
+            /* Q: 16 bytes per thread, rows beyond the last as zeros */
+            for (uint32_t e = wt; e < kManyRows * HD / 8u; e += 128u) {
+                const uint32_t r = e / (HD / 8u), ch = e % (HD / 8u), row = my_row0 + r;
+                uint4 w = make_uint4(0u, 0u, 0u, 0u);
+                if (row < rows) w = *reinterpret_cast<const uint4 *>(a.q + (uint64_t)(row / group) * a.ldq + (uint64_t)(kvh * group + row % group) * HD + ch * 8u);
+                sts128u(base + F::kQ + q_tile * F::kTile + (ch >> 3) * F::kHalfBytes + swizzled(r, ch & 7u), w.x, w.y, w.z, w.w);
+            }
+            async_proxy_fence();
+            arrive(q_full + q_tile * 8u);
+        }
+        const uint32_t row = my_row0 + wt, row_ok = row < rows, token = min(row, rows - 1u) / group, idx_pos = (uint32_t)pos - span.first + span.lead;      /* (tree) list index of the first draft */
+        const uint32_t own = (uint32_t)pos + (a.depth ? (uint32_t)a.depth[token] : token), words = (a.T + 31u) / 32u;
+        /* in list indices this row sees [lo, hi) and what lies below `always` of it */
+        const int32_t hi = a.visible ? (int32_t)idx_pos : (int32_t)(own - span.first + span.lead + 1u);
+        const int32_t lo = a.c.window && own + 1u > a.c.window + span.first ? (int32_t)(span.lead + own + 1u - a.c.window - span.first) : (int32_t)span.lead;
+        const int32_t always = min((int32_t)(a.c.window ? max(a.c.sinks, span.lead) : span.lead), hi);
+        const uint32_t *seen = a.visible ? a.visible + (uint64_t)token * words : nullptr;
+        const uint32_t tm_s = tmem + s * 128u + ((warp & 3u) << 21), tm_o = tmem + 256u + s * 128u + ((warp & 3u) << 21);
+        float m = -INFINITY, l = 0.f;
+        uint32_t v[32];
+        for (uint32_t i = 0; i < my_n && alive; i++) {
+            const int32_t key0 = (int32_t)((tile0 + (solo ? 2u * i + s : i)) * kManyKeys);
+            /* what of the tile the row sees; a warp whose rows see it whole does without */
+            uint32_t vis[4];
+            bool whole = true;
+#pragma unroll
+            for (uint32_t ch = 0; ch < 4u; ch++) {
+                const int32_t k0 = key0 + (int32_t)(ch * 32u);
+                vis[ch] = bit_range(lo - k0, hi - k0) | bit_range(0 - k0, always - k0);
+                if (seen) {
+                    const int32_t d = k0 - (int32_t)idx_pos;                             /* draft of the chunk's first key */
+                    if (d > -32 && d < (int32_t)a.T) {
+                        const uint32_t w0 = d >= 0 ? (uint32_t)d >> 5 : 0u, lo_word = seen[w0], hi_word = d >= 0 && w0 + 1u < words ? seen[w0 + 1u] : 0u;
+                        vis[ch] |= (d >= 0 ? __funnelshift_r(lo_word, hi_word, (uint32_t)d & 31u) : lo_word << (uint32_t)(-d)) & bit_range(-d, (int32_t)a.T - d);
+                    }
+                }
+                whole = whole && vis[ch] == 0xFFFFFFFFu;
+            }
+            whole = __all_sync(0xffffffffu, whole || !row_ok);
+            alive = mbar_wait(s_full + s * 8u, i & 1u);
+            if (!alive) break;
+            tm_fence_after();
+            float top = -INFINITY;
+#pragma unroll
+            for (uint32_t ch = 0; ch < 4u; ch++) {
+                tm_load32(tm_s + ch * 32u, v);
+                tm_wait_load();
+                if (!whole) {
+#pragma unroll
+                    for (uint32_t e = 0; e < 32u; e++) if (!((vis[ch] >> e) & 1u)) v[e] = 0xFF800000u;
+                }
+#pragma unroll
+                for (uint32_t e = 0; e < 32u; e += 2u) top = fmaxf(top, fmaxf(__uint_as_float(v[e]), __uint_as_float(v[e + 1])));
+            }
+            top *= a.scale;
+            const bool raise = top > m + 8.f;
+            if (__any_sync(0xffffffffu, raise)) {
+                const float up = raise ? top : m, f = up == -INFINITY ? 1.f : exp2_fast(m - up);
+                if (i) {
+#pragma unroll
+                    for (uint32_t ch = 0; ch < HD / 32u; ch++) {
+                        tm_load32(tm_o + ch * 32u, v);
+                        tm_wait_load();
+#pragma unroll
+                        for (uint32_t e = 0; e < 32u; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+                        tm_store32(tm_o + ch * 32u, v);
+                    }
+                }
+                m = up; l *= f;
+            }
+            const float below = m == -INFINITY ? 0.f : m;
+            float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+            for (uint32_t ch = 0; ch < 4u; ch++) {
+                tm_load32(tm_s + ch * 32u, v);
+                tm_wait_load();
+                uint32_t p[16];
+#pragma unroll
+                for (uint32_t e = 0; e < 32u; e += 2u) {
+                    float x = __uint_as_float(v[e]), y = __uint_as_float(v[e + 1]);
+                    if (!whole) { if (!((vis[ch] >> e) & 1u)) x = -INFINITY; if (!((vis[ch] >> (e + 1u)) & 1u)) y = -INFINITY; }
+                    x = exp2_fast(fmaf(x, a.scale, -below)); y = exp2_fast(fmaf(y, a.scale, -below));
+                    l0 += x; l1 += y;
+                    p[e >> 1] = pack_bf16(x, y);
+                }
+                tm_store16(tm_s + ch * 16u, p);
+            }
+            l += l0 + l1;
+            tm_wait_store();
+            tm_fence_before();
+            arrive(p_full + s * 8u);
+        }
+        /* O, then the row's share or result */
+        if (alive && my_n) { alive = mbar_wait(o_full + s * 8u, 0u); tm_fence_after(); }
+        if (solo) {
+            /* the second stream's share through shared memory (Q, K and V are done with: O1 is complete and O0 is awaited) */
+            float *there = reinterpret_cast<float *>(many_raw + (base - smem_addr(many_raw)));
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            if (s == 1) {
+                if (alive && my_n) {
+#pragma unroll
+                    for (uint32_t ch = 0; ch < HD / 32u; ch++) {
+                        tm_load32(tm_o + ch * 32u, v);
+                        tm_wait_load();
+#pragma unroll
+                        for (uint32_t e = 0; e < 32u; e++) there[(ch * 32u + e) * 128u + wt] = __uint_as_float(v[e]);
+                    }
+                }
+                there[HD * 128u + wt] = my_n ? m : -INFINITY; there[HD * 128u + 128u + wt] = l;
+            }
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+        }
+        if (alive && pos_ok && !(solo && s)) {
+            const float *there = reinterpret_cast<const float *>(many_raw + (base - smem_addr(many_raw)));
+            float f0 = 1.f, f1 = 0.f, total = l, top = m;
+            if (solo) {
+                const float m1 = there[HD * 128u + wt];
+                top = fmaxf(m, m1);
+                f0 = m == -INFINITY ? 0.f : exp2_fast(m - top); f1 = m1 == -INFINITY ? 0.f : exp2_fast(m1 - top);
+                total = l * f0 + there[HD * 128u + 128u + wt] * f1;
+            }
+            const uint64_t line = (uint64_t)token * a.n_q + kvh * group + row % group;
+            const float r = total == 0.f ? 0.f : 1.f / total;
+            float *part = a.splits > 1u ? a.part_o + ((uint64_t)split * a.T * a.n_q + line) * HD : nullptr;
+            if (a.splits > 1u && row_ok) *reinterpret_cast<float2 *>(a.part_ml + ((uint64_t)split * a.T * a.n_q + line) * 2u) = make_float2(n ? top : -INFINITY, total);
+#pragma unroll
+            for (uint32_t ch = 0; ch < HD / 32u; ch++) {
+                if (my_n) { tm_load32(tm_o + ch * 32u, v); tm_wait_load(); }
+                else {
+#pragma unroll
+                    for (uint32_t e = 0; e < 32u; e++) v[e] = 0u;
+                }
+                if (solo) {
+#pragma unroll
+                    for (uint32_t e = 0; e < 32u; e++) {
+                        float x = __uint_as_float(v[e]) * f0;
+                        if (f1 != 0.f) x = fmaf(there[(ch * 32u + e) * 128u + wt], f1, x);
+                        v[e] = __float_as_uint(x);
+                    }
+                }
+                if (row_ok && part) {
+#pragma unroll
+                    for (uint32_t e = 0; e < 32u; e += 4u) *reinterpret_cast<uint4 *>(part + ch * 32u + e) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                } else if (row_ok) {
+                    uint16_t *to = a.out + line * HD + ch * 32u;
+#pragma unroll
+                    for (uint32_t e = 0; e < 32u; e += 8u) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (uint32_t j = 0; j < 4u; j++) w[j] = total == 0.f ? 0u : pack_bf16(__uint_as_float(v[e + 2u * j]) * r, __uint_as_float(v[e + 2u * j + 1u]) * r);
+                        *reinterpret_cast<uint4 *>(to + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+                __syncwarp();
+            }
+        }
+    } else if (warp < 12u) {
+        /* ---- K and V into shared memory ---- */
+        const uint32_t pt = tid - 256u, items = 2u * n;
+        constexpr uint32_t kChunks = HD * (ELEM == kKvE4m3 ? 1u : 2u) / 16u, kPasses = kManyKeys * kChunks / 128u, kRowsPerPass = 128u / kChunks;
+        const uint32_t ch = pt % kChunks, r0 = pt / kChunks;                            /* this thread's chunk of rows r0, r0 + kRowsPerPass, ... */
+        const uint64_t head = (uint64_t)kvh * a.c.capacity;
+        auto tile_of = [&](uint32_t x) { return x == 0u ? 0u : x + 1u == items ? n - 1u : x & 1u ? (x + 1u) / 2u : (x - 2u) / 2u; };
+        auto is_v = [&](uint32_t x) { return x != 0u && (x + 1u == items || !(x & 1u)); };
+        auto cell_of = [&](uint32_t i) -> uint64_t {                                    /* slot of list index i < span.count */
+            uint32_t sl = i < span.lead ? i : slot_first + (i - span.lead);
+            if (i >= span.lead && sl >= a.c.capacity) sl -= ring;
+            return head + sl;
+        };
+        auto fetch = [&](uint32_t x, uint32_t dst_tile) {                              /* the item's rows as they are: bf16 into the operand's places, codes into this thread's staging */
+            const uint8_t *from = is_v(x) ? a.c.v : a.c.k;
+            const uint32_t i0 = (tile0 + tile_of(x)) * kManyKeys;
+#pragma unroll
+            for (uint32_t e = 0; e < kPasses; e++) {
+                const uint32_t r = r0 + e * kRowsPerPass, i = i0 + r, ok = i < span.count;
+                const uint64_t cell = ok ? cell_of(i) : head;
+                if (ELEM == kKvE4m3) copy16(dst_tile + (e * 128u + pt) * 16u, from + cell * HD + ch * 16u, ok ? 16u : 0u);
+                else copy16(dst_tile + (ch >> 3) * F::kHalfBytes + swizzled(r, ch & 7u), from + (cell * HD + ch * 8u) * 2u, ok ? 16u : 0u);
+            }
+        };
+        if (ELEM == kKvBf16) {
+            for (uint32_t x = 0; x < items + F::kAhead && alive; x++) {
+                if (x < items) {
+                    if (x >= NS) alive = mbar_wait(empty + (x % NS) * 8u, ((x / NS) - 1u) & 1u);
+                    if (!alive) break;
+                    fetch(x, base + F::kRing + (x % NS) * F::kTile);
+                }
+                copies_commit();
+                if (x >= F::kAhead) {
+                    copies_wait<F::kAhead>();
+                    async_proxy_fence();
+                    arrive(full + ((x - F::kAhead) % NS) * 8u);
+                }
+            }
+        } else {
+            uint8_t unit[kPasses];
+            auto units = [&](uint32_t x) {
+                const uint8_t *from = is_v(x) ? a.c.v_exp : a.c.k_exp;
+                const uint32_t i0 = (tile0 + tile_of(x)) * kManyKeys;
+#pragma unroll
+                for (uint32_t e = 0; e < kPasses; e++) { const uint32_t i = i0 + r0 + e * kRowsPerPass; unit[e] = from[i < span.count ? cell_of(i) : head]; }
+            };
+            for (uint32_t x = 0; x < F::kAhead; x++) { if (x < items) fetch(x, base + F::kStage + (x % F::kStaging) * F::kStagingBytes); copies_commit(); }
+            if (items) units(0u);
+            for (uint32_t x = 0; x < items && alive; x++) {
+                if (x + F::kAhead < items) fetch(x + F::kAhead, base + F::kStage + ((x + F::kAhead) % F::kStaging) * F::kStagingBytes);
+                copies_commit();
+                copies_wait<F::kAhead>();
+                uint8_t now[kPasses];
+#pragma unroll
+                for (uint32_t e = 0; e < kPasses; e++) now[e] = unit[e];
+                if (x + 1u < items) units(x + 1u);
+                if (x >= NS) alive = mbar_wait(empty + (x % NS) * 8u, ((x / NS) - 1u) & 1u);
+                if (!alive) break;
+                const uint32_t dst = base + F::kRing + (x % NS) * F::kTile, src = base + F::kStage + (x % F::kStaging) * F::kStagingBytes;
+#pragma unroll
+                for (uint32_t e = 0; e < kPasses; e++) {
+                    const uint4 w = lds128(src + (e * 128u + pt) * 16u);
+                    const uint32_t u2 = kv_unit2(now[e]);
+                    uint4 lo, hi;
+                    kv_values4(w.x, u2, lo.x, lo.y); kv_values4(w.y, u2, lo.z, lo.w); kv_values4(w.z, u2, hi.x, hi.y); kv_values4(w.w, u2, hi.z, hi.w);
+                    const uint32_t r = r0 + e * kRowsPerPass, at = dst + (ch >> 2) * F::kHalfBytes, c8 = (ch & 3u) * 2u;
+                    sts128u(at + swizzled(r, c8), lo.x, lo.y, lo.z, lo.w);
+                    sts128u(at + swizzled(r, c8 + 1u), hi.x, hi.y, hi.z, hi.w);
+                }
+                async_proxy_fence();
+                arrive(full + (x % NS) * 8u);
+            }
+        }
+        copies_wait<0>();
+    } else if (lane == 0 && n) {
+        /* ---- matrix products ---- */
+        const uint32_t q_desc_base = base + F::kQ, ring0 = base + F::kRing;
+        constexpr uint32_t kIdescS = idesc_bf16(128u, kManyKeys, false), kIdescO = idesc_bf16(128u, HD, true);
+        auto ready = [&](uint32_t item) { return mbar_wait_one(full + (item % NS) * 8u, (item / NS) & 1u); };
+        auto scores = [&](uint32_t s, uint32_t t) {
+            const uint32_t kt = ring0 + (item_k(t) % NS) * F::kTile, qt = q_desc_base + (solo ? 0u : s) * F::kTile;
+#pragma unroll
+            for (uint32_t kk = 0; kk < HD / 16u; kk++)
+                mma_ss(tmem + s * 128u, desc_sw128(qt + (kk >> 2) * F::kHalfBytes + (kk & 3u) * 32u, 16u), desc_sw128(kt + (kk >> 2) * F::kHalfBytes + (kk & 3u) * 32u, 16u), kIdescS, kk ? 1u : 0u);
+            mma_commit(s_full + s * 8u);
+        };
+        auto outputs = [&](uint32_t s, uint32_t t, bool first) {
+            const uint32_t vt = ring0 + (item_v(t) % NS) * F::kTile;
+#pragma unroll
+            for (uint32_t kk = 0; kk < kManyKeys / 16u; kk++)
+                mma_ts(tmem + 256u + s * 128u, tmem + s * 128u + kk * 8u, desc_sw128(vt + kk * 2048u, F::kHalfBytes), kIdescO, first && !kk ? 0u : 1u);
+        };
+        auto release = [&](uint32_t item) { mma_commit(empty + (item % NS) * 8u); };
+        alive = mbar_wait_one(q_full, 0u) && (solo || mbar_wait_one(q_full + 8u, 0u)) && ready(0u);
+        if (alive) {
+            tm_fence_after();
+            scores(0u, 0u);
+            if (solo) {
+                release(item_k(0u));
+                if (n > 1u) { alive = ready(item_k(1u)); if (alive) { tm_fence_after(); scores(1u, 1u); release(item_k(1u)); } }
+            } else { scores(1u, 0u); release(item_k(0u)); }
+        }
+        if (solo) {
+            for (uint32_t t = 0; t < n && alive; t++) {                                 /* tile t belongs to stream t & 1 */
+                const uint32_t s = t & 1u;
+                alive = ready(item_v(t)) && mbar_wait_one(p_full + s * 8u, (t >> 1) & 1u);
+                if (!alive) break;
+                tm_fence_after();
+                outputs(s, t, t < 2u);
+                release(item_v(t));
+                if (t + 2u >= n) mma_commit(o_full + s * 8u);
+                else {
+                    alive = ready(item_k(t + 2u));
+                    if (!alive) break;
+                    tm_fence_after();
+                    scores(s, t + 2u);
+                    release(item_k(t + 2u));
+                }
+            }
+        } else {
+            for (uint32_t t = 0; t < n && alive; t++) {
+                const bool more = t + 1u < n;
+                alive = ready(item_v(t)) && (!more || ready(item_k(t + 1u)));
+                for (uint32_t s = 0; s < 2u && alive; s++) {
+                    alive = mbar_wait_one(p_full + s * 8u, t & 1u);
+                    if (!alive) break;
+                    tm_fence_after();
+                    outputs(s, t, t == 0u);
+                    if (s) release(item_v(t));
+                    if (more) { scores(s, t + 1u); if (s) release(item_k(t + 1u)); }
+                    else mma_commit(o_full + s * 8u);
+                }
+            }
+        }
+        if (!alive) {                                                                   /* what was issued must end before the memory is given back */
+            mma_commit(o_full); mma_commit(o_full + 8u);
+            for (uint32_t i = 0; i < (1u << 20); i++) if (mbar_poll(o_full, 0u) && mbar_poll(o_full + 8u, 0u)) break;
+        }
+    }
+    if (!pos_ok && tid == 0) atomicOr(a.status, kKvStatusPosition);
+    __syncwarp();
+    tm_fence_before();
+    __syncthreads();
+    tm_fence_after();
+    if (warp == 12u) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+template <int HD, int ELEM>
+static cudaError_t launch_many(cudaStream_t st, const KvAttention &a) {
+    const uint64_t rows = (uint64_t)a.T * (a.n_q / a.c.n_kv), pairs = (rows + 2u * kManyRows - 1u) / (2u * kManyRows);
+    if (pairs * a.c.n_kv > 65535u) return cudaErrorInvalidValue;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.splits, (uint32_t)(pairs * a.c.n_kv)); cfg.blockDim = dim3(kManyThreads); cfg.dynamicSmemBytes = Many<HD, ELEM>::kSmem; cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr; cfg.numAttrs = dependent_launch() ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kv_attention_many_kernel<HD, ELEM>, a);
+}
+
+cudaError_t launch_kv_many(cudaStream_t st, int elem, uint32_t head_dim, const KvAttention &a) {
+    if (elem == kKvE4m3) return head_dim == 64u ? launch_many<64, kKvE4m3>(st, a) : launch_many<128, kKvE4m3>(st, a);
+    return head_dim == 64u ? launch_many<64, kKvBf16>(st, a) : launch_many<128, kKvBf16>(st, a);
+}
+
+void configure_kv_many() {
+    cudaFuncSetAttribute(kv_attention_many_kernel<64, kKvBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Many<64, kKvBf16>::kSmem);
+    cudaFuncSetAttribute(kv_attention_many_kernel<64, kKvE4m3>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Many<64, kKvE4m3>::kSmem);
+    cudaFuncSetAttribute(kv_attention_many_kernel<128, kKvBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Many<128, kKvBf16>::kSmem);
+    cudaFuncSetAttribute(kv_attention_many_kernel<128, kKvE4m3>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Many<128, kKvE4m3>::kSmem);
+}
+
+int read_kv_many_status(bool clear) {
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_kernel_status, sizeof(int)) != cudaSuccess) return -1;
+    if (clear && v) { const int z = 0; cudaMemcpyToSymbol(g_kernel_status, &z, sizeof(int)); }
+    return v;
+}
+
+}  // namespace nwc
