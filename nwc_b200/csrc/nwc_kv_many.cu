@@ -16,8 +16,8 @@
  * Bound: 4 * 128 * 128 * head_dim multiply-adds per pair of tiles on the tensor cores (2048 clocks at head_dim 128), and as
  * many clocks of the exponential unit (16 per SM and clock) for 2 * 128 * 128 weights.
  *
- * Roles: warps 0-3 and 4-7 weights of stream 0 and 1 (they also load Q, rescale and write out O), warps 8-11 bring K and V
- * into shared memory, one thread of warp 12 issues the MMAs.  The copies are 16 bytes per thread, so a tile may begin, end and
+ * Roles: warps 0-3 and 4-7 weights of stream 0 and 1 (they also load Q, rescale and write out O), warps 8-15 bring K and V
+ * into shared memory, one thread of warp 16 issues the MMAs.  The copies are 16 bytes per thread, so a tile may begin, end and
  * wrap anywhere in the ring and a row that is no key of the call is written as zeros (whatever its slot holds, weight 0 times
  * it must be 0).  e4m3 rows become bf16 on the way, exactly: code and unit have fewer bits than a bf16 number.  All waits are
  * bounded; a role that gives up records the status word and stops, the others run out, tensor memory is freed.
@@ -33,10 +33,10 @@ namespace nwc {
 
 namespace {
 
-constexpr uint32_t kManyRows = 128u, kManyKeys = 128u, kManyThreads = 13u * 32u;
+constexpr uint32_t kManyRows = 128u, kManyKeys = 128u, kManyThreads = 20u * 32u, kProducers = 256u;
 
 template <int HD, int ELEM> struct Many {
-    static constexpr uint32_t kHalves = HD / 64u, kTile = kManyKeys * HD * 2u, kHalfBytes = kManyKeys * 128u;      /* a bf16 tile: halves of 64 dimensions, 128-byte rows, swizzled */
+    static constexpr uint32_t kTile = kManyKeys * HD * 2u, kHalfBytes = kManyKeys * 128u;      /* a bf16 tile: halves of 64 dimensions, 128-byte rows, swizzled */
     static constexpr uint32_t kSlots = ELEM == kKvE4m3 ? (HD == 64 ? 6u : 3u) : (HD == 64 ? 8u : 5u);
     static constexpr uint32_t kStaging = ELEM == kKvE4m3 ? 4u : 0u, kStagingBytes = kManyKeys * HD;              /* raw codes in flight */
     static constexpr uint32_t kAhead = ELEM == kKvE4m3 ? 3u : 2u;                                                 /* tiles in flight beyond the one awaited */
@@ -74,10 +74,21 @@ __device__ __forceinline__ void tm_store32(uint32_t addr, const uint32_t (&v)[32
                  ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
                    "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]) : "memory");
 }
-__device__ __forceinline__ void tm_store16(uint32_t addr, const uint32_t (&v)[16]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
-                 ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
+__device__ __forceinline__ void tm_load16(uint32_t addr, uint32_t (&v)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                 : "r"(addr) : "memory");
 }
+/* the wait names the registers that it makes valid, so that nothing reads them above it */
+__device__ __forceinline__ void tm_wait_load16(uint32_t (&v)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]) :: "memory");
+}
+/* two fp32 operations in one instruction */
+__device__ __forceinline__ uint64_t pack2(float a, float b) { uint64_t d; asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b)); return d; }
+__device__ __forceinline__ void unpack2(uint64_t v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) { uint64_t d; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c)); return d; }
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) { uint64_t d; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b)); return d; }
 __device__ __forceinline__ void tm_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tm_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tm_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -103,9 +114,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attention_many_kernel(cons
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
     const uint32_t group = a.n_q / a.c.n_kv, rows = a.T * group, kvh = blockIdx.y % a.c.n_kv, row0 = (blockIdx.y / a.c.n_kv) * 2u * kManyRows, split = blockIdx.x;
     const bool solo = rows - row0 <= kManyRows;
-    if (warp == 12u) {
+    if (warp == 16u) {
         if (lane == 0) {
-            for (uint32_t s = 0; s < NS; s++) { mbar_init(full + s * 8u, 128u); mbar_init(empty + s * 8u, 1u); }
+            for (uint32_t s = 0; s < NS; s++) { mbar_init(full + s * 8u, kProducers); mbar_init(empty + s * 8u, 1u); }
             for (uint32_t s = 0; s < 2u; s++) { mbar_init(q_full + s * 8u, 128u); mbar_init(s_full + s * 8u, 1u); mbar_init(p_full + s * 8u, 128u); mbar_init(o_full + s * 8u, 1u); }
             mbar_init_fence();
         }
@@ -131,8 +142,10 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attention_many_kernel(cons
     auto item_k = [](uint32_t t) { return t ? 2u * t - 1u : 0u; };
     auto item_v = [n](uint32_t t) { return t + 1u < n ? 2u * t + 2u : 2u * n - 1u; };
     bool alive = true;
+    /* registers: 20 warps start with 96 each; 8 x 144 + 8 x 64 + 4 x 64 = 20 x 96 */
     if (warp < 8u) {
         /* ---- weights ---- */
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
         const uint32_t s = warp >> 2, wt = tid & 127u, q_tile = solo ? 0u : s, my_row0 = row0 + q_tile * kManyRows;
         const uint32_t my_n = solo ? (s ? n / 2u : (n + 1u) / 2u) : n;                 /* tiles of this stream */
         if (n && !(solo && s)) {
@@ -154,76 +167,98 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attention_many_kernel(cons
         const int32_t always = min((int32_t)(a.c.window ? max(a.c.sinks, span.lead) : span.lead), hi);
         const uint32_t *seen = a.visible ? a.visible + (uint64_t)token * words : nullptr;
         const uint32_t tm_s = tmem + s * 128u + ((warp & 3u) << 21), tm_o = tmem + 256u + s * 128u + ((warp & 3u) << 21);
+        const int32_t lo_all = __reduce_max_sync(0xffffffffu, row_ok ? lo : 0), hi_all = __reduce_min_sync(0xffffffffu, row_ok ? hi : 0x7FFFFFFF);
         float m = -INFINITY, l = 0.f;
         uint32_t v[32];
         for (uint32_t i = 0; i < my_n && alive; i++) {
             const int32_t key0 = (int32_t)((tile0 + (solo ? 2u * i + s : i)) * kManyKeys);
             /* what of the tile the row sees; a warp whose rows see it whole does without */
+            const bool whole = key0 >= lo_all && key0 + (int32_t)kManyKeys <= hi_all;
             uint32_t vis[4];
-            bool whole = true;
+            if (!whole) {
 #pragma unroll
-            for (uint32_t ch = 0; ch < 4u; ch++) {
-                const int32_t k0 = key0 + (int32_t)(ch * 32u);
-                vis[ch] = bit_range(lo - k0, hi - k0) | bit_range(0 - k0, always - k0);
-                if (seen) {
-                    const int32_t d = k0 - (int32_t)idx_pos;                             /* draft of the chunk's first key */
-                    if (d > -32 && d < (int32_t)a.T) {
-                        const uint32_t w0 = d >= 0 ? (uint32_t)d >> 5 : 0u, lo_word = seen[w0], hi_word = d >= 0 && w0 + 1u < words ? seen[w0 + 1u] : 0u;
-                        vis[ch] |= (d >= 0 ? __funnelshift_r(lo_word, hi_word, (uint32_t)d & 31u) : lo_word << (uint32_t)(-d)) & bit_range(-d, (int32_t)a.T - d);
+                for (uint32_t ch = 0; ch < 4u; ch++) {
+                    const int32_t k0 = key0 + (int32_t)(ch * 32u);
+                    vis[ch] = bit_range(lo - k0, hi - k0) | bit_range(0 - k0, always - k0);
+                    if (seen) {
+                        const int32_t d = k0 - (int32_t)idx_pos;                         /* draft of the chunk's first key */
+                        if (d > -32 && d < (int32_t)a.T) {
+                            const uint32_t w0 = d >= 0 ? (uint32_t)d >> 5 : 0u, lo_word = seen[w0], hi_word = d >= 0 && w0 + 1u < words ? seen[w0 + 1u] : 0u;
+                            vis[ch] |= (d >= 0 ? __funnelshift_r(lo_word, hi_word, (uint32_t)d & 31u) : lo_word << (uint32_t)(-d)) & bit_range(-d, (int32_t)a.T - d);
+                        }
                     }
                 }
-                whole = whole && vis[ch] == 0xFFFFFFFFu;
             }
-            whole = __all_sync(0xffffffffu, whole || !row_ok);
             alive = mbar_wait(s_full + s * 8u, i & 1u);
             if (!alive) break;
             tm_fence_after();
-            float top = -INFINITY;
+            /* One pass over the scores with the maximum as it stands: it is passed by more than 2^8 hardly ever after the first
+               tile, and then the pass is repeated (the weights stay in registers until it is known). */
+            bool raised = i == 0u;
+            if (raised) {
+                float top = -INFINITY;
 #pragma unroll
-            for (uint32_t ch = 0; ch < 4u; ch++) {
-                tm_load32(tm_s + ch * 32u, v);
-                tm_wait_load();
-                if (!whole) {
+                for (uint32_t ch = 0; ch < 4u; ch++) {
+                    tm_load32(tm_s + ch * 32u, v);
+                    tm_wait_load();
+                    if (!whole) {
 #pragma unroll
-                    for (uint32_t e = 0; e < 32u; e++) if (!((vis[ch] >> e) & 1u)) v[e] = 0xFF800000u;
-                }
-#pragma unroll
-                for (uint32_t e = 0; e < 32u; e += 2u) top = fmaxf(top, fmaxf(__uint_as_float(v[e]), __uint_as_float(v[e + 1])));
-            }
-            top *= a.scale;
-            const bool raise = top > m + 8.f;
-            if (__any_sync(0xffffffffu, raise)) {
-                const float up = raise ? top : m, f = up == -INFINITY ? 1.f : exp2_fast(m - up);
-                if (i) {
-#pragma unroll
-                    for (uint32_t ch = 0; ch < HD / 32u; ch++) {
-                        tm_load32(tm_o + ch * 32u, v);
-                        tm_wait_load();
-#pragma unroll
-                        for (uint32_t e = 0; e < 32u; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
-                        tm_store32(tm_o + ch * 32u, v);
+                        for (uint32_t e = 0; e < 32u; e++) if (!((vis[ch] >> e) & 1u)) v[e] = 0xFF800000u;
                     }
+#pragma unroll
+                    for (uint32_t e = 0; e < 32u; e += 2u) top = fmaxf(top, fmaxf(__uint_as_float(v[e]), __uint_as_float(v[e + 1])));
+                }
+                m = top * a.scale;
+            }
+            uint32_t p[64];
+            float sum;
+            for (;;) {
+                const float below = m == -INFINITY ? 0.f : -m;
+                const uint64_t scale2 = pack2(a.scale, a.scale), below2 = pack2(below, below);
+                uint64_t sum2 = 0ull;
+                float top = -INFINITY;
+                uint32_t w[2][16];
+                tm_load16(tm_s, w[0]);
+#pragma unroll
+                for (uint32_t ch = 0; ch < 8u; ch++) {
+                    uint32_t (&x)[16] = w[ch & 1u];
+                    tm_wait_load16(x);
+                    if (ch < 7u) tm_load16(tm_s + (ch + 1u) * 16u, w[(ch + 1u) & 1u]);
+                    if (!whole) {
+#pragma unroll
+                        for (uint32_t e = 0; e < 16u; e++) if (!((vis[ch >> 1] >> ((ch & 1u) * 16u + e)) & 1u)) x[e] = 0xFF800000u;
+                    }
+#pragma unroll
+                    for (uint32_t e = 0; e < 16u; e += 2u) {
+                        top = fmaxf(top, fmaxf(__uint_as_float(x[e]), __uint_as_float(x[e + 1])));
+                        float y0, y1;
+                        unpack2(fma2(pack2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), scale2, below2), y0, y1);
+                        y0 = exp2_fast(y0); y1 = exp2_fast(y1);
+                        sum2 = add2(sum2, pack2(y0, y1));
+                        p[ch * 8u + (e >> 1)] = pack_bf16(y0, y1);
+                    }
+                }
+                float s0, s1;
+                unpack2(sum2, s0, s1);
+                sum = s0 + s1;
+                top *= a.scale;
+                const bool raise = top > m + 8.f;
+                if (raised || !__any_sync(0xffffffffu, raise)) break;
+                raised = true;
+                const float up = raise ? top : m, f = up == -INFINITY ? 1.f : exp2_fast(m - up);
+#pragma unroll
+                for (uint32_t ch = 0; ch < HD / 32u; ch++) {
+                    tm_load32(tm_o + ch * 32u, v);
+                    tm_wait_load();
+#pragma unroll
+                    for (uint32_t e = 0; e < 32u; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+                    tm_store32(tm_o + ch * 32u, v);
                 }
                 m = up; l *= f;
             }
-            const float below = m == -INFINITY ? 0.f : m;
-            float l0 = 0.f, l1 = 0.f;
-#pragma unroll
-            for (uint32_t ch = 0; ch < 4u; ch++) {
-                tm_load32(tm_s + ch * 32u, v);
-                tm_wait_load();
-                uint32_t p[16];
-#pragma unroll
-                for (uint32_t e = 0; e < 32u; e += 2u) {
-                    float x = __uint_as_float(v[e]), y = __uint_as_float(v[e + 1]);
-                    if (!whole) { if (!((vis[ch] >> e) & 1u)) x = -INFINITY; if (!((vis[ch] >> (e + 1u)) & 1u)) y = -INFINITY; }
-                    x = exp2_fast(fmaf(x, a.scale, -below)); y = exp2_fast(fmaf(y, a.scale, -below));
-                    l0 += x; l1 += y;
-                    p[e >> 1] = pack_bf16(x, y);
-                }
-                tm_store16(tm_s + ch * 16u, p);
-            }
-            l += l0 + l1;
+            l += sum;
+            tm_store32(tm_s, *reinterpret_cast<uint32_t (*)[32]>(p));
+            tm_store32(tm_s + 32u, *reinterpret_cast<uint32_t (*)[32]>(p + 32));
             tm_wait_store();
             tm_fence_before();
             arrive(p_full + s * 8u);
@@ -292,36 +327,44 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attention_many_kernel(cons
                 __syncwarp();
             }
         }
-    } else if (warp < 12u) {
+    } else if (warp < 16u) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         /* ---- K and V into shared memory ---- */
         const uint32_t pt = tid - 256u, items = 2u * n;
-        constexpr uint32_t kChunks = HD * (ELEM == kKvE4m3 ? 1u : 2u) / 16u, kPasses = kManyKeys * kChunks / 128u, kRowsPerPass = 128u / kChunks;
+        constexpr uint32_t kRowBytes = HD * (ELEM == kKvE4m3 ? 1u : 2u), kChunks = kRowBytes / 16u, kPasses = kManyKeys * kChunks / kProducers, kRowsPerPass = kProducers / kChunks;
+        static_assert(kRowsPerPass % 8u == 0u, "a thread's rows take the same place in the swizzle");
         const uint32_t ch = pt % kChunks, r0 = pt / kChunks;                            /* this thread's chunk of rows r0, r0 + kRowsPerPass, ... */
         const uint64_t head = (uint64_t)kvh * a.c.capacity;
         auto tile_of = [&](uint32_t x) { return x == 0u ? 0u : x + 1u == items ? n - 1u : x & 1u ? (x + 1u) / 2u : (x - 2u) / 2u; };
         auto is_v = [&](uint32_t x) { return x != 0u && (x + 1u == items || !(x & 1u)); };
-        auto cell_of = [&](uint32_t i) -> uint64_t {                                    /* slot of list index i < span.count */
-            uint32_t sl = i < span.lead ? i : slot_first + (i - span.lead);
-            if (i >= span.lead && sl >= a.c.capacity) sl -= ring;
-            return head + sl;
+        auto slot_of = [&](uint32_t i) -> uint32_t {                                    /* of list index i < span.count */
+            const uint32_t sl = i < span.lead ? i : slot_first + (i - span.lead);
+            return i >= span.lead && sl >= a.c.capacity ? sl - ring : sl;
         };
-        auto fetch = [&](uint32_t x, uint32_t dst_tile) {                              /* the item's rows as they are: bf16 into the operand's places, codes into this thread's staging */
-            const uint8_t *from = is_v(x) ? a.c.v : a.c.k;
+        /* a tile of 128 keys whose slots follow one another needs one address */
+        auto straight = [&](uint32_t i0) { return i0 + kManyKeys <= span.count && slot_of(i0 + kManyKeys - 1u) == slot_of(i0) + kManyKeys - 1u && (i0 >= span.lead || i0 + kManyKeys <= span.lead); };
+        auto fetch = [&](uint32_t x, uint32_t dst, uint32_t step) {                    /* rows as they are, pass e to dst + e * step */
+            const uint8_t *from = (is_v(x) ? a.c.v : a.c.k) + ch * 16u;
             const uint32_t i0 = (tile0 + tile_of(x)) * kManyKeys;
+            if (straight(i0)) {
+                from += (head + slot_of(i0) + r0) * kRowBytes;
 #pragma unroll
-            for (uint32_t e = 0; e < kPasses; e++) {
-                const uint32_t r = r0 + e * kRowsPerPass, i = i0 + r, ok = i < span.count;
-                const uint64_t cell = ok ? cell_of(i) : head;
-                if (ELEM == kKvE4m3) copy16(dst_tile + (e * 128u + pt) * 16u, from + cell * HD + ch * 16u, ok ? 16u : 0u);
-                else copy16(dst_tile + (ch >> 3) * F::kHalfBytes + swizzled(r, ch & 7u), from + (cell * HD + ch * 8u) * 2u, ok ? 16u : 0u);
+                for (uint32_t e = 0; e < kPasses; e++) copy16(dst + e * step, from + e * kRowsPerPass * kRowBytes, 16u);
+            } else {
+#pragma unroll
+                for (uint32_t e = 0; e < kPasses; e++) {
+                    const uint32_t i = i0 + r0 + e * kRowsPerPass;
+                    copy16(dst + e * step, from + (head + (i < span.count ? slot_of(i) : 0u)) * kRowBytes, i < span.count ? 16u : 0u);
+                }
             }
         };
-        if (ELEM == kKvBf16) {
+        if constexpr (ELEM == kKvBf16) {
+            const uint32_t place = base + F::kRing + (ch >> 3) * F::kHalfBytes + swizzled(r0, ch & 7u);
             for (uint32_t x = 0; x < items + F::kAhead && alive; x++) {
                 if (x < items) {
                     if (x >= NS) alive = mbar_wait(empty + (x % NS) * 8u, ((x / NS) - 1u) & 1u);
                     if (!alive) break;
-                    fetch(x, base + F::kRing + (x % NS) * F::kTile);
+                    fetch(x, place + (x % NS) * F::kTile, kRowsPerPass * 128u);
                 }
                 copies_commit();
                 if (x >= F::kAhead) {
@@ -331,42 +374,67 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attention_many_kernel(cons
                 }
             }
         } else {
+            const uint32_t c8 = (ch & 3u) * 2u, place = base + F::kRing + (ch >> 2) * F::kHalfBytes, place_lo = place + swizzled(r0, c8), place_hi = place + swizzled(r0, c8 + 1u), staged = base + F::kStage + pt * 16u;
             uint8_t unit[kPasses];
             auto units = [&](uint32_t x) {
                 const uint8_t *from = is_v(x) ? a.c.v_exp : a.c.k_exp;
                 const uint32_t i0 = (tile0 + tile_of(x)) * kManyKeys;
+                if (straight(i0)) {
+                    from += head + slot_of(i0) + r0;
 #pragma unroll
-                for (uint32_t e = 0; e < kPasses; e++) { const uint32_t i = i0 + r0 + e * kRowsPerPass; unit[e] = from[i < span.count ? cell_of(i) : head]; }
+                    for (uint32_t e = 0; e < kPasses; e++) unit[e] = from[e * kRowsPerPass];
+                } else {
+#pragma unroll
+                    for (uint32_t e = 0; e < kPasses; e++) { const uint32_t i = i0 + r0 + e * kRowsPerPass; unit[e] = from[head + (i < span.count ? slot_of(i) : 0u)]; }
+                }
             };
-            for (uint32_t x = 0; x < F::kAhead; x++) { if (x < items) fetch(x, base + F::kStage + (x % F::kStaging) * F::kStagingBytes); copies_commit(); }
+            for (uint32_t x = 0; x < F::kAhead; x++) { if (x < items) fetch(x, staged + (x % F::kStaging) * F::kStagingBytes, kProducers * 16u); copies_commit(); }
             if (items) units(0u);
             for (uint32_t x = 0; x < items && alive; x++) {
-                if (x + F::kAhead < items) fetch(x + F::kAhead, base + F::kStage + ((x + F::kAhead) % F::kStaging) * F::kStagingBytes);
+                if (x + F::kAhead < items) fetch(x + F::kAhead, staged + ((x + F::kAhead) % F::kStaging) * F::kStagingBytes, kProducers * 16u);
                 copies_commit();
                 copies_wait<F::kAhead>();
-                uint8_t now[kPasses];
+                /* code bits in bf16's places are the value times 2^-120: times 2^(120 + e), one exact multiplication while that
+                   is a bf16 number (rows below 2^16), two beyond */
+                uint32_t f[kPasses];
+                bool large = false;
 #pragma unroll
-                for (uint32_t e = 0; e < kPasses; e++) now[e] = unit[e];
+                for (uint32_t e = 0; e < kPasses; e++) { const uint32_t b = unit[e]; f[e] = min(b + 120u, 254u) * 0x00800080u; large = large || b > 134u; }
+                large = __any_sync(0xffffffffu, large);
+                uint32_t f2[kPasses];
+                if (large) {
+#pragma unroll
+                    for (uint32_t e = 0; e < kPasses; e++) f2[e] = (max((uint32_t)unit[e], 134u) - 7u) * 0x00800080u;
+                }
                 if (x + 1u < items) units(x + 1u);
                 if (x >= NS) alive = mbar_wait(empty + (x % NS) * 8u, ((x / NS) - 1u) & 1u);
                 if (!alive) break;
-                const uint32_t dst = base + F::kRing + (x % NS) * F::kTile, src = base + F::kStage + (x % F::kStaging) * F::kStagingBytes;
+                const uint32_t to = (x % NS) * F::kTile, src = staged + (x % F::kStaging) * F::kStagingBytes;
 #pragma unroll
                 for (uint32_t e = 0; e < kPasses; e++) {
-                    const uint4 w = lds128(src + (e * 128u + pt) * 16u);
-                    const uint32_t u2 = kv_unit2(now[e]);
-                    uint4 lo, hi;
-                    kv_values4(w.x, u2, lo.x, lo.y); kv_values4(w.y, u2, lo.z, lo.w); kv_values4(w.z, u2, hi.x, hi.y); kv_values4(w.w, u2, hi.z, hi.w);
-                    const uint32_t r = r0 + e * kRowsPerPass, at = dst + (ch >> 2) * F::kHalfBytes, c8 = (ch & 3u) * 2u;
-                    sts128u(at + swizzled(r, c8), lo.x, lo.y, lo.z, lo.w);
-                    sts128u(at + swizzled(r, c8 + 1u), hi.x, hi.y, hi.z, hi.w);
+                    const uint4 w = lds128(src + e * kProducers * 16u);
+                    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+                    uint32_t y[8];
+#pragma unroll
+                    for (uint32_t j = 0; j < 4u; j++) {
+                        kv_spread(u[j], y[2 * j], y[2 * j + 1]);
+                        y[2 * j] = kv_mul2(y[2 * j], f[e]); y[2 * j + 1] = kv_mul2(y[2 * j + 1], f[e]);
+                    }
+                    if (large) {
+#pragma unroll
+                        for (uint32_t j = 0; j < 8u; j++) y[j] = kv_mul2(y[j], f2[e]);
+                    }
+                    sts128u(place_lo + to + e * kRowsPerPass * 128u, y[0], y[1], y[2], y[3]);
+                    sts128u(place_hi + to + e * kRowsPerPass * 128u, y[4], y[5], y[6], y[7]);
                 }
                 async_proxy_fence();
                 arrive(full + (x % NS) * 8u);
             }
         }
         copies_wait<0>();
-    } else if (lane == 0 && n) {
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        if (warp == 16u && lane == 0 && n) {
         /* ---- matrix products ---- */
         const uint32_t q_desc_base = base + F::kQ, ring0 = base + F::kRing;
         constexpr uint32_t kIdescS = idesc_bf16(128u, kManyKeys, false), kIdescO = idesc_bf16(128u, HD, true);
@@ -430,13 +498,14 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attention_many_kernel(cons
             mma_commit(o_full); mma_commit(o_full + 8u);
             for (uint32_t i = 0; i < (1u << 20); i++) if (mbar_poll(o_full, 0u) && mbar_poll(o_full + 8u, 0u)) break;
         }
+        }
     }
     if (!pos_ok && tid == 0) atomicOr(a.status, kKvStatusPosition);
     __syncwarp();
     tm_fence_before();
     __syncthreads();
     tm_fence_after();
-    if (warp == 12u) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    if (warp == 16u) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
 template <int HD, int ELEM>
