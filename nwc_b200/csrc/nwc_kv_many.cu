@@ -16,8 +16,8 @@
  * Bound: 4 * 128 * 128 * head_dim multiply-adds per pair of tiles on the tensor cores (2048 clocks at head_dim 128), and as
  * many clocks of the exponential unit (16 per SM and clock) for 2 * 128 * 128 weights.
  *
- * Roles: warps 0-3 and 4-7 weights of stream 0 and 1 (they also load Q, rescale and write out O), warps 8-15 bring K and V
- * into shared memory, one thread of warp 16 issues the MMAs.  The copies are 16 bytes per thread, so a tile may begin, end and
+ * Roles: warps 0-3 and 4-7 weights of stream 0 and 1 (they also load Q, rescale and write out O), the next four or eight
+ * bring K and V into shared memory, one thread behind them issues the MMAs.  The copies are 16 bytes per thread, so a tile may begin, end and
  * wrap anywhere in the ring and a row that is no key of the call is written as zeros (whatever its slot holds, weight 0 times
  * it must be 0).  e4m3 rows become bf16 on the way, exactly: code and unit have fewer bits than a bf16 number.  All waits are
  * bounded; a role that gives up records the status word and stops, the others run out, tensor memory is freed.
@@ -33,13 +33,18 @@ namespace nwc {
 
 namespace {
 
-constexpr uint32_t kManyRows = 128u, kManyKeys = 128u, kManyThreads = 20u * 32u, kProducers = 256u;
+constexpr uint32_t kManyRows = 128u, kManyKeys = 128u;
 
 template <int HD, int ELEM> struct Many {
     static constexpr uint32_t kTile = kManyKeys * HD * 2u, kHalfBytes = kManyKeys * 128u;      /* a bf16 tile: halves of 64 dimensions, 128-byte rows, swizzled */
     static constexpr uint32_t kSlots = ELEM == kKvE4m3 ? (HD == 64 ? 6u : 3u) : (HD == 64 ? 8u : 5u);
     static constexpr uint32_t kStaging = ELEM == kKvE4m3 ? 4u : 0u, kStagingBytes = kManyKeys * HD;              /* raw codes in flight */
     static constexpr uint32_t kAhead = ELEM == kKvE4m3 ? 3u : 2u;                                                 /* tiles in flight beyond the one awaited */
+    /* Registers: the warps start with 65536 / threads (a multiple of 8) each; those that hold a row of scores take what the
+       others give back: 8 x 184 + 4 x 72 + 4 x 72 = 16 x 128, 8 x 160 + 8 x 56 + 4 x 48 = 20 x 96.  Widening e4m3 rows takes
+       eight warps, copying bf16 ones four. */
+    static constexpr uint32_t kProducers = ELEM == kKvE4m3 ? 256u : 128u, kMmaWarp = 8u + kProducers / 32u, kThreads = 256u + kProducers + 128u;
+    static constexpr int kRegsWeights = ELEM == kKvE4m3 ? 160 : 184, kRegsProduce = ELEM == kKvE4m3 ? 56 : 72, kRegsMma = ELEM == kKvE4m3 ? 48 : 72;
     static constexpr uint32_t kQ = 0u, kRing = 2u * kTile, kStage = kRing + kSlots * kTile, kBars = kStage + kStaging * kStagingBytes;
     static constexpr uint32_t kSmem = 1024u + kBars + (2u * kSlots + 8u) * 8u + 16u;
 };
@@ -69,32 +74,93 @@ __device__ __forceinline__ void tm_load32(uint32_t addr, uint32_t (&v)[32]) {
                    "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
                  : "r"(addr) : "memory");
 }
-__device__ __forceinline__ void tm_store32(uint32_t addr, const uint32_t (&v)[32]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
-                 ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
-                   "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]) : "memory");
+__device__ __forceinline__ void tm_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tm_store16(uint32_t addr, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
 }
-__device__ __forceinline__ void tm_load16(uint32_t addr, uint32_t (&v)[16]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-                 : "r"(addr) : "memory");
+__device__ __forceinline__ void tm_load8(uint32_t addr, uint32_t (&v)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "r"(addr) : "memory");
 }
-/* the wait names the registers that it makes valid, so that nothing reads them above it */
-__device__ __forceinline__ void tm_wait_load16(uint32_t (&v)[16]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]) :: "memory");
+__device__ __forceinline__ void tm_store8(uint32_t addr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
+/* names registers that a wait has made valid, so that nothing reads them above it (no instruction) */
+template <int N> __device__ __forceinline__ void tm_hold(uint32_t (&v)[N]) {
+#pragma unroll
+    for (int e = 0; e < N; e++) asm volatile("" : "+r"(v[e]));
 }
 /* two fp32 operations in one instruction */
 __device__ __forceinline__ uint64_t pack2(float a, float b) { uint64_t d; asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b)); return d; }
 __device__ __forceinline__ void unpack2(uint64_t v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) { uint64_t d; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c)); return d; }
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) { uint64_t d; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b)); return d; }
-__device__ __forceinline__ void tm_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tm_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tm_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tm_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) { uint32_t d; asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(b), "f"(a)); return d; }
 __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+/* One row's scores of a tile -> weights: running maximum m (log2) and sum l updated, P (bf16) over the scores' first columns,
+   O rescaled where m was raised.  The 128 scores are in registers throughout. */
+template <bool WHOLE>
+__device__ __forceinline__ void weights(float scale, uint32_t tm_s, uint32_t tm_o, uint32_t hd, bool have_o, const uint32_t (&vis)[4], float &m, float &l) {
+    uint32_t v[4][32];
+#pragma unroll
+    for (uint32_t ch = 0; ch < 4u; ch++) tm_load32(tm_s + ch * 32u, v[ch]);
+    tm_wait_load();
+#pragma unroll
+    for (uint32_t ch = 0; ch < 4u; ch++) tm_hold(v[ch]);
+    float top4[4];
+#pragma unroll
+    for (uint32_t ch = 0; ch < 4u; ch++) {
+        if (!WHOLE) {
+#pragma unroll
+            for (uint32_t e = 0; e < 32u; e++) if (!((vis[ch] >> e) & 1u)) v[ch][e] = 0xFF800000u;
+        }
+        float t = __uint_as_float(v[ch][0]);
+#pragma unroll
+        for (uint32_t e = 1; e < 31u; e += 2u) t = fmaxf(t, fmaxf(__uint_as_float(v[ch][e]), __uint_as_float(v[ch][e + 1])));
+        top4[ch] = fmaxf(t, __uint_as_float(v[ch][31]));
+    }
+    const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * scale;
+    const bool raise = top > m + 8.f;
+    if (__any_sync(0xffffffffu, raise)) {
+        const float up = raise ? top : m, f = up == -INFINITY ? 1.f : exp2_fast(m - up);
+        m = up; l *= f;
+        if (have_o) {
+            for (uint32_t c = 0; c < hd; c += 8u) {                                     /* (rare; few registers beside the scores) */
+                uint32_t o[8];
+                tm_load8(tm_o + c, o);
+                tm_wait_load();
+                tm_hold(o);
+#pragma unroll
+                for (uint32_t e = 0; e < 8u; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                tm_store8(tm_o + c, o);
+            }
+        }
+    }
+    const float below = m == -INFINITY ? 0.f : -m;
+    const uint64_t scale2 = pack2(scale, scale), below2 = pack2(below, below);
+    uint64_t sum0 = 0ull, sum1 = 0ull;
+#pragma unroll
+    for (uint32_t ch = 0; ch < 4u; ch++) {
+        uint32_t p[16];
+#pragma unroll
+        for (uint32_t e = 0; e < 32u; e += 4u) {
+            float y0, y1, y2, y3;
+            unpack2(fma2(pack2(__uint_as_float(v[ch][e]), __uint_as_float(v[ch][e + 1])), scale2, below2), y0, y1);
+            unpack2(fma2(pack2(__uint_as_float(v[ch][e + 2]), __uint_as_float(v[ch][e + 3])), scale2, below2), y2, y3);
+            y0 = exp2_fast(y0); y1 = exp2_fast(y1); y2 = exp2_fast(y2); y3 = exp2_fast(y3);
+            sum0 = add2(sum0, pack2(y0, y1)); sum1 = add2(sum1, pack2(y2, y3));
+            p[e >> 1] = pack_bf16(y0, y1); p[(e >> 1) + 1u] = pack_bf16(y2, y3);
+        }
+        tm_store16(tm_s + ch * 16u, p);
+    }
+    float s0, s1;
+    unpack2(add2(sum0, sum1), s0, s1);
+    l += s0 + s1;
+}
 /* bits [lo, hi) of a word whose bit 0 is number 0; lo and hi may lie anywhere */
 __device__ __forceinline__ uint32_t bit_range(int32_t lo, int32_t hi) {
     lo = max(lo, 0); hi = min(hi, 32);
@@ -105,16 +171,16 @@ __device__ __forceinline__ uint32_t bit_range(int32_t lo, int32_t hi) {
 }  // namespace
 
 template <int HD, int ELEM>
-__global__ void __launch_bounds__(kManyThreads, 1) kv_attention_many_kernel(const KvAttention a) {
+__global__ void __launch_bounds__(Many<HD, ELEM>::kThreads, 1) kv_attention_many_kernel(const KvAttention a) {
     using F = Many<HD, ELEM>;
-    constexpr uint32_t NS = F::kSlots;
+    constexpr uint32_t NS = F::kSlots, kProducers = F::kProducers;
     extern __shared__ uint8_t many_raw[];
     const uint32_t base = (smem_addr(many_raw) + 1023u) & ~1023u;
     const uint32_t bars = base + F::kBars, full = bars, empty = bars + NS * 8u, q_full = bars + 2u * NS * 8u, s_full = q_full + 16u, p_full = s_full + 16u, o_full = p_full + 16u, tmem_slot = o_full + 16u;
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
     const uint32_t group = a.n_q / a.c.n_kv, rows = a.T * group, kvh = blockIdx.y % a.c.n_kv, row0 = (blockIdx.y / a.c.n_kv) * 2u * kManyRows, split = blockIdx.x;
     const bool solo = rows - row0 <= kManyRows;
-    if (warp == 16u) {
+    if (warp == F::kMmaWarp) {
         if (lane == 0) {
             for (uint32_t s = 0; s < NS; s++) { mbar_init(full + s * 8u, kProducers); mbar_init(empty + s * 8u, 1u); }
             for (uint32_t s = 0; s < 2u; s++) { mbar_init(q_full + s * 8u, 128u); mbar_init(s_full + s * 8u, 1u); mbar_init(p_full + s * 8u, 128u); mbar_init(o_full + s * 8u, 1u); }
@@ -142,10 +208,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attention_many_kernel(cons
     auto item_k = [](uint32_t t) { return t ? 2u * t - 1u : 0u; };
     auto item_v = [n](uint32_t t) { return t + 1u < n ? 2u * t + 2u : 2u * n - 1u; };
     bool alive = true;
-    /* registers: 20 warps start with 96 each; 8 x 144 + 8 x 64 + 4 x 64 = 20 x 96 */
     if (warp < 8u) {
         /* ---- weights ---- */
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(F::kRegsWeights));
         const uint32_t s = warp >> 2, wt = tid & 127u, q_tile = solo ? 0u : s, my_row0 = row0 + q_tile * kManyRows;
         const uint32_t my_n = solo ? (s ? n / 2u : (n + 1u) / 2u) : n;                 /* tiles of this stream */
         if (n && !(solo && s)) {
@@ -169,12 +234,11 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attention_many_kernel(cons
         const uint32_t tm_s = tmem + s * 128u + ((warp & 3u) << 21), tm_o = tmem + 256u + s * 128u + ((warp & 3u) << 21);
         const int32_t lo_all = __reduce_max_sync(0xffffffffu, row_ok ? lo : 0), hi_all = __reduce_min_sync(0xffffffffu, row_ok ? hi : 0x7FFFFFFF);
         float m = -INFINITY, l = 0.f;
-        uint32_t v[32];
         for (uint32_t i = 0; i < my_n && alive; i++) {
             const int32_t key0 = (int32_t)((tile0 + (solo ? 2u * i + s : i)) * kManyKeys);
             /* what of the tile the row sees; a warp whose rows see it whole does without */
             const bool whole = key0 >= lo_all && key0 + (int32_t)kManyKeys <= hi_all;
-            uint32_t vis[4];
+            uint32_t vis[4] = {0u, 0u, 0u, 0u};
             if (!whole) {
 #pragma unroll
                 for (uint32_t ch = 0; ch < 4u; ch++) {
@@ -192,77 +256,13 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attention_many_kernel(cons
             alive = mbar_wait(s_full + s * 8u, i & 1u);
             if (!alive) break;
             tm_fence_after();
-            /* One pass over the scores with the maximum as it stands: it is passed by more than 2^8 hardly ever after the first
-               tile, and then the pass is repeated (the weights stay in registers until it is known). */
-            bool raised = i == 0u;
-            if (raised) {
-                float top = -INFINITY;
-#pragma unroll
-                for (uint32_t ch = 0; ch < 4u; ch++) {
-                    tm_load32(tm_s + ch * 32u, v);
-                    tm_wait_load();
-                    if (!whole) {
-#pragma unroll
-                        for (uint32_t e = 0; e < 32u; e++) if (!((vis[ch] >> e) & 1u)) v[e] = 0xFF800000u;
-                    }
-#pragma unroll
-                    for (uint32_t e = 0; e < 32u; e += 2u) top = fmaxf(top, fmaxf(__uint_as_float(v[e]), __uint_as_float(v[e + 1])));
-                }
-                m = top * a.scale;
-            }
-            uint32_t p[64];
-            float sum;
-            for (;;) {
-                const float below = m == -INFINITY ? 0.f : -m;
-                const uint64_t scale2 = pack2(a.scale, a.scale), below2 = pack2(below, below);
-                uint64_t sum2 = 0ull;
-                float top = -INFINITY;
-                uint32_t w[2][16];
-                tm_load16(tm_s, w[0]);
-#pragma unroll
-                for (uint32_t ch = 0; ch < 8u; ch++) {
-                    uint32_t (&x)[16] = w[ch & 1u];
-                    tm_wait_load16(x);
-                    if (ch < 7u) tm_load16(tm_s + (ch + 1u) * 16u, w[(ch + 1u) & 1u]);
-                    if (!whole) {
-#pragma unroll
-                        for (uint32_t e = 0; e < 16u; e++) if (!((vis[ch >> 1] >> ((ch & 1u) * 16u + e)) & 1u)) x[e] = 0xFF800000u;
-                    }
-#pragma unroll
-                    for (uint32_t e = 0; e < 16u; e += 2u) {
-                        top = fmaxf(top, fmaxf(__uint_as_float(x[e]), __uint_as_float(x[e + 1])));
-                        float y0, y1;
-                        unpack2(fma2(pack2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), scale2, below2), y0, y1);
-                        y0 = exp2_fast(y0); y1 = exp2_fast(y1);
-                        sum2 = add2(sum2, pack2(y0, y1));
-                        p[ch * 8u + (e >> 1)] = pack_bf16(y0, y1);
-                    }
-                }
-                float s0, s1;
-                unpack2(sum2, s0, s1);
-                sum = s0 + s1;
-                top *= a.scale;
-                const bool raise = top > m + 8.f;
-                if (raised || !__any_sync(0xffffffffu, raise)) break;
-                raised = true;
-                const float up = raise ? top : m, f = up == -INFINITY ? 1.f : exp2_fast(m - up);
-#pragma unroll
-                for (uint32_t ch = 0; ch < HD / 32u; ch++) {
-                    tm_load32(tm_o + ch * 32u, v);
-                    tm_wait_load();
-#pragma unroll
-                    for (uint32_t e = 0; e < 32u; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
-                    tm_store32(tm_o + ch * 32u, v);
-                }
-                m = up; l *= f;
-            }
-            l += sum;
-            tm_store32(tm_s, *reinterpret_cast<uint32_t (*)[32]>(p));
-            tm_store32(tm_s + 32u, *reinterpret_cast<uint32_t (*)[32]>(p + 32));
+            if (whole) weights<true>(a.scale, tm_s, tm_o, HD, i != 0u, vis, m, l);
+            else weights<false>(a.scale, tm_s, tm_o, HD, i != 0u, vis, m, l);
             tm_wait_store();
             tm_fence_before();
             arrive(p_full + s * 8u);
         }
+        uint32_t v[32];
         /* O, then the row's share or result */
         if (alive && my_n) { alive = mbar_wait(o_full + s * 8u, 0u); tm_fence_after(); }
         if (solo) {
@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attention_many_kernel(cons
 #pragma unroll
                     for (uint32_t ch = 0; ch < HD / 32u; ch++) {
                         tm_load32(tm_o + ch * 32u, v);
-                        tm_wait_load();
+                        tm_wait_load(); tm_hold(v);
 #pragma unroll
                         for (uint32_t e = 0; e < 32u; e++) there[(ch * 32u + e) * 128u + wt] = __uint_as_float(v[e]);
                     }
@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attention_many_kernel(cons
             if (a.splits > 1u && row_ok) *reinterpret_cast<float2 *>(a.part_ml + ((uint64_t)split * a.T * a.n_q + line) * 2u) = make_float2(n ? top : -INFINITY, total);
 #pragma unroll
             for (uint32_t ch = 0; ch < HD / 32u; ch++) {
-                if (my_n) { tm_load32(tm_o + ch * 32u, v); tm_wait_load(); }
+                if (my_n) { tm_load32(tm_o + ch * 32u, v); tm_wait_load(); tm_hold(v); }
                 else {
 #pragma unroll
                     for (uint32_t e = 0; e < 32u; e++) v[e] = 0u;
@@ -327,8 +327,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attention_many_kernel(cons
                 __syncwarp();
             }
         }
-    } else if (warp < 16u) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    } else if (warp < F::kMmaWarp) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F::kRegsProduce));
         /* ---- K and V into shared memory ---- */
         const uint32_t pt = tid - 256u, items = 2u * n;
         constexpr uint32_t kRowBytes = HD * (ELEM == kKvE4m3 ? 1u : 2u), kChunks = kRowBytes / 16u, kPasses = kManyKeys * kChunks / kProducers, kRowsPerPass = kProducers / kChunks;
@@ -433,8 +433,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attention_many_kernel(cons
         }
         copies_wait<0>();
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-        if (warp == 16u && lane == 0 && n) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F::kRegsMma));
+        if (warp == F::kMmaWarp && lane == 0 && n) {
         /* ---- matrix products ---- */
         const uint32_t q_desc_base = base + F::kQ, ring0 = base + F::kRing;
         constexpr uint32_t kIdescS = idesc_bf16(128u, kManyKeys, false), kIdescO = idesc_bf16(128u, HD, true);
@@ -505,7 +505,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) kv_attention_many_kernel(cons
     tm_fence_before();
     __syncthreads();
     tm_fence_after();
-    if (warp == 16u) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    if (warp == F::kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
 template <int HD, int ELEM>
@@ -513,7 +513,7 @@ static cudaError_t launch_many(cudaStream_t st, const KvAttention &a) {
     const uint64_t rows = (uint64_t)a.T * (a.n_q / a.c.n_kv), pairs = (rows + 2u * kManyRows - 1u) / (2u * kManyRows);
     if (pairs * a.c.n_kv > 65535u) return cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(a.splits, (uint32_t)(pairs * a.c.n_kv)); cfg.blockDim = dim3(kManyThreads); cfg.dynamicSmemBytes = Many<HD, ELEM>::kSmem; cfg.stream = st;
+    cfg.gridDim = dim3(a.splits, (uint32_t)(pairs * a.c.n_kv)); cfg.blockDim = dim3(Many<HD, ELEM>::kThreads); cfg.dynamicSmemBytes = Many<HD, ELEM>::kSmem; cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr; cfg.numAttrs = dependent_launch() ? 1 : 0;
