@@ -87,6 +87,7 @@ struct KvAttention {
        part_o fp32 [splits][T * n_q][head_dim] unnormalised, part_ml fp32 [splits][T * n_q][2] = running maximum (log2), sum */
     float *part_o, *part_ml;
     uint32_t splits;
+    uint32_t layer, layers;      /* which layer of how many `c` is */
 };
 /* How a call is divided.  It goes by sizes that the host knows (a captured call is replayed at other positions): the most
    keys that the cache can show, not the position. */

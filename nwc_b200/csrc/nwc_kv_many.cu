@@ -17,14 +17,17 @@
  * many clocks of the exponential unit (16 per SM and clock) for 2 * 128 * 128 weights.
  *
  * Roles: warps 0-3 and 4-7 weights of stream 0 and 1 (they also load Q, rescale and write out O), the next four or eight
- * bring K and V into shared memory, one thread behind them issues the MMAs.  The copies are 16 bytes per thread, so a tile may begin, end and
- * wrap anywhere in the ring and a row that is no key of the call is written as zeros (whatever its slot holds, weight 0 times
- * it must be 0).  e4m3 rows become bf16 on the way, exactly: code and unit have fewer bits than a bf16 number.  All waits are
+ * bring K and V into shared memory, one thread behind them issues the MMAs.  A tile
+ * of the list of keys may begin, end and wrap anywhere in the ring; a row that is no key of the call is written as zeros
+ * (whatever its slot holds, weight 0 times it must be 0).  Whole bf16 tiles are tensor-map copies; e4m3 rows become bf16 on
+ * the way, exactly: code and unit have fewer bits than a bf16 number.  All waits are
  * bounded; a role that gives up records the status word and stops, the others run out, tensor memory is freed.
  *
  * O is rescaled in tensor memory only when a row's maximum passes the one it is scaled by by more than 2^8 (weights stay below
  * 2^8, sums are fp32): after the first tiles hardly ever.  P is rounded to bf16 (2^-8 relative), the sum of the weights is not.
  */
+#include <atomic>
+#include <cuda.h>
 #include "nwc_kv.h"
 #include "nwc_async.cuh"
 #include "nwc_launch.h"
@@ -37,36 +40,54 @@ constexpr uint32_t kManyRows = 128u, kManyKeys = 128u;
 
 template <int HD, int ELEM> struct Many {
     static constexpr uint32_t kTile = kManyKeys * HD * 2u, kHalfBytes = kManyKeys * 128u;      /* a bf16 tile: halves of 64 dimensions, 128-byte rows, swizzled */
-    static constexpr uint32_t kSlots = ELEM == kKvE4m3 ? (HD == 64 ? 6u : 3u) : (HD == 64 ? 8u : 5u);
-    static constexpr uint32_t kStaging = ELEM == kKvE4m3 ? 4u : 0u, kStagingBytes = kManyKeys * HD;              /* raw codes in flight */
-    static constexpr uint32_t kAhead = ELEM == kKvE4m3 ? 3u : 2u;                                                 /* tiles in flight beyond the one awaited */
+    /* Operand slots.  Both streams' products with a tile must end before its slot is filled again, and the filling itself takes
+       a while, so three slots run dry: the products wait for V, V for the slot, the slot for the products. */
+    static constexpr uint32_t kSlots = HD == 64 ? 8u : 5u;
     /* Registers: the warps start with 65536 / threads (a multiple of 8) each; those that hold a row of scores take what the
-       others give back: 8 x 184 + 4 x 72 + 4 x 72 = 16 x 128, 8 x 160 + 8 x 56 + 4 x 48 = 20 x 96.  Widening e4m3 rows takes
+       others give back: 8 x 184 + 4 x 72 + 4 x 72 = 16 x 128, 8 x 152 + 8 x 64 + 4 x 48 = 20 x 96.  Widening e4m3 rows takes
        eight warps, copying bf16 ones four. */
     static constexpr uint32_t kProducers = ELEM == kKvE4m3 ? 256u : 128u, kMmaWarp = 8u + kProducers / 32u, kThreads = 256u + kProducers + 128u;
-    static constexpr int kRegsWeights = ELEM == kKvE4m3 ? 160 : 184, kRegsProduce = ELEM == kKvE4m3 ? 56 : 72, kRegsMma = ELEM == kKvE4m3 ? 48 : 72;
-    static constexpr uint32_t kQ = 0u, kRing = 2u * kTile, kStage = kRing + kSlots * kTile, kBars = kStage + kStaging * kStagingBytes;
+    static constexpr int kRegsWeights = ELEM == kKvE4m3 ? 152 : 184, kRegsProduce = ELEM == kKvE4m3 ? 64 : 72, kRegsMma = ELEM == kKvE4m3 ? 48 : 72;
+    static constexpr uint32_t kQ = 0u, kRing = 2u * kTile, kBars = kRing + kSlots * kTile;
     static constexpr uint32_t kSmem = 1024u + kBars + (2u * kSlots + 8u) * 8u + 16u;
 };
 
-__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr, uint32_t lead_bytes) {
-    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(lead_bytes >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) | ((uint64_t)1u << 46) | ((uint64_t)2u << 61);
-}
+/* shared-memory descriptor, 128-byte swizzle, groups of eight rows 1024 bytes apart: address (in 16 bytes) and leading offset in
+   the low word, the rest in the high one */
+__device__ __forceinline__ uint32_t desc_low(uint32_t addr, uint32_t lead_bytes) { return ((addr & 0x3FFFFu) >> 4) | ((lead_bytes >> 4) << 16); }
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
 __host__ __device__ constexpr uint32_t idesc_bf16(uint32_t M, uint32_t N, bool b_mn_major) {
     return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn_major ? 1u << 16 : 0u) | ((N >> 3) << 17) | ((M >> 4) << 24);
 }
 __device__ __forceinline__ uint32_t swizzled(uint32_t row, uint32_t chunk) { return row * 128u + ((chunk ^ (row & 7u)) << 4); }
 __device__ __forceinline__ void sts128u(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) { asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory"); }
-__device__ __forceinline__ void arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+/* one arrival for the warp (32 arrivals of single lanes queue up at the barrier: a tile took a thousand clocks longer) */
+__device__ __forceinline__ void arrive_warp(uint32_t bar) { __syncwarp(); if ((threadIdx.x & 31u) == 0u) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, uint32_t bytes) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory"); }
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ void mma_commit(uint32_t bar) { asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory"); }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+__device__ __forceinline__ void copies_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+/* one box of 64 dimensions x 128 rows of this GPU's own memory into this CTA's shared memory; x is 0 or 64 elements = 128 bytes */
+__device__ __forceinline__ void tensor_load(uint32_t dst, const CUtensorMap *map, uint32_t x, uint32_t row, uint32_t plane, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(row), "r"(plane), "r"(bar) : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+/* The issuing warp stays together and all of its lanes hold the same descriptors, so that they live in uniform registers; one
+   elected lane (`leader`) issues.  (One lane in a branch of its own moves every operand over for each MMA: measured 110
+   clocks an MMA that takes 64.) */
+__device__ __forceinline__ uint32_t elect_lane() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+    return p;
+}
+__device__ __forceinline__ void mma_commit(uint32_t leader, uint32_t bar) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(leader) : "memory");
+}
+__device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, q;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\tmov.b64 x, {%1, %6};\n\tmov.b64 y, {%2, %6};\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(leader), "r"(kDescHigh) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t leader, uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, q;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\tmov.b64 y, {%2, %6};\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(leader), "r"(kDescHigh) : "memory");
 }
 __device__ __forceinline__ void tm_load32(uint32_t addr, uint32_t (&v)[32]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
@@ -171,7 +192,7 @@ __device__ __forceinline__ uint32_t bit_range(int32_t lo, int32_t hi) {
 }  // namespace
 
 template <int HD, int ELEM>
-__global__ void __launch_bounds__(Many<HD, ELEM>::kThreads, 1) kv_attention_many_kernel(const KvAttention a) {
+__global__ void __launch_bounds__(Many<HD, ELEM>::kThreads, 1) kv_attention_many_kernel(const KvAttention a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     using F = Many<HD, ELEM>;
     constexpr uint32_t NS = F::kSlots, kProducers = F::kProducers;
     extern __shared__ uint8_t many_raw[];
@@ -182,8 +203,8 @@ __global__ void __launch_bounds__(Many<HD, ELEM>::kThreads, 1) kv_attention_many
     const bool solo = rows - row0 <= kManyRows;
     if (warp == F::kMmaWarp) {
         if (lane == 0) {
-            for (uint32_t s = 0; s < NS; s++) { mbar_init(full + s * 8u, kProducers); mbar_init(empty + s * 8u, 1u); }
-            for (uint32_t s = 0; s < 2u; s++) { mbar_init(q_full + s * 8u, 128u); mbar_init(s_full + s * 8u, 1u); mbar_init(p_full + s * 8u, 128u); mbar_init(o_full + s * 8u, 1u); }
+            for (uint32_t s = 0; s < NS; s++) { mbar_init(full + s * 8u, kProducers / 32u); mbar_init(empty + s * 8u, 1u); }
+            for (uint32_t s = 0; s < 2u; s++) { mbar_init(q_full + s * 8u, 4u); mbar_init(s_full + s * 8u, 1u); mbar_init(p_full + s * 8u, 4u); mbar_init(o_full + s * 8u, 1u); }
             mbar_init_fence();
         }
         __syncwarp();
@@ -222,7 +243,7 @@ __global__ void __launch_bounds__(Many<HD, ELEM>::kThreads, 1) kv_attention_many
                 sts128u(base + F::kQ + q_tile * F::kTile + (ch >> 3) * F::kHalfBytes + swizzled(r, ch & 7u), w.x, w.y, w.z, w.w);
             }
             async_proxy_fence();
-            arrive(q_full + q_tile * 8u);
+            arrive_warp(q_full + q_tile * 8u);
         }
         const uint32_t row = my_row0 + wt, row_ok = row < rows, token = min(row, rows - 1u) / group, idx_pos = (uint32_t)pos - span.first + span.lead;      /* (tree) list index of the first draft */
         const uint32_t own = (uint32_t)pos + (a.depth ? (uint32_t)a.depth[token] : token), words = (a.T + 31u) / 32u;
@@ -260,7 +281,7 @@ __global__ void __launch_bounds__(Many<HD, ELEM>::kThreads, 1) kv_attention_many
             else weights<false>(a.scale, tm_s, tm_o, HD, i != 0u, vis, m, l);
             tm_wait_store();
             tm_fence_before();
-            arrive(p_full + s * 8u);
+            arrive_warp(p_full + s * 8u);
         }
         uint32_t v[32];
         /* O, then the row's share or result */
@@ -343,161 +364,149 @@ __global__ void __launch_bounds__(Many<HD, ELEM>::kThreads, 1) kv_attention_many
         };
         /* a tile of 128 keys whose slots follow one another needs one address */
         auto straight = [&](uint32_t i0) { return i0 + kManyKeys <= span.count && slot_of(i0 + kManyKeys - 1u) == slot_of(i0) + kManyKeys - 1u && (i0 >= span.lead || i0 + kManyKeys <= span.lead); };
-        auto fetch = [&](uint32_t x, uint32_t dst, uint32_t step) {                    /* rows as they are, pass e to dst + e * step */
-            const uint8_t *from = (is_v(x) ? a.c.v : a.c.k) + ch * 16u;
-            const uint32_t i0 = (tile0 + tile_of(x)) * kManyKeys;
-            if (straight(i0)) {
-                from += (head + slot_of(i0) + r0) * kRowBytes;
+        if constexpr (ELEM == kKvBf16) {
+            /* a straight tile is one tensor-map copy per 64 dimensions (one thread, no multicast), any other is copied row by row */
+            const uint32_t place = base + F::kRing + (ch >> 3) * F::kHalfBytes + swizzled(r0, ch & 7u), plane = a.layer * a.c.n_kv + kvh;
+            for (uint32_t x = 0; x < items && alive; x++) {
+                const uint32_t i0 = (tile0 + tile_of(x)) * kManyKeys, to = base + F::kRing + (x % NS) * F::kTile, bar = full + (x % NS) * 8u;
+                if (x >= NS) alive = mbar_wait(empty + (x % NS) * 8u, ((x / NS) - 1u) & 1u);
+                if (!alive) break;
+                if (straight(i0)) {
+                    if (warp == 8u && lane == 0) {
+                        mbar_expect(bar, F::kTile);
 #pragma unroll
-                for (uint32_t e = 0; e < kPasses; e++) copy16(dst + e * step, from + e * kRowsPerPass * kRowBytes, 16u);
-            } else {
+                        for (uint32_t h = 0; h < HD / 64u; h++) tensor_load(to + h * F::kHalfBytes, is_v(x) ? &vmap : &kmap, h * 64u, slot_of(i0), plane, bar);
+                    }
+                    __syncwarp();
+                    if (warp != 8u) arrive_warp(bar);
+                    continue;
+                }
+                const uint8_t *from = (is_v(x) ? a.c.v : a.c.k) + ch * 16u;
 #pragma unroll
                 for (uint32_t e = 0; e < kPasses; e++) {
                     const uint32_t i = i0 + r0 + e * kRowsPerPass;
-                    copy16(dst + e * step, from + (head + (i < span.count ? slot_of(i) : 0u)) * kRowBytes, i < span.count ? 16u : 0u);
+                    copy16(place + (x % NS) * F::kTile + e * kRowsPerPass * 128u, from + (head + (i < span.count ? slot_of(i) : 0u)) * kRowBytes, i < span.count ? 16u : 0u);
                 }
-            }
-        };
-        if constexpr (ELEM == kKvBf16) {
-            const uint32_t place = base + F::kRing + (ch >> 3) * F::kHalfBytes + swizzled(r0, ch & 7u);
-            for (uint32_t x = 0; x < items + F::kAhead && alive; x++) {
-                if (x < items) {
-                    if (x >= NS) alive = mbar_wait(empty + (x % NS) * 8u, ((x / NS) - 1u) & 1u);
-                    if (!alive) break;
-                    fetch(x, place + (x % NS) * F::kTile, kRowsPerPass * 128u);
-                }
-                copies_commit();
-                if (x >= F::kAhead) {
-                    copies_wait<F::kAhead>();
-                    async_proxy_fence();
-                    arrive(full + ((x - F::kAhead) % NS) * 8u);
-                }
+                copies_wait_all();
+                async_proxy_fence();
+                arrive_warp(bar);
             }
         } else {
-            const uint32_t c8 = (ch & 3u) * 2u, place = base + F::kRing + (ch >> 2) * F::kHalfBytes, place_lo = place + swizzled(r0, c8), place_hi = place + swizzled(r0, c8 + 1u), staged = base + F::kStage + pt * 16u;
-            uint8_t unit[kPasses];
-            auto units = [&](uint32_t x) {
-                const uint8_t *from = is_v(x) ? a.c.v_exp : a.c.k_exp;
+            /* codes in registers a tile early (two sets, used in turn), widened into the operand's places */
+            const uint32_t c8 = (ch & 3u) * 2u, place = base + F::kRing + (ch >> 2) * F::kHalfBytes, place_lo = place + swizzled(r0, c8), place_hi = place + swizzled(r0, c8 + 1u);
+            auto load = [&](uint32_t x, uint4 (&w)[kPasses], uint8_t (&unit)[kPasses]) {
+                if (x >= items) return;
+                const bool v = is_v(x);
+                const uint8_t *from = (v ? a.c.v : a.c.k) + ch * 16u, *exps = v ? a.c.v_exp : a.c.k_exp;
                 const uint32_t i0 = (tile0 + tile_of(x)) * kManyKeys;
                 if (straight(i0)) {
-                    from += head + slot_of(i0) + r0;
+                    const uint64_t cell = head + slot_of(i0) + r0;
+                    from += cell * kRowBytes; exps += cell;
 #pragma unroll
-                    for (uint32_t e = 0; e < kPasses; e++) unit[e] = from[e * kRowsPerPass];
+                    for (uint32_t e = 0; e < kPasses; e++) { w[e] = *reinterpret_cast<const uint4 *>(from + e * kRowsPerPass * kRowBytes); unit[e] = exps[e * kRowsPerPass]; }
                 } else {
 #pragma unroll
-                    for (uint32_t e = 0; e < kPasses; e++) { const uint32_t i = i0 + r0 + e * kRowsPerPass; unit[e] = from[head + (i < span.count ? slot_of(i) : 0u)]; }
+                    for (uint32_t e = 0; e < kPasses; e++) {
+                        const uint32_t i = i0 + r0 + e * kRowsPerPass;
+                        w[e] = make_uint4(0u, 0u, 0u, 0u); unit[e] = 0;
+                        if (i < span.count) { const uint64_t cell = head + slot_of(i); w[e] = *reinterpret_cast<const uint4 *>(from + cell * kRowBytes); unit[e] = exps[cell]; }
+                    }
                 }
             };
-            for (uint32_t x = 0; x < F::kAhead; x++) { if (x < items) fetch(x, staged + (x % F::kStaging) * F::kStagingBytes, kProducers * 16u); copies_commit(); }
-            if (items) units(0u);
-            for (uint32_t x = 0; x < items && alive; x++) {
-                if (x + F::kAhead < items) fetch(x + F::kAhead, staged + ((x + F::kAhead) % F::kStaging) * F::kStagingBytes, kProducers * 16u);
-                copies_commit();
-                copies_wait<F::kAhead>();
-                /* code bits in bf16's places are the value times 2^-120: times 2^(120 + e), one exact multiplication while that
-                   is a bf16 number (rows below 2^16), two beyond */
-                uint32_t f[kPasses];
+            auto widen = [&](uint32_t x, const uint4 (&w)[kPasses], const uint8_t (&unit)[kPasses]) {
+                if (x >= NS) alive = mbar_wait(empty + (x % NS) * 8u, ((x / NS) - 1u) & 1u);
+                if (!alive) return;
+                const uint32_t to = (x % NS) * F::kTile;
                 bool large = false;
 #pragma unroll
-                for (uint32_t e = 0; e < kPasses; e++) { const uint32_t b = unit[e]; f[e] = min(b + 120u, 254u) * 0x00800080u; large = large || b > 134u; }
+                for (uint32_t e = 0; e < kPasses; e++) large = large || unit[e] > 134u;
                 large = __any_sync(0xffffffffu, large);
-                uint32_t f2[kPasses];
-                if (large) {
-#pragma unroll
-                    for (uint32_t e = 0; e < kPasses; e++) f2[e] = (max((uint32_t)unit[e], 134u) - 7u) * 0x00800080u;
-                }
-                if (x + 1u < items) units(x + 1u);
-                if (x >= NS) alive = mbar_wait(empty + (x % NS) * 8u, ((x / NS) - 1u) & 1u);
-                if (!alive) break;
-                const uint32_t to = (x % NS) * F::kTile, src = staged + (x % F::kStaging) * F::kStagingBytes;
 #pragma unroll
                 for (uint32_t e = 0; e < kPasses; e++) {
-                    const uint4 w = lds128(src + e * kProducers * 16u);
-                    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+                    /* code bits in bf16's places are the value times 2^-120: times 2^(120 + e), one exact multiplication while
+                       that is a bf16 number (rows below 2^16), two beyond */
+                    const uint32_t b = unit[e], f = min(b + 120u, 254u) * 0x00800080u, u[4] = {w[e].x, w[e].y, w[e].z, w[e].w};
                     uint32_t y[8];
 #pragma unroll
                     for (uint32_t j = 0; j < 4u; j++) {
                         kv_spread(u[j], y[2 * j], y[2 * j + 1]);
-                        y[2 * j] = kv_mul2(y[2 * j], f[e]); y[2 * j + 1] = kv_mul2(y[2 * j + 1], f[e]);
+                        y[2 * j] = kv_mul2(y[2 * j], f); y[2 * j + 1] = kv_mul2(y[2 * j + 1], f);
                     }
                     if (large) {
+                        const uint32_t f2 = (max(b, 134u) - 7u) * 0x00800080u;
 #pragma unroll
-                        for (uint32_t j = 0; j < 8u; j++) y[j] = kv_mul2(y[j], f2[e]);
+                        for (uint32_t j = 0; j < 8u; j++) y[j] = kv_mul2(y[j], f2);
                     }
                     sts128u(place_lo + to + e * kRowsPerPass * 128u, y[0], y[1], y[2], y[3]);
                     sts128u(place_hi + to + e * kRowsPerPass * 128u, y[4], y[5], y[6], y[7]);
                 }
                 async_proxy_fence();
-                arrive(full + (x % NS) * 8u);
+                arrive_warp(full + (x % NS) * 8u);
+            };
+            uint4 w0[kPasses], w1[kPasses];
+            uint8_t u0[kPasses], u1[kPasses];
+            load(0u, w0, u0);
+            for (uint32_t x = 0; x < items && alive; x += 2u) {                         /* (the number of items is even) */
+                load(x + 1u, w1, u1);
+                widen(x, w0, u0);
+                if (!alive) break;
+                load(x + 2u, w0, u0);
+                widen(x + 1u, w1, u1);
             }
         }
-        copies_wait<0>();
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F::kRegsMma));
-        if (warp == F::kMmaWarp && lane == 0 && n) {
-        /* ---- matrix products ---- */
-        const uint32_t q_desc_base = base + F::kQ, ring0 = base + F::kRing;
-        constexpr uint32_t kIdescS = idesc_bf16(128u, kManyKeys, false), kIdescO = idesc_bf16(128u, HD, true);
-        auto ready = [&](uint32_t item) { return mbar_wait_one(full + (item % NS) * 8u, (item / NS) & 1u); };
-        auto scores = [&](uint32_t s, uint32_t t) {
-            const uint32_t kt = ring0 + (item_k(t) % NS) * F::kTile, qt = q_desc_base + (solo ? 0u : s) * F::kTile;
+        if (warp == F::kMmaWarp && n) {
+            /* ---- matrix products ---- */
+            constexpr uint32_t kIdescS = idesc_bf16(128u, kManyKeys, false), kIdescO = idesc_bf16(128u, HD, true);
+            const uint32_t leader = elect_lane();
+            /* descriptors of Q and of the ring's first slot, as a row-major (K) and as a transposed operand (V); the address field counts 16 bytes */
+            const uint32_t q_desc = desc_low(base + F::kQ, 16u), k_desc = desc_low(base + F::kRing, 16u), v_desc = desc_low(base + F::kRing, F::kHalfBytes);
+            auto ready = [&](uint32_t item) { return mbar_wait(full + (item % NS) * 8u, (item / NS) & 1u); };
+            auto scores = [&](uint32_t s, uint32_t t) {
+                const uint32_t qd = q_desc + (solo ? 0u : s * (F::kTile >> 4)), kd = k_desc + (item_k(t) % NS) * (F::kTile >> 4);
 #pragma unroll
-            for (uint32_t kk = 0; kk < HD / 16u; kk++)
-                mma_ss(tmem + s * 128u, desc_sw128(qt + (kk >> 2) * F::kHalfBytes + (kk & 3u) * 32u, 16u), desc_sw128(kt + (kk >> 2) * F::kHalfBytes + (kk & 3u) * 32u, 16u), kIdescS, kk ? 1u : 0u);
-            mma_commit(s_full + s * 8u);
-        };
-        auto outputs = [&](uint32_t s, uint32_t t, bool first) {
-            const uint32_t vt = ring0 + (item_v(t) % NS) * F::kTile;
+                for (uint32_t kk = 0; kk < HD / 16u; kk++) {
+                    constexpr uint32_t kHalf = F::kHalfBytes >> 4;
+                    mma_ss(leader, tmem + s * 128u, qd + (kk >> 2) * kHalf + (kk & 3u) * 2u, kd + (kk >> 2) * kHalf + (kk & 3u) * 2u, kIdescS, kk ? 1u : 0u);
+                }
+                mma_commit(leader, s_full + s * 8u);
+            };
+            auto outputs = [&](uint32_t s, uint32_t t, bool first) {
+                const uint32_t vd = v_desc + (item_v(t) % NS) * (F::kTile >> 4);
 #pragma unroll
-            for (uint32_t kk = 0; kk < kManyKeys / 16u; kk++)
-                mma_ts(tmem + 256u + s * 128u, tmem + s * 128u + kk * 8u, desc_sw128(vt + kk * 2048u, F::kHalfBytes), kIdescO, first && !kk ? 0u : 1u);
-        };
-        auto release = [&](uint32_t item) { mma_commit(empty + (item % NS) * 8u); };
-        alive = mbar_wait_one(q_full, 0u) && (solo || mbar_wait_one(q_full + 8u, 0u)) && ready(0u);
-        if (alive) {
-            tm_fence_after();
-            scores(0u, 0u);
-            if (solo) {
-                release(item_k(0u));
-                if (n > 1u) { alive = ready(item_k(1u)); if (alive) { tm_fence_after(); scores(1u, 1u); release(item_k(1u)); } }
-            } else { scores(1u, 0u); release(item_k(0u)); }
-        }
-        if (solo) {
-            for (uint32_t t = 0; t < n && alive; t++) {                                 /* tile t belongs to stream t & 1 */
-                const uint32_t s = t & 1u;
-                alive = ready(item_v(t)) && mbar_wait_one(p_full + s * 8u, (t >> 1) & 1u);
-                if (!alive) break;
-                tm_fence_after();
-                outputs(s, t, t < 2u);
-                release(item_v(t));
-                if (t + 2u >= n) mma_commit(o_full + s * 8u);
-                else {
-                    alive = ready(item_k(t + 2u));
+                for (uint32_t kk = 0; kk < kManyKeys / 16u; kk++)
+                    mma_ts(leader, tmem + 256u + s * 128u, tmem + s * 128u + kk * 8u, vd + kk * (2048u >> 4), kIdescO, first && !kk ? 0u : 1u);
+            };
+            auto release = [&](uint32_t item) { mma_commit(leader, empty + (item % NS) * 8u); };
+            /* step x = one stream's tile: S of the first tile of each, then per step O += P V and the S that follows it.  Alone
+               (solo), tile x belongs to stream x & 1; together, both streams take tile x / 2. */
+            const uint32_t steps = solo ? n : 2u * n;
+            alive = mbar_wait(q_full, 0u) && (solo || mbar_wait(q_full + 8u, 0u));
+            for (uint32_t x = 0; x < steps + 2u && alive; x++) {
+                const uint32_t s = x & 1u;
+                if (x >= 2u) {
+                    const uint32_t y = x - 2u, t = solo ? y : y >> 1;
+                    alive = ready(item_v(t)) && mbar_wait(p_full + s * 8u, (y >> 1) & 1u);
                     if (!alive) break;
                     tm_fence_after();
-                    scores(s, t + 2u);
-                    release(item_k(t + 2u));
+                    outputs(s, t, y < 2u);
+                    if (solo || s) release(item_v(t));
+                    if (x >= steps) mma_commit(leader, o_full + s * 8u);
                 }
-            }
-        } else {
-            for (uint32_t t = 0; t < n && alive; t++) {
-                const bool more = t + 1u < n;
-                alive = ready(item_v(t)) && (!more || ready(item_k(t + 1u)));
-                for (uint32_t s = 0; s < 2u && alive; s++) {
-                    alive = mbar_wait_one(p_full + s * 8u, t & 1u);
+                if (x < steps) {
+                    const uint32_t t = solo ? x : x >> 1;
+                    alive = ready(item_k(t));
                     if (!alive) break;
                     tm_fence_after();
-                    outputs(s, t, t == 0u);
-                    if (s) release(item_v(t));
-                    if (more) { scores(s, t + 1u); if (s) release(item_k(t + 1u)); }
-                    else mma_commit(o_full + s * 8u);
+                    scores(s, t);
+                    if (solo || s) release(item_k(t));
                 }
             }
-        }
-        if (!alive) {                                                                   /* what was issued must end before the memory is given back */
-            mma_commit(o_full); mma_commit(o_full + 8u);
-            for (uint32_t i = 0; i < (1u << 20); i++) if (mbar_poll(o_full, 0u) && mbar_poll(o_full + 8u, 0u)) break;
-        }
+            if (!alive) {                                                               /* what was issued must end before the memory is given back */
+                mma_commit(leader, o_full); mma_commit(leader, o_full + 8u);
+                for (uint32_t i = 0; i < (1u << 20); i++) if (__all_sync(0xffffffffu, mbar_poll(o_full, 0u) && mbar_poll(o_full + 8u, 0u))) break;
+            }
         }
     }
     if (!pos_ok && tid == 0) atomicOr(a.status, kKvStatusPosition);
@@ -506,6 +515,20 @@ __global__ void __launch_bounds__(Many<HD, ELEM>::kThreads, 1) kv_attention_many
     __syncthreads();
     tm_fence_after();
     if (warp == F::kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+/* cuTensorMapEncodeTiled through the runtime's driver entry point (the library does not link against the driver) */
+typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                  const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeTiledFn encode_tiled() {
+    static std::atomic<void *> cached{nullptr};
+    void *fn = cached.load(std::memory_order_acquire);
+    if (!fn) {
+        cudaDriverEntryPointQueryResult res;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &res) != cudaSuccess || res != cudaDriverEntryPointSuccess) { cudaGetLastError(); return nullptr; }
+        cached.store(fn, std::memory_order_release);
+    }
+    return reinterpret_cast<EncodeTiledFn>(fn);
 }
 
 template <int HD, int ELEM>
@@ -517,7 +540,19 @@ static cudaError_t launch_many(cudaStream_t st, const KvAttention &a) {
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr; cfg.numAttrs = dependent_launch() ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kv_attention_many_kernel<HD, ELEM>, a);
+    /* bf16: K and V as [planes][capacity][HD], boxes of 64 dimensions x 128 rows, swizzled as the operands are */
+    alignas(64) CUtensorMap maps[2] = {};
+    if (ELEM == kKvBf16) {
+        const EncodeTiledFn encode = encode_tiled();
+        if (!encode) return cudaErrorNotSupported;
+        const cuuint64_t dims[3] = {HD, a.c.capacity, (cuuint64_t)a.layers * a.c.n_kv}, strides[2] = {HD * 2u, (cuuint64_t)a.c.capacity * HD * 2u};
+        const cuuint32_t box[3] = {64u, kManyKeys, 1u}, ones[3] = {1u, 1u, 1u};
+        const uint64_t below = (uint64_t)a.layer * a.c.n_kv * a.c.capacity * HD * 2u;
+        for (int i = 0; i < 2; i++)
+            if (encode(&maps[i], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3u, (i ? a.c.v : a.c.k) - below, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                       CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) return cudaErrorInvalidValue;
+    }
+    return cudaLaunchKernelEx(&cfg, kv_attention_many_kernel<HD, ELEM>, a, maps[0], maps[1]);
 }
 
 cudaError_t launch_kv_many(cudaStream_t st, int elem, uint32_t head_dim, const KvAttention &a) {
