@@ -235,13 +235,18 @@ __global__ void __launch_bounds__(Many<HD, ELEM>::kThreads, 1) kv_attention_many
         const uint32_t s = warp >> 2, wt = tid & 127u, q_tile = solo ? 0u : s, my_row0 = row0 + q_tile * kManyRows;
         const uint32_t my_n = solo ? (s ? n / 2u : (n + 1u) / 2u) : n;                 /* tiles of this stream */
         if (n && !(solo && s)) {
-            /* Q: 16 bytes per thread, rows beyond the last as zeros */
-            for (uint32_t e = wt; e < kManyRows * HD / 8u; e += 128u) {
-                const uint32_t r = e / (HD / 8u), ch = e % (HD / 8u), row = my_row0 + r;
-                uint4 w = make_uint4(0u, 0u, 0u, 0u);
-                if (row < rows) w = *reinterpret_cast<const uint4 *>(a.q + (uint64_t)(row / group) * a.ldq + (uint64_t)(kvh * group + row % group) * HD + ch * 8u);
-                sts128u(base + F::kQ + q_tile * F::kTile + (ch >> 3) * F::kHalfBytes + swizzled(r, ch & 7u), w.x, w.y, w.z, w.w);
+            /* Q: 16 bytes per thread (all loads in flight together), rows beyond the last as zeros */
+            constexpr uint32_t kQChunks = HD / 8u, kQPasses = kManyRows * kQChunks / 128u, kQRows = 128u / kQChunks;
+            const uint32_t qr = wt / kQChunks, qc = wt % kQChunks;
+            uint4 w[kQPasses];
+#pragma unroll
+            for (uint32_t e = 0; e < kQPasses; e++) {
+                const uint32_t row = my_row0 + qr + e * kQRows;
+                w[e] = make_uint4(0u, 0u, 0u, 0u);
+                if (row < rows) w[e] = *reinterpret_cast<const uint4 *>(a.q + (uint64_t)(row / group) * a.ldq + (uint64_t)(kvh * group + row % group) * HD + qc * 8u);
             }
+#pragma unroll
+            for (uint32_t e = 0; e < kQPasses; e++) sts128u(base + F::kQ + q_tile * F::kTile + (qc >> 3) * F::kHalfBytes + swizzled(qr + e * kQRows, qc & 7u), w[e].x, w[e].y, w[e].z, w[e].w);
             async_proxy_fence();
             arrive_warp(q_full + q_tile * 8u);
         }
