@@ -46,8 +46,8 @@ template <int HD, int ELEM> struct Many {
     /* Registers: the warps start with 65536 / threads (a multiple of 8) each; those that hold a row of scores take what the
        others give back: 8 x 184 + 4 x 72 + 4 x 72 = 16 x 128, 8 x 152 + 8 x 64 + 4 x 48 = 20 x 96.  Widening e4m3 rows takes
        eight warps, copying bf16 ones four. */
-    static constexpr uint32_t kProducers = ELEM == kKvE4m3 ? 256u : 128u, kMmaWarp = 8u + kProducers / 32u, kThreads = 256u + kProducers + 128u;
-    static constexpr int kRegsWeights = ELEM == kKvE4m3 ? 152 : 184, kRegsProduce = ELEM == kKvE4m3 ? 64 : 72, kRegsMma = ELEM == kKvE4m3 ? 48 : 72;
+    static constexpr uint32_t kProducers = 128u, kMmaWarp = 8u + kProducers / 32u, kThreads = 256u + kProducers + 128u;
+    static constexpr int kRegsWeights = ELEM == kKvE4m3 ? 168 : 184, kRegsProduce = ELEM == kKvE4m3 ? 112 : 72, kRegsMma = ELEM == kKvE4m3 ? 64 : 72;
     static constexpr uint32_t kQ = 0u, kRing = 2u * kTile, kBars = kRing + kSlots * kTile;
     static constexpr uint32_t kSmem = 1024u + kBars + (2u * kSlots + 8u) * 8u + 16u;
 };
