@@ -24,6 +24,19 @@ __device__ __forceinline__ uint16_t pack_e4m3(float a, float b) { return __nv_cv
 
 __device__ __forceinline__ uint4 pack8(const float (&y)[8]) { return make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7])); }
 constexpr float kLargestBf16 = 3.3895313892515355e38f;
+/* 1.875 * 2^127: the largest value of three mantissa bits in range; rounding a larger one up would reach 2^128 */
+constexpr float kLargestE4m3 = 3.1901471898837980e38f;
+/* a + b as the rounded sum and what the rounding left (Knuth's two-sum) */
+__device__ __forceinline__ float two_sum(float a, float b, float &e) {
+    const float s = __fadd_rn(a, b), t = __fsub_rn(s, a);
+    e = __fadd_rn(__fsub_rn(a, __fsub_rn(s, t)), __fsub_rn(b, t));
+    return s;
+}
+/* exponent byte of a row: smallest e with top <= 1.75 * 2^(8 + e), from top's exponent field, one more where its mantissa is above 0.75 */
+__device__ __forceinline__ int32_t unit_byte(float top) {
+    const uint32_t bits = __float_as_uint(top);
+    return max(0, (int32_t)(bits >> 23) - 8 + ((bits & 0x7FFFFFu) > 0x600000u ? 1 : 0));
+}
 
 struct StoreArgs {
     KvLayer c;
@@ -38,93 +51,173 @@ struct StoreArgs {
 };
 
 /* HD / 8 lanes hold one row, eight numbers each, so a row is one 16-byte load per lane; the rotary partner of a number lives
-   in the lane HD / 16 away.  A warp takes kRows rows of one token at a time (their loads are in flight together and share the
-   token's cos / sin).  Everything between the loaded bf16 numbers and what is stored is fp32, rounded once. */
+   in the lane HD / 16 away.  A warp takes PASSES x kSide rows of one kind (query, key or value) of one token: their loads are in
+   flight together, before the position is known, and they share the token's cos / sin.  (Rows of all kinds in one warp make
+   one long piece of code, four times unrolled: 100 us for 4096 tokens of 64 + 16 heads where this takes less than half, most of it waiting
+   for instructions.)
+   Between the loaded bf16 numbers and what is stored is fp32, rounded once.  Keys that become e4m3 codes are kept to twice
+   fp32's precision on the way (with fp32's few roundings some four of a million land on the wrong side of a code's border):
+   a product of three bf16 numbers is exact in fp32, so x w cos and x' w' sin are, their sum is two numbers, and so is the
+   reciprocal norm after one Newton step. */
+template <int HD> struct Row {
+    static constexpr uint32_t kLanes = HD / 8, kSide = 32 / kLanes;
+    template <class T> static __device__ __forceinline__ T partner(T v) { return __shfl_xor_sync(0xffffffffu, v, kLanes / 2); }
+    static __device__ __forceinline__ float sum(float v) {
+#pragma unroll
+        for (uint32_t o = kLanes / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        return v;
+    }
+    static __device__ __forceinline__ float max(float v) {
+#pragma unroll
+        for (uint32_t o = kLanes / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+        return v;
+    }
+};
+__device__ __forceinline__ void unpack8(const uint4 &w, float (&x)[8]) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int j = 0; j < 4; j++) { x[2 * j] = lo16(u[j]); x[2 * j + 1] = hi16(u[j]); }
+}
+/* x w / norm, turned; `sign` is that of the partner's share in this lane */
+template <int HD>
+__device__ __forceinline__ void normed_and_turned(float (&y)[8], bool norm, const float (&w)[8], float eps, const float (&c)[8], const float (&s)[8], float sign) {
+    if (norm) {
+        float ss = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) ss = fmaf(y[j], y[j], ss);
+        const float inv = rsqrtf(Row<HD>::sum(ss) * (1.f / HD) + eps);
+#pragma unroll
+        for (int j = 0; j < 8; j++) y[j] *= inv * w[j];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) { const float other = Row<HD>::partner(y[j]); y[j] = fmaf(y[j], c[j], sign * other * s[j]); }
+}
+/* the same as a sum of two numbers each */
+template <int HD>
+__device__ __forceinline__ void normed_and_turned_exactly(float (&y)[8], float (&low)[8], bool norm, const float (&w)[8], float eps, const float (&c)[8], const float (&s)[8], float sign) {
+    float inv = 1.f, inv_low = 0.f;
+    if (norm) {
+        float sh = 0.f, sl = 0.f, e;
+#pragma unroll
+        for (int j = 0; j < 8; j++) { sh = two_sum(sh, y[j] * y[j], e); sl += e; }
+#pragma unroll
+        for (uint32_t o = Row<HD>::kLanes / 2; o > 0; o >>= 1) {
+            const float oh = __shfl_xor_sync(0xffffffffu, sh, o), ol = __shfl_xor_sync(0xffffffffu, sl, o);
+            sh = two_sum(sh, oh, e); sl = sl + ol + e;
+        }
+        const float mh = two_sum(sh * (1.f / HD), eps, e), ml = sl * (1.f / HD) + e;
+        inv = rsqrtf(mh);
+        const float ph = __fmul_rn(inv, inv), pl = fmaf(inv, inv, -ph);
+        inv_low = 0.5f * inv * (fmaf(-mh, ph, 1.f) - fmaf(mh, pl, ml * ph));
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const float xw = norm ? __fmul_rn(y[j], w[j]) : y[j], other = Row<HD>::partner(xw);
+        float e, h = two_sum(__fmul_rn(xw, c[j]), sign * __fmul_rn(other, s[j]), e);
+        if (norm) {
+            const float p = __fmul_rn(h, inv), q = fmaf(h, inv, -p) + fmaf(e, inv, h * inv_low);
+            h = __fadd_rn(p, q); e = __fsub_rn(q, __fsub_rn(h, p));
+        }
+        y[j] = h; low[j] = e;
+    }
+}
+/* One row's eight numbers y + low of this lane into the cache.  What is not finite would reach every query: it is kept out (0)
+   and reported. */
+template <int HD, int ELEM>
+__device__ __forceinline__ void store_row(const StoreArgs &a, uint8_t *plane, uint8_t *exps, uint64_t cell, uint32_t sub, bool live, float (&y)[8], float (&low)[8]) {
+    bool fine = true;
+    float top = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        if (!(fabsf(y[j]) <= kLargestBf16)) { fine = false; y[j] = low[j] = 0.f; }
+        if (ELEM == kKvE4m3) {
+            if (fabsf(y[j]) >= kLargestE4m3) { y[j] = copysignf(kLargestE4m3, y[j]); low[j] = 0.f; }
+            /* the magnitude rounded up: what the row's unit goes by */
+            top = fmaxf(top, __uint_as_float(__float_as_uint(fabsf(y[j])) + (low[j] != 0.f && (low[j] > 0.f) == (y[j] > 0.f) ? 1u : 0u)));
+        }
+    }
+    if (ELEM == kKvE4m3) {
+        const int32_t b = unit_byte(Row<HD>::max(top));
+        const float up = __uint_as_float((uint32_t)(254 - b) << 23);  /* 2^(127 - b): exact */
+#pragma unroll
+        for (int j = 0; j < 8; j++) {                                 /* truncated with a sticky last bit: rounding that to e4m3 is rounding the sum of both numbers */
+            uint32_t f = __float_as_uint(y[j]);
+            if (low[j] != 0.f) f = (f - ((low[j] > 0.f) == (y[j] > 0.f) ? 0u : 1u)) | 1u;
+            y[j] = __uint_as_float(f) * up;
+        }
+        if (live) {
+            uint2 codes;
+            codes.x = pack_e4m3(y[0], y[1]) | ((uint32_t)pack_e4m3(y[2], y[3]) << 16);
+            codes.y = pack_e4m3(y[4], y[5]) | ((uint32_t)pack_e4m3(y[6], y[7]) << 16);
+            *reinterpret_cast<uint2 *>(plane + cell * HD + sub * 8u) = codes;
+            if (sub == 0) exps[cell] = (uint8_t)b;
+        }
+    } else if (live) *reinterpret_cast<uint4 *>(plane + (cell * HD + sub * 8u) * 2u) = pack8(y);
+    if (live && !fine) atomicOr(a.status, kKvStatusNotFinite);
+}
+
+constexpr uint32_t kStoreQ = 4, kStoreK = 1, kStoreV = 2;             /* passes of a warp */
+template <int HD> __host__ __device__ constexpr uint32_t store_groups(uint32_t n, uint32_t passes) { return (n + passes * (256u / HD) - 1u) / (passes * (256u / HD)); }
+
 template <int HD, int ELEM>
 __global__ void __launch_bounds__(256) kv_store_kernel(const StoreArgs a) {
-    constexpr uint32_t kLanesPerRow = HD / 8, kSide = 32 / kLanesPerRow, kPasses = 4, kRows = kSide * kPasses;
-    const uint32_t lane = threadIdx.x & 31u, sub = lane % kLanesPerRow, side = lane / kLanesPerRow, d0 = sub * 8u;
-    const uint32_t heads = a.n_q + 2u * a.c.n_kv, groups = (heads + kRows - 1u) / kRows;
-    const uint64_t unit = (uint64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    using R = Row<HD>;
+    const uint32_t lane = threadIdx.x & 31u, sub = lane % R::kLanes, side = lane / R::kLanes, d0 = sub * 8u, n_q = a.n_q, n_kv = a.c.n_kv;
+    const uint32_t gq = store_groups<HD>(n_q, kStoreQ), gk = store_groups<HD>(n_kv, kStoreK), gv = store_groups<HD>(n_kv, kStoreV), groups = gq + gk + gv;
+    const uint32_t unit = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);           /* (below 2^31: the launcher checks) */
     dependency_sync();
-    if (unit >= (uint64_t)groups * a.T) return;
-    const uint32_t t = (uint32_t)(unit / groups), row0 = (uint32_t)(unit % groups) * kRows;
+    if (unit >= groups * a.T) return;
+    const uint32_t t = unit / groups, group = unit - t * groups;
+    const int kind = group < gq ? 0 : group < gq + gk ? 1 : 2;        /* of the whole warp */
+    const uint32_t n = kind ? n_kv : n_q, row0 = kind == 0 ? group * kStoreQ * R::kSide : kind == 1 ? (group - gq) * kStoreK * R::kSide : (group - gq - gk) * kStoreV * R::kSide;
+    const uint16_t *from = a.qkv + (uint64_t)t * a.ldqkv + (uint64_t)(kind == 0 ? 0u : kind == 1 ? n_q : n_q + n_kv) * HD + d0;
+    uint4 raw[kStoreQ];
+#pragma unroll
+    for (uint32_t i = 0; i < kStoreQ; i++) {
+        const uint32_t row = row0 + i * R::kSide + side;
+        raw[i] = row < n && (i == 0u || kind == 0 || (kind == 2 && i < kStoreV)) ? __ldcs(reinterpret_cast<const uint4 *>(from + (uint64_t)row * HD)) : make_uint4(0u, 0u, 0u, 0u);
+    }
     const int32_t pos = *a.pos, depth = a.depth ? a.depth[t] : (int32_t)t;
     const uint32_t limit = a.c.window ? 0x7FFFFFFFu : a.c.capacity;
     const bool ok = pos >= 0 && (uint64_t)pos + a.T <= limit && depth >= 0 && (uint32_t)depth < a.T && (uint64_t)pos + (a.depth ? (uint32_t)depth + 1u : a.T) <= a.max_pos;
     if (!ok) { if (lane == 0) atomicOr(a.status, kKvStatusPosition); return; }
-    const uint32_t slot = kv_slot((uint32_t)pos + t, a.c.capacity, a.c.window, a.c.sinks);
-    uint4 raw[kPasses];
+    const uint64_t slot = kv_slot((uint32_t)pos + t, a.c.capacity, a.c.window, a.c.sinks);
+    if (kind == 2) {
 #pragma unroll
-    for (uint32_t i = 0; i < kPasses; i++) {
-        const uint32_t row = row0 + i * kSide + side;
-        raw[i] = row < heads ? *reinterpret_cast<const uint4 *>(a.qkv + (uint64_t)t * a.ldqkv + (uint64_t)row * HD + d0) : make_uint4(0u, 0u, 0u, 0u);
+        for (uint32_t i = 0; i < kStoreV; i++) {
+            const uint32_t row = row0 + i * R::kSide + side;
+            float y[8], low[8];
+            unpack8(raw[i], y);
+#pragma unroll
+            for (int j = 0; j < 8; j++) low[j] = 0.f;
+            store_row<HD, ELEM>(a, a.c.v, a.c.v_exp, (uint64_t)row * a.c.capacity + slot, sub, row < n, y, low);
+        }
+        return;
     }
     const uint64_t at = ((uint64_t)pos + (uint32_t)depth) * HD + d0;
-    const uint4 cw = *reinterpret_cast<const uint4 *>(a.cos_t + at), sw = *reinterpret_cast<const uint4 *>(a.sin_t + at);
-    const uint32_t cu[4] = {cw.x, cw.y, cw.z, cw.w}, su[4] = {sw.x, sw.y, sw.z, sw.w};
+    const bool norm = a.q_norm != nullptr;
+    float c[8], s[8], w[8];
+    unpack8(*reinterpret_cast<const uint4 *>(a.cos_t + at), c);
+    unpack8(*reinterpret_cast<const uint4 *>(a.sin_t + at), s);
+    if (norm) unpack8(*reinterpret_cast<const uint4 *>((kind ? a.k_norm : a.q_norm) + d0), w);
+    const float sign = sub < R::kLanes / 2 ? -1.f : 1.f;
+    if (kind == 1) {
+        static_assert(kStoreK == 1, "one pass of keys");
+        const uint32_t row = row0 + side;
+        float y[8], low[8];
+        unpack8(raw[0], y);
+        if (ELEM == kKvE4m3) normed_and_turned_exactly<HD>(y, low, norm, w, a.eps, c, s, sign);
+        else normed_and_turned<HD>(y, norm, w, a.eps, c, s, sign);
+        store_row<HD, ELEM>(a, a.c.k, a.c.k_exp, (uint64_t)row * a.c.capacity + slot, sub, row < n, y, low);
+        return;
+    }
 #pragma unroll
-    for (uint32_t i = 0; i < kPasses; i++) {
-        const uint32_t row = row0 + i * kSide + side;
-        const bool live = row < heads, is_q = row < a.n_q, is_v = row >= a.n_q + a.c.n_kv;
-        const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-        float x[8];
-#pragma unroll
-        for (int j = 0; j < 4; j++) { x[2 * j] = lo16(u[j]); x[2 * j + 1] = hi16(u[j]); }
-        const uint16_t *weight = is_q ? a.q_norm : a.k_norm;
-        if (a.q_norm) {                                               /* (the sum of a V row is not used) */
-            float ss = 0.f;
-#pragma unroll
-            for (int j = 0; j < 8; j++) ss = fmaf(x[j], x[j], ss);
-#pragma unroll
-            for (uint32_t o = kLanesPerRow / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            const float inv = rsqrtf(ss * (1.f / HD) + a.eps);
-            if (!is_v) {
-                const uint4 ww = *reinterpret_cast<const uint4 *>(weight + d0);
-                const uint32_t wu[4] = {ww.x, ww.y, ww.z, ww.w};
-#pragma unroll
-                for (int j = 0; j < 4; j++) { x[2 * j] *= inv * lo16(wu[j]); x[2 * j + 1] *= inv * hi16(wu[j]); }
-            }
-        }
-        const float sign = sub < kLanesPerRow / 2 ? -1.f : 1.f;
+    for (uint32_t i = 0; i < kStoreQ; i++) {
+        const uint32_t row = row0 + i * R::kSide + side;
         float y[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const float other = __shfl_xor_sync(0xffffffffu, x[j], kLanesPerRow / 2);
-            const float c = j & 1 ? hi16(cu[j >> 1]) : lo16(cu[j >> 1]), s = j & 1 ? hi16(su[j >> 1]) : lo16(su[j >> 1]);
-            y[j] = is_v ? x[j] : fmaf(x[j], c, sign * other * s);
-        }
-        if (is_q) *reinterpret_cast<uint4 *>(a.q_out + ((uint64_t)t * a.n_q + row) * HD + d0) = pack8(y);
-        /* a key or value that is not finite would reach every query through the cache: it is kept out (0) and reported */
-        bool fine = true;
-        float top = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            if (!(fabsf(y[j]) <= kLargestBf16)) { fine = false; y[j] = 0.f; }
-            /* (1.875 * 2^127: the largest value of three mantissa bits in range; rounding a larger one up would reach 2^128) */
-            if (ELEM == kKvE4m3) y[j] = fminf(fmaxf(y[j], -3.1901471898837980e38f), 3.1901471898837980e38f);
-            top = fmaxf(top, fabsf(y[j]));
-        }
-        const uint32_t kvh = is_v ? row - a.n_q - a.c.n_kv : row - a.n_q;
-        const uint64_t cell = (uint64_t)kvh * a.c.capacity + slot;
-        if (ELEM == kKvE4m3) {
-#pragma unroll
-            for (uint32_t o = kLanesPerRow / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            /* smallest e with top <= 1.75 * 2^(8 + e): from top's exponent field, one more where its mantissa is above 0.75 */
-            const uint32_t bits = __float_as_uint(top);
-            const int32_t b = max(0, (int32_t)(bits >> 23) - 8 + ((bits & 0x7FFFFFu) > 0x600000u ? 1 : 0));
-            const float inv = __uint_as_float((uint32_t)(254 - b) << 23);         /* 2^(127 - b): exact */
-            if (live && !is_q) {
-                uint2 codes;
-                codes.x = pack_e4m3(y[0] * inv, y[1] * inv) | ((uint32_t)pack_e4m3(y[2] * inv, y[3] * inv) << 16);
-                codes.y = pack_e4m3(y[4] * inv, y[5] * inv) | ((uint32_t)pack_e4m3(y[6] * inv, y[7] * inv) << 16);
-                *reinterpret_cast<uint2 *>((is_v ? a.c.v : a.c.k) + cell * HD + d0) = codes;
-                if (sub == 0) (is_v ? a.c.v_exp : a.c.k_exp)[cell] = (uint8_t)b;
-            }
-        } else if (live && !is_q) {
-            *reinterpret_cast<uint4 *>((is_v ? a.c.v : a.c.k) + (cell * HD + d0) * 2u) = pack8(y);
-        }
-        if (live && !is_q && !fine) atomicOr(a.status, kKvStatusNotFinite);
+        unpack8(raw[i], y);
+        normed_and_turned<HD>(y, norm, w, a.eps, c, s, sign);
+        if (row < n) *reinterpret_cast<uint4 *>(a.q_out + ((uint64_t)t * n_q + row) * HD + d0) = pack8(y);
     }
 }
 
@@ -215,9 +308,8 @@ KvLayer layer_of(const nwc_kv_cache *c, uint32_t layer) {
 
 template <int HD>
 cudaError_t launch_store(int elem, const StoreArgs &a, void *stream) {
-    constexpr uint32_t rows = 4u * 32u / (HD / 8u);
-    const uint64_t units = (uint64_t)((a.n_q + 2u * a.c.n_kv + rows - 1u) / rows) * a.T, blocks = (units + 7u) / 8u;
-    if (blocks > 0x7FFFFFFFull) return cudaErrorInvalidValue;
+    const uint64_t units = (uint64_t)(store_groups<HD>(a.n_q, kStoreQ) + store_groups<HD>(a.c.n_kv, kStoreK) + store_groups<HD>(a.c.n_kv, kStoreV)) * a.T, blocks = (units + 7u) / 8u;
+    if (units > 0x7FFFFFFFull) return cudaErrorInvalidValue;
     const uint32_t threads = units >= 8u ? 256u : (uint32_t)units * 32u;
     return elem == kKvE4m3 ? launch(kv_store_kernel<HD, kKvE4m3>, dim3((uint32_t)blocks), dim3(threads), stream, a)
                            : launch(kv_store_kernel<HD, kKvBf16>, dim3((uint32_t)blocks), dim3(threads), stream, a);

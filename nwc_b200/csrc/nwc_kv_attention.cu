@@ -17,8 +17,8 @@
  * bf16 caches take bf16 products.  e4m3 codes become f16 (exactly, one conversion for two codes; bf16 would take bit moves and a
  * multiplication, 640 instead of 230 instructions of the 1150 per tile of 32 keys, and the kernel is bound by its issue rate),
  * with a query row scaled by a power of two to fill f16's range; the unit 2^e of a K row multiplies its scores, that of a V
- * row, relative to the largest met so far, its weights.  The weights are rounded for the second product to bf16 (2^-8) or f16
- * (2^-11); their sum, the running maximum and all accumulators are fp32.
+ * row, relative to the largest met so far, its weights.  Tiles with V rows more than 2^10 smaller than that take bf16 products
+ * for them.  The weights are rounded for the second product to bf16 (2^-8) or f16 (2^-11); their sum, the running maximum and all accumulators are fp32.
  */
 #include "nwc_kv.h"
 #include "nwc_async.cuh"
@@ -47,6 +47,8 @@ __device__ __forceinline__ uint32_t pack_half(float a, float b) { uint32_t d; as
 __device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t &lo, uint32_t &hi) {
     asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
 }
+/* codes (in the high bytes of both halves of w; the low bytes may hold anything) -> bf16 pair */
+__device__ __forceinline__ uint32_t codes_to_bf16(uint32_t w) { return kv_mul2(((w >> 4) & 0x07F007F0u) | (w & 0x80008000u), kTwoTo120); }
 /* 2^e for -126 <= e <= 127 */
 __device__ __forceinline__ float power_of_two(int32_t e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
@@ -85,7 +87,7 @@ __device__ __forceinline__ void cluster_barrier() {
 template <int HD, int ELEM, int MT, int SHORT>
 __global__ void __launch_bounds__(32 * Few<HD, ELEM, MT, SHORT>::kWarps, 1) kv_attention_few_kernel(const KvAttention a) {
     using F = Few<HD, ELEM, MT, SHORT>;
-    constexpr uint32_t kRows = F::kRows, kNT = F::kKeys / 8u, kSteps = HD / 16u, kWarps = F::kWarps;
+    constexpr uint32_t kRows = F::kRows, kNT = F::kKeys / 8u, kWarps = F::kWarps;
     extern __shared__ __align__(128) uint8_t few_raw[];
     const uint32_t ring = smem_addr(few_raw), tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, g = lane >> 2, c = lane & 3u;
     uint8_t *qs = few_raw + F::kQ;                                                  /* Q in fragment order: [kSteps][MT][32 lanes] uint4 */
@@ -300,6 +302,8 @@ __global__ void __launch_bounds__(32 * Few<HD, ELEM, MT, SHORT>::kWarps, 1) kv_a
 #pragma unroll
         for (uint32_t i = 0; i < 2u * MT; i++) base[i] = m[i] == -INFINITY ? 0.f : m[i];
         const float v_unit = power_of_two(max((int32_t)(v_byte - top_byte), -126));
+        /* rows more than 2^10 smaller than the largest met: their weights would reach f16's subnormal numbers */
+        const bool wide = ELEM == kKvE4m3 && __any_sync(0xffffffffu, v_byte && v_byte + 10u < top_byte);
 #pragma unroll
         for (uint32_t j = 0; j < kNT; j++)
 #pragma unroll
@@ -319,7 +323,7 @@ __global__ void __launch_bounds__(32 * Few<HD, ELEM, MT, SHORT>::kWarps, 1) kv_a
             uint4 pf[MT];
 #pragma unroll
             for (uint32_t i = 0; i < MT; i++) {
-                auto pack = [](float x, float y) { return ELEM == kKvE4m3 ? pack_half(x, y) : pack_bf16(x, y); };
+                auto pack = [&](float x, float y) { return ELEM == kKvE4m3 && !wide ? pack_half(x, y) : pack_bf16(x, y); };
                 pf[i] = make_uint4(pack(sc[i][2 * h][0], sc[i][2 * h][1]), pack(sc[i][2 * h][2], sc[i][2 * h][3]),
                                    pack(sc[i][2 * h + 1][0], sc[i][2 * h + 1][1]), pack(sc[i][2 * h + 1][2], sc[i][2 * h + 1][3]));
             }
@@ -334,7 +338,15 @@ __global__ void __launch_bounds__(32 * Few<HD, ELEM, MT, SHORT>::kWarps, 1) kv_a
                     if (ELEM == kKvE4m3 && HD == 64) { const uint2 x = lds64(from + g * 8u); w[e][0] = x.x; w[e][1] = x.y; }
                     else { const uint4 x = lds128(from + pc * 128u + g * 16u); w[e][0] = x.x; w[e][1] = x.y; w[e][2] = x.z; w[e][3] = x.w; }
                 }
-                if (ELEM == kKvE4m3) {
+                if (ELEM == kKvE4m3 && wide) {
+#pragma unroll
+                    for (uint32_t d = 0; d < kPieceDims; d++) {
+                        const uint32_t sel = (d & 3u) << 4 | ((d & 3u) + 4u) << 12;
+                        const uint32_t b0 = codes_to_bf16(__byte_perm(w[0][d >> 2], w[1][d >> 2], sel)), b1 = codes_to_bf16(__byte_perm(w[2][d >> 2], w[3][d >> 2], sel));
+#pragma unroll
+                        for (uint32_t i = 0; i < MT; i++) mma16816(o[i][pc * kPieceDims + d], pf[i], b0, b1);
+                    }
+                } else if (ELEM == kKvE4m3) {
 #pragma unroll
                     for (uint32_t d = 0; d < kPieceDims; d += 2u) {
                         /* bytes d % 4 and d % 4 + 1 of the two keys' words, side by side */

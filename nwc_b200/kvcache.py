@@ -16,6 +16,9 @@ import torch
 
 from . import _lib as L
 
+BF16, INT32 = torch.bfloat16, torch.int32
+current_device, raw_stream = getattr(torch._C, "_cuda_getDevice", None), getattr(torch._C, "_cuda_getCurrentRawStream", None)     # (absent without CUDA)
+MAX_TREE = 1024
 ELEMS = {"bf16": (0, torch.bfloat16), "fp8": (1, torch.float8_e4m3fn)}
 STATUS_TEXT = ((1, "a position outside the cache or the rotary tables"), (2, "a key or value that is not finite"), (4, "an accepted path that is not one"))
 
@@ -25,7 +28,7 @@ def draft_tree(parents, device="cuda"):
     Returns (visible int32 [T, ceil(T / 32)], depth int32 [T]): every token sees its ancestors and itself."""
     T = len(parents)
     if not T: raise ValueError("a draft tree has at least one token")
-    if T > 1024: raise ValueError(f"a draft tree has at most 1024 tokens, not {T}")
+    if T > MAX_TREE: raise ValueError(f"a draft tree has at most {MAX_TREE} tokens, not {T}")
     masks, depth = [], []
     for i, p in enumerate(parents):
         p = int(p)
@@ -87,6 +90,7 @@ class KVCache:
         self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
         at = lambda t: None if t is None else t.data_ptr()
         self._c = L.KvCache(at(k), at(v), at(k_exp), at(v_exp), self.layers, self.n_kv, self.head_dim, self.capacity, window, sinks, 1 if quantised else 0)
+        self._at, self._bf16 = k.get_device(), torch.empty(0, dtype=BF16, device=k.device)
         self._need = {}                                               # workspace bytes per (tokens, query heads)
         self._ref, self._status = ctypes.byref(self._c), self.status.data_ptr()
 
@@ -98,19 +102,21 @@ class KVCache:
         Returns the queries, bf16 [T, n_q, head_dim]."""
         if qkv.dim() == 1: qkv = qkv[None]
         T, width = self._tokens(qkv, 2, "qkv")
-        heads, hd = width // self.head_dim, self.head_dim
-        n_q = heads - 2 * self.n_kv
+        hd, at = self.head_dim, self._at
+        n_q = width // hd - 2 * self.n_kv
         if width % hd or n_q <= 0 or n_q % self.n_kv: raise ValueError(f"qkv rows of {width} are not (n_q + 2 * {self.n_kv}) heads of {hd}, n_q a multiple of {self.n_kv}")
         if (q_norm is None) != (k_norm is None): raise ValueError("q_norm and k_norm come together")
-        for t, shape in ((cos, None), (sin, cos.shape), (q_norm, (hd,)), (k_norm, (hd,))):
-            if t is not None and (t.dtype != torch.bfloat16 or t.device != self.device or not t.is_contiguous() or t.shape[-1] != hd or shape is not None and tuple(t.shape) != tuple(shape)):
-                raise ValueError(f"cos and sin are bf16 [positions, {hd}], q_norm and k_norm bf16 [{hd}], on the cache's device")
+        rows = cos.size(0)
+        if cos.dim() != 2 or sin.dim() != 2 or sin.size(0) != rows: raise ValueError(f"cos and sin are both [positions, {hd}]")
+        for t in (cos, sin) if q_norm is None else (cos, sin, q_norm, k_norm):
+            if t.dtype is not BF16 or t.get_device() != at or t.size(-1) != hd or not t.is_contiguous(): raise ValueError(f"cos and sin are contiguous bf16 [positions, {hd}], q_norm and k_norm bf16 [{hd}], on {self.device}")
+        if q_norm is not None and (q_norm.dim() != 1 or k_norm.dim() != 1): raise ValueError(f"q_norm and k_norm are bf16 [{hd}]")
         if depth is not None: self._int32(depth, T, "depth")
         self._int32(pos, 1, "pos")
         self._layer(layer)
         out = qkv.new_empty((T, n_q, hd))
-        self._call("nwc_kv_append", L.lib.nwc_kv_append, layer, qkv.data_ptr(), qkv.stride(0), T, n_q, None if q_norm is None else q_norm.data_ptr(),
-                   None if k_norm is None else k_norm.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0], pos.data_ptr(), None if depth is None else depth.data_ptr(),
+        self._call("nwc_kv_append", L.lib.nwc_kv_append, self._ref, layer, qkv.data_ptr(), qkv.stride(0), T, n_q, None if q_norm is None else q_norm.data_ptr(),
+                   None if k_norm is None else k_norm.data_ptr(), cos.data_ptr(), sin.data_ptr(), rows, pos.data_ptr(), None if depth is None else depth.data_ptr(),
                    eps, out.data_ptr(), self._status)
         return out
 
@@ -122,7 +128,7 @@ class KVCache:
         if hd != self.head_dim or n_q % self.n_kv or q.stride(1) != hd: raise ValueError(f"q is [T, n_q, {self.head_dim}] with n_q a multiple of {self.n_kv} and a token's heads side by side")
         if (visible is None) != (depth is None): raise ValueError("visible and depth come together (draft_tree makes them)")
         if visible is not None:
-            if T > 1024: raise ValueError(f"a draft tree has at most 1024 tokens, not {T}")
+            if T > MAX_TREE: raise ValueError(f"a draft tree has at most {MAX_TREE} tokens, not {T}")
             self._int32(visible, T * ((T + 31) // 32), "visible"); self._int32(depth, T, "depth")
         self._int32(pos, 1, "pos")
         self._layer(layer)
@@ -132,7 +138,7 @@ class KVCache:
             with torch.cuda.device(self.device): need = self._need[T, n_q] = L.lib.nwc_kv_attention_workspace(self._ref, T, n_q)
         # a workspace of the call's own: the allocator keeps it from calls on other streams, a graph keeps it in its pool
         work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-        self._call("nwc_kv_attention", L.lib.nwc_kv_attention, layer, q.data_ptr(), q.stride(0), T, n_q, pos.data_ptr(), None if visible is None else visible.data_ptr(),
+        self._call("nwc_kv_attention", L.lib.nwc_kv_attention, self._ref, layer, q.data_ptr(), q.stride(0), T, n_q, pos.data_ptr(), None if visible is None else visible.data_ptr(),
                    None if depth is None else depth.data_ptr(), 1.0 / math.sqrt(hd) if scale is None else float(scale), out.data_ptr(), None if work is None else work.data_ptr(), need, self._status)
         return out
 
@@ -144,9 +150,9 @@ class KVCache:
         if not self.window and first + count > self.capacity: raise ValueError(f"positions {first} .. {first + count - 1} are outside a cache of {self.capacity}")
         if self.window and first + count - max(first, self.sinks) > self.capacity - self.sinks: raise ValueError(f"{count} positions do not lie in a ring of {self.capacity - self.sinks} at the same time")
         self._layer(layer)
-        k = torch.empty((self.n_kv, count, self.head_dim), dtype=torch.bfloat16, device=self.device)
-        v = torch.empty_like(k)
-        self._call("nwc_kv_read", L.lib.nwc_kv_read, layer, first, count, k.data_ptr(), v.data_ptr())
+        shape = (self.n_kv, count, self.head_dim)
+        k, v = self._bf16.new_empty(shape), self._bf16.new_empty(shape)
+        self._call("nwc_kv_read", L.lib.nwc_kv_read, self._ref, layer, first, count, k.data_ptr(), v.data_ptr())
         return k, v
 
     def commit(self, pos, path, count, tokens=None):
@@ -155,8 +161,8 @@ class KVCache:
         told apart from a wrong path).  The caller then advances pos by count."""
         if path.dim() != 1: raise ValueError("path is a vector of draft numbers")
         self._int32(path, path.numel(), "path"); self._int32(count, 1, "count"); self._int32(pos, 1, "pos")
-        if tokens is None: tokens = min(1024, self.capacity - self.sinks - self.window + 1 if self.window else self.capacity)
-        self._call("nwc_kv_commit", L.lib.nwc_kv_commit, None, tokens, pos.data_ptr(), path.data_ptr(), count.data_ptr(), min(path.numel(), tokens), self._status)
+        if tokens is None: tokens = min(MAX_TREE, self.capacity - self.sinks - self.window + 1 if self.window else self.capacity)
+        self._call("nwc_kv_commit", L.lib.nwc_kv_commit, self._ref, tokens, pos.data_ptr(), path.data_ptr(), count.data_ptr(), min(path.numel(), tokens), self._status)
 
     def check(self):
         """Waits for the device; raises when a call since the last check met one of STATUS_TEXT."""
@@ -165,26 +171,25 @@ class KVCache:
             self.status.zero_()
             raise RuntimeError("key/value cache: " + "; ".join(text for bit, text in STATUS_TEXT if bits & bit))
 
-    # ---- helpers ----
+    # ---- helpers (a call of one token takes microseconds on the device: what every call checks is kept to plain comparisons) ----
     def _tokens(self, t, dims, name):
-        if t.dim() != dims or t.dtype != torch.bfloat16 or t.device != self.device or t.stride(-1) != 1 or t.stride(0) % 8 or t.data_ptr() % 16:
+        if t.dim() != dims or t.dtype is not BF16 or t.get_device() != self._at or t.stride(-1) != 1 or t.stride(0) % 8 or t.data_ptr() % 16:
             raise ValueError(f"{name} is a {dims}-dimensional bf16 tensor on {self.device}, rows contiguous and 16-byte aligned")
-        if not 0 < t.shape[0] <= 65535: raise ValueError(f"a call takes 1 to 65535 tokens, not {t.shape[0]}")
-        return t.shape
+        shape = t.shape
+        if not 0 < shape[0] <= 65535: raise ValueError(f"a call takes 1 to 65535 tokens, not {shape[0]}")
+        return shape
 
     def _int32(self, t, n, name):
-        if t.dtype != torch.int32 or t.device != self.device or t.numel() != n or not t.is_contiguous(): raise ValueError(f"{name} is int32 with {n} elements on {self.device}")
+        if t.dtype is not INT32 or t.get_device() != self._at or t.numel() != n or not t.is_contiguous(): raise ValueError(f"{name} is int32 with {n} elements on {self.device}")
 
     def _layer(self, layer):
         if not 0 <= layer < self.layers: raise IndexError(f"layer {layer} of a cache of {self.layers}")
 
-    def _call(self, name, fn, layer, *args):
+    def _call(self, name, fn, *args):
         """One library call on the current stream of the cache's device."""
-        head = (self._ref,) if layer is None else (self._ref, layer)
-        index = self.device.index
-        if torch._C._cuda_getDevice() == index: err = fn(torch._C._cuda_getCurrentRawStream(index), *head, *args)
+        if current_device() == self._at: err = fn(raw_stream(self._at), *args)
         else:
-            with torch.cuda.device(index): err = fn(torch._C._cuda_getCurrentRawStream(index), *head, *args)
+            with torch.cuda.device(self._at): err = fn(raw_stream(self._at), *args)
         if err == -1: raise ValueError(f"{name}: the cache ({self.capacity} slots, window {self.window}, {self.sinks} sinks) does not take this call")
         if err: raise RuntimeError(f"{name} error {err}")
 

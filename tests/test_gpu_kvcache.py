@@ -258,6 +258,35 @@ def test_scores_of_any_size(T):
     assert_attention(out, *R.attend(q.double(), k[0], v[0], pos, scale=0.5))
 
 
+@pytest.mark.parametrize("T", [1, 5, 40])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_value_rows_of_very_different_size(T, hd):
+    """Every second position holds values 2^-22 of its neighbours'; the keys make queries prefer the small ones so clearly
+    (scores 60 apart) that the large ones weigh nothing: the small values come out to the usual precision."""
+    from nwc_b200 import KVCache
+    n_q, n_kv, pos = 8, 2, 300
+    g = torch.Generator().manual_seed(T)
+    c = KVCache(n_kv, hd, pos + T, "fp8")
+    small = torch.arange(pos + T) % 2 == 1
+    k = torch.randn(n_kv, pos + T, hd, generator=g, dtype=torch.float64) * 0.1
+    k[:, small, 0] += 8.0; k[:, ~small, 0] -= 8.0
+    v = torch.randn(n_kv, pos + T, hd, generator=g, dtype=torch.float64) * torch.where(small, 2.0 ** -22, 1.0)[:, None].double()
+    held = []
+    for x, t, e in ((k, c.k, c.k_exp), (v, c.v, c.v_exp)):
+        u = R.unit_exponent(x)
+        codes = R.rounded_e4m3(x * torch.exp2(-u.double())[..., None])
+        t[0].copy_(codes.to(torch.float32).to(torch.float8_e4m3fn)); e[0].copy_((u + 127).to(torch.uint8))
+        held.append(codes * torch.exp2(u.double())[..., None])
+    q = torch.randn(T, n_q, hd, generator=g) * 0.1
+    q[:, :, 0] = 4.0 * hd ** 0.5
+    q = q.to(torch.bfloat16)
+    out = c.attend(q.cuda(), at(pos))
+    c.check()
+    want, weight = R.attend(q.double(), held[0], held[1], pos)
+    assert want.abs().max() < 2.0 ** -18
+    assert_attention(out, want, weight)
+
+
 def test_query_rows_may_be_slices():
     n_q, n_kv, hd, pos, T = 8, 2, 128, 90, 20
     c, k, v = filled(n_kv, hd, pos + T, "fp8")
