@@ -285,6 +285,13 @@ int nwc_argmax(void *stream, const uint16_t *logits, uint32_t V, int64_t *cur, i
 int nwc_argmax_tp(void *stream, const uint16_t *logits, uint32_t V, int64_t *cur, int64_t *log, int32_t *pos,
                   int32_t *step, uint32_t log_len, uint32_t max_pos, void *const *buffers, int rank, int world);
 
+/* nwc_add_rmsnorm, nwc_swiglu and the greedy choice for `rows` tokens at once: h, delta, xn [rows][H], gate_up [rows][2 I],
+   a [rows][I], logits [rows][V], best int64[rows] (lowest index wins ties). */
+int nwc_add_rmsnorm_rows(void *stream, const uint16_t *h_in, const uint16_t *delta, uint16_t *h_out, const uint16_t *weight,
+                         float eps, uint32_t H, uint32_t rows, uint16_t *xn);
+int nwc_swiglu_rows(void *stream, const uint16_t *gate_up, uint32_t I, uint32_t rows, uint16_t *a);
+int nwc_argmax_rows(void *stream, const uint16_t *logits, uint32_t V, uint32_t rows, int64_t *best);
+
 /* ---- a cache for long sessions and for several tokens at once (no counterpart in the reference, which leaves the cache to
    Transformers) -------------------------------------------------------------------------------------------------------
 

@@ -69,6 +69,9 @@ _SIGNATURES = {
     "nwc_comm_import": (I, [P, P]),
     "nwc_comm_release": (I, [P]),
     "nwc_comm_slot": (P, [P, U32, I]),
+    "nwc_add_rmsnorm_rows": (I, [P, P, P, P, P, ctypes.c_float, U32, U32, P]),
+    "nwc_swiglu_rows": (I, [P, P, U32, U32, P]),
+    "nwc_argmax_rows": (I, [P, P, U32, U32, P]),
     "nwc_kv_append": (I, [P, P, U32, P, U64, U32, U32, P, P, P, P, U32, P, P, ctypes.c_float, P, P]),
     "nwc_kv_read": (I, [P, P, U32, U32, U32, P, P]),
     "nwc_kv_attention": (I, [P, P, U32, P, U64, U32, U32, P, P, P, ctypes.c_float, P, P, U64, P]),

@@ -48,6 +48,7 @@ struct StoreArgs {
     float eps;
     uint16_t *q_out;
     int *status;
+    uint32_t chunks;             /* kStoreQ passes of query rows that a warp takes one after the other */
 };
 
 /* HD / 8 lanes hold one row, eight numbers each, so a row is one 16-byte load per lane; the rotary partner of a number lives
@@ -78,9 +79,9 @@ __device__ __forceinline__ void unpack8(const uint4 &w, float (&x)[8]) {
 #pragma unroll
     for (int j = 0; j < 4; j++) { x[2 * j] = lo16(u[j]); x[2 * j + 1] = hi16(u[j]); }
 }
-/* x w / norm, turned; `sign` is that of the partner's share in this lane */
+/* x w / norm, turned (s: with the sign of the partner's share in this lane) */
 template <int HD>
-__device__ __forceinline__ void normed_and_turned(float (&y)[8], bool norm, const float (&w)[8], float eps, const float (&c)[8], const float (&s)[8], float sign) {
+__device__ __forceinline__ void normed_and_turned(float (&y)[8], bool norm, const float (&w)[8], float eps, const float (&c)[8], const float (&s)[8]) {
     if (norm) {
         float ss = 0.f;
 #pragma unroll
@@ -90,11 +91,11 @@ __device__ __forceinline__ void normed_and_turned(float (&y)[8], bool norm, cons
         for (int j = 0; j < 8; j++) y[j] *= inv * w[j];
     }
 #pragma unroll
-    for (int j = 0; j < 8; j++) { const float other = Row<HD>::partner(y[j]); y[j] = fmaf(y[j], c[j], sign * other * s[j]); }
+    for (int j = 0; j < 8; j++) { const float other = Row<HD>::partner(y[j]); y[j] = fmaf(y[j], c[j], other * s[j]); }
 }
 /* the same as a sum of two numbers each */
 template <int HD>
-__device__ __forceinline__ void normed_and_turned_exactly(float (&y)[8], float (&low)[8], bool norm, const float (&w)[8], float eps, const float (&c)[8], const float (&s)[8], float sign) {
+__device__ __forceinline__ void normed_and_turned_exactly(float (&y)[8], float (&low)[8], bool norm, const float (&w)[8], float eps, const float (&c)[8], const float (&s)[8]) {
     float inv = 1.f, inv_low = 0.f;
     if (norm) {
         float sh = 0.f, sl = 0.f, e;
@@ -113,7 +114,7 @@ __device__ __forceinline__ void normed_and_turned_exactly(float (&y)[8], float (
 #pragma unroll
     for (int j = 0; j < 8; j++) {
         const float xw = norm ? __fmul_rn(y[j], w[j]) : y[j], other = Row<HD>::partner(xw);
-        float e, h = two_sum(__fmul_rn(xw, c[j]), sign * __fmul_rn(other, s[j]), e);
+        float e, h = two_sum(__fmul_rn(xw, c[j]), __fmul_rn(other, s[j]), e);
         if (norm) {
             const float p = __fmul_rn(h, inv), q = fmaf(h, inv, -p) + fmaf(e, inv, h * inv_low);
             h = __fadd_rn(p, q); e = __fsub_rn(q, __fsub_rn(h, p));
@@ -163,13 +164,13 @@ template <int HD, int ELEM>
 __global__ void __launch_bounds__(256) kv_store_kernel(const StoreArgs a) {
     using R = Row<HD>;
     const uint32_t lane = threadIdx.x & 31u, sub = lane % R::kLanes, side = lane / R::kLanes, d0 = sub * 8u, n_q = a.n_q, n_kv = a.c.n_kv;
-    const uint32_t gq = store_groups<HD>(n_q, kStoreQ), gk = store_groups<HD>(n_kv, kStoreK), gv = store_groups<HD>(n_kv, kStoreV), groups = gq + gk + gv;
+    const uint32_t gq = store_groups<HD>(n_q, kStoreQ * a.chunks), gk = store_groups<HD>(n_kv, kStoreK), gv = store_groups<HD>(n_kv, kStoreV), groups = gq + gk + gv;
     const uint32_t unit = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);           /* (below 2^31: the launcher checks) */
     dependency_sync();
     if (unit >= groups * a.T) return;
     const uint32_t t = unit / groups, group = unit - t * groups;
     const int kind = group < gq ? 0 : group < gq + gk ? 1 : 2;        /* of the whole warp */
-    const uint32_t n = kind ? n_kv : n_q, row0 = kind == 0 ? group * kStoreQ * R::kSide : kind == 1 ? (group - gq) * kStoreK * R::kSide : (group - gq - gk) * kStoreV * R::kSide;
+    const uint32_t n = kind ? n_kv : n_q, row0 = kind == 0 ? group * a.chunks * kStoreQ * R::kSide : kind == 1 ? (group - gq) * kStoreK * R::kSide : (group - gq - gk) * kStoreV * R::kSide;
     const uint16_t *from = a.qkv + (uint64_t)t * a.ldqkv + (uint64_t)(kind == 0 ? 0u : kind == 1 ? n_q : n_q + n_kv) * HD + d0;
     uint4 raw[kStoreQ];
 #pragma unroll
@@ -200,24 +201,37 @@ __global__ void __launch_bounds__(256) kv_store_kernel(const StoreArgs a) {
     unpack8(*reinterpret_cast<const uint4 *>(a.cos_t + at), c);
     unpack8(*reinterpret_cast<const uint4 *>(a.sin_t + at), s);
     if (norm) unpack8(*reinterpret_cast<const uint4 *>((kind ? a.k_norm : a.q_norm) + d0), w);
-    const float sign = sub < R::kLanes / 2 ? -1.f : 1.f;
+    if (sub < R::kLanes / 2) {                                        /* the lower half takes the upper one's numbers negated */
+#pragma unroll
+        for (int j = 0; j < 8; j++) s[j] = -s[j];
+    }
     if (kind == 1) {
         static_assert(kStoreK == 1, "one pass of keys");
         const uint32_t row = row0 + side;
         float y[8], low[8];
         unpack8(raw[0], y);
-        if (ELEM == kKvE4m3) normed_and_turned_exactly<HD>(y, low, norm, w, a.eps, c, s, sign);
-        else normed_and_turned<HD>(y, norm, w, a.eps, c, s, sign);
+        if (ELEM == kKvE4m3) normed_and_turned_exactly<HD>(y, low, norm, w, a.eps, c, s);
+        else normed_and_turned<HD>(y, norm, w, a.eps, c, s);
         store_row<HD, ELEM>(a, a.c.k, a.c.k_exp, (uint64_t)row * a.c.capacity + slot, sub, row < n, y, low);
         return;
     }
+    for (uint32_t chunk = 0; chunk < a.chunks; chunk++) {
+        const uint32_t first = row0 + chunk * kStoreQ * R::kSide + side;
+        uint4 next[kStoreQ];
 #pragma unroll
-    for (uint32_t i = 0; i < kStoreQ; i++) {
-        const uint32_t row = row0 + i * R::kSide + side;
-        float y[8];
-        unpack8(raw[i], y);
-        normed_and_turned<HD>(y, norm, w, a.eps, c, s, sign);
-        if (row < n) *reinterpret_cast<uint4 *>(a.q_out + ((uint64_t)t * n_q + row) * HD + d0) = pack8(y);
+        for (uint32_t i = 0; i < kStoreQ; i++) {
+            const uint32_t row = first + (kStoreQ + i) * R::kSide;
+            next[i] = chunk + 1u < a.chunks && row < n ? __ldcs(reinterpret_cast<const uint4 *>(from + (uint64_t)row * HD)) : make_uint4(0u, 0u, 0u, 0u);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kStoreQ; i++) {
+            const uint32_t row = first + i * R::kSide;
+            float y[8];
+            unpack8(raw[i], y);
+            normed_and_turned<HD>(y, norm, w, a.eps, c, s);
+            if (row < n) *reinterpret_cast<uint4 *>(a.q_out + ((uint64_t)t * n_q + row) * HD + d0) = pack8(y);
+            raw[i] = next[i];
+        }
     }
 }
 
@@ -307,8 +321,11 @@ KvLayer layer_of(const nwc_kv_cache *c, uint32_t layer) {
 }
 
 template <int HD>
-cudaError_t launch_store(int elem, const StoreArgs &a, void *stream) {
-    const uint64_t units = (uint64_t)(store_groups<HD>(a.n_q, kStoreQ) + store_groups<HD>(a.c.n_kv, kStoreK) + store_groups<HD>(a.c.n_kv, kStoreV)) * a.T, blocks = (units + 7u) / 8u;
+cudaError_t launch_store(int elem, const StoreArgs &given, void *stream) {
+    /* more query rows to a warp once there are warps enough: position, cos and sin are read once for them */
+    StoreArgs a = given;
+    a.chunks = (uint64_t)a.T * a.n_q * (HD / 8u) >= 1u << 20 ? 2u : 1u;
+    const uint64_t units = (uint64_t)(store_groups<HD>(a.n_q, kStoreQ * a.chunks) + store_groups<HD>(a.c.n_kv, kStoreK) + store_groups<HD>(a.c.n_kv, kStoreV)) * a.T, blocks = (units + 7u) / 8u;
     if (units > 0x7FFFFFFFull) return cudaErrorInvalidValue;
     const uint32_t threads = units >= 8u ? 256u : (uint32_t)units * 32u;
     return elem == kKvE4m3 ? launch(kv_store_kernel<HD, kKvE4m3>, dim3((uint32_t)blocks), dim3(threads), stream, a)
@@ -325,7 +342,7 @@ NWC_EXPORT int nwc_kv_append(void *stream, const nwc_kv_cache *cache, uint32_t l
     const uint64_t width = (uint64_t)(n_q + 2u * cache->n_kv) * cache->head_dim;
     if (ldqkv < width || ldqkv % 8u) return -1;
     if (!aligned16(qkv) || !aligned16(cos_t) || !aligned16(sin_t) || !aligned16(q_out) || !aligned16(q_norm) || !aligned16(k_norm)) return -1;
-    const StoreArgs a{layer_of(cache, layer), qkv, ldqkv, T, n_q, q_norm, k_norm, cos_t, sin_t, max_pos, pos, depth, eps, q_out, status};
+    const StoreArgs a{layer_of(cache, layer), qkv, ldqkv, T, n_q, q_norm, k_norm, cos_t, sin_t, max_pos, pos, depth, eps, q_out, status, 1u};
     return (int)(cache->head_dim == 64u ? launch_store<64>(cache->elem, a, stream) : cache->head_dim == 128u ? launch_store<128>(cache->elem, a, stream) : launch_store<256>(cache->elem, a, stream));
 }
 
@@ -357,7 +374,7 @@ NWC_EXPORT uint64_t nwc_kv_attention_workspace(const nwc_kv_cache *cache, uint32
     if (!cache || !T || T > NWC_KV_MAX_TOKENS || !n_q || n_q > 65535u || !cache->n_kv || n_q % cache->n_kv) return 0;
     const int sms = nwc_setup();
     if (sms <= 0) return 0;
-    return workspace_bytes(kv_attention_plan(cache->head_dim, cache->n_kv, cache->capacity, cache->window, cache->sinks, T, n_q, sms), T, n_q, cache->head_dim);
+    return workspace_bytes(kv_attention_plan(cache->elem, cache->head_dim, cache->n_kv, cache->capacity, cache->window, cache->sinks, T, n_q, sms), T, n_q, cache->head_dim);
 }
 
 NWC_EXPORT int nwc_kv_attention(void *stream, const nwc_kv_cache *cache, uint32_t layer, const uint16_t *q, uint64_t ldq, uint32_t T, uint32_t n_q,
@@ -369,7 +386,7 @@ NWC_EXPORT int nwc_kv_attention(void *stream, const nwc_kv_cache *cache, uint32_
     if (!(scale > 0.f) || scale > 3e38f) return -1;
     const int sms = nwc_setup();
     if (sms <= 0) return (int)cudaErrorNoDevice;
-    const KvPlan plan = kv_attention_plan(cache->head_dim, cache->n_kv, cache->capacity, cache->window, cache->sinks, T, n_q, sms);
+    const KvPlan plan = kv_attention_plan(cache->elem, cache->head_dim, cache->n_kv, cache->capacity, cache->window, cache->sinks, T, n_q, sms);
     const uint64_t need = workspace_bytes(plan, T, n_q, cache->head_dim);
     if (need && (!workspace || workspace_size < need)) return -1;
     float *part_o = static_cast<float *>(workspace), *part_ml = need ? part_o + (uint64_t)plan.splits * T * n_q * cache->head_dim : nullptr;

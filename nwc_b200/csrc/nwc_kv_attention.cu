@@ -519,9 +519,9 @@ cudaError_t launch_all(cudaStream_t st, const KvAttention &a, const KvPlan &p) {
     const bool in_clusters = p.in_clusters;
     cudaError_t err;
     if (p.many) err = launch_kv_many(st, ELEM, HD, a); else
-    if constexpr (HD == 256) err = in_clusters ? launch_few<HD, ELEM, 1, 1>(st, a) : launch_few<HD, ELEM, 1, 0>(st, a);
-    else if (in_clusters) err = rows > 16u ? launch_few<HD, ELEM, 2, 1>(st, a) : launch_few<HD, ELEM, 1, 1>(st, a);
-    else err = rows > 16u ? launch_few<HD, ELEM, 2, 0>(st, a) : launch_few<HD, ELEM, 1, 0>(st, a);
+    if (in_clusters) err = launch_few<HD, ELEM, 1, 1>(st, a);
+    else if constexpr (HD != 256 && ELEM == kKvE4m3) err = rows > 16u /* the plan lets no more than 32 come here */ ? launch_few<HD, ELEM, 2, 0>(st, a) : launch_few<HD, ELEM, 1, 0>(st, a);
+    else err = launch_few<HD, ELEM, 1, 0>(st, a);
     if (err != cudaSuccess || a.splits == 1u || in_clusters) return err;
     const uint64_t units = (uint64_t)a.T * a.n_q * (HD >= 128 ? HD / 128 : 1);
     /* (an ordinary dependent launch: the join's set-up overlaps the last CTAs; it waits for the whole grid before it reads) */
@@ -531,28 +531,40 @@ template <int HD, int ELEM, int MT, int SHORT> void configure_one() {
     cudaFuncSetAttribute(kv_attention_few_kernel<HD, ELEM, MT, SHORT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Few<HD, ELEM, MT, SHORT>::kSmem);
     if (SHORT) cudaFuncSetAttribute(kv_attention_few_kernel<HD, ELEM, MT, SHORT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
 }
-template <int HD, int MT> void configure_few() {
-    configure_one<HD, kKvBf16, MT, 0>(); configure_one<HD, kKvBf16, MT, 1>(); configure_one<HD, kKvE4m3, MT, 0>(); configure_one<HD, kKvE4m3, MT, 1>();
+template <int HD> void configure_few() {
+    configure_one<HD, kKvBf16, 1, 0>(); configure_one<HD, kKvBf16, 1, 1>(); configure_one<HD, kKvE4m3, 1, 0>(); configure_one<HD, kKvE4m3, 1, 1>();
+    if constexpr (HD != 256) configure_one<HD, kKvE4m3, 2, 0>();
 }
 
 }  // namespace
 
-KvPlan kv_attention_plan(uint32_t head_dim, uint32_t n_kv, uint32_t capacity, uint32_t window, uint32_t sinks, uint32_t T, uint32_t n_q, int sms) {
-    const uint32_t rows = T * (n_q / n_kv), per = head_dim == 256u ? 16u : (rows > 16u ? 32u : 16u);
-    const uint64_t ctas = (uint64_t)n_kv * ((rows + per - 1u) / per), keys = window ? (uint64_t)sinks + window + T - 1u : capacity;
-    KvPlan p{1u, false, head_dim != 256u && rows > kKvFewRows};
+/* Which kernel and how many CTAs (times in us on B200, head_dim 128, eight key/value heads, calls of one kind in a graph):
+     rows per key/value head   keys     e4m3: few / many      bf16: few / many
+     32                        32768    36 / 45               47 / 36
+     32                        131072   104 / 149             118 / 91
+     32                        4096     32 / 16               34 / 14
+   The many-rows kernel multiplies 128 rows whatever there are, on tensor cores that make nothing of it, but it takes a while to
+   fill and widens e4m3 rows at a rate of its own: the few-rows kernel takes up to 16 rows, and up to 32 of a long e4m3 cache. */
+KvPlan kv_attention_plan(int elem, uint32_t head_dim, uint32_t n_kv, uint32_t capacity, uint32_t window, uint32_t sinks, uint32_t T, uint32_t n_q, int sms) {
+    const uint32_t rows = T * (n_q / n_kv);
+    const uint64_t keys = window ? (uint64_t)sinks + window + T - 1u : capacity;
+    const bool longer = keys > kKvShortKeys;
+    KvPlan p{1u, false, head_dim != 256u && rows > (elem == kKvE4m3 && longer ? 32u : 16u)};
     if (p.many) {
         /* a CTA per SM, each with at least two tiles of 128 keys */
-        const uint64_t ctas = (uint64_t)n_kv * ((rows + 255u) / 256u), keys = window ? (uint64_t)sinks + window + (T < 256u ? T : 256u) : capacity;
-        const uint64_t most = (keys + 255u) / 256u, want = ctas < (uint64_t)sms ? (uint64_t)sms / ctas : 1u;
+        const uint64_t ctas = (uint64_t)n_kv * ((rows + 255u) / 256u), seen = window ? (uint64_t)sinks + window + (T < 256u ? T : 256u) : capacity;
+        const uint64_t most = (seen + 255u) / 256u, want = ctas < (uint64_t)sms ? (uint64_t)sms / ctas : 1u;
         p.splits = (uint32_t)(want < most ? want : most);
         return p;
     }
+    const uint32_t per = head_dim == 256u || rows <= 16u ? 16u : 32u;
+    const uint64_t ctas = (uint64_t)n_kv * ((rows + per - 1u) / per);
     if (ctas >= (uint64_t)sms * 2u) return p;
-    if (keys <= kKvShortKeys) {
-        /* clusters of 2^k CTAs, a tile of 16 keys for each of their four warps, as long as the GPU has room for them */
+    if (!longer) {
+        /* Clusters of 2^k CTAs, a tile of 16 keys for each of their four warps, as long as the GPU has room for them side by
+           side (sixteen clusters of sixteen one after the other: 34 us where eight are 13). */
         p.in_clusters = true;
-        while (p.splits < 16u && (uint64_t)p.splits * 64u < keys && ctas * p.splits < (uint64_t)sms) p.splits *= 2u;
+        while (p.splits < 16u && (uint64_t)p.splits * 64u < keys && ctas * p.splits * 2u <= (uint64_t)sms * 5u / 4u) p.splits *= 2u;
         return p;
     }
     /* no CTA below a tile for each of its warps */
@@ -566,7 +578,7 @@ cudaError_t launch_kv_attention(cudaStream_t st, int elem, uint32_t head_dim, co
     return head_dim == 64u ? launch_all<64, kKvBf16>(st, a, p) : head_dim == 128u ? launch_all<128, kKvBf16>(st, a, p) : launch_all<256, kKvBf16>(st, a, p);
 }
 
-void configure_kv_kernels() { configure_kv_many(); configure_few<64, 1>(); configure_few<64, 2>(); configure_few<128, 1>(); configure_few<128, 2>(); configure_few<256, 1>(); }
+void configure_kv_kernels() { configure_kv_many(); configure_few<64>(); configure_few<128>(); configure_few<256>(); }
 
 int read_kv_status(bool clear) {
     int v = 0;

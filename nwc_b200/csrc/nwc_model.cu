@@ -76,6 +76,23 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_kernel(const uint16_t *h_in,
     }
 }
 
+/* The same for rows of several tokens, one CTA each (h may be h_in). */
+__global__ void __launch_bounds__(1024) add_rmsnorm_rows_kernel(const uint16_t *h_in, const uint16_t *__restrict__ delta, uint16_t *h, const uint16_t *__restrict__ weight,
+                                                                 float eps, uint32_t H, uint16_t *__restrict__ xn) {
+    __shared__ float red[32];
+    const uint64_t row = (uint64_t)blockIdx.x * H;
+    dependency_sync();
+    float ss = 0.f;
+    for (uint32_t i = threadIdx.x; i < H; i += blockDim.x) {
+        float v = bf2f(h_in[row + i]);
+        if (delta) v = bfround(v + bf2f(delta[row + i]));
+        if (delta || h != h_in) h[row + i] = f2bf(v);
+        ss += v * v;
+    }
+    const float inv = rsqrtf(block_sum(ss, red) / (float)H + eps);
+    for (uint32_t i = threadIdx.x; i < H; i += blockDim.x) xn[row + i] = f2bf(bf2f(weight[i]) * bfround(bf2f(h[row + i]) * inv));
+}
+
 /* One CTA per query head.  qkv = [q heads | k heads | v heads] x head_dim of the current token.
    cos / sin: bf16 [max_pos][head_dim] tables.  Caches: bf16 [n_kv][max_len][head_dim].  pos_ptr: position of the token. */
 __global__ void __launch_bounds__(256) attention_decode_kernel(const uint16_t *__restrict__ qkv, const uint16_t *__restrict__ q_norm, const uint16_t *__restrict__ k_norm,
@@ -365,6 +382,16 @@ __global__ void swiglu_kernel(const uint16_t *__restrict__ gu, uint32_t I, uint1
     if (a32) a32[i] = y;
 }
 
+/* the same for rows of several tokens */
+__global__ void swiglu_rows_kernel(const uint16_t *__restrict__ gu, uint32_t I, uint16_t *__restrict__ a) {
+    const uint32_t i = blockIdx.x * blockDim.x + threadIdx.x;
+    const uint64_t t = blockIdx.y;
+    dependency_sync();
+    if (i >= I) return;
+    const float g = bf2f(gu[t * 2u * I + i]), u = bf2f(gu[t * 2u * I + I + i]);
+    a[t * I + i] = f2bf(bfround(g / (1.f + __expf(-g))) * u);
+}
+
 /* Greedy choice: smallest index of the largest logit.  Every CTA folds its slice into one 64-bit key (order-preserving
    image of the value in the high word, inverted index in the low word) and takes the maximum into a device word; the
    CTA that arrives last writes the token for the next step, logs it, advances pos and step (only while the log and the
@@ -449,6 +476,23 @@ __global__ void __launch_bounds__(256) argmax_kernel(const uint16_t *__restrict_
     }
 }
 
+/* Greedy choice of every row: one CTA per token. */
+__global__ void __launch_bounds__(512) argmax_rows_kernel(const uint16_t *__restrict__ logits, uint32_t V, int64_t *__restrict__ best_of) {
+    __shared__ unsigned long long best_of_warp[16];
+    dependency_sync();
+    const uint16_t *row = logits + (uint64_t)blockIdx.x * V;
+    unsigned long long best = 0ull;
+    for (uint32_t i = threadIdx.x; i < V; i += blockDim.x) { const unsigned long long k = argmax_key(bf2f(row[i]), i); best = k > best ? k : best; }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) { const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o); best = other > best ? other : best; }
+    if ((threadIdx.x & 31) == 0) best_of_warp[threadIdx.x >> 5] = best;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (uint32_t w = 1; w < (blockDim.x >> 5); w++) best = best_of_warp[w] > best ? best_of_warp[w] : best;
+        best_of[blockIdx.x] = (int64_t)(0xFFFFFFFFu - (uint32_t)best);
+    }
+}
+
 bool g_plain_attention = false;          /* tests: route every head size through the general kernel */
 
 template <class... Params, class... Args>
@@ -497,6 +541,22 @@ NWC_EXPORT void nwc_set_plain_attention(int on) { g_plain_attention = on != 0; }
 NWC_EXPORT int nwc_swiglu(void *stream, const uint16_t *gate_up, uint32_t I, uint16_t *a16, float *a32) {
     if (!I) return -1;
     return (int)launch(swiglu_kernel, dim3((I + 255) / 256), dim3(256), 0, stream, gate_up, I, a16, a32);
+}
+
+NWC_EXPORT int nwc_add_rmsnorm_rows(void *stream, const uint16_t *h_in, const uint16_t *delta, uint16_t *h_out, const uint16_t *weight, float eps, uint32_t H,
+                                    uint32_t rows, uint16_t *xn) {
+    if (!H || !rows || !h_in || !h_out || !weight || !xn) return -1;
+    return (int)launch(add_rmsnorm_rows_kernel, dim3(rows), dim3(H >= 4096 ? 1024 : (H >= 1024 ? 512 : 256)), 0, stream, h_in, delta, h_out, weight, eps, H, xn);
+}
+
+NWC_EXPORT int nwc_swiglu_rows(void *stream, const uint16_t *gate_up, uint32_t I, uint32_t rows, uint16_t *a) {
+    if (!I || !rows || rows > 65535u || !gate_up || !a) return -1;
+    return (int)launch(swiglu_rows_kernel, dim3((I + 255) / 256, rows), dim3(256), 0, stream, gate_up, I, a);
+}
+
+NWC_EXPORT int nwc_argmax_rows(void *stream, const uint16_t *logits, uint32_t V, uint32_t rows, int64_t *best) {
+    if (!V || !rows || !logits || !best) return -1;
+    return (int)launch(argmax_rows_kernel, dim3(rows), dim3(512), 0, stream, logits, V, best);
 }
 
 static int run_argmax(void *stream, const uint16_t *logits, uint32_t V, int64_t *cur, int64_t *log, int32_t *pos, int32_t *step, uint32_t log_len,

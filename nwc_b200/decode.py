@@ -14,6 +14,7 @@ import torch
 
 from . import _lib as L
 from . import tp as TP
+from .kvcache import KVCache, draft_tree
 from .presets import PRESETS, DecoderConfig
 from .weight import NWCWeight
 
@@ -197,7 +198,8 @@ def rope_tables(cfg, max_len, device):
 
 
 class DecodeEngine:
-    def __init__(self, weights: DecoderWeights, max_len=1024, device="cuda", dependent_launch=False, tp_group=None, tp_reduce="push", side_tables=False, prefetch_next=True):
+    def __init__(self, weights: DecoderWeights, max_len=1024, device="cuda", dependent_launch=False, tp_group=None, tp_reduce="push", side_tables=False, prefetch_next=True,
+                 kv="bf16", window=0, sinks=0, chunk=0):
         """tp_group: torch.distributed process group of the tensor-parallel ranks (weights.tp_world > 1), else None.
         tp_reduce, how the ranks' partial o / down outputs are summed:
           "push"  the row-parallel matvec stores its partial into every rank's exchange buffer over NVLink and the next
@@ -205,7 +207,12 @@ class DecodeEngine:
           "pull"  one kernel of this library per sum reads the peers' partials over NVLink (also called "peer");
           "nccl"  one NCCL all-reduce per sum.
         prefetch_next: every matvec names the matrix of the matvec after it, whose first bytes then travel to L2 across the
-        kernel boundary (layout-2 matrices)."""
+        kernel boundary (layout-2 matrices).
+        kv, window, sinks, chunk: any of them off its default keeps keys and values in a KVCache instead of plain bf16 arrays:
+        kv = "fp8" quantises them as they are written; window > 0 lets a token see the last `window` positions and the first
+        `sinks` (the cache then holds that many slots, max_len bounds the positions only); chunk > 0 is the most tokens that
+        extend(), verify() and prefill(chunked) hand over at once.  Keys are then rounded once on their way into the cache
+        (the plain arrays round after every operation, as Transformers does)."""
         L.require_cuda()
         self.prefetch_next = bool(prefetch_next)
         self.dependent_launch = bool(dependent_launch)
@@ -239,8 +246,13 @@ class DecodeEngine:
         self.gu = bf(2 * c.intermediate)
         self.logits = bf(c.vocab)                                   # this rank's vocabulary rows
         self.logits_all = bf(c.vocab * self.tp_world) if self.tp_world > 1 else self.logits
-        self.k_cache = torch.zeros(c.layers, c.n_kv, max_len, c.head_dim, dtype=torch.bfloat16, device=device)
-        self.v_cache = torch.zeros_like(self.k_cache)
+        self.cache, self.chunk = None, int(chunk)
+        if kv != "bf16" or window or sinks or chunk:
+            if self.chunk < 0: raise ValueError("chunk is not negative")
+            self.cache = KVCache(c.n_kv, c.head_dim, sinks + window + max(self.chunk, 1) - 1 if window else max_len, kv, layers=c.layers, window=window, sinks=sinks, device=device)
+        else:
+            self.k_cache = torch.zeros(c.layers, c.n_kv, max_len, c.head_dim, dtype=torch.bfloat16, device=device)
+            self.v_cache = torch.zeros_like(self.k_cache)
         self.cos, self.sin = rope_tables(c, max_len, device)
         self.cur = torch.zeros(1, dtype=torch.int64, device=device)
         self.pos = torch.zeros(1, dtype=torch.int32, device=device)
@@ -340,6 +352,18 @@ class DecodeEngine:
             L.lib.nwc_set_dependent_launch(0)
         self.launches_per_step = self._count
 
+    def _attend(self, i, l, c, st):
+        """Keys and values of self.qkv enter layer i's cache, its query attends; returns the input of the o projection."""
+        if self.cache is not None:
+            q = self.cache.append(self.qkv, self.pos, self.cos, self.sin, l["q_norm"], l["k_norm"], c.eps, layer=i)
+            out = self.cache.attend(q, self.pos, layer=i)
+            self._count += 2
+            return out
+        self._check(L.lib.nwc_attention_decode(st(), L.ptr(self.qkv), L.ptr(l["q_norm"]), L.ptr(l["k_norm"]), L.ptr(self.cos), L.ptr(self.sin),
+                                               L.ptr(self.k_cache[i]), L.ptr(self.v_cache[i]), L.ptr(self.pos), c.n_q, c.n_kv, c.head_dim, self.max_len,
+                                               c.eps, L.ptr(self.attn), L.ptr(self.status)), "nwc_attention_decode")
+        return self.attn
+
     def _forward_peer(self, c, w, st, e, h, h_next):
         """Tensor-parallel step with the partial sums exchanged through peer memory: every linear takes a ready x, the
         kernel after o / down adds the ranks' partials, the residual and applies the next RMSNorm."""
@@ -348,10 +372,8 @@ class DecodeEngine:
         self._check(L.lib.nwc_add_rmsnorm(st(), L.ptr(h), None, L.ptr(h), L.ptr(w.layers[0]["in_norm"]), c.eps, c.hidden, L.ptr(self.xn), None), "nwc_add_rmsnorm")
         for i, l in enumerate(w.layers):
             self._linear(l["qkv"], self.xn, self.qkv)
-            self._check(L.lib.nwc_attention_decode(st(), L.ptr(self.qkv), L.ptr(l["q_norm"]), L.ptr(l["k_norm"]), L.ptr(self.cos), L.ptr(self.sin),
-                                                   L.ptr(self.k_cache[i]), L.ptr(self.v_cache[i]), L.ptr(self.pos), c.n_q, c.n_kv, c.head_dim, self.max_len,
-                                                   c.eps, L.ptr(self.attn), L.ptr(self.status)), "nwc_attention_decode")
-            self._linear(l["o"], self.attn, self.peers.slot(0))
+            att = self._attend(i, l, c, st)
+            self._linear(l["o"], att, self.peers.slot(0))
             self.peers.allreduce_add_rmsnorm(0, h, h_next, l["post_norm"], c.eps, self.xn); self._count += 1
             h, h_next = h_next, h
             self._linear(l["gate_up"], self.xn, self.gu)
@@ -372,10 +394,8 @@ class DecodeEngine:
             after = (w.layers[i + 1]["qkv"], 1) if i + 1 < len(w.layers) else (w.lm_head, 1)
             self._linear(l["qkv"], None, self.qkv, mode=1, h_in=h, h_out=h_next, norm_w=l["in_norm"], tp_in=1 if i else -1, then=(l["o"], 0))
             h, h_next = h_next, h
-            self._check(L.lib.nwc_attention_decode(st(), L.ptr(self.qkv), L.ptr(l["q_norm"]), L.ptr(l["k_norm"]), L.ptr(self.cos), L.ptr(self.sin),
-                                                   L.ptr(self.k_cache[i]), L.ptr(self.v_cache[i]), L.ptr(self.pos), c.n_q, c.n_kv, c.head_dim, self.max_len,
-                                                   c.eps, L.ptr(self.attn), L.ptr(self.status)), "nwc_attention_decode")
-            self._linear(l["o"], self.attn, None, tp_out=0, then=(l["gate_up"], 1))
+            att = self._attend(i, l, c, st)
+            self._linear(l["o"], att, None, tp_out=0, then=(l["gate_up"], 1))
             self._linear(l["gate_up"], None, self.gu, mode=1, h_in=h, h_out=h_next, norm_w=l["post_norm"], tp_in=0, then=(l["down"], 2))
             h, h_next = h_next, h
             self._linear(l["down"], None, None, mode=2, gate_up=self.gu, tp_out=1, then=after)
@@ -396,10 +416,8 @@ class DecodeEngine:
             after = (w.layers[i + 1]["qkv"], 1) if i + 1 < len(w.layers) else (w.lm_head, 1)
             self._linear(l["qkv"], None, self.qkv, mode=1, h_in=h, delta=delta, h_out=h_next, norm_w=l["in_norm"], then=(l["o"], 0))
             h, h_next = h_next, h
-            self._check(L.lib.nwc_attention_decode(st(), L.ptr(self.qkv), L.ptr(l["q_norm"]), L.ptr(l["k_norm"]), L.ptr(self.cos), L.ptr(self.sin),
-                                                   L.ptr(self.k_cache[i]), L.ptr(self.v_cache[i]), L.ptr(self.pos), c.n_q, c.n_kv, c.head_dim, self.max_len,
-                                                   c.eps, L.ptr(self.attn), L.ptr(self.status)), "nwc_attention_decode")
-            self._linear(l["o"], self.attn, self.proj, then=(l["gate_up"], 1))
+            att = self._attend(i, l, c, st)
+            self._linear(l["o"], att, self.proj, then=(l["gate_up"], 1))
             self._all_reduce(self.proj)
             self._linear(l["gate_up"], None, self.gu, mode=1, h_in=h, delta=self.proj, h_out=h_next, norm_w=l["post_norm"], then=(l["down"], 2))
             h, h_next = h_next, h
@@ -438,13 +456,92 @@ class DecodeEngine:
         """After a synchronise: the position must have stayed inside the KV cache and no bounded wait inside a kernel
         (bulk copy, peer rank) may have run out - a step that did is not a valid token."""
         if int(self.status.item()): raise RuntimeError("decode position left the KV cache")
+        if self.cache is not None: self.cache.check()
         st = L.lib.nwc_kernel_status(1)
         if st: raise RuntimeError(f"a bounded wait inside a kernel gave up (status {st}: 2 = bulk copy, 3 = a tensor-parallel rank did not answer)")
 
-    def prefill(self, prompt_ids):
-        """Feed the prompt token by token through the decode step (teacher forcing); returns the first generated token
-        id as a device tensor.  Positions restart at 0."""
+    # ---- several tokens at once (engines with a chunk) ----
+    def _rows(self, tokens, visible=None, depth=None):
+        """One pass of T tokens at positions pos .. pos + T - 1; returns the greedy next token after each, int64 [T].  Every
+        kernel is the T-row form of the decode step's."""
+        c, w, st = self.cfg, self.w, L.stream
+        if self.cache is None or not self.chunk: raise ValueError("build the engine with chunk > 0 to hand over several tokens at once")
+        if self.tp_world > 1: raise NotImplementedError("several tokens at once run on one GPU")
+        T = tokens.numel()
+        if not 0 < T <= self.chunk: raise ValueError(f"{T} tokens at once; the engine takes 1 to {self.chunk}")
+        h = w.embed.gather(tokens)
+        fresh = lambda width: torch.empty(T, width, dtype=torch.bfloat16, device=self.device)
+        xn, delta = fresh(c.hidden), None
+        def norm(weight):
+            self._check(L.lib.nwc_add_rmsnorm_rows(st(), L.ptr(h), L.ptr(delta), L.ptr(h), L.ptr(weight), c.eps, c.hidden, T, L.ptr(xn)), "nwc_add_rmsnorm_rows")
+        def linear(weight, x):
+            y = weight.linear_prefill(x)
+            return torch.nn.functional.linear(x, weight.dense()) if y is None else y
+        for i, l in enumerate(w.layers):
+            norm(l["in_norm"])
+            q = self.cache.append(linear(l["qkv"], xn), self.pos, self.cos, self.sin, l["q_norm"], l["k_norm"], c.eps, depth=depth, layer=i)
+            delta = linear(l["o"], self.cache.attend(q, self.pos, visible=visible, depth=depth, layer=i))
+            norm(l["post_norm"])
+            gate_up, act = linear(l["gate_up"], xn), fresh(c.intermediate)
+            self._check(L.lib.nwc_swiglu_rows(st(), L.ptr(gate_up), c.intermediate, T, L.ptr(act)), "nwc_swiglu_rows")
+            delta = linear(l["down"], act)
+        norm(w.final_norm)
+        self.logits_rows = linear(w.lm_head, xn)
+        best = torch.empty(T, dtype=torch.int64, device=self.device)
+        self._check(L.lib.nwc_argmax_rows(st(), L.ptr(self.logits_rows), c.vocab, T, L.ptr(best)), "nwc_argmax_rows")
+        return best
+
+    def extend(self, token_ids):
+        """Feed tokens at the current position, `chunk` at a time; returns the greedy next token after each (int64, on the
+        device).  The last one becomes the current token."""
+        tokens = torch.as_tensor(token_ids, dtype=torch.int64, device=self.device).reshape(-1)
+        pos = int(self.pos.item())
+        if not tokens.numel(): raise ValueError("no tokens")
+        if pos + tokens.numel() > self.max_len: raise ValueError(f"{tokens.numel()} more tokens from position {pos} do not fit {self.max_len}")
+        out = []
+        for part in tokens.split(max(self.chunk, 1)):
+            out.append(self._rows(part)); self.pos += part.numel()
+        out = torch.cat(out)
+        self.cur.copy_(out[-1:])
+        return out
+
+    def verify(self, drafts, parents):
+        """One step of speculative decoding.  drafts: proposed token ids; parents[i] < i: the draft that draft i continues, -1 =
+        the current token.  The current token and all drafts run at once (at most `chunk` together), each seeing its
+        ancestors; the longest path of drafts that greedy decoding would have chosen is kept in the cache.  Returns the new
+        tokens: the accepted drafts and the one that follows them (at least one), which becomes the current token."""
+        drafts = [int(t) for t in drafts]
+        if len(drafts) != len(parents): raise ValueError("every draft has a parent")
+        visible, depth = draft_tree([-1] + [int(p) + 1 for p in parents], self.device)
+        start, pos = int(self.step_no.item()), int(self.pos.item())
+        deepest = int(depth.max())
+        if pos + len(drafts) + 1 > self.max_len or start + deepest + 1 > self.log.numel(): raise ValueError(f"{len(drafts)} drafts from position {pos} do not fit {self.max_len}")
+        tokens = torch.cat([self.cur, torch.tensor(drafts, dtype=torch.int64, device=self.device)])
+        best = self._rows(tokens, visible, depth)
+        greedy = best.tolist()                                          # (waits for the device)
+        path, new = [0], [greedy[0]]
+        while True:
+            child = next((i + 1 for i, p in enumerate(parents) if int(p) + 1 == path[-1] and drafts[i] == new[-1]), None)
+            if child is None: break
+            path.append(child); new.append(greedy[child])
+        n = torch.tensor([len(path)], dtype=torch.int32, device=self.device)
+        self.cache.commit(self.pos, torch.tensor(path, dtype=torch.int32, device=self.device), n, tokens=tokens.numel())
+        self.pos += n
+        self.log[start:start + len(new)] = torch.tensor(new, dtype=torch.int64, device=self.device)
+        self.step_no += len(new)
+        self.cur.fill_(new[-1])
+        self._check_status()
+        return new
+
+    def prefill(self, prompt_ids, chunked=False):
+        """Feed the prompt token by token through the decode step (teacher forcing), or, chunked, `chunk` tokens at a time;
+        returns the first generated token id as a device tensor.  Positions restart at 0."""
         self.reset()
+        if chunked:
+            self.extend(prompt_ids)
+            torch.cuda.synchronize()
+            self._check_status()
+            return self.cur
         prompt = torch.as_tensor(prompt_ids, dtype=torch.int64, device=self.device).reshape(-1)
         if prompt.numel() > self.max_len: raise ValueError(f"prompt of {prompt.numel()} tokens does not fit the KV cache ({self.max_len})")
         for i in range(prompt.numel()):
