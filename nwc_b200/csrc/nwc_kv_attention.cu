@@ -7,7 +7,7 @@
  *
  * One token reads every visible row once and computes little: the bound is the memory's rate.  So the rows of a key/value
  * head are read once for all of its query rows (T * group of them, 16 or 32 at a time: the M of mma.m16n8k16), the keys are
- * divided over the CTAs of the whole GPU, and every warp streams its own tiles through a ring of bulk copies in shared memory,
+ * divided over the CTAs of the whole GPU, and every warp streams its own tiles through a ring of asynchronous copies in shared memory,
  * deep enough to keep the memory busy.  There is no barrier between the warps of a CTA until their shares are joined.
  *
  * Fragments.  A dot product may add its terms in any order, so the B fragment of K takes the 16-byte piece that a lane reads
@@ -42,6 +42,9 @@ __device__ __forceinline__ void mma16816_half(float (&c)[4], const uint4 &a, uin
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, uint32_t bytes) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory"); }
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ uint32_t pack_half(float a, float b) { uint32_t d; asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(b), "f"(a)); return d; }
 /* four codes -> two f16 pairs (codes 0, 1 and 2, 3): exact */
 __device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t &lo, uint32_t &hi) {
@@ -68,7 +71,7 @@ template <int HD, int ELEM, int MT, int SHORT> struct Few {
        stores in fragment order and the loads in order of dimensions meet different banks */
     static constexpr uint32_t kPitch = (HD / 8u * 10u + 23u) / 32u * 32u + 8u;
     static constexpr uint32_t kRing = larger(kWarps * kStages * kStageBytes, kWarps * kRows * kPitch * 4u);
-    static constexpr uint32_t kQ = kRing, kBars = kQ + kRows * HD * 2u, kPart = kBars + kWarps * kStages * 8u, kQUnit = kPart + 2u * kWarps * kRows * 4u, kShare = (kQUnit + kRows * 4u + 15u) / 16u * 16u;
+    static constexpr uint32_t kQ = kRing, kPart = kQ + kRows * HD * 2u, kQUnit = kPart + 2u * kWarps * kRows * 4u, kShare = (kQUnit + kRows * 4u + 15u) / 16u * 16u;
     static constexpr uint32_t kSmem = kShare + (SHORT ? kRows * (HD + 2u) * 4u + 16u * kRows * 8u : kRows * 8u);
 };
 __device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
@@ -91,14 +94,9 @@ __global__ void __launch_bounds__(32 * Few<HD, ELEM, MT, SHORT>::kWarps, 1) kv_a
     extern __shared__ __align__(128) uint8_t few_raw[];
     const uint32_t ring = smem_addr(few_raw), tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, g = lane >> 2, c = lane & 3u;
     uint8_t *qs = few_raw + F::kQ;                                                  /* Q in fragment order: [kSteps][MT][32 lanes] uint4 */
-    const uint32_t bars = ring + F::kBars, mine = ring + warp * F::kStages * F::kStageBytes, my_bars = bars + warp * F::kStages * 8u;
+    const uint32_t mine = ring + warp * F::kStages * F::kStageBytes;
     float *part_m = reinterpret_cast<float *>(few_raw + F::kPart), *part_l = part_m + kWarps * kRows, *q_unit = reinterpret_cast<float *>(few_raw + F::kQUnit);
     const uint32_t group = a.n_q / a.c.n_kv, rows = a.T * group, kvh = blockIdx.y % a.c.n_kv, row0 = (blockIdx.y / a.c.n_kv) * kRows, split = blockIdx.x;
-    if (lane == 0) {
-        for (uint32_t s = 0; s < F::kStages; s++) mbar_init(my_bars + s * 8u, 1u);
-        mbar_init_fence();
-    }
-    __syncwarp();
     kv_dependency_sync();
     const int32_t pos = *a.pos;
     if (pos < 0 || (uint64_t)pos + a.T > (a.c.window ? 0x7FFFFFFFu : a.c.capacity)) { if (tid == 0) atomicOr(a.status, kKvStatusPosition); return; }
@@ -108,25 +106,35 @@ __global__ void __launch_bounds__(32 * Few<HD, ELEM, MT, SHORT>::kWarps, 1) kv_a
     const uint32_t my_tiles = last_tile - first_tile > warp ? (last_tile - first_tile - warp + kWarps - 1u) / kWarps : 0u;
     auto position = [&](uint32_t i) { return i < span.lead ? i : span.first + (i - span.lead); };
     auto slot_of = [&](uint32_t i) { return kv_slot(position(i), a.c.capacity, a.c.window, a.c.sinks); };
+    /* The copies are 16 bytes per lane.  Pieces of a row change places so that the lanes of a quarter warp, which read K at four
+       pieces of two rows and V at two pieces of four, meet eight different bank groups: piece ^ 4 in odd rows of K, piece ^ (row &
+       6) in V.  (Bulk copies lay the rows down as they are: 63 us for 131071 e4m3 positions where this takes TIME_HERE.) */
+    constexpr uint32_t kCopies = F::kKeys * F::kRowBytes / 512u;      /* per lane and plane */
+    auto k_place = [](uint32_t row, uint32_t piece) { return row * F::kRowBytes + ((F::kRowBytes >= 128u ? piece ^ ((row & 1u) << 2) : piece) << 4); };
+    auto v_place = [](uint32_t row, uint32_t piece) {
+        if (F::kRowBytes >= 128u) return row * F::kRowBytes + ((piece ^ (row & 6u)) << 4);
+        return (row >> 1) * 128u + (((((row & 1u) << 2) | piece) ^ (row & 6u)) << 4);          /* 64-byte rows: two of them share a line */
+    };
     auto issue = [&](uint32_t i) {
         const uint32_t s = i % F::kStages, key0 = (first_tile + warp + i * kWarps) * F::kKeys, n = min(F::kKeys, span.count - key0);
-        const uint32_t dst = mine + s * F::kStageBytes, bar = my_bars + s * 8u;
-        const uint32_t a0 = slot_of(key0);
-        const bool straight = slot_of(key0 + n - 1u) == a0 + n - 1u;                    /* neither the end of the sinks nor of the ring inside */
+        const uint32_t dst = mine + s * F::kStageBytes;
         const uint64_t cell = (uint64_t)kvh * a.c.capacity;
-        if (lane == 0) {
-            mbar_expect(bar, 2u * n * F::kRowBytes);
-            if (straight) {
-                bulk_load(dst, a.c.k + (cell + a0) * F::kRowBytes, n * F::kRowBytes, bar);
-                bulk_load(dst + F::kKeys * F::kRowBytes, a.c.v + (cell + a0) * F::kRowBytes, n * F::kRowBytes, bar);
+        const uint32_t a0 = slot_of(key0);
+        if (n == F::kKeys && slot_of(key0 + n - 1u) == a0 + n - 1u) {                   /* neither the end of the sinks nor of the ring inside */
+            const uint8_t *kf = a.c.k + (cell + a0) * F::kRowBytes + lane * 16u, *vf = a.c.v + (cell + a0) * F::kRowBytes + lane * 16u;
+#pragma unroll
+            for (uint32_t e = 0; e < kCopies; e++) {
+                const uint32_t at = e * 512u + lane * 16u, row = at / F::kRowBytes, piece = (at % F::kRowBytes) >> 4;
+                copy16(dst + k_place(row, piece), kf + e * 512u, 16u);
+                copy16(dst + F::kKeys * F::kRowBytes + v_place(row, piece), vf + e * 512u, 16u);
             }
-        }
-        if (!straight) {
-            __syncwarp();
-            if (lane < n) {
-                const uint64_t row = cell + slot_of(key0 + lane);
-                bulk_load(dst + lane * F::kRowBytes, a.c.k + row * F::kRowBytes, F::kRowBytes, bar);
-                bulk_load(dst + (F::kKeys + lane) * F::kRowBytes, a.c.v + row * F::kRowBytes, F::kRowBytes, bar);
+        } else {
+#pragma unroll
+            for (uint32_t e = 0; e < kCopies; e++) {                                    /* rows behind the last key arrive as zeros: weight 0 times whatever lies there must be 0 */
+                const uint32_t at = e * 512u + lane * 16u, row = at / F::kRowBytes, piece = (at % F::kRowBytes) >> 4;
+                const uint64_t from = (cell + (row < n ? slot_of(key0 + row) : 0u)) * F::kRowBytes + piece * 16u;
+                copy16(dst + k_place(row, piece), a.c.k + from, row < n ? 16u : 0u);
+                copy16(dst + F::kKeys * F::kRowBytes + v_place(row, piece), a.c.v + from, row < n ? 16u : 0u);
             }
         }
     };
@@ -137,7 +145,7 @@ __global__ void __launch_bounds__(32 * Few<HD, ELEM, MT, SHORT>::kWarps, 1) kv_a
         const uint64_t cell = (uint64_t)kvh * a.c.capacity + slot_of(min((first_tile + warp + i * kWarps) * F::kKeys + lane, span.count - 1u));
         k_next = a.c.k_exp[cell]; v_next = a.c.v_exp[cell];
     };
-    for (uint32_t i = 0; i < F::kStages && i < my_tiles; i++) issue(i);
+    for (uint32_t i = 0; i < F::kStages; i++) { if (i < my_tiles) issue(i); copies_commit(); }
     units(0u);
     /* Q: the 16-byte piece of a row that meets the K piece of lane c, in the order its words are used.  A row is one warp's. */
     for (uint32_t r = warp; r < kRows; r += kWarps) {
@@ -192,19 +200,13 @@ __global__ void __launch_bounds__(32 * Few<HD, ELEM, MT, SHORT>::kWarps, 1) kv_a
             for (uint32_t e = 0; e < 4u; e++) o[i][j][e] = 0.f;
 #pragma unroll
     for (uint32_t i = 0; i < 2u * MT; i++) { m[i] = -INFINITY; l[i] = 0.f; }
-    bool alive = true;                                                                  /* a wait that gave up: no new copies, but those in flight are waited for */
-    uint32_t issued = min(F::kStages, my_tiles);
-    for (uint32_t it = 0; it < issued; it++) {
+    for (uint32_t it = 0; it < my_tiles; it++) {
         const uint32_t s = it % F::kStages, key0 = (first_tile + warp + it * kWarps) * F::kKeys, n = min(F::kKeys, span.count - key0);
         const uint32_t kt = mine + s * F::kStageBytes, vt = kt + F::kKeys * F::kRowBytes;
         const uint32_t k_byte = k_next, v_byte = v_next;
-        alive = mbar_wait(my_bars + s * 8u, (it / F::kStages) & 1u) && alive;
-        if (!alive) continue;
+        copies_wait<F::kStages - 1u>();                                                 /* this lane's copies of the tile ... */
+        __syncwarp();                                                                   /* ... and the other lanes' */
         units(it + 1u);
-        if (n < F::kKeys) {                                                             /* V rows behind the last key: weight 0 times whatever lies there must be 0 */
-            for (uint32_t e = lane; e < (F::kKeys - n) * (F::kRowBytes / 16u); e += 32u) asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vt + n * F::kRowBytes + e * 16u), "r"(0u) : "memory");
-            __syncwarp();
-        }
         /* scores */
         float sc[MT][kNT][4];
 #pragma unroll
@@ -223,7 +225,7 @@ __global__ void __launch_bounds__(32 * Few<HD, ELEM, MT, SHORT>::kWarps, 1) kv_a
                 for (uint32_t i = 0; i < MT; i++) qf[st][i] = reinterpret_cast<const uint4 *>(qs)[((pc * kStepsPerPiece + st) * MT + i) * 32u + lane];
 #pragma unroll
             for (uint32_t j = 0; j < kNT; j++) {
-                const uint4 w = lds128(kt + (j * 8u + g) * F::kRowBytes + pc * 64u + c * 16u);
+                const uint4 w = lds128(kt + j * 8u * F::kRowBytes + k_place(g, pc * 4u + c));
                 const uint32_t u[4] = {w.x, w.y, w.z, w.w};
                 if (ELEM == kKvE4m3) {
 #pragma unroll
@@ -327,16 +329,16 @@ __global__ void __launch_bounds__(32 * Few<HD, ELEM, MT, SHORT>::kWarps, 1) kv_a
                 pf[i] = make_uint4(pack(sc[i][2 * h][0], sc[i][2 * h][1]), pack(sc[i][2 * h][2], sc[i][2 * h][3]),
                                    pack(sc[i][2 * h + 1][0], sc[i][2 * h + 1][1]), pack(sc[i][2 * h + 1][2], sc[i][2 * h + 1][3]));
             }
-            const uint32_t v0 = vt + (h * 16u + 2u * c) * F::kRowBytes;
+            const uint32_t v0 = vt + h * 16u * F::kRowBytes;
             constexpr uint32_t kPieceDims = ELEM == kKvE4m3 ? (HD == 64 ? 8u : 16u) : 8u, kVPieces = HD / (8u * kPieceDims);
 #pragma unroll
             for (uint32_t pc = 0; pc < kVPieces; pc++) {
                 uint32_t w[4][4];                                                       /* [key][word] */
 #pragma unroll
                 for (uint32_t e = 0; e < 4u; e++) {
-                    const uint32_t from = v0 + ((e & 1u) + (e >> 1) * 8u) * F::kRowBytes;
-                    if (ELEM == kKvE4m3 && HD == 64) { const uint2 x = lds64(from + g * 8u); w[e][0] = x.x; w[e][1] = x.y; }
-                    else { const uint4 x = lds128(from + pc * 128u + g * 16u); w[e][0] = x.x; w[e][1] = x.y; w[e][2] = x.z; w[e][3] = x.w; }
+                    const uint32_t row = 2u * c + (e & 1u), below = (e >> 1) * 8u * F::kRowBytes;       /* (eight rows on, the places are the same) */
+                    if (ELEM == kKvE4m3 && HD == 64) { const uint2 x = lds64(v0 + below + v_place(row, g >> 1) + (g & 1u) * 8u); w[e][0] = x.x; w[e][1] = x.y; }
+                    else { const uint4 x = lds128(v0 + below + v_place(row, pc * 8u + g)); w[e][0] = x.x; w[e][1] = x.y; w[e][2] = x.z; w[e][3] = x.w; }
                 }
                 if (ELEM == kKvE4m3 && wide) {
 #pragma unroll
@@ -370,9 +372,9 @@ __global__ void __launch_bounds__(32 * Few<HD, ELEM, MT, SHORT>::kWarps, 1) kv_a
                 }
             }
         }
-        async_proxy_fence();
         __syncwarp();
-        if (issued < my_tiles) issue(issued++);
+        if (it + F::kStages < my_tiles) issue(it + F::kStages);
+        copies_commit();
     }
     /* join the warps: common maximum, then sums and outputs rescaled to it, in warp order */
 #pragma unroll
