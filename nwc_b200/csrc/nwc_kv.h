@@ -97,7 +97,6 @@ KvPlan kv_attention_plan(int elem, uint32_t head_dim, uint32_t n_kv, uint32_t ca
 cudaError_t launch_kv_attention(cudaStream_t st, int elem, uint32_t head_dim, const KvAttention &a, const KvPlan &plan);
 cudaError_t launch_kv_many(cudaStream_t st, int elem, uint32_t head_dim, const KvAttention &a);
 void configure_kv_many();
-int read_kv_many_status(bool clear);
 void configure_kv_kernels();                 /* per-device shared-memory opt-ins */
 int read_kv_status(bool clear);              /* 0, or 2 when a bounded wait gave up */
 

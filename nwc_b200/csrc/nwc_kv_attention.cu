@@ -457,38 +457,53 @@ __global__ void __launch_bounds__(32 * Few<HD, ELEM, MT, SHORT>::kWarps, 1) kv_a
     }
 }
 
-/* The shares of the splits joined in split order: one warp per output row and 128 (64) of its dimensions. */
+/* The shares of the splits joined: `ways` warps per output row and 128 (64) of its dimensions take the splits in turn, and meet
+   in shared memory in their order.  (One warp alone reads one share after another: 148 of them took 22 us.) */
 template <int HD>
-__global__ void __launch_bounds__(128) kv_attention_join_kernel(const KvAttention a) {
-    constexpr uint32_t kPer = HD >= 128 ? 4u : 2u, kWarpsPerRow = HD / (32u * kPer);
-    const uint32_t lane = threadIdx.x & 31u;
-    const uint64_t unit = (uint64_t)blockIdx.x * 4u + (threadIdx.x >> 5), lines = (uint64_t)a.T * a.n_q;
+__global__ void __launch_bounds__(256) kv_attention_join_kernel(const KvAttention a, uint32_t ways) {
+    constexpr uint32_t kPer = HD >= 128 ? 4u : 2u, kPieces = HD / (32u * kPer);
+    __shared__ float sums[8][32u * kPer + 1u];
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, way = warp % ways;
+    const uint64_t unit = (uint64_t)blockIdx.x * (8u / ways) + warp / ways, lines = (uint64_t)a.T * a.n_q, line = unit / kPieces;
+    const uint32_t d = (uint32_t)(unit % kPieces) * 32u * kPer + lane * kPer;
     kv_dependency_sync();
-    if (unit >= lines * kWarpsPerRow) return;
-    const uint64_t line = unit / kWarpsPerRow;
-    const uint32_t d = (uint32_t)(unit % kWarpsPerRow) * 32u * kPer + lane * kPer;
     const int32_t pos = *a.pos;
     if (pos < 0 || (uint64_t)pos + a.T > (a.c.window ? 0x7FFFFFFFu : a.c.capacity)) return;
-    float top = -INFINITY;
-    for (uint32_t s = lane; s < a.splits; s += 32u) top = fmaxf(top, __ldcg(a.part_ml + ((uint64_t)s * lines + line) * 2u));
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-    float total = 0.f, sum[kPer];
+    const bool live = line < lines;
+    float top = -INFINITY, total = 0.f, sum[kPer];
 #pragma unroll
     for (uint32_t j = 0; j < kPer; j++) sum[j] = 0.f;
-#pragma unroll 4
-    for (uint32_t s = 0; s < a.splits; s++) {
-        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(a.part_ml) + (uint64_t)s * lines + line);
-        const float *from = a.part_o + ((uint64_t)s * lines + line) * HD + d;
-        float x[kPer];
-        if (kPer == 4u) { const float4 v = __ldcg(reinterpret_cast<const float4 *>(from)); x[0] = v.x; x[1] = v.y; x[kPer - 2] = v.z; x[kPer - 1] = v.w; }
-        else { const float2 v = __ldcg(reinterpret_cast<const float2 *>(from)); x[0] = v.x; x[1] = v.y; }
-        if (ml.x == -INFINITY) continue;
-        const float f = exp2_fast(ml.x - top);
-        total = fmaf(ml.y, f, total);
+    if (live) {
+        for (uint32_t s = lane; s < a.splits; s += 32u) top = fmaxf(top, __ldcg(a.part_ml + ((uint64_t)s * lines + line) * 2u));
 #pragma unroll
-        for (uint32_t j = 0; j < kPer; j++) sum[j] = fmaf(x[j], f, sum[j]);
+        for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+#pragma unroll 4
+        for (uint32_t s = way; s < a.splits; s += ways) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2 *>(a.part_ml) + (uint64_t)s * lines + line);
+            const float *from = a.part_o + ((uint64_t)s * lines + line) * HD + d;
+            float x[kPer];
+            if (kPer == 4u) { const float4 v = __ldcg(reinterpret_cast<const float4 *>(from)); x[0] = v.x; x[1] = v.y; x[kPer - 2] = v.z; x[kPer - 1] = v.w; }
+            else { const float2 v = __ldcg(reinterpret_cast<const float2 *>(from)); x[0] = v.x; x[1] = v.y; }
+            if (ml.x == -INFINITY) continue;                                            /* (such a share has no outputs) */
+            const float f = exp2_fast(ml.x - top);
+            total = fmaf(ml.y, f, total);
+#pragma unroll
+            for (uint32_t j = 0; j < kPer; j++) sum[j] = fmaf(x[j], f, sum[j]);
+        }
     }
+    if (ways > 1u) {
+#pragma unroll
+        for (uint32_t j = 0; j < kPer; j++) sums[warp][lane * kPer + j] = sum[j];
+        if (lane == 0) sums[warp][32u * kPer] = total;
+        __syncthreads();
+        if (way) return;
+        for (uint32_t w = 1; w < ways; w++) {
+            total += sums[warp + w][32u * kPer];
+#pragma unroll
+            for (uint32_t j = 0; j < kPer; j++) sum[j] += sums[warp + w][lane * kPer + j];
+        }
+    }
+    if (!live) return;
     const float r = total == 0.f ? 0.f : 1.f / total;
     uint16_t *to = a.out + line * HD + d;
 #pragma unroll
@@ -526,8 +541,9 @@ cudaError_t launch_all(cudaStream_t st, const KvAttention &a, const KvPlan &p) {
     else err = launch_few<HD, ELEM, 1, 0>(st, a);
     if (err != cudaSuccess || a.splits == 1u || in_clusters) return err;
     const uint64_t units = (uint64_t)a.T * a.n_q * (HD >= 128 ? HD / 128 : 1);
+    const uint32_t ways = a.splits >= 16u ? 8u : a.splits >= 8u ? 4u : 1u, per_block = 8u / ways;
     /* (an ordinary dependent launch: the join's set-up overlaps the last CTAs; it waits for the whole grid before it reads) */
-    return launch(kv_attention_join_kernel<HD>, dim3((uint32_t)((units + 3u) / 4u)), dim3(128), 0, st, true, 1u, a);
+    return launch(kv_attention_join_kernel<HD>, dim3((uint32_t)((units + per_block - 1u) / per_block)), dim3(256), 0, st, true, 1u, a, ways);
 }
 template <int HD, int ELEM, int MT, int SHORT> void configure_one() {
     cudaFuncSetAttribute(kv_attention_few_kernel<HD, ELEM, MT, SHORT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Few<HD, ELEM, MT, SHORT>::kSmem);
@@ -581,13 +597,5 @@ cudaError_t launch_kv_attention(cudaStream_t st, int elem, uint32_t head_dim, co
 }
 
 void configure_kv_kernels() { configure_kv_many(); configure_few<64>(); configure_few<128>(); configure_few<256>(); }
-
-int read_kv_status(bool clear) {
-    int v = 0;
-    if (cudaMemcpyFromSymbol(&v, g_kernel_status, sizeof(int)) != cudaSuccess) return -1;
-    if (clear && v) { const int z = 0; cudaMemcpyToSymbol(g_kernel_status, &z, sizeof(int)); }
-    const int w = read_kv_many_status(clear);
-    return v ? v : w;
-}
 
 }  // namespace nwc

@@ -572,7 +572,7 @@ void configure_kv_many() {
     cudaFuncSetAttribute(kv_attention_many_kernel<128, kKvE4m3>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Many<128, kKvE4m3>::kSmem);
 }
 
-int read_kv_many_status(bool clear) {
+int read_kv_status(bool clear) {
     int v = 0;
     if (cudaMemcpyFromSymbol(&v, g_kernel_status, sizeof(int)) != cudaSuccess) return -1;
     if (clear && v) { const int z = 0; cudaMemcpyToSymbol(g_kernel_status, &z, sizeof(int)); }
