@@ -96,7 +96,7 @@ __global__ void __launch_bounds__(32 * Few<HD, ELEM, MT, SHORT>::kWarps, 1) kv_a
     uint8_t *qs = few_raw + F::kQ;                                                  /* Q in fragment order: [kSteps][MT][32 lanes] uint4 */
     const uint32_t mine = ring + warp * F::kStages * F::kStageBytes;
     float *part_m = reinterpret_cast<float *>(few_raw + F::kPart), *part_l = part_m + kWarps * kRows, *q_unit = reinterpret_cast<float *>(few_raw + F::kQUnit);
-    const uint32_t group = a.n_q / a.c.n_kv, rows = a.T * group, kvh = blockIdx.y % a.c.n_kv, row0 = (blockIdx.y / a.c.n_kv) * kRows, split = blockIdx.x;
+    const uint32_t group = a.n_q / a.c.n_kv, rows = a.T * group, kvh = blockIdx.x % a.c.n_kv, row0 = (blockIdx.x / a.c.n_kv) * kRows, split = blockIdx.y;
     kv_dependency_sync();
     const int32_t pos = *a.pos;
     if (pos < 0 || (uint64_t)pos + a.T > (a.c.window ? 0x7FFFFFFFu : a.c.capacity)) { if (tid == 0) atomicOr(a.status, kKvStatusPosition); return; }
@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(32 * Few<HD, ELEM, MT, SHORT>::kWarps, 1) kv_a
             total = fmaf(part_l[w * kRows + tid], f, total);
             part_m[w * kRows + tid] = f;                                                /* from here on the warp's factor */
         }
-        share_ml[2u * tid] = top; share_ml[2u * tid + 1u] = total;
+        share_ml[2u * tid] = total == total ? top : 0.f; share_ml[2u * tid + 1u] = total;      /* (a query that is not a number has no maximum, but its share counts) */
     }
     __syncthreads();
     for (uint32_t at = tid; at < live * HD; at += 32u * kWarps) {
@@ -519,7 +519,7 @@ cudaError_t launch(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem
     cudaLaunchAttribute attr[2];
     uint32_t n = 0;
     if (dependent) { attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[n++].val.programmaticStreamSerializationAllowed = 1; }
-    if (cluster > 1u) { attr[n].id = cudaLaunchAttributeClusterDimension; attr[n].val.clusterDim.x = cluster; attr[n].val.clusterDim.y = 1; attr[n++].val.clusterDim.z = 1; }
+    if (cluster > 1u) { attr[n].id = cudaLaunchAttributeClusterDimension; attr[n].val.clusterDim.x = 1; attr[n].val.clusterDim.y = cluster; attr[n++].val.clusterDim.z = 1; }
     cfg.attrs = attr; cfg.numAttrs = n;
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
 }
@@ -528,7 +528,7 @@ template <int HD, int ELEM, int MT, int SHORT>
 cudaError_t launch_few(cudaStream_t st, const KvAttention &a) {
     using F = Few<HD, ELEM, MT, SHORT>;
     const uint32_t rows = a.T * (a.n_q / a.c.n_kv), tiles = (rows + F::kRows - 1u) / F::kRows;
-    return launch(kv_attention_few_kernel<HD, ELEM, MT, SHORT>, dim3(a.splits, a.c.n_kv * tiles), dim3(32u * F::kWarps), F::kSmem, st, dependent_launch(), SHORT ? a.splits : 1u, a);
+    return launch(kv_attention_few_kernel<HD, ELEM, MT, SHORT>, dim3(a.c.n_kv * tiles, a.splits), dim3(32u * F::kWarps), F::kSmem, st, dependent_launch(), SHORT ? a.splits : 1u, a);
 }
 template <int HD, int ELEM>
 cudaError_t launch_all(cudaStream_t st, const KvAttention &a, const KvPlan &p) {

@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(Many<HD, ELEM>::kThreads, 1) kv_attention_many
     const uint32_t base = (smem_addr(many_raw) + 1023u) & ~1023u;
     const uint32_t bars = base + F::kBars, full = bars, empty = bars + NS * 8u, q_full = bars + 2u * NS * 8u, s_full = q_full + 16u, p_full = s_full + 16u, o_full = p_full + 16u, tmem_slot = o_full + 16u;
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
-    const uint32_t group = a.n_q / a.c.n_kv, rows = a.T * group, kvh = blockIdx.y % a.c.n_kv, row0 = (blockIdx.y / a.c.n_kv) * 2u * kManyRows, split = blockIdx.x;
+    const uint32_t group = a.n_q / a.c.n_kv, rows = a.T * group, kvh = blockIdx.x % a.c.n_kv, row0 = (blockIdx.x / a.c.n_kv) * 2u * kManyRows, split = blockIdx.y;
     const bool solo = rows - row0 <= kManyRows;
     if (warp == F::kMmaWarp) {
         if (lane == 0) {
@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(Many<HD, ELEM>::kThreads, 1) kv_attention_many
             const uint64_t line = (uint64_t)token * a.n_q + kvh * group + row % group;
             const float r = total == 0.f ? 0.f : 1.f / total;
             float *part = a.splits > 1u ? a.part_o + ((uint64_t)split * a.T * a.n_q + line) * HD : nullptr;
-            if (a.splits > 1u && row_ok) *reinterpret_cast<float2 *>(a.part_ml + ((uint64_t)split * a.T * a.n_q + line) * 2u) = make_float2(n ? top : -INFINITY, total);
+            if (a.splits > 1u && row_ok) *reinterpret_cast<float2 *>(a.part_ml + ((uint64_t)split * a.T * a.n_q + line) * 2u) = make_float2(!n ? -INFINITY : total == total ? top : 0.f /* a query that is not a number has no maximum, but its share counts */, total);
 #pragma unroll
             for (uint32_t ch = 0; ch < HD / 32u; ch++) {
                 if (my_n) { tm_load32(tm_o + ch * 32u, v); tm_wait_load(); tm_hold(v); }
@@ -539,9 +539,8 @@ static EncodeTiledFn encode_tiled() {
 template <int HD, int ELEM>
 static cudaError_t launch_many(cudaStream_t st, const KvAttention &a) {
     const uint64_t rows = (uint64_t)a.T * (a.n_q / a.c.n_kv), pairs = (rows + 2u * kManyRows - 1u) / (2u * kManyRows);
-    if (pairs * a.c.n_kv > 65535u) return cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(a.splits, (uint32_t)(pairs * a.c.n_kv)); cfg.blockDim = dim3(Many<HD, ELEM>::kThreads); cfg.dynamicSmemBytes = Many<HD, ELEM>::kSmem; cfg.stream = st;
+    cfg.gridDim = dim3((uint32_t)(pairs * a.c.n_kv), a.splits); cfg.blockDim = dim3(Many<HD, ELEM>::kThreads); cfg.dynamicSmemBytes = Many<HD, ELEM>::kSmem; cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr; cfg.numAttrs = dependent_launch() ? 1 : 0;

@@ -325,6 +325,54 @@ def test_offsets_beyond_32_bits(elem):
     assert (err <= 2.0 ** -8 * want.abs() + 2.0 ** -6 * weight).all()
 
 
+@pytest.mark.parametrize("n_q,n_kv,hd", [(32, 2, 256), (256, 8, 64)])
+def test_the_most_tokens_of_a_call(n_q, n_kv, hd):
+    """65535 tokens of so many heads that the row tiles pass 65535, each seeing itself alone: its value comes back."""
+    from nwc_b200 import KVCache
+    T = 65535
+    c = KVCache(n_kv, hd, T, "bf16", window=1)
+    c.v.copy_(torch.randn(c.v.shape[2:], device="cuda").to(torch.bfloat16)[None, None].expand_as(c.v))
+    q = torch.ones(T, n_q, hd, dtype=torch.bfloat16, device="cuda")
+    out = c.attend(q, at(7)).view(T, n_q, hd)
+    c.check()
+    slots = (7 + torch.arange(T, device="cuda")) % T
+    assert torch.equal(out, c.v[0, 0][slots][:, None].expand_as(out))
+
+
+@pytest.mark.parametrize("T,pos", [(1, 200), (60, 200), (1, 9000), (5, 9000), (300, 700)])
+def test_queries_that_are_not_finite_spoil_their_own_rows_only(T, pos):
+    n_q, n_kv, hd = 8, 2, 128
+    c, k, v = filled(n_kv, hd, pos + T, "fp8")
+    q = queries(T, n_q, hd)
+    q[0, 3, 5] = float("nan")
+    out = c.attend(q.cuda(), at(pos)).view(T, n_q, hd)
+    c.check()
+    assert torch.isnan(out[0, 3]).all()
+    keep = torch.ones(T, n_q, dtype=torch.bool); keep[0, 3] = False
+    q[0, 3] = 0
+    want, weight = R.attend(q.double(), k[0], v[0], pos)
+    assert_attention(out[keep.cuda()], want[keep], weight[keep])
+
+
+def test_calls_on_other_streams_and_from_two_caches():
+    """A call's workspace is its own: two caches attended from two streams at the same time, many times."""
+    n_q, n_kv, hd, pos = 16, 2, 128, 6000
+    made = [filled(n_kv, hd, pos + 64, "fp8", seed=s) for s in (1, 2)]
+    qs = [queries(T, n_q, hd, seed=T).cuda() for T in (1, 40)]
+    p = at(pos)
+    want = [[c.attend(q, p) for q in qs] for c, _, _ in made]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s): got[i].append([made[i][0].attend(q, p) for q in qs])
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        made[i][0].check()
+        for outs in got[i]: assert all(torch.equal(a, b) for a, b in zip(outs, want[i]))
+
+
 # ---- the operators together ----
 
 @pytest.mark.parametrize("elem", ["bf16", "fp8"])
