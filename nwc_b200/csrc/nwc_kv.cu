@@ -390,6 +390,6 @@ NWC_EXPORT int nwc_kv_attention(void *stream, const nwc_kv_cache *cache, uint32_
     const uint64_t need = workspace_bytes(plan, T, n_q, cache->head_dim);
     if (need && (!workspace || workspace_size < need)) return -1;
     float *part_o = static_cast<float *>(workspace), *part_ml = need ? part_o + (uint64_t)plan.splits * T * n_q * cache->head_dim : nullptr;
-    const KvAttention a{layer_of(cache, layer), q, ldq, T, n_q, pos, visible, depth, scale * 1.4426950408889634f, out, status, part_o, part_ml, plan.splits, layer, cache->layers};
-    return (int)launch_kv_attention((cudaStream_t)stream, cache->elem, cache->head_dim, a, plan);
+    const KvAttention a{layer_of(cache, layer), q, ldq, T, n_q, pos, visible, depth, scale * 1.4426950408889634f, out, status, part_o, part_ml, plan.splits, layer, cache->layers, 0u};
+    return (int)launch_kv_attention((cudaStream_t)stream, cache->elem, cache->head_dim, a, plan, sms);
 }

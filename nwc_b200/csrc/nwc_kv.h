@@ -88,14 +88,15 @@ struct KvAttention {
     float *part_o, *part_ml;
     uint32_t splits;
     uint32_t layer, layers;      /* which layer of how many `c` is */
+    uint32_t pairs;              /* many: units of two row tiles; those behind them have one */
 };
 /* How a call is divided.  It goes by sizes that the host knows (a captured call is replayed at other positions): the most
    keys that the cache can show, not the position. */
 constexpr uint32_t kKvShortKeys = 4096;
 struct KvPlan { uint32_t splits; bool in_clusters, many; };       /* many: the tensor-memory kernel of nwc_kv_many.cu */
 KvPlan kv_attention_plan(int elem, uint32_t head_dim, uint32_t n_kv, uint32_t capacity, uint32_t window, uint32_t sinks, uint32_t T, uint32_t n_q, int sms);
-cudaError_t launch_kv_attention(cudaStream_t st, int elem, uint32_t head_dim, const KvAttention &a, const KvPlan &plan);
-cudaError_t launch_kv_many(cudaStream_t st, int elem, uint32_t head_dim, const KvAttention &a);
+cudaError_t launch_kv_attention(cudaStream_t st, int elem, uint32_t head_dim, const KvAttention &a, const KvPlan &plan, int sms);
+cudaError_t launch_kv_many(cudaStream_t st, int elem, uint32_t head_dim, const KvAttention &a, int sms);
 void configure_kv_many();
 void configure_kv_kernels();                 /* per-device shared-memory opt-ins */
 int read_kv_status(bool clear);              /* 0, or 2 when a bounded wait gave up */

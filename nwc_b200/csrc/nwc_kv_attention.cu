@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(32 * Few<HD, ELEM, MT, SHORT>::kWarps, 1) kv_a
     auto slot_of = [&](uint32_t i) { return kv_slot(position(i), a.c.capacity, a.c.window, a.c.sinks); };
     /* The copies are 16 bytes per lane.  Pieces of a row change places so that the lanes of a quarter warp, which read K at four
        pieces of two rows and V at two pieces of four, meet eight different bank groups: piece ^ 4 in odd rows of K, piece ^ (row &
-       6) in V.  (Bulk copies lay the rows down as they are: 63 us for 131071 e4m3 positions where this takes TIME_HERE.) */
+       6) in V.  (Bulk copies lay the rows down as they are: 63 us for 131071 e4m3 positions where this takes 53.) */
     constexpr uint32_t kCopies = F::kKeys * F::kRowBytes / 512u;      /* per lane and plane */
     auto k_place = [](uint32_t row, uint32_t piece) { return row * F::kRowBytes + ((F::kRowBytes >= 128u ? piece ^ ((row & 1u) << 2) : piece) << 4); };
     auto v_place = [](uint32_t row, uint32_t piece) {
@@ -531,11 +531,11 @@ cudaError_t launch_few(cudaStream_t st, const KvAttention &a) {
     return launch(kv_attention_few_kernel<HD, ELEM, MT, SHORT>, dim3(a.c.n_kv * tiles, a.splits), dim3(32u * F::kWarps), F::kSmem, st, dependent_launch(), SHORT ? a.splits : 1u, a);
 }
 template <int HD, int ELEM>
-cudaError_t launch_all(cudaStream_t st, const KvAttention &a, const KvPlan &p) {
+cudaError_t launch_all(cudaStream_t st, const KvAttention &a, const KvPlan &p, int sms) {
     const uint32_t rows = a.T * (a.n_q / a.c.n_kv);
     const bool in_clusters = p.in_clusters;
     cudaError_t err;
-    if (p.many) err = launch_kv_many(st, ELEM, HD, a); else
+    if (p.many) err = launch_kv_many(st, ELEM, HD, a, sms); else
     if (in_clusters) err = launch_few<HD, ELEM, 1, 1>(st, a);
     else if constexpr (HD != 256 && ELEM == kKvE4m3) err = rows > 16u /* the plan lets no more than 32 come here */ ? launch_few<HD, ELEM, 2, 0>(st, a) : launch_few<HD, ELEM, 1, 0>(st, a);
     else err = launch_few<HD, ELEM, 1, 0>(st, a);
@@ -591,9 +591,9 @@ KvPlan kv_attention_plan(int elem, uint32_t head_dim, uint32_t n_kv, uint32_t ca
     return p;
 }
 
-cudaError_t launch_kv_attention(cudaStream_t st, int elem, uint32_t head_dim, const KvAttention &a, const KvPlan &p) {
-    if (elem == kKvE4m3) return head_dim == 64u ? launch_all<64, kKvE4m3>(st, a, p) : head_dim == 128u ? launch_all<128, kKvE4m3>(st, a, p) : launch_all<256, kKvE4m3>(st, a, p);
-    return head_dim == 64u ? launch_all<64, kKvBf16>(st, a, p) : head_dim == 128u ? launch_all<128, kKvBf16>(st, a, p) : launch_all<256, kKvBf16>(st, a, p);
+cudaError_t launch_kv_attention(cudaStream_t st, int elem, uint32_t head_dim, const KvAttention &a, const KvPlan &p, int sms) {
+    if (elem == kKvE4m3) return head_dim == 64u ? launch_all<64, kKvE4m3>(st, a, p, sms) : head_dim == 128u ? launch_all<128, kKvE4m3>(st, a, p, sms) : launch_all<256, kKvE4m3>(st, a, p, sms);
+    return head_dim == 64u ? launch_all<64, kKvBf16>(st, a, p, sms) : head_dim == 128u ? launch_all<128, kKvBf16>(st, a, p, sms) : launch_all<256, kKvBf16>(st, a, p, sms);
 }
 
 void configure_kv_kernels() { configure_kv_many(); configure_few<64>(); configure_few<128>(); configure_few<256>(); }

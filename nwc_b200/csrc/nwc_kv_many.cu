@@ -199,8 +199,11 @@ __global__ void __launch_bounds__(Many<HD, ELEM>::kThreads, 1) kv_attention_many
     const uint32_t base = (smem_addr(many_raw) + 1023u) & ~1023u;
     const uint32_t bars = base + F::kBars, full = bars, empty = bars + NS * 8u, q_full = bars + 2u * NS * 8u, s_full = q_full + 16u, p_full = s_full + 16u, o_full = p_full + 16u, tmem_slot = o_full + 16u;
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
-    const uint32_t group = a.n_q / a.c.n_kv, rows = a.T * group, kvh = blockIdx.x % a.c.n_kv, row0 = (blockIdx.x / a.c.n_kv) * 2u * kManyRows, split = blockIdx.y;
-    const bool solo = rows - row0 <= kManyRows;
+    /* the first `pairs` units are two row tiles, the others one (see the launcher) */
+    const uint32_t group = a.n_q / a.c.n_kv, rows = a.T * group, unit = blockIdx.x, split = blockIdx.y;
+    const uint32_t kvh = unit % a.c.n_kv, row0 = unit < a.pairs ? unit / a.c.n_kv * 2u * kManyRows : a.pairs / a.c.n_kv * 2u * kManyRows + (unit - a.pairs) / a.c.n_kv * kManyRows;
+    const bool solo = unit >= a.pairs || rows - row0 <= kManyRows;
+    const uint32_t my_rows = solo ? kManyRows : 2u * kManyRows;
     if (warp == F::kMmaWarp) {
         if (lane == 0) {
             for (uint32_t s = 0; s < NS; s++) { mbar_init(full + s * 8u, kProducers / 32u); mbar_init(empty + s * 8u, 1u); }
@@ -220,7 +223,7 @@ __global__ void __launch_bounds__(Many<HD, ELEM>::kThreads, 1) kv_attention_many
     tm_fence_after();
     uint32_t tmem; asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
     /* the keys that this CTA's tokens see: as kv_span, for their positions; list index = lead sinks, then positions from first */
-    const uint32_t t_first = row0 / group, t_last = min(a.T - 1u, (row0 + 2u * kManyRows - 1u) / group);
+    const uint32_t t_first = row0 / group, t_last = min(a.T - 1u, (row0 + my_rows - 1u) / group);
     KvSpan span{0u, 0u, 0u};
     if (pos_ok) span = a.visible ? kv_span(pos, a.T, a.c.window, a.c.sinks) : kv_span((uint32_t)pos + t_first, t_last - t_first + 1u, a.c.window, a.c.sinks);
     const uint32_t slot_first = kv_slot(span.first, a.c.capacity, a.c.window, a.c.sinks), ring = a.c.capacity - a.c.sinks;
@@ -537,10 +540,23 @@ static EncodeTiledFn encode_tiled() {
 }
 
 template <int HD, int ELEM>
-static cudaError_t launch_many(cudaStream_t st, const KvAttention &a) {
-    const uint64_t rows = (uint64_t)a.T * (a.n_q / a.c.n_kv), pairs = (rows + 2u * kManyRows - 1u) / (2u * kManyRows);
+static cudaError_t launch_many(cudaStream_t st, const KvAttention &given, int sms) {
+    /* Units of one key/value head's 256 rows, one CTA each (times the splits of the keys).  Where the last wave of CTAs would fill
+       less than half of the GPU, its rows go out as units of 128: twice as many, each done in half the time (its two streams
+       take the key tiles in turn).  4096 tokens of 32 + 8 heads under a window of 4096, 512 units: 286 us, with halved ones 258. */
+    const uint64_t rows = (uint64_t)given.T * (given.n_q / given.c.n_kv), all = (rows + 2u * kManyRows - 1u) / (2u * kManyRows) * given.c.n_kv, last = all % (uint64_t)sms;
+    KvAttention a = given;
+    uint64_t units = all;
+    a.pairs = (uint32_t)all;
+    if (a.splits == 1u && all > (uint64_t)sms && last && last * 2u <= (uint64_t)sms) {
+        const uint64_t halved = (last + given.c.n_kv - 1u) / given.c.n_kv;              /* pairs of row tiles of every head */
+        if (halved * given.c.n_kv * 2u <= (uint64_t)sms) {
+            const uint64_t kept = all / given.c.n_kv - halved, left = rows - kept * 2u * kManyRows;
+            a.pairs = (uint32_t)(kept * given.c.n_kv); units = a.pairs + (left + kManyRows - 1u) / kManyRows * given.c.n_kv;
+        }
+    }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((uint32_t)(pairs * a.c.n_kv), a.splits); cfg.blockDim = dim3(Many<HD, ELEM>::kThreads); cfg.dynamicSmemBytes = Many<HD, ELEM>::kSmem; cfg.stream = st;
+    cfg.gridDim = dim3((uint32_t)units, a.splits); cfg.blockDim = dim3(Many<HD, ELEM>::kThreads); cfg.dynamicSmemBytes = Many<HD, ELEM>::kSmem; cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr; cfg.numAttrs = dependent_launch() ? 1 : 0;
@@ -559,9 +575,9 @@ static cudaError_t launch_many(cudaStream_t st, const KvAttention &a) {
     return cudaLaunchKernelEx(&cfg, kv_attention_many_kernel<HD, ELEM>, a, maps[0], maps[1]);
 }
 
-cudaError_t launch_kv_many(cudaStream_t st, int elem, uint32_t head_dim, const KvAttention &a) {
-    if (elem == kKvE4m3) return head_dim == 64u ? launch_many<64, kKvE4m3>(st, a) : launch_many<128, kKvE4m3>(st, a);
-    return head_dim == 64u ? launch_many<64, kKvBf16>(st, a) : launch_many<128, kKvBf16>(st, a);
+cudaError_t launch_kv_many(cudaStream_t st, int elem, uint32_t head_dim, const KvAttention &a, int sms) {
+    if (elem == kKvE4m3) return head_dim == 64u ? launch_many<64, kKvE4m3>(st, a, sms) : launch_many<128, kKvE4m3>(st, a, sms);
+    return head_dim == 64u ? launch_many<64, kKvBf16>(st, a, sms) : launch_many<128, kKvBf16>(st, a, sms);
 }
 
 void configure_kv_many() {

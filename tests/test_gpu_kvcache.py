@@ -246,6 +246,26 @@ def test_what_lies_outside_the_visible_span_does_not_matter(elem, T):
     assert_attention(out, *R.attend(q.double(), k[0], v[0], pos, window, sinks))
 
 
+@pytest.mark.parametrize("T,n_q,n_kv,hd", [(1300, 128, 8, 64), (1199, 128, 8, 64), (650, 128, 4, 64), (1215, 16, 1, 64), (5200, 8, 1, 64)])
+def test_more_row_tiles_than_the_gpu_has_places(T, n_q, n_kv, hd):
+    """Waves of units whose last one is halved (whole, with an odd tile, with few rows left), or is not; against torch in fp32
+    here, its error (2^-20) being no part of the bound."""
+    pos, window, sinks = 100, 70, 3
+    c, k, v = filled(n_kv, hd, sinks + window + T - 1, "bf16", window, sinks, seed=T)
+    q = queries(T, n_q, hd).cuda()
+    out = c.attend(q, at(pos)).view(T, n_q, hd)
+    c.check()
+    k, v = k[0].float().cuda(), v[0].float().cuda()
+    p = torch.tensor([x for x in range(pos + T) if x < sinks or x > pos - window], device="cuda")
+    slots = torch.tensor([R.slot(int(x), sinks + window + T - 1, window, sinks) for x in p], device="cuda")
+    own = pos + torch.arange(T, device="cuda")[:, None]
+    sees = (p <= own) & ((p < sinks) | (p > own - window))
+    for h in range(0, n_q, max(1, n_q // 16)):
+        g = h // (n_q // n_kv)
+        w = torch.softmax((q[:, h].float() @ k[g, slots].T / hd ** 0.5).masked_fill(~sees, float("-inf")), -1)
+        assert_attention(out[:, h], (w @ v[g, slots]).double().cpu(), (w @ v[g, slots].abs()).double().cpu())
+
+
 @pytest.mark.parametrize("T", [1, 40, 200])
 def test_scores_of_any_size(T):
     """Score differences of hundreds (one position takes all the weight) and a scale of the caller's; scores that large stay
