@@ -340,7 +340,7 @@ int nwc_kv_attention(void *stream, const nwc_kv_cache *cache, uint32_t layer, co
                      uint16_t *out, void *workspace, uint64_t workspace_size, int *status);
 
 /* The accepted path of a draft tree of T tokens at *pos: row path[i] of the drafts becomes row i for i < *count (<= most <= T),
-   in all layers; path (device, `most` entries) rises strictly.  The caller then advances *pos by *count; the drafts behind
+   in all layers; path (device, `most` entries) rises strictly and stays below T and the cache's end.  The caller then advances *pos by *count; the drafts behind
    the path count as never stored. */
 int nwc_kv_commit(void *stream, const nwc_kv_cache *cache, uint32_t T, const int32_t *pos, const int32_t *path,
                   const int32_t *count, uint32_t most, int *status);

@@ -272,8 +272,9 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const ReadArgs a) {
 __global__ void __launch_bounds__(64) kv_commit_kernel(KvLayer c, uint32_t row_bytes, uint32_t T, const int32_t *pos_ptr, const int32_t *path, const int32_t *count_ptr, uint32_t most, int *status) {
     dependency_sync();
     const int32_t pos = *pos_ptr, count = *count_ptr;
-    bool ok = pos >= 0 && count >= 0 && (uint32_t)count <= most && (uint64_t)pos + T <= (c.window ? 0x7FFFFFFFu : c.capacity);
-    for (int32_t i = 0, last = -1; ok && i < count; i++) { const int32_t p = path[i]; ok = p > last && (uint32_t)p < T; last = p; }
+    const uint64_t end = c.window ? 0x7FFFFFFFu : c.capacity;
+    bool ok = pos >= 0 && count >= 0 && (uint32_t)count <= most;
+    for (int32_t i = 0, last = -1; ok && i < count; i++) { const int32_t p = path[i]; ok = p > last && (uint32_t)p < T && (uint64_t)pos + (uint32_t)p < end; last = p; }
     if (!ok) { if (threadIdx.x == 0) atomicOr(status, kKvStatusPath); return; }
     const uint64_t head = blockIdx.x, cell0 = head * c.capacity;
     const uint32_t columns = row_bytes >> 4;

@@ -157,8 +157,8 @@ class KVCache:
 
     def commit(self, pos, path, count, tokens=None):
         """The accepted path of the draft tree stored at pos, in all layers: row path[i] of the drafts becomes row i for i <
-        count (int32 [1]; path int32, strictly rising).  `tokens`: size of the tree (default: as many as the cache allows to be
-        told apart from a wrong path).  The caller then advances pos by count."""
+        count (int32 [1]; path int32, strictly rising).  `tokens`: size of the tree (default: the largest that the
+        cache could have taken), beyond which a path is refused.  The caller then advances pos by count."""
         if path.dim() != 1: raise ValueError("path is a vector of draft numbers")
         self._int32(path, path.numel(), "path"); self._int32(count, 1, "count"); self._int32(pos, 1, "pos")
         if tokens is None: tokens = min(MAX_TREE, self.capacity - self.sinks - self.window + 1 if self.window else self.capacity)

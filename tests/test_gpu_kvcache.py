@@ -446,6 +446,19 @@ def test_the_first_layer_is_not_moved_by_another_caches_commit_and_all_layers_ar
         assert torch.equal(t, w)
 
 
+@pytest.mark.parametrize("window,sinks,capacity,pos", [(0, 0, 40, 33), (0, 0, 40, 0), (20, 3, 30, 33), (20, 3, 30, 1000)])
+def test_commit_finds_the_trees_limits_itself(window, sinks, capacity, pos):
+    c, k, v = filled(2, 64, capacity, "fp8", window, sinks)
+    was = c.read(pos, 7)
+    path = [0, 2, 3, 6]
+    c.commit(at(pos), torch.tensor(path, dtype=torch.int32, device="cuda"), torch.tensor([4], dtype=torch.int32, device="cuda"))
+    c.check()
+    for a, b in zip(was, c.read(pos, 7)): assert torch.equal(b[:, :4], a[:, path]) and torch.equal(b[:, 4:], a[:, 4:])
+    beyond = 40 - pos if not window else 8                              # the first draft that the cache could not have taken
+    c.commit(at(pos), torch.tensor([beyond], dtype=torch.int32, device="cuda"), torch.tensor([1], dtype=torch.int32, device="cuda"))
+    with pytest.raises(RuntimeError, match="path"): c.check()
+
+
 @pytest.mark.parametrize("path,count,tokens", [([2, 1], 2, 4), ([0, 0], 2, 4), ([0, 4], 2, 4), ([-1, 0], 2, 4), ([0, 1], 3, 4), ([0, 1], -1, 4)])
 def test_wrong_paths_move_nothing(path, count, tokens):
     c, _, _ = filled(2, 64, 32, "bf16")
