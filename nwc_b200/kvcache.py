@@ -17,6 +17,10 @@ import torch
 from . import _lib as L
 
 BF16, INT32 = torch.bfloat16, torch.int32
+try:                                                                  # an allocation without the dispatcher's way: 0.8 us instead of 1.9
+    from torch._C._dynamo.guards import _empty_strided_cuda as empty_strided
+except ImportError:
+    def empty_strided(shape, strides, dtype): return torch.empty(shape, dtype=dtype, device="cuda")
 current_device, raw_stream = getattr(torch._C, "_cuda_getDevice", None), getattr(torch._C, "_cuda_getCurrentRawStream", None)     # (absent without CUDA)
 MAX_TREE = 1024
 ELEMS = {"bf16": (0, torch.bfloat16), "fp8": (1, torch.float8_e4m3fn)}
@@ -90,7 +94,7 @@ class KVCache:
         self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
         at = lambda t: None if t is None else t.data_ptr()
         self._c = L.KvCache(at(k), at(v), at(k_exp), at(v_exp), self.layers, self.n_kv, self.head_dim, self.capacity, window, sinks, 1 if quantised else 0)
-        self._at, self._bf16 = k.get_device(), torch.empty(0, dtype=BF16, device=k.device)
+        self._at = k.get_device()
         self._need = {}                                               # workspace bytes per (tokens, query heads)
         self._ref, self._status = ctypes.byref(self._c), self.status.data_ptr()
 
@@ -102,22 +106,25 @@ class KVCache:
         Returns the queries, bf16 [T, n_q, head_dim]."""
         if qkv.dim() == 1: qkv = qkv[None]
         T, width = self._tokens(qkv, 2, "qkv")
-        hd, at = self.head_dim, self._at
-        n_q = width // hd - 2 * self.n_kv
-        if width % hd or n_q <= 0 or n_q % self.n_kv: raise ValueError(f"qkv rows of {width} are not (n_q + 2 * {self.n_kv}) heads of {hd}, n_q a multiple of {self.n_kv}")
-        if (q_norm is None) != (k_norm is None): raise ValueError("q_norm and k_norm come together")
-        rows = cos.size(0)
-        if cos.dim() != 2 or sin.dim() != 2 or sin.size(0) != rows: raise ValueError(f"cos and sin are both [positions, {hd}]")
-        for t in (cos, sin) if q_norm is None else (cos, sin, q_norm, k_norm):
-            if t.dtype is not BF16 or t.get_device() != at or t.size(-1) != hd or not t.is_contiguous(): raise ValueError(f"cos and sin are contiguous bf16 [positions, {hd}], q_norm and k_norm bf16 [{hd}], on {self.device}")
-        if q_norm is not None and (q_norm.dim() != 1 or k_norm.dim() != 1): raise ValueError(f"q_norm and k_norm are bf16 [{hd}]")
-        if depth is not None: self._int32(depth, T, "depth")
+        hd, at, n_kv = self.head_dim, self._at, self.n_kv
+        n_q = width // hd - 2 * n_kv
+        if width % hd or n_q <= 0 or n_q % n_kv: raise ValueError(f"qkv rows of {width} are not (n_q + 2 * {n_kv}) heads of {hd}, n_q a multiple of {n_kv}")
+        rows = cos.shape[0]
+        if cos.shape != (rows, hd) or sin.shape != (rows, hd): raise ValueError(f"cos and sin are both [positions, {hd}]")
+        if cos.dtype is not BF16 or sin.dtype is not BF16 or cos.get_device() != at or sin.get_device() != at or not cos.is_contiguous() or not sin.is_contiguous():
+            raise ValueError(f"cos and sin are contiguous bf16 on {self.device}")
+        qn = kn = dp = None
+        if q_norm is not None and k_norm is not None:
+            for t in (q_norm, k_norm):
+                if t.dtype is not BF16 or t.get_device() != at or t.shape != (hd,) or not t.is_contiguous(): raise ValueError(f"q_norm and k_norm are contiguous bf16 [{hd}] on {self.device}")
+            qn, kn = q_norm.data_ptr(), k_norm.data_ptr()
+        elif q_norm is not None or k_norm is not None: raise ValueError("q_norm and k_norm come together")
+        if depth is not None: self._int32(depth, T, "depth"); dp = depth.data_ptr()
         self._int32(pos, 1, "pos")
-        self._layer(layer)
-        out = qkv.new_empty((T, n_q, hd))
-        self._call("nwc_kv_append", L.lib.nwc_kv_append, self._ref, layer, qkv.data_ptr(), qkv.stride(0), T, n_q, None if q_norm is None else q_norm.data_ptr(),
-                   None if k_norm is None else k_norm.data_ptr(), cos.data_ptr(), sin.data_ptr(), rows, pos.data_ptr(), None if depth is None else depth.data_ptr(),
-                   eps, out.data_ptr(), self._status)
+        if not 0 <= layer < self.layers: self._layer(layer)
+        out = self._empty((T, n_q, hd), (n_q * hd, hd, 1))
+        self._call("nwc_kv_append", L.lib.nwc_kv_append, self._ref, layer, qkv.data_ptr(), qkv.stride(0), T, n_q, qn, kn, cos.data_ptr(), sin.data_ptr(), rows,
+                   pos.data_ptr(), dp, eps, out.data_ptr(), self._status)
         return out
 
     def attend(self, q, pos, visible=None, depth=None, layer=0, scale=None):
@@ -131,13 +138,13 @@ class KVCache:
             if T > MAX_TREE: raise ValueError(f"a draft tree has at most {MAX_TREE} tokens, not {T}")
             self._int32(visible, T * ((T + 31) // 32), "visible"); self._int32(depth, T, "depth")
         self._int32(pos, 1, "pos")
-        self._layer(layer)
-        out = q.new_empty((T, n_q * hd))
+        if not 0 <= layer < self.layers: self._layer(layer)
+        out = self._empty((T, n_q * hd), (n_q * hd, 1))
         need = self._need.get((T, n_q))
         if need is None:
             with torch.cuda.device(self.device): need = self._need[T, n_q] = L.lib.nwc_kv_attention_workspace(self._ref, T, n_q)
         # a workspace of the call's own: the allocator keeps it from calls on other streams, a graph keeps it in its pool
-        work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        work = self._empty((need // 2,), (1,)) if need else None
         self._call("nwc_kv_attention", L.lib.nwc_kv_attention, self._ref, layer, q.data_ptr(), q.stride(0), T, n_q, pos.data_ptr(), None if visible is None else visible.data_ptr(),
                    None if depth is None else depth.data_ptr(), 1.0 / math.sqrt(hd) if scale is None else float(scale), out.data_ptr(), None if work is None else work.data_ptr(), need, self._status)
         return out
@@ -149,9 +156,10 @@ class KVCache:
         if first < 0 or count < 1: raise ValueError("positions from 0 on, at least one")
         if not self.window and first + count > self.capacity: raise ValueError(f"positions {first} .. {first + count - 1} are outside a cache of {self.capacity}")
         if self.window and first + count - max(first, self.sinks) > self.capacity - self.sinks: raise ValueError(f"{count} positions do not lie in a ring of {self.capacity - self.sinks} at the same time")
-        self._layer(layer)
-        shape = (self.n_kv, count, self.head_dim)
-        k, v = self._bf16.new_empty(shape), self._bf16.new_empty(shape)
+        if not 0 <= layer < self.layers: self._layer(layer)
+        hd = self.head_dim
+        shape, strides = (self.n_kv, count, hd), (count * hd, hd, 1)
+        k, v = self._empty(shape, strides), self._empty(shape, strides)
         self._call("nwc_kv_read", L.lib.nwc_kv_read, self._ref, layer, first, count, k.data_ptr(), v.data_ptr())
         return k, v
 
@@ -182,8 +190,12 @@ class KVCache:
     def _int32(self, t, n, name):
         if t.dtype is not INT32 or t.get_device() != self._at or t.numel() != n or not t.is_contiguous(): raise ValueError(f"{name} is int32 with {n} elements on {self.device}")
 
+    def _empty(self, shape, strides):
+        """bf16 on the cache's device."""
+        return empty_strided(shape, strides, BF16) if current_device() == self._at else torch.empty(shape, dtype=BF16, device=self.device)
+
     def _layer(self, layer):
-        if not 0 <= layer < self.layers: raise IndexError(f"layer {layer} of a cache of {self.layers}")
+        raise IndexError(f"layer {layer} of a cache of {self.layers}")
 
     def _call(self, name, fn, *args):
         """One library call on the current stream of the cache's device."""

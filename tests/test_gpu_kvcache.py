@@ -523,3 +523,34 @@ def test_captured_and_replayed_calls_follow_the_position(T):
             want = c.attend(c.append(xi, p, cos, sin), p)
             c.check()
             assert torch.equal(got, want)
+
+
+def test_what_the_python_calls_refuse():
+    from nwc_b200 import KVCache
+    c = KVCache(2, 64, 32, "fp8", layers=2)
+    bf = lambda *s: torch.zeros(*s, dtype=torch.bfloat16, device="cuda")
+    x, p, t, w = bf(3, 8 * 64), at(0), bf(40, 64), bf(64)
+    good = dict(qkv=x, pos=p, cos=t, sin=t, q_norm=w, k_norm=w)
+    for bad in (dict(qkv=x.float()), dict(qkv=x.cpu()), dict(qkv=bf(3, 8 * 64 + 1)), dict(qkv=bf(3, 3 * 64)), dict(qkv=bf(3, 7 * 64)), dict(qkv=bf(8 * 64, 3).T), dict(qkv=bf(0, 8 * 64)),
+                dict(pos=torch.zeros(1, device="cuda")), dict(pos=p.cpu()), dict(pos=p.repeat(2)), dict(cos=t[:, :32]), dict(cos=t.float()), dict(cos=bf(39, 64)), dict(sin=bf(64, 40).T),
+                dict(q_norm=None), dict(k_norm=w[:32]), dict(q_norm=w.float()), dict(depth=p), dict(depth=torch.zeros(3, device="cuda"))):
+        with pytest.raises(ValueError): c.append(**{**good, **bad})
+    for layer in (-1, 2):
+        with pytest.raises(IndexError): c.append(**good, layer=layer)
+        with pytest.raises(IndexError): c.read(0, 1, layer=layer)
+    q, words = bf(3, 4, 64), torch.zeros(3, 1, dtype=torch.int32, device="cuda")
+    good = dict(q=q, pos=p)
+    for bad in (dict(q=q.float()), dict(q=bf(3, 5, 64)), dict(q=bf(3, 4, 128)), dict(q=bf(3, 4 * 64)), dict(q=bf(4, 3, 64).transpose(0, 1)), dict(visible=words), dict(depth=p),
+                dict(visible=words, depth=p), dict(visible=words[:2], depth=words.view(3)), dict(scale=0.0), dict(scale=float("nan")), dict(q=bf(33, 4, 64))):
+        with pytest.raises(ValueError): c.attend(**{**good, **bad})
+    with pytest.raises(IndexError): c.attend(q, p, layer=5)
+    for first, count in ((-1, 2), (0, 0), (30, 3)):
+        with pytest.raises(ValueError): c.read(first, count)
+    for path, count in ((torch.zeros(2, 1, dtype=torch.int32, device="cuda"), p), (p.float(), p), (p, p.cpu())):
+        with pytest.raises(ValueError): c.commit(p, path, count)
+    ring = KVCache(2, 64, 32, window=20, sinks=2)
+    with pytest.raises(ValueError): ring.append(bf(12, 8 * 64), p, t, t)                # 30 slots hold a window of 20 and 11 tokens, not 12
+    ring.append(bf(11, 8 * 64), p, t, t)
+    with pytest.raises(ValueError): ring.read(2, 31)
+    c.append(**dict(qkv=x[0], pos=p, cos=t, sin=t))                                     # a vector is one token
+    c.check(); ring.check()
