@@ -266,29 +266,49 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const ReadArgs a) {
     }
 }
 
-/* The accepted path of a draft tree, moved together: row pos + path[i] -> row pos + i for i < count, in every layer and
-   head.  path rises strictly, so path[i] >= i and a row is read before anything overwrites it when the moves run in order;
-   each thread owns one 16-byte column (or the exponent bytes) of all rows and therefore needs no synchronisation. */
-__global__ void __launch_bounds__(64) kv_commit_kernel(KvLayer c, uint32_t row_bytes, uint32_t T, const int32_t *pos_ptr, const int32_t *path, const int32_t *count_ptr, uint32_t most, int *status) {
+/* The accepted path of a draft tree, moved together: row pos + path[i] -> row pos + i for i < count, in every layer and head
+   (one CTA each).  path rises strictly, so path[i] >= i: a row is never overwritten before the moves that read it, as long as
+   the moves run in order or read before they write.  A CTA takes kMoves x 256 pieces of 16 bytes at a time, all read before
+   any is written.  (One thread per piece's column, row after row: 5 us for 15 rows, a load's latency each, where this takes 3.) */
+constexpr uint32_t kMoves = 4;
+__global__ void __launch_bounds__(256) kv_commit_kernel(KvLayer c, uint32_t row_bytes, uint32_t T, const int32_t *pos_ptr, const int32_t *path, const int32_t *count_ptr, uint32_t most, int *status) {
+    __shared__ uint32_t from[NWC_KV_MAX_TREE];                        /* slots */
+    const uint32_t tid = threadIdx.x;
     dependency_sync();
     const int32_t pos = *pos_ptr, count = *count_ptr;
     const uint64_t end = c.window ? 0x7FFFFFFFu : c.capacity;
     bool ok = pos >= 0 && count >= 0 && (uint32_t)count <= most;
-    for (int32_t i = 0, last = -1; ok && i < count; i++) { const int32_t p = path[i]; ok = p > last && (uint32_t)p < T && (uint64_t)pos + (uint32_t)p < end; last = p; }
-    if (!ok) { if (threadIdx.x == 0) atomicOr(status, kKvStatusPath); return; }
-    const uint64_t head = blockIdx.x, cell0 = head * c.capacity;
-    const uint32_t columns = row_bytes >> 4;
-    for (uint32_t j = threadIdx.x; j < 2u * columns + (c.k_exp ? 2u : 0u); j += blockDim.x) {
-        if (j < 2u * columns) {
-            uint8_t *base = (j < columns ? c.k : c.v) + cell0 * row_bytes + (j % columns) * 16u;
-            for (int32_t i = 0; i < count; i++) {
-                const int32_t p = path[i];
-                if (p != i) *reinterpret_cast<uint4 *>(base + (uint64_t)kv_slot(pos + i, c.capacity, c.window, c.sinks) * row_bytes) = *reinterpret_cast<const uint4 *>(base + (uint64_t)kv_slot(pos + p, c.capacity, c.window, c.sinks) * row_bytes);
-            }
-        } else {
-            uint8_t *base = (j == 2u * columns ? c.k_exp : c.v_exp) + cell0;
-            for (int32_t i = 0; i < count; i++) { const int32_t p = path[i]; if (p != i) base[kv_slot(pos + i, c.capacity, c.window, c.sinks)] = base[kv_slot(pos + p, c.capacity, c.window, c.sinks)]; }
+    if (ok) {
+        for (uint32_t i = tid; i < (uint32_t)count; i += 256u) {
+            const int32_t p = path[i], before = i ? path[i - 1u] : -1;
+            ok = ok && p > before && (uint32_t)p < T && (uint64_t)pos + (uint32_t)p < end;
+            from[i] = kv_slot((uint32_t)(pos + p), c.capacity, c.window, c.sinks);
         }
+    }
+    if (!__syncthreads_and(ok)) { if (tid == 0) atomicOr(status, kKvStatusPath); return; }
+    const uint64_t cell0 = (uint64_t)blockIdx.x * c.capacity;
+    const uint32_t columns = row_bytes >> 4, pieces = 2u * columns * (uint32_t)count;
+    auto place = [&](uint32_t e, uint32_t slot) {                    /* piece e = row i, K's columns, V's columns */
+        const uint32_t j = e % (2u * columns);
+        return reinterpret_cast<uint4 *>((j < columns ? c.k : c.v) + (cell0 + slot) * row_bytes + (j % columns) * 16u);
+    };
+    auto target = [&](uint32_t i) { return kv_slot((uint32_t)pos + i, c.capacity, c.window, c.sinks); };
+    for (uint32_t e0 = 0; e0 < pieces; e0 += kMoves * 256u) {
+        uint4 w[kMoves];
+#pragma unroll
+        for (uint32_t m = 0; m < kMoves; m++) { const uint32_t e = e0 + m * 256u + tid; if (e < pieces) w[m] = *place(e, from[e / (2u * columns)]); }
+        __syncthreads();
+#pragma unroll
+        for (uint32_t m = 0; m < kMoves; m++) { const uint32_t e = e0 + m * 256u + tid; if (e < pieces) *place(e, target(e / (2u * columns))) = w[m]; }
+        __syncthreads();
+    }
+    for (uint32_t e0 = 0; c.k_exp && e0 < 2u * (uint32_t)count; e0 += 256u) {
+        const uint32_t e = e0 + tid;
+        uint8_t *exps = (e & 1u ? c.v_exp : c.k_exp) + cell0, w = 0;
+        if (e < 2u * (uint32_t)count) w = exps[from[e >> 1]];
+        __syncthreads();
+        if (e < 2u * (uint32_t)count) exps[target(e >> 1)] = w;
+        __syncthreads();
     }
 }
 
@@ -363,7 +383,7 @@ NWC_EXPORT int nwc_kv_commit(void *stream, const nwc_kv_cache *cache, uint32_t T
     if (!cache_ok(cache, 0u, T) || !T || T > NWC_KV_MAX_TREE || most > T || !pos || !path || !count || !status) return -1;
     if (!most) return 0;
     const uint32_t row_bytes = cache->head_dim * (cache->elem == kKvBf16 ? 2u : 1u);
-    return (int)launch(kv_commit_kernel, dim3(cache->layers * cache->n_kv), dim3(64), stream, layer_of(cache, 0u), row_bytes, T, pos, path, count, most, status);
+    return (int)launch(kv_commit_kernel, dim3(cache->layers * cache->n_kv), dim3(256), stream, layer_of(cache, 0u), row_bytes, T, pos, path, count, most, status);
 }
 
 /* fp32 sums and (maximum, sum) pairs of every split: 0 where the keys are not divided or a cluster joins its shares */
