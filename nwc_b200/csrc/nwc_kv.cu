@@ -386,16 +386,13 @@ NWC_EXPORT int nwc_kv_commit(void *stream, const nwc_kv_cache *cache, uint32_t T
     return (int)launch(kv_commit_kernel, dim3(cache->layers * cache->n_kv), dim3(256), stream, layer_of(cache, 0u), row_bytes, T, pos, path, count, most, status);
 }
 
-/* fp32 sums and (maximum, sum) pairs of every split: 0 where the keys are not divided or a cluster joins its shares */
-static uint64_t workspace_bytes(const KvPlan &p, uint32_t T, uint32_t n_q, uint32_t head_dim) {
-    return p.splits == 1u || p.in_clusters ? 0u : (uint64_t)p.splits * T * n_q * (head_dim + 2u) * sizeof(float);
-}
+static uint64_t workspace_bytes(const KvPlan &p, uint32_t head_dim) { return p.cells * (head_dim + 2u) * sizeof(float); }
 
 NWC_EXPORT uint64_t nwc_kv_attention_workspace(const nwc_kv_cache *cache, uint32_t T, uint32_t n_q) {
     if (!cache || !T || T > NWC_KV_MAX_TOKENS || !n_q || n_q > 65535u || !cache->n_kv || n_q % cache->n_kv) return 0;
     const int sms = nwc_setup();
     if (sms <= 0) return 0;
-    return workspace_bytes(kv_attention_plan(cache->elem, cache->head_dim, cache->n_kv, cache->capacity, cache->window, cache->sinks, T, n_q, sms), T, n_q, cache->head_dim);
+    return workspace_bytes(kv_attention_plan(cache->elem, cache->head_dim, cache->n_kv, cache->capacity, cache->window, cache->sinks, T, n_q, sms), cache->head_dim);
 }
 
 NWC_EXPORT int nwc_kv_attention(void *stream, const nwc_kv_cache *cache, uint32_t layer, const uint16_t *q, uint64_t ldq, uint32_t T, uint32_t n_q,
@@ -408,9 +405,9 @@ NWC_EXPORT int nwc_kv_attention(void *stream, const nwc_kv_cache *cache, uint32_
     const int sms = nwc_setup();
     if (sms <= 0) return (int)cudaErrorNoDevice;
     const KvPlan plan = kv_attention_plan(cache->elem, cache->head_dim, cache->n_kv, cache->capacity, cache->window, cache->sinks, T, n_q, sms);
-    const uint64_t need = workspace_bytes(plan, T, n_q, cache->head_dim);
+    const uint64_t need = workspace_bytes(plan, cache->head_dim);
     if (need && (!workspace || workspace_size < need)) return -1;
-    float *part_o = static_cast<float *>(workspace), *part_ml = need ? part_o + (uint64_t)plan.splits * T * n_q * cache->head_dim : nullptr;
+    float *part_o = static_cast<float *>(workspace), *part_ml = need ? part_o + plan.cells * cache->head_dim : nullptr;
     const KvAttention a{layer_of(cache, layer), q, ldq, T, n_q, pos, visible, depth, scale * 1.4426950408889634f, out, status, part_o, part_ml, plan.splits, layer, cache->layers, 0u};
     return (int)launch_kv_attention((cudaStream_t)stream, cache->elem, cache->head_dim, a, plan, sms);
 }

@@ -83,8 +83,9 @@ struct KvAttention {
     float scale;                 /* softmax scale times log2(e) */
     uint16_t *out;               /* bf16 [T][n_q * head_dim] */
     int *status;
-    /* where the keys are divided over `splits` CTAs, each leaves its share here (row = token * n_q + head):
-       part_o fp32 [splits][T * n_q][head_dim] unnormalised, part_ml fp32 [splits][T * n_q][2] = running maximum (log2), sum */
+    /* Where a row's keys are divided over `splits` CTAs, each leaves its share here, fp32: the unnormalised outputs, and running
+       maximum (log2) and sum.  Few rows: part_o [splits][T * n_q][head_dim], part_ml [splits][T * n_q][2].  Many: part_o
+       [splits][units][2][head_dim / 4][128][4], part_ml [splits][units][2][128][2]. */
     float *part_o, *part_ml;
     uint32_t splits;
     uint32_t layer, layers;      /* which layer of how many `c` is */
@@ -93,7 +94,11 @@ struct KvAttention {
 /* How a call is divided.  It goes by sizes that the host knows (a captured call is replayed at other positions): the most
    keys that the cache can show, not the position. */
 constexpr uint32_t kKvShortKeys = 4096;
-struct KvPlan { uint32_t splits; bool in_clusters, many; };       /* many: the tensor-memory kernel of nwc_kv_many.cu */
+struct KvPlan {
+    uint32_t splits;             /* CTAs that divide the keys of one head's rows */
+    bool in_clusters, many;      /* many: the tensor-memory kernel of nwc_kv_many.cu */
+    uint64_t cells;              /* rows of shares in the workspace, head_dim + 2 fp32 numbers each */
+};
 KvPlan kv_attention_plan(int elem, uint32_t head_dim, uint32_t n_kv, uint32_t capacity, uint32_t window, uint32_t sinks, uint32_t T, uint32_t n_q, int sms);
 cudaError_t launch_kv_attention(cudaStream_t st, int elem, uint32_t head_dim, const KvAttention &a, const KvPlan &plan, int sms);
 cudaError_t launch_kv_many(cudaStream_t st, int elem, uint32_t head_dim, const KvAttention &a, int sms);

@@ -531,11 +531,10 @@ cudaError_t launch_few(cudaStream_t st, const KvAttention &a) {
     return launch(kv_attention_few_kernel<HD, ELEM, MT, SHORT>, dim3(a.c.n_kv * tiles, a.splits), dim3(32u * F::kWarps), F::kSmem, st, dependent_launch(), SHORT ? a.splits : 1u, a);
 }
 template <int HD, int ELEM>
-cudaError_t launch_all(cudaStream_t st, const KvAttention &a, const KvPlan &p, int sms) {
+cudaError_t launch_all(cudaStream_t st, const KvAttention &a, const KvPlan &p) {
     const uint32_t rows = a.T * (a.n_q / a.c.n_kv);
     const bool in_clusters = p.in_clusters;
     cudaError_t err;
-    if (p.many) err = launch_kv_many(st, ELEM, HD, a, sms); else
     if (in_clusters) err = launch_few<HD, ELEM, 1, 1>(st, a);
     else if constexpr (HD != 256 && ELEM == kKvE4m3) err = rows > 16u /* the plan lets no more than 32 come here */ ? launch_few<HD, ELEM, 2, 0>(st, a) : launch_few<HD, ELEM, 1, 0>(st, a);
     else err = launch_few<HD, ELEM, 1, 0>(st, a);
@@ -567,12 +566,13 @@ KvPlan kv_attention_plan(int elem, uint32_t head_dim, uint32_t n_kv, uint32_t ca
     const uint32_t rows = T * (n_q / n_kv);
     const uint64_t keys = window ? (uint64_t)sinks + window + T - 1u : capacity;
     const bool longer = keys > kKvShortKeys;
-    KvPlan p{1u, false, head_dim != 256u && rows > (elem == kKvE4m3 && longer ? 32u : 16u)};
+    KvPlan p{1u, false, head_dim != 256u && rows > (elem == kKvE4m3 && longer ? 32u : 16u), 0u};
     if (p.many) {
         /* a CTA per SM, each with at least two tiles of 128 keys */
         const uint64_t ctas = (uint64_t)n_kv * ((rows + 255u) / 256u), seen = window ? (uint64_t)sinks + window + (T < 256u ? T : 256u) : capacity;
         const uint64_t most = (seen + 255u) / 256u, want = ctas < (uint64_t)sms ? (uint64_t)sms / ctas : 1u;
         p.splits = (uint32_t)(want < most ? want : most);
+        p.cells = p.splits > 1u ? (uint64_t)p.splits * ctas * 256u : 0u;
         return p;
     }
     const uint32_t per = head_dim == 256u || rows <= 16u ? 16u : 32u;
@@ -588,12 +588,14 @@ KvPlan kv_attention_plan(int elem, uint32_t head_dim, uint32_t n_kv, uint32_t ca
     /* no CTA below a tile for each of its warps */
     const uint64_t most = (keys + 383u) / 384u, want = (uint64_t)sms > ctas ? (uint64_t)sms / ctas : 1u;
     p.splits = (uint32_t)(want < most ? want : most);
+    p.cells = p.splits > 1u ? (uint64_t)p.splits * T * n_q : 0u;
     return p;
 }
 
 cudaError_t launch_kv_attention(cudaStream_t st, int elem, uint32_t head_dim, const KvAttention &a, const KvPlan &p, int sms) {
-    if (elem == kKvE4m3) return head_dim == 64u ? launch_all<64, kKvE4m3>(st, a, p, sms) : head_dim == 128u ? launch_all<128, kKvE4m3>(st, a, p, sms) : launch_all<256, kKvE4m3>(st, a, p, sms);
-    return head_dim == 64u ? launch_all<64, kKvBf16>(st, a, p, sms) : head_dim == 128u ? launch_all<128, kKvBf16>(st, a, p, sms) : launch_all<256, kKvBf16>(st, a, p, sms);
+    if (p.many) return launch_kv_many(st, elem, head_dim, a, sms);
+    if (elem == kKvE4m3) return head_dim == 64u ? launch_all<64, kKvE4m3>(st, a, p) : head_dim == 128u ? launch_all<128, kKvE4m3>(st, a, p) : launch_all<256, kKvE4m3>(st, a, p);
+    return head_dim == 64u ? launch_all<64, kKvBf16>(st, a, p) : head_dim == 128u ? launch_all<128, kKvBf16>(st, a, p) : launch_all<256, kKvBf16>(st, a, p);
 }
 
 void configure_kv_kernels() { configure_kv_many(); configure_few<64>(); configure_few<128>(); configure_few<256>(); }

@@ -11,7 +11,7 @@
  *   stream 1:                  weights of S1(j+1)
  *
  * With at most 128 rows in all, both streams hold the same rows and take the key tiles in turn; their shares meet at the end.
- * Few rows over a long cache: the keys are divided over several CTAs and joined by kv_attention_join_kernel.
+ * Few rows over a long cache: the keys are divided over several CTAs and joined by a second kernel.
  *
  * Bound: 4 * 128 * 128 * head_dim multiply-adds per pair of tiles on the tensor cores (2048 clocks at head_dim 128), and as
  * many clocks of the exponential unit (16 per SM and clock) for 2 * 128 * 128 weights.
@@ -121,6 +121,10 @@ __device__ __forceinline__ void tm_wait_store() { asm volatile("tcgen05.wait::st
 __device__ __forceinline__ void tm_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tm_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) { uint32_t d; asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(b), "f"(a)); return d; }
+__device__ __forceinline__ void kv_dependency_sync() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
 __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 /* One row's scores of a tile -> weights: running maximum m (log2) and sum l updated, P (bf16) over the scores' first columns,
    O rescaled where m was raised.  The 128 scores are in registers throughout. */
@@ -214,8 +218,7 @@ __global__ void __launch_bounds__(Many<HD, ELEM>::kThreads, 1) kv_attention_many
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tmem_slot) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    kv_dependency_sync();
     const int32_t pos = *a.pos;
     const bool pos_ok = pos >= 0 && (uint64_t)pos + a.T <= (a.c.window ? 0x7FFFFFFFu : a.c.capacity);
     tm_fence_before();
@@ -323,8 +326,10 @@ __global__ void __launch_bounds__(Many<HD, ELEM>::kThreads, 1) kv_attention_many
             }
             const uint64_t line = (uint64_t)token * a.n_q + kvh * group + row % group;
             const float r = total == 0.f ? 0.f : 1.f / total;
-            float *part = a.splits > 1u ? a.part_o + ((uint64_t)split * a.T * a.n_q + line) * HD : nullptr;
-            if (a.splits > 1u && row_ok) *reinterpret_cast<float2 *>(a.part_ml + ((uint64_t)split * a.T * a.n_q + line) * 2u) = make_float2(!n ? -INFINITY : total == total ? top : 0.f /* a query that is not a number has no maximum, but its share counts */, total);
+            /* a share's outputs four dimensions at a time, rows side by side: what a warp writes (and the join reads) is one piece */
+            const uint64_t block = ((uint64_t)split * gridDim.x + unit) * 2u + s;
+            float *part = a.splits > 1u ? a.part_o + block * kManyRows * HD + wt * 4u : nullptr;
+            if (a.splits > 1u && row_ok) *reinterpret_cast<float2 *>(a.part_ml + (block * kManyRows + wt) * 2u) = make_float2(!n ? -INFINITY : total == total ? top : 0.f /* a query that is not a number has no maximum, but its share counts */, total);
 #pragma unroll
             for (uint32_t ch = 0; ch < HD / 32u; ch++) {
                 if (my_n) { tm_load32(tm_o + ch * 32u, v); tm_wait_load(); tm_hold(v); }
@@ -342,7 +347,7 @@ __global__ void __launch_bounds__(Many<HD, ELEM>::kThreads, 1) kv_attention_many
                 }
                 if (row_ok && part) {
 #pragma unroll
-                    for (uint32_t e = 0; e < 32u; e += 4u) *reinterpret_cast<uint4 *>(part + ch * 32u + e) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                    for (uint32_t e = 0; e < 32u; e += 4u) *reinterpret_cast<uint4 *>(part + (uint64_t)(ch * 8u + e / 4u) * kManyRows * 4u) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
                 } else if (row_ok) {
                     uint16_t *to = a.out + line * HD + ch * 32u;
 #pragma unroll
@@ -525,6 +530,69 @@ __global__ void __launch_bounds__(Many<HD, ELEM>::kThreads, 1) kv_attention_many
     if (warp == F::kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
+/* The shares of the splits joined, in their order.  A lane is a row, a warp 32 rows and 16 dimensions of them; `ways` warps take
+   the splits in turn and meet in shared memory. */
+template <int HD>
+__global__ void __launch_bounds__(256) kv_attention_many_join_kernel(const KvAttention a, uint32_t units, uint32_t ways) {
+    constexpr uint32_t kPieces = HD / 16u;
+    __shared__ float sums[8][17][32];
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, way = warp % ways;
+    const uint64_t item = (uint64_t)blockIdx.x * (8u / ways) + warp / ways;             /* unit, stream, 32 rows, 16 dimensions */
+    const uint32_t piece = (uint32_t)(item % kPieces), part = (uint32_t)(item / kPieces) & 3u, s = (uint32_t)(item / (kPieces * 4u)) & 1u;
+    const uint64_t unit = item / (kPieces * 8u);
+    kv_dependency_sync();
+    const int32_t pos = *a.pos;
+    if (pos < 0 || (uint64_t)pos + a.T > (a.c.window ? 0x7FFFFFFFu : a.c.capacity)) return;
+    const uint32_t group = a.n_q / a.c.n_kv, rows = a.T * group, kvh = (uint32_t)(unit % a.c.n_kv), row0 = (uint32_t)(unit / a.c.n_kv) * 2u * kManyRows, r = part * 32u + lane, row = row0 + s * kManyRows + r;
+    const bool here = unit < units && row0 < rows && !(s && rows - row0 <= kManyRows), live = here && row < rows;      /* (a unit of one row tile: the streams' shares are one) */
+    float top = -INFINITY, total = 0.f, sum[16];
+#pragma unroll
+    for (uint32_t j = 0; j < 16u; j++) sum[j] = 0.f;
+    if (live) {
+        const float2 *ml = reinterpret_cast<const float2 *>(a.part_ml) + (unit * 2u + s) * kManyRows + r;
+        const float4 *from = reinterpret_cast<const float4 *>(a.part_o) + (unit * 2u + s) * kManyRows * (HD / 4u) + (uint64_t)piece * 4u * kManyRows + r;
+        const uint64_t step = (uint64_t)units * 2u * kManyRows;                         /* from split to split */
+#pragma unroll 4
+        for (uint32_t y = 0; y < a.splits; y++) top = fmaxf(top, __ldcg(ml + y * step).x);
+#pragma unroll 2
+        for (uint32_t y = way; y < a.splits; y += ways) {
+            const float2 w = __ldcg(ml + y * step);
+            float4 v[4];
+#pragma unroll
+            for (uint32_t j = 0; j < 4u; j++) v[j] = __ldcg(from + y * step * (HD / 4u) + j * kManyRows);
+            const bool share = w.x != -INFINITY;                                        /* (one without keys left no outputs) */
+            const float f = share ? exp2_fast(w.x - top) : 0.f;
+            total = fmaf(w.y, f, total);
+            if (share) {
+#pragma unroll
+                for (uint32_t j = 0; j < 4u; j++) {
+                    sum[4 * j] = fmaf(v[j].x, f, sum[4 * j]); sum[4 * j + 1] = fmaf(v[j].y, f, sum[4 * j + 1]);
+                    sum[4 * j + 2] = fmaf(v[j].z, f, sum[4 * j + 2]); sum[4 * j + 3] = fmaf(v[j].w, f, sum[4 * j + 3]);
+                }
+            }
+        }
+    }
+    if (ways > 1u) {
+#pragma unroll
+        for (uint32_t j = 0; j < 16u; j++) sums[warp][j][lane] = sum[j];
+        sums[warp][16][lane] = total;
+        __syncthreads();
+        if (way) return;
+        for (uint32_t w = 1; w < ways; w++) {
+            total += sums[warp + w][16][lane];
+#pragma unroll
+            for (uint32_t j = 0; j < 16u; j++) sum[j] += sums[warp + w][j][lane];
+        }
+    }
+    if (!live) return;
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    uint4 *to = reinterpret_cast<uint4 *>(a.out + ((uint64_t)(row / group) * a.n_q + kvh * group + row % group) * HD + piece * 16u);
+#pragma unroll
+    for (uint32_t j = 0; j < 2u; j++)
+        to[j] = make_uint4(pack_bf16(sum[8 * j] * inv, sum[8 * j + 1] * inv), pack_bf16(sum[8 * j + 2] * inv, sum[8 * j + 3] * inv),
+                           pack_bf16(sum[8 * j + 4] * inv, sum[8 * j + 5] * inv), pack_bf16(sum[8 * j + 6] * inv, sum[8 * j + 7] * inv));
+}
+
 /* cuTensorMapEncodeTiled through the runtime's driver entry point (the library does not link against the driver) */
 typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
                                   const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -572,7 +640,12 @@ static cudaError_t launch_many(cudaStream_t st, const KvAttention &given, int sm
             if (encode(&maps[i], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3u, (i ? a.c.v : a.c.k) - below, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) return cudaErrorInvalidValue;
     }
-    return cudaLaunchKernelEx(&cfg, kv_attention_many_kernel<HD, ELEM>, a, maps[0], maps[1]);
+    const cudaError_t err = cudaLaunchKernelEx(&cfg, kv_attention_many_kernel<HD, ELEM>, a, maps[0], maps[1]);
+    if (err != cudaSuccess || a.splits == 1u) return err;
+    const uint32_t ways = a.splits >= 16u ? 8u : a.splits >= 6u ? 4u : a.splits >= 3u ? 2u : 1u;
+    cfg.gridDim = dim3((uint32_t)((units * 8u * (HD / 16u) * ways + 7u) / 8u)); cfg.blockDim = dim3(256); cfg.dynamicSmemBytes = 0;
+    cfg.numAttrs = 1;                                                                   /* (its set-up overlaps the last CTAs; it waits for the whole grid before it reads) */
+    return cudaLaunchKernelEx(&cfg, kv_attention_many_join_kernel<HD>, a, (uint32_t)units, ways);
 }
 
 cudaError_t launch_kv_many(cudaStream_t st, int elem, uint32_t head_dim, const KvAttention &a, int sms) {
