@@ -324,8 +324,9 @@ __global__ void __launch_bounds__(Many<HD, ELEM>::kThreads, 1) kv_attention_many
                 f0 = m == -INFINITY ? 0.f : exp2_fast(m - top); f1 = m1 == -INFINITY ? 0.f : exp2_fast(m1 - top);
                 total = l * f0 + there[HD * 128u + 128u + wt] * f1;
             }
-            const uint64_t line = (uint64_t)token * a.n_q + kvh * group + row % group;
             const float r = total == 0.f ? 0.f : 1.f / total;
+            /* (Q's place: this stream's products with it are done; solo: the ring's, where every product is, behind the second stream's share) */
+            const uint32_t staged = base + (solo ? F::kRing + 8192u : F::kQ + s * F::kTile) + (warp & 3u) * 32u * HD * 2u;
             /* a share's outputs four dimensions at a time, rows side by side: what a warp writes (and the join reads) is one piece */
             const uint64_t block = ((uint64_t)split * gridDim.x + unit) * 2u + s;
             float *part = a.splits > 1u ? a.part_o + block * kManyRows * HD + wt * 4u : nullptr;
@@ -348,17 +349,26 @@ __global__ void __launch_bounds__(Many<HD, ELEM>::kThreads, 1) kv_attention_many
                 if (row_ok && part) {
 #pragma unroll
                     for (uint32_t e = 0; e < 32u; e += 4u) *reinterpret_cast<uint4 *>(part + (uint64_t)(ch * 8u + e / 4u) * kManyRows * 4u) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-                } else if (row_ok) {
-                    uint16_t *to = a.out + line * HD + ch * 32u;
+                } else if (!part) {
 #pragma unroll
                     for (uint32_t e = 0; e < 32u; e += 8u) {
                         uint32_t w[4];
 #pragma unroll
                         for (uint32_t j = 0; j < 4u; j++) w[j] = total == 0.f ? 0u : pack_bf16(__uint_as_float(v[e + 2u * j]) * r, __uint_as_float(v[e + 2u * j + 1u]) * r);
-                        *reinterpret_cast<uint4 *>(to + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                        sts128u(staged + lane * (HD * 2u) + (((ch * 4u + e / 8u) ^ (lane & 7u)) << 4), w[0], w[1], w[2], w[3]);
                     }
                 }
                 __syncwarp();
+            }
+            if (!part) {
+                /* the warp's 32 rows through shared memory, so that a store is whole rows */
+                constexpr uint32_t kPieces = HD / 8u, kRowsOnce = 32u / kPieces;
+#pragma unroll 4
+                for (uint32_t r0 = 0; r0 < 32u; r0 += kRowsOnce) {
+                    const uint32_t rr = r0 + lane / kPieces, piece = lane % kPieces, there_row = my_row0 + (warp & 3u) * 32u + rr;
+                    const uint4 w = lds128(staged + rr * (HD * 2u) + ((piece ^ (rr & 7u)) << 4));
+                    if (there_row < rows) *reinterpret_cast<uint4 *>(a.out + ((uint64_t)(there_row / group) * a.n_q + kvh * group + there_row % group) * HD + piece * 8u) = w;
+                }
             }
         }
     } else if (warp < F::kMmaWarp) {
