@@ -51,8 +51,8 @@ struct StoreArgs {
     uint32_t chunks;             /* kStoreQ passes of query rows that a warp takes one after the other */
 };
 
-/* HD / 8 lanes hold one row, eight numbers each, so a row is one 16-byte load per lane; the rotary partner of a number lives
-   in the lane HD / 16 away.  A warp takes PASSES x kSide rows of one kind (query, key or value) of one token: their loads are in
+/* HD / 8 lanes hold one row, eight numbers each: four of the lower half and the four that rotary embedding pairs them with, so a
+   row is two 8-byte loads per lane and no number has to be fetched from another lane.  A warp takes PASSES x kSide rows of one kind (query, key or value) of one token: their loads are in
    flight together, before the position is known, and they share the token's cos / sin.  (Rows of all kinds in one warp make
    one long piece of code, four times unrolled: 100 us for 4096 tokens of 64 + 16 heads where this takes less than half, most of it waiting
    for instructions.)
@@ -62,7 +62,6 @@ struct StoreArgs {
    reciprocal norm after one Newton step. */
 template <int HD> struct Row {
     static constexpr uint32_t kLanes = HD / 8, kSide = 32 / kLanes;
-    template <class T> static __device__ __forceinline__ T partner(T v) { return __shfl_xor_sync(0xffffffffu, v, kLanes / 2); }
     static __device__ __forceinline__ float sum(float v) {
 #pragma unroll
         for (uint32_t o = kLanes / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -79,7 +78,19 @@ __device__ __forceinline__ void unpack8(const uint4 &w, float (&x)[8]) {
 #pragma unroll
     for (int j = 0; j < 4; j++) { x[2 * j] = lo16(u[j]); x[2 * j + 1] = hi16(u[j]); }
 }
-/* x w / norm, turned (s: with the sign of the partner's share in this lane) */
+/* a lane's eight numbers of a row: 4 sub .. 4 sub + 3 and the same of the upper half */
+template <int HD> __device__ __forceinline__ uint4 load_streamed(const uint16_t *row) {
+    const uint2 a = __ldcs(reinterpret_cast<const uint2 *>(row)), b = __ldcs(reinterpret_cast<const uint2 *>(row + HD / 2));
+    return make_uint4(a.x, a.y, b.x, b.y);
+}
+template <int HD> __device__ __forceinline__ uint4 load_again(const uint16_t *row) {
+    const uint2 a = *reinterpret_cast<const uint2 *>(row), b = *reinterpret_cast<const uint2 *>(row + HD / 2);
+    return make_uint4(a.x, a.y, b.x, b.y);
+}
+template <int HD> __device__ __forceinline__ void store_halves(uint16_t *row, const uint4 &w) {
+    *reinterpret_cast<uint2 *>(row) = make_uint2(w.x, w.y); *reinterpret_cast<uint2 *>(row + HD / 2) = make_uint2(w.z, w.w);
+}
+/* x w / norm, turned (s: with the sign of the partner's share) */
 template <int HD>
 __device__ __forceinline__ void normed_and_turned(float (&y)[8], bool norm, const float (&w)[8], float eps, const float (&c)[8], const float (&s)[8]) {
     if (norm) {
@@ -91,7 +102,7 @@ __device__ __forceinline__ void normed_and_turned(float (&y)[8], bool norm, cons
         for (int j = 0; j < 8; j++) y[j] *= inv * w[j];
     }
 #pragma unroll
-    for (int j = 0; j < 8; j++) { const float other = Row<HD>::partner(y[j]); y[j] = fmaf(y[j], c[j], other * s[j]); }
+    for (int j = 0; j < 4; j++) { const float a = y[j], b = y[j + 4]; y[j] = fmaf(a, c[j], b * s[j]); y[j + 4] = fmaf(b, c[j + 4], a * s[j + 4]); }
 }
 /* the same as a sum of two numbers each */
 template <int HD>
@@ -111,10 +122,12 @@ __device__ __forceinline__ void normed_and_turned_exactly(float (&y)[8], float (
         const float ph = __fmul_rn(inv, inv), pl = fmaf(inv, inv, -ph);
         inv_low = 0.5f * inv * (fmaf(-mh, ph, 1.f) - fmaf(mh, pl, ml * ph));
     }
+    float xw[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) xw[j] = norm ? __fmul_rn(y[j], w[j]) : y[j];
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-        const float xw = norm ? __fmul_rn(y[j], w[j]) : y[j], other = Row<HD>::partner(xw);
-        float e, h = two_sum(__fmul_rn(xw, c[j]), __fmul_rn(other, s[j]), e);
+        float e, h = two_sum(__fmul_rn(xw[j], c[j]), __fmul_rn(xw[j ^ 4], s[j]), e);
         if (norm) {
             const float p = __fmul_rn(h, inv), q = fmaf(h, inv, -p) + fmaf(e, inv, h * inv_low);
             h = __fadd_rn(p, q); e = __fsub_rn(q, __fsub_rn(h, p));
@@ -147,13 +160,11 @@ __device__ __forceinline__ void store_row(const StoreArgs &a, uint8_t *plane, ui
             y[j] = __uint_as_float(f) * up;
         }
         if (live) {
-            uint2 codes;
-            codes.x = pack_e4m3(y[0], y[1]) | ((uint32_t)pack_e4m3(y[2], y[3]) << 16);
-            codes.y = pack_e4m3(y[4], y[5]) | ((uint32_t)pack_e4m3(y[6], y[7]) << 16);
-            *reinterpret_cast<uint2 *>(plane + cell * HD + sub * 8u) = codes;
+            *reinterpret_cast<uint32_t *>(plane + cell * HD + sub * 4u) = pack_e4m3(y[0], y[1]) | ((uint32_t)pack_e4m3(y[2], y[3]) << 16);
+            *reinterpret_cast<uint32_t *>(plane + cell * HD + HD / 2 + sub * 4u) = pack_e4m3(y[4], y[5]) | ((uint32_t)pack_e4m3(y[6], y[7]) << 16);
             if (sub == 0) exps[cell] = (uint8_t)b;
         }
-    } else if (live) *reinterpret_cast<uint4 *>(plane + (cell * HD + sub * 8u) * 2u) = pack8(y);
+    } else if (live) store_halves<HD>(reinterpret_cast<uint16_t *>(plane) + cell * HD + sub * 4u, pack8(y));
     if (live && !fine) atomicOr(a.status, kKvStatusNotFinite);
 }
 
@@ -163,7 +174,7 @@ template <int HD> __host__ __device__ constexpr uint32_t store_groups(uint32_t n
 template <int HD, int ELEM>
 __global__ void __launch_bounds__(256) kv_store_kernel(const StoreArgs a) {
     using R = Row<HD>;
-    const uint32_t lane = threadIdx.x & 31u, sub = lane % R::kLanes, side = lane / R::kLanes, d0 = sub * 8u, n_q = a.n_q, n_kv = a.c.n_kv;
+    const uint32_t lane = threadIdx.x & 31u, sub = lane % R::kLanes, side = lane / R::kLanes, d0 = sub * 4u, n_q = a.n_q, n_kv = a.c.n_kv;
     const uint32_t gq = store_groups<HD>(n_q, kStoreQ * a.chunks), gk = store_groups<HD>(n_kv, kStoreK), gv = store_groups<HD>(n_kv, kStoreV), groups = gq + gk + gv;
     const uint32_t unit = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);           /* (below 2^31: the launcher checks) */
     dependency_sync();
@@ -176,7 +187,7 @@ __global__ void __launch_bounds__(256) kv_store_kernel(const StoreArgs a) {
 #pragma unroll
     for (uint32_t i = 0; i < kStoreQ; i++) {
         const uint32_t row = row0 + i * R::kSide + side;
-        raw[i] = row < n && (i == 0u || kind == 0 || (kind == 2 && i < kStoreV)) ? __ldcs(reinterpret_cast<const uint4 *>(from + (uint64_t)row * HD)) : make_uint4(0u, 0u, 0u, 0u);
+        raw[i] = row < n && (i == 0u || kind == 0 || (kind == 2 && i < kStoreV)) ? load_streamed<HD>(from + (uint64_t)row * HD) : make_uint4(0u, 0u, 0u, 0u);
     }
     const int32_t pos = *a.pos, depth = a.depth ? a.depth[t] : (int32_t)t;
     const uint32_t limit = a.c.window ? 0x7FFFFFFFu : a.c.capacity;
@@ -198,13 +209,11 @@ __global__ void __launch_bounds__(256) kv_store_kernel(const StoreArgs a) {
     const uint64_t at = ((uint64_t)pos + (uint32_t)depth) * HD + d0;
     const bool norm = a.q_norm != nullptr;
     float c[8], s[8], w[8];
-    unpack8(*reinterpret_cast<const uint4 *>(a.cos_t + at), c);
-    unpack8(*reinterpret_cast<const uint4 *>(a.sin_t + at), s);
-    if (norm) unpack8(*reinterpret_cast<const uint4 *>((kind ? a.k_norm : a.q_norm) + d0), w);
-    if (sub < R::kLanes / 2) {                                        /* the lower half takes the upper one's numbers negated */
+    unpack8(load_again<HD>(a.cos_t + at), c);
+    unpack8(load_again<HD>(a.sin_t + at), s);
+    if (norm) unpack8(load_again<HD>((kind ? a.k_norm : a.q_norm) + d0), w);
 #pragma unroll
-        for (int j = 0; j < 8; j++) s[j] = -s[j];
-    }
+    for (int j = 0; j < 4; j++) s[j] = -s[j];                         /* the lower half takes the upper one's numbers negated */
     if (kind == 1) {
         static_assert(kStoreK == 1, "one pass of keys");
         const uint32_t row = row0 + side;
@@ -221,7 +230,7 @@ __global__ void __launch_bounds__(256) kv_store_kernel(const StoreArgs a) {
 #pragma unroll
         for (uint32_t i = 0; i < kStoreQ; i++) {
             const uint32_t row = first + (kStoreQ + i) * R::kSide;
-            next[i] = chunk + 1u < a.chunks && row < n ? __ldcs(reinterpret_cast<const uint4 *>(from + (uint64_t)row * HD)) : make_uint4(0u, 0u, 0u, 0u);
+            next[i] = chunk + 1u < a.chunks && row < n ? load_streamed<HD>(from + (uint64_t)row * HD) : make_uint4(0u, 0u, 0u, 0u);
         }
 #pragma unroll
         for (uint32_t i = 0; i < kStoreQ; i++) {
@@ -229,7 +238,7 @@ __global__ void __launch_bounds__(256) kv_store_kernel(const StoreArgs a) {
             float y[8];
             unpack8(raw[i], y);
             normed_and_turned<HD>(y, norm, w, a.eps, c, s);
-            if (row < n) *reinterpret_cast<uint4 *>(a.q_out + ((uint64_t)t * n_q + row) * HD + d0) = pack8(y);
+            if (row < n) store_halves<HD>(a.q_out + ((uint64_t)t * n_q + row) * HD + d0, pack8(y));
             raw[i] = next[i];
         }
     }

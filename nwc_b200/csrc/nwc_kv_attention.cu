@@ -557,9 +557,9 @@ template <int HD> void configure_few() {
 
 /* Which kernel and how many CTAs (times in us on B200, head_dim 128, eight key/value heads, calls of one kind in a graph):
      rows per key/value head   keys     e4m3: few / many      bf16: few / many
-     32                        32768    31 / 43               47 / 36
-     32                        131072   93 / 147              118 / 91
-     32                        4096     32 / 16               34 / 14
+     32                        32768    31 / 44               41 / 34
+     32                        131072   93 / 143              104 / 92
+     32                        4096     23 / 17               22 / 15
    The many-rows kernel multiplies 128 rows whatever there are, on tensor cores that make nothing of it, but it takes a while to
    fill and widens e4m3 rows at a rate of its own: the few-rows kernel takes up to 16 rows, and up to 32 of a long e4m3 cache. */
 KvPlan kv_attention_plan(int elem, uint32_t head_dim, uint32_t n_kv, uint32_t capacity, uint32_t window, uint32_t sinks, uint32_t T, uint32_t n_q, int sms) {

@@ -43,9 +43,9 @@ template <int HD, int ELEM> struct Many {
     /* Operand slots.  Both streams' products with a tile must end before its slot is filled again, and the filling itself takes
        a while, so three slots run dry: the products wait for V, V for the slot, the slot for the products. */
     static constexpr uint32_t kSlots = HD == 64 ? 8u : 5u;
-    /* Registers: the warps start with 65536 / threads (a multiple of 8) each; those that hold a row of scores take what the
-       others give back: 8 x 184 + 4 x 72 + 4 x 72 = 16 x 128, 8 x 152 + 8 x 64 + 4 x 48 = 20 x 96.  Widening e4m3 rows takes
-       eight warps, copying bf16 ones four. */
+    /* Registers: the 16 warps start with 65536 / 512 = 128 each; those that hold a row of scores take what the others give back:
+       8 x 184 + 4 x 72 + 4 x 72 = 16 x 128 (bf16: the producers only start copies), 8 x 168 + 4 x 112 + 4 x 64 = 16 x 128 (e4m3:
+       they hold two sets of codes; at 176 / 96 / 64 the tree of 64 over 32768 takes 107 us instead of 90). */
     static constexpr uint32_t kProducers = 128u, kMmaWarp = 8u + kProducers / 32u, kThreads = 256u + kProducers + 128u;
     static constexpr int kRegsWeights = ELEM == kKvE4m3 ? 168 : 184, kRegsProduce = ELEM == kKvE4m3 ? 112 : 72, kRegsMma = ELEM == kKvE4m3 ? 64 : 72;
     static constexpr uint32_t kQ = 0u, kRing = 2u * kTile, kBars = kRing + kSlots * kTile;
@@ -621,7 +621,7 @@ template <int HD, int ELEM>
 static cudaError_t launch_many(cudaStream_t st, const KvAttention &given, int sms) {
     /* Units of one key/value head's 256 rows, one CTA each (times the splits of the keys).  Where the last wave of CTAs would fill
        less than half of the GPU, its rows go out as units of 128: twice as many, each done in half the time (its two streams
-       take the key tiles in turn).  4096 tokens of 32 + 8 heads under a window of 4096, 512 units: 286 us, with halved ones 258. */
+       take the key tiles in turn).  4096 tokens of 32 + 8 heads under a window of 4096, 512 units: 308 us (sustained), with halved ones 292. */
     const uint64_t rows = (uint64_t)given.T * (given.n_q / given.c.n_kv), all = (rows + 2u * kManyRows - 1u) / (2u * kManyRows) * given.c.n_kv, last = all % (uint64_t)sms;
     KvAttention a = given;
     uint64_t units = all;

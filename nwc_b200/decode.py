@@ -447,6 +447,7 @@ class DecodeEngine:
 
     def reset(self):
         self.pos.zero_(); self.step_no.zero_(); self.log.zero_(); self.status.zero_()
+        if self.cache is not None: self.cache.status.zero_()
 
     def _run(self):
         if self.graph is not None: self.graph.replay()
@@ -497,6 +498,8 @@ class DecodeEngine:
         tokens = torch.as_tensor(token_ids, dtype=torch.int64, device=self.device).reshape(-1)
         pos = int(self.pos.item())
         if not tokens.numel(): raise ValueError("no tokens")
+        low, high = int(tokens.min()), int(tokens.max())
+        if low < 0 or high >= self.cfg.vocab: raise ValueError(f"token ids {low} .. {high} are not all below {self.cfg.vocab}")
         if pos + tokens.numel() > self.max_len: raise ValueError(f"{tokens.numel()} more tokens from position {pos} do not fit {self.max_len}")
         out = []
         for part in tokens.split(max(self.chunk, 1)):
@@ -512,6 +515,7 @@ class DecodeEngine:
         tokens: the accepted drafts and the one that follows them (at least one), which becomes the current token."""
         drafts = [int(t) for t in drafts]
         if len(drafts) != len(parents): raise ValueError("every draft has a parent")
+        if any(not 0 <= t < self.cfg.vocab for t in drafts): raise ValueError(f"draft token ids are not all below {self.cfg.vocab}")
         visible, depth = draft_tree([-1] + [int(p) + 1 for p in parents], self.device)
         start, pos = int(self.step_no.item()), int(self.pos.item())
         deepest = int(depth.max())

@@ -95,6 +95,7 @@ class KVCache:
         at = lambda t: None if t is None else t.data_ptr()
         self._c = L.KvCache(at(k), at(v), at(k_exp), at(v_exp), self.layers, self.n_kv, self.head_dim, self.capacity, window, sinks, 1 if quantised else 0)
         self._at = k.get_device()
+        with torch.cuda.device(self._at): L.lib.nwc_setup()           # not in the first call, which may be one that is captured
         self._need = {}                                               # workspace bytes per (tokens, query heads)
         self._ref, self._status = ctypes.byref(self._c), self.status.data_ptr()
 

@@ -144,6 +144,25 @@ def test_what_the_engine_refuses():
     with pytest.raises(ValueError, match="elem"): engine(kv="int8")
 
 
+def test_token_ids_outside_the_vocabulary_are_refused():
+    """Their embedding rows would be whatever lay in the buffer."""
+    eng = engine(chunk=4, max_len=16)
+    for ids in ([1, 2048], [-1], [5, -2048, 3]):
+        with pytest.raises(ValueError, match="below 2048"): eng.extend(ids)
+        with pytest.raises(ValueError, match="below 2048"): eng.verify(ids, [-1] * len(ids))
+    assert int(eng.pos) == 0 and eng.extend([0, 2047]).numel() == 2
+
+
+def test_a_reset_engine_has_forgotten_a_session_that_left_its_cache():
+    eng = engine(kv="fp8", max_len=8, chunk=4)
+    eng.prefill(TOKENS[:8], chunked=True)
+    eng.forward_token()                                                 # position 8 of a cache of 8: refused by the kernels, reported by check()
+    torch.cuda.synchronize()
+    assert int(eng.cache.status) != 0
+    want = engine(kv="fp8", max_len=8, chunk=4).prefill(TOKENS[:5], chunked=True)
+    assert int(eng.prefill(TOKENS[:5], chunked=True)) == int(want)
+
+
 @pytest.mark.parametrize("H,rows", [(256, 1), (1000, 3), (8192, 70)])
 def test_row_kernels_equal_the_single_row_ones(H, rows):
     from nwc_b200 import _lib as L
