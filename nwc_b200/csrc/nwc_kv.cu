@@ -52,9 +52,10 @@ struct StoreArgs {
 };
 
 /* HD / 8 lanes hold one row, eight numbers each: four of the lower half and the four that rotary embedding pairs them with, so a
-   row is two 8-byte loads per lane and no number has to be fetched from another lane.  A warp takes PASSES x kSide rows of one kind (query, key or value) of one token: their loads are in
+   row is two 8-byte loads per lane and no number has to be fetched from another lane (41 us with shuffles, 39 without, for the
+   call below).  A warp takes PASSES x kSide rows of one kind (query, key or value) of one token: their loads are in
    flight together, before the position is known, and they share the token's cos / sin.  (Rows of all kinds in one warp make
-   one long piece of code, four times unrolled: 100 us for 4096 tokens of 64 + 16 heads where this takes less than half, most of it waiting
+   one long piece of code, four times unrolled: 100 us for 4096 tokens of 64 + 16 heads where this takes a third, most of it waiting
    for instructions.)
    Between the loaded bf16 numbers and what is stored is fp32, rounded once.  Keys that become e4m3 codes are kept to twice
    fp32's precision on the way (with fp32's few roundings some four of a million land on the wrong side of a code's border):
@@ -171,8 +172,12 @@ __device__ __forceinline__ void store_row(const StoreArgs &a, uint8_t *plane, ui
 constexpr uint32_t kStoreQ = 4, kStoreK = 1, kStoreV = 2;             /* passes of a warp */
 template <int HD> __host__ __device__ constexpr uint32_t store_groups(uint32_t n, uint32_t passes) { return (n + passes * (256u / HD) - 1u) / (passes * (256u / HD)); }
 
-template <int HD, int ELEM>
-__global__ void __launch_bounds__(256) kv_store_kernel(const StoreArgs a) {
+/* Bound: integer work (unpacking, packing) and the dependent start of a warp (position, cos / sin, rows), 4096 tokens of 64 +
+   16 heads without norms: 34 us for 160 MB, 0.73 of measured bandwidth.  So the warps that fit count: without the norm weights the
+   kernel is held to 64 registers (four CTAs per SM; with 80 and three it takes 39), with them it would spill (one token 2.8 -> 3.3
+   us, 517 tokens 5.9 -> 7.1, 4096 tokens no faster). */
+template <int HD, int ELEM, bool NORM>
+__global__ void __launch_bounds__(256, NORM ? 3 : 4) kv_store_kernel(const StoreArgs a) {
     using R = Row<HD>;
     const uint32_t lane = threadIdx.x & 31u, sub = lane % R::kLanes, side = lane / R::kLanes, d0 = sub * 4u, n_q = a.n_q, n_kv = a.c.n_kv;
     const uint32_t gq = store_groups<HD>(n_q, kStoreQ * a.chunks), gk = store_groups<HD>(n_kv, kStoreK), gv = store_groups<HD>(n_kv, kStoreV), groups = gq + gk + gv;
@@ -207,11 +212,10 @@ __global__ void __launch_bounds__(256) kv_store_kernel(const StoreArgs a) {
         return;
     }
     const uint64_t at = ((uint64_t)pos + (uint32_t)depth) * HD + d0;
-    const bool norm = a.q_norm != nullptr;
     float c[8], s[8], w[8];
     unpack8(load_again<HD>(a.cos_t + at), c);
     unpack8(load_again<HD>(a.sin_t + at), s);
-    if (norm) unpack8(load_again<HD>((kind ? a.k_norm : a.q_norm) + d0), w);
+    if (NORM) unpack8(load_again<HD>((kind ? a.k_norm : a.q_norm) + d0), w);
 #pragma unroll
     for (int j = 0; j < 4; j++) s[j] = -s[j];                         /* the lower half takes the upper one's numbers negated */
     if (kind == 1) {
@@ -219,8 +223,8 @@ __global__ void __launch_bounds__(256) kv_store_kernel(const StoreArgs a) {
         const uint32_t row = row0 + side;
         float y[8], low[8];
         unpack8(raw[0], y);
-        if (ELEM == kKvE4m3) normed_and_turned_exactly<HD>(y, low, norm, w, a.eps, c, s);
-        else normed_and_turned<HD>(y, norm, w, a.eps, c, s);
+        if (ELEM == kKvE4m3) normed_and_turned_exactly<HD>(y, low, NORM, w, a.eps, c, s);
+        else normed_and_turned<HD>(y, NORM, w, a.eps, c, s);
         store_row<HD, ELEM>(a, a.c.k, a.c.k_exp, (uint64_t)row * a.c.capacity + slot, sub, row < n, y, low);
         return;
     }
@@ -237,7 +241,7 @@ __global__ void __launch_bounds__(256) kv_store_kernel(const StoreArgs a) {
             const uint32_t row = first + i * R::kSide;
             float y[8];
             unpack8(raw[i], y);
-            normed_and_turned<HD>(y, norm, w, a.eps, c, s);
+            normed_and_turned<HD>(y, NORM, w, a.eps, c, s);
             if (row < n) store_halves<HD>(a.q_out + ((uint64_t)t * n_q + row) * HD + d0, pack8(y));
             raw[i] = next[i];
         }
@@ -358,8 +362,9 @@ cudaError_t launch_store(int elem, const StoreArgs &given, void *stream) {
     const uint64_t units = (uint64_t)(store_groups<HD>(a.n_q, kStoreQ * a.chunks) + store_groups<HD>(a.c.n_kv, kStoreK) + store_groups<HD>(a.c.n_kv, kStoreV)) * a.T, blocks = (units + 7u) / 8u;
     if (units > 0x7FFFFFFFull) return cudaErrorInvalidValue;
     const uint32_t threads = units >= 8u ? 256u : (uint32_t)units * 32u;
-    return elem == kKvE4m3 ? launch(kv_store_kernel<HD, kKvE4m3>, dim3((uint32_t)blocks), dim3(threads), stream, a)
-                           : launch(kv_store_kernel<HD, kKvBf16>, dim3((uint32_t)blocks), dim3(threads), stream, a);
+    const auto kernel = elem == kKvE4m3 ? (a.q_norm ? kv_store_kernel<HD, kKvE4m3, true> : kv_store_kernel<HD, kKvE4m3, false>)
+                                        : (a.q_norm ? kv_store_kernel<HD, kKvBf16, true> : kv_store_kernel<HD, kKvBf16, false>);
+    return launch(kernel, dim3((uint32_t)blocks), dim3(threads), stream, a);
 }
 
 }  // namespace
