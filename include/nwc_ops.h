@@ -305,7 +305,8 @@ int nwc_argmax_rows(void *stream, const uint16_t *logits, uint32_t V, uint32_t r
    k, v, qkv, q and out are 16-byte aligned; every call is asynchronous on its stream, allocates nothing and can be captured.
    *pos (device) is the position of a call's first token.  *status (device) collects bits, 0 = fine: 1 a position outside the
    cache or the rotary tables (the call, or with `depth` that token, wrote nothing), 2 a key or value that was not finite (0
-   was stored in its place), 4 a path that is not one (nothing was moved). */
+   was stored in its place), 4 a path that is not one (nothing was moved), 8 a bounded wait inside the attention gave up (its outputs are
+   not valid; nwc_kernel_status() reports it as well). */
 #define NWC_KV_MAX_TOKENS 65535
 #define NWC_KV_MAX_TREE 1024
 typedef struct {
@@ -344,6 +345,9 @@ int nwc_kv_attention(void *stream, const nwc_kv_cache *cache, uint32_t layer, co
    the path count as never stored. */
 int nwc_kv_commit(void *stream, const nwc_kv_cache *cache, uint32_t T, const int32_t *pos, const int32_t *path,
                   const int32_t *count, uint32_t most, int *status);
+
+/* tests: a wait of the attention's kind that runs out after a moment, and what it leaves in *status and in nwc_kernel_status() */
+int nwc_kv_wait_probe(void *stream, int *status);
 
 #ifdef __cplusplus
 }

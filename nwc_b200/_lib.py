@@ -77,6 +77,7 @@ _SIGNATURES = {
     "nwc_kv_attention": (I, [P, P, U32, P, U64, U32, U32, P, P, P, ctypes.c_float, P, P, U64, P]),
     "nwc_kv_attention_workspace": (U64, [P, U32, U32]),
     "nwc_kv_commit": (I, [P, P, U32, P, P, P, U32, P]),
+    "nwc_kv_wait_probe": (I, [P, P]),
     "nwc_allreduce_add_rmsnorm": (I, [P, P, I, I, I, P, P, P, ctypes.c_float, U32, P]),
 }
 for _name, (_res, _args) in _SIGNATURES.items():

@@ -255,9 +255,9 @@ NWC_EXPORT int nwc_ref_fp8(void *stream, const uint8_t *w, const float *scale, c
 NWC_EXPORT int nwc_setup(void) { return device_sms(); }
 
 NWC_EXPORT int nwc_kernel_status(int clear) {
-    const int v[5] = {read_kernel_status(clear != 0), read_prefill_status(clear != 0), read_comm_status(clear != 0), read_model_status(clear != 0), read_kv_status(clear != 0)};
-    int worst = v[0];
-    for (int i = 1; i < 4; i++) if (v[i] > worst) worst = v[i];
+    const int v[] = {read_kernel_status(clear != 0), read_prefill_status(clear != 0), read_comm_status(clear != 0), read_model_status(clear != 0), read_kv_status(clear != 0)};
+    int worst = 0;
+    for (const int one : v) if (one > worst) worst = one;
     return worst;
 }
 

@@ -32,11 +32,11 @@ __device__ __forceinline__ bool mbar_poll(uint32_t bar, uint32_t parity) {
     asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
 }
-/* Whole-warp wait: true when the phase completed for every lane; false after kWaitPolls polls (status word set).
+/* Whole-warp wait: true when the phase completed for every lane; false after `polls` polls (status word set).
    The answer is made warp-uniform so that the lanes never disagree about leaving their loop. */
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint32_t polls = kWaitPolls) {
     bool ok = false;
-    for (uint32_t i = 0; i < kWaitPolls && !ok; i++) ok = mbar_poll(bar, parity);
+    for (uint32_t i = 0; i < polls && !ok; i++) ok = mbar_poll(bar, parity);
     ok = __all_sync(0xffffffffu, ok);
     if (!ok) atomicExch(&g_kernel_status, kStatusWaitTimeout);
     return ok;

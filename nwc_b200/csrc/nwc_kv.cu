@@ -400,6 +400,8 @@ NWC_EXPORT int nwc_kv_commit(void *stream, const nwc_kv_cache *cache, uint32_t T
     return (int)launch(kv_commit_kernel, dim3(cache->layers * cache->n_kv), dim3(256), stream, layer_of(cache, 0u), row_bytes, T, pos, path, count, most, status);
 }
 
+NWC_EXPORT int nwc_kv_wait_probe(void *stream, int *status) { return status ? (int)launch_kv_wait_probe((cudaStream_t)stream, status) : -1; }
+
 static uint64_t workspace_bytes(const KvPlan &p, uint32_t head_dim) { return p.cells * (head_dim + 2u) * sizeof(float); }
 
 NWC_EXPORT uint64_t nwc_kv_attention_workspace(const nwc_kv_cache *cache, uint32_t T, uint32_t n_q) {

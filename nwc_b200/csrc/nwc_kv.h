@@ -18,7 +18,7 @@
 namespace nwc {
 
 constexpr int kKvBf16 = 0, kKvE4m3 = 1;
-constexpr int kKvStatusPosition = 1, kKvStatusNotFinite = 2, kKvStatusPath = 4;      /* bits of the status word */
+constexpr int kKvStatusPosition = 1, kKvStatusNotFinite = 2, kKvStatusPath = 4, kKvStatusWait = 8;      /* bits of the status word */
 
 /* One layer of a cache. */
 struct KvLayer {
@@ -103,6 +103,7 @@ KvPlan kv_attention_plan(int elem, uint32_t head_dim, uint32_t n_kv, uint32_t ca
 cudaError_t launch_kv_attention(cudaStream_t st, int elem, uint32_t head_dim, const KvAttention &a, const KvPlan &plan, int sms);
 cudaError_t launch_kv_many(cudaStream_t st, int elem, uint32_t head_dim, const KvAttention &a, int sms);
 void configure_kv_many();
+cudaError_t launch_kv_wait_probe(cudaStream_t st, int *status);
 void configure_kv_kernels();                 /* per-device shared-memory opt-ins */
 int read_kv_status(bool clear);              /* 0, or 2 when a bounded wait gave up */
 

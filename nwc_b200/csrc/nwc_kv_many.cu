@@ -193,6 +193,9 @@ __device__ __forceinline__ uint32_t bit_range(int32_t lo, int32_t hi) {
     return (0xFFFFFFFFu >> (32 - (hi - lo))) << lo;
 }
 
+/* a warp that gave up waiting says so in the call's status word too: its outputs, or its share of them, were not written */
+__device__ __forceinline__ void report_wait(bool alive, int *status) { if (!alive && (threadIdx.x & 31u) == 0u) atomicOr(status, kKvStatusWait); }
+
 }  // namespace
 
 template <int HD, int ELEM>
@@ -533,6 +536,7 @@ __global__ void __launch_bounds__(Many<HD, ELEM>::kThreads, 1) kv_attention_many
         }
     }
     if (!pos_ok && tid == 0) atomicOr(a.status, kKvStatusPosition);
+    report_wait(alive, a.status);
     __syncwarp();
     tm_fence_before();
     __syncthreads();
@@ -661,6 +665,18 @@ static cudaError_t launch_many(cudaStream_t st, const KvAttention &given, int sm
 cudaError_t launch_kv_many(cudaStream_t st, int elem, uint32_t head_dim, const KvAttention &a, int sms) {
     if (elem == kKvE4m3) return head_dim == 64u ? launch_many<64, kKvE4m3>(st, a, sms) : launch_many<128, kKvE4m3>(st, a, sms);
     return head_dim == 64u ? launch_many<64, kKvBf16>(st, a, sms) : launch_many<128, kKvBf16>(st, a, sms);
+}
+
+/* One warp waits, with a short limit, for a barrier that nothing arrives at, and reports it as the attention does. */
+__global__ void kv_wait_probe_kernel(int *status) {
+    __shared__ __align__(8) uint64_t bar;
+    if (threadIdx.x == 0) { mbar_init(smem_addr(&bar), 1u); mbar_init_fence(); }
+    __syncwarp();
+    report_wait(mbar_wait(smem_addr(&bar), 0u, 64u), status);
+}
+cudaError_t launch_kv_wait_probe(cudaStream_t st, int *status) {
+    kv_wait_probe_kernel<<<1, 32, 0, st>>>(status);
+    return cudaGetLastError();
 }
 
 void configure_kv_many() {

@@ -457,8 +457,8 @@ class DecodeEngine:
         """After a synchronise: the position must have stayed inside the KV cache and no bounded wait inside a kernel
         (bulk copy, peer rank) may have run out - a step that did is not a valid token."""
         if int(self.status.item()): raise RuntimeError("decode position left the KV cache")
-        if self.cache is not None: self.cache.check()
         st = L.lib.nwc_kernel_status(1)
+        if self.cache is not None: self.cache.check()               # (a wait of its kernels is in both words: said once)
         if st: raise RuntimeError(f"a bounded wait inside a kernel gave up (status {st}: 2 = bulk copy, 3 = a tensor-parallel rank did not answer)")
 
     # ---- several tokens at once (engines with a chunk) ----

@@ -24,7 +24,8 @@ except ImportError:
 current_device, raw_stream = getattr(torch._C, "_cuda_getDevice", None), getattr(torch._C, "_cuda_getCurrentRawStream", None)     # (absent without CUDA)
 MAX_TREE = 1024
 ELEMS = {"bf16": (0, torch.bfloat16), "fp8": (1, torch.float8_e4m3fn)}
-STATUS_TEXT = ((1, "a position outside the cache or the rotary tables"), (2, "a key or value that is not finite"), (4, "an accepted path that is not one"))
+STATUS_TEXT = ((1, "a position outside the cache or the rotary tables"), (2, "a key or value that is not finite"), (4, "an accepted path that is not one"),
+               (8, "a bounded wait inside the attention gave up, its outputs are not valid"))
 
 
 def draft_tree(parents, device="cuda"):

@@ -163,6 +163,17 @@ def test_a_reset_engine_has_forgotten_a_session_that_left_its_cache():
     assert int(eng.prefill(TOKENS[:5], chunked=True)) == int(want)
 
 
+def test_the_engine_reports_a_wait_that_ran_out_once():
+    from nwc_b200 import _lib as L
+    eng = engine(chunk=4, max_len=16)
+    assert L.lib.nwc_kv_wait_probe(L.stream(), L.ptr(eng.cache.status)) == 0
+    with pytest.raises(RuntimeError, match="gave up"): eng._check_status()
+    eng._check_status()
+    assert L.lib.nwc_kv_wait_probe(L.stream(), L.ptr(torch.zeros(1, dtype=torch.int32, device="cuda"))) == 0       # in the library's word alone
+    with pytest.raises(RuntimeError, match="gave up"): eng._check_status()
+    eng._check_status()
+
+
 @pytest.mark.parametrize("H,rows", [(256, 1), (1000, 3), (8192, 70)])
 def test_row_kernels_equal_the_single_row_ones(H, rows):
     from nwc_b200 import _lib as L

@@ -554,3 +554,14 @@ def test_what_the_python_calls_refuse():
     with pytest.raises(ValueError): ring.read(2, 31)
     c.append(**dict(qkv=x[0], pos=p, cos=t, sin=t))                                     # a vector is one token
     c.check(); ring.check()
+
+
+def test_a_wait_that_ran_out_is_reported_by_the_cache_and_by_the_library():
+    """The probe waits, for a moment, for a barrier that nothing arrives at, and reports it as the attention kernel does."""
+    from nwc_b200 import KVCache, _lib as L
+    c = KVCache(2, 64, 32)
+    assert L.lib.nwc_kernel_status(1) == 0
+    assert L.lib.nwc_kv_wait_probe(L.stream(), L.ptr(c.status)) == 0
+    with pytest.raises(RuntimeError, match="gave up"): c.check()
+    c.check()                                                            # reported once
+    assert L.lib.nwc_kernel_status(0) == 2 and L.lib.nwc_kernel_status(1) == 2 and L.lib.nwc_kernel_status(1) == 0

@@ -109,3 +109,7 @@ def test_reference_attention_in_a_case_done_by_hand():
     # ring of three behind one sink: position 4 lives in slot 1, 5 in slot 2
     out, _ = R.attend(q[:1], k, v, pos=4, window=1, sinks=1)
     assert out.item() == 2.0
+
+
+def test_the_wait_probe_refuses_no_status_word(L):
+    assert L.lib.nwc_kv_wait_probe(None, None) == -1
