@@ -393,7 +393,8 @@ __global__ void __launch_bounds__(Many<HD, ELEM>::kThreads, 1) kv_attention_many
         if constexpr (ELEM == kKvBf16) {
             /* a straight tile is one tensor-map copy per 64 dimensions (one thread, no multicast), any other is copied row by row */
             const uint32_t place = base + F::kRing + (ch >> 3) * F::kHalfBytes + swizzled(r0, ch & 7u), plane = a.layer * a.c.n_kv + kvh;
-            for (uint32_t x = 0; x < items && alive; x++) {
+            uint32_t x = 0;
+            for (; x < items && alive; x++) {
                 const uint32_t i0 = (tile0 + tile_of(x)) * kManyKeys, to = base + F::kRing + (x % NS) * F::kTile, bar = full + (x % NS) * 8u;
                 if (x >= NS) alive = mbar_wait(empty + (x % NS) * 8u, ((x / NS) - 1u) & 1u);
                 if (!alive) break;
@@ -417,6 +418,9 @@ __global__ void __launch_bounds__(Many<HD, ELEM>::kThreads, 1) kv_attention_many
                 async_proxy_fence();
                 arrive_warp(bar);
             }
+            /* Where the products gave up, copies may still be on their way: the CTA does not end before those of the last NS tiles
+               have arrived (elsewhere they long have). */
+            if (warp == 8u) for (uint32_t y = x > NS ? x - NS : 0u; y < x; y++) mbar_wait(full + (y % NS) * 8u, (y / NS) & 1u);
         } else {
             /* codes in registers a tile early (two sets, used in turn), widened into the operand's places */
             const uint32_t c8 = (ch & 3u) * 2u, place = base + F::kRing + (ch >> 2) * F::kHalfBytes, place_lo = place + swizzled(r0, c8), place_hi = place + swizzled(r0, c8 + 1u);
