@@ -333,7 +333,8 @@ int nwc_kv_read(void *stream, const nwc_kv_cache *cache, uint32_t layer, uint32_
    [T][n_q * head_dim]) over the positions that token t sees; a token that sees none gets zeros.  q rows are ldq apart (a multiple
    of 8).  visible != NULL: the tokens are drafts of a tree (T <= NWC_KV_MAX_TREE); token t stands at position *pos + depth[t],
    sees what is cached below *pos as above, and of the drafts those whose bit is set: bit j of word visible[t][j / 32]
-   ([T][(T + 31) / 32]), its own included or not.  workspace: nwc_kv_attention_workspace() bytes of device memory (16-byte
+   ([T][(T + 31) / 32]), its own included or not.  The window is not applied to the drafts: masks of paths longer than it leave
+   out the ancestors that it no longer reaches (depth[t] - depth[j] >= window and *pos + depth[j] >= sinks).  workspace: nwc_kv_attention_workspace() bytes of device memory (16-byte
    aligned; none for 0) that belong to this call until it is done: calls that may overlap use different ones. */
 uint64_t nwc_kv_attention_workspace(const nwc_kv_cache *cache, uint32_t T, uint32_t n_q);
 int nwc_kv_attention(void *stream, const nwc_kv_cache *cache, uint32_t layer, const uint16_t *q, uint64_t ldq, uint32_t T,

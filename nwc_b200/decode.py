@@ -510,14 +510,15 @@ class DecodeEngine:
 
     def verify(self, drafts, parents):
         """One step of speculative decoding.  drafts: proposed token ids; parents[i] < i: the draft that draft i continues, -1 =
-        the current token.  The current token and all drafts run at once (at most `chunk` together), each seeing its
-        ancestors; the longest path of drafts that greedy decoding would have chosen is kept in the cache.  Returns the new
+        the current token.  The current token and all drafts run at once (at most `chunk` together), each seeing what
+        it would see as a single token behind its ancestors; the longest path of drafts that greedy decoding would have chosen is kept in the cache.  Returns the new
         tokens: the accepted drafts and the one that follows them (at least one), which becomes the current token."""
         drafts = [int(t) for t in drafts]
         if len(drafts) != len(parents): raise ValueError("every draft has a parent")
         if any(not 0 <= t < self.cfg.vocab for t in drafts): raise ValueError(f"draft token ids are not all below {self.cfg.vocab}")
-        visible, depth = draft_tree([-1] + [int(p) + 1 for p in parents], self.device)
         start, pos = int(self.step_no.item()), int(self.pos.item())
+        window, sinks = (self.cache.window, self.cache.sinks) if self.cache is not None else (0, 0)
+        visible, depth = draft_tree([-1] + [int(p) + 1 for p in parents], self.device, window, sinks, pos)
         deepest = int(depth.max())
         if pos + len(drafts) + 1 > self.max_len or start + deepest + 1 > self.log.numel(): raise ValueError(f"{len(drafts)} drafts from position {pos} do not fit {self.max_len}")
         tokens = torch.cat([self.cur, torch.tensor(drafts, dtype=torch.int64, device=self.device)])

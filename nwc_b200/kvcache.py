@@ -7,7 +7,8 @@ stream; positions live in device memory, so every call can be captured in a CUDA
     q = cache.append(qkv, pos, cos, sin, q_norm, k_norm, layer=i)        # T tokens at positions pos .. pos + T - 1
     out = cache.attend(q, pos, layer=i)                                  # [T, n_q * head_dim]
 
-A draft tree is verified with the same two calls and the masks of `draft_tree`, then `commit` moves the accepted path together.
+A draft tree is verified with the same two calls and the masks of `draft_tree` (which takes the cache's window), then `commit`
+moves the accepted path together.
 """
 import ctypes
 import math
@@ -28,18 +29,26 @@ STATUS_TEXT = ((1, "a position outside the cache or the rotary tables"), (2, "a 
                (8, "a bounded wait inside the attention gave up, its outputs are not valid"))
 
 
-def draft_tree(parents, device="cuda"):
+def draft_tree(parents, device="cuda", window=0, sinks=0, pos=None):
     """Masks of a draft tree: parents[i] < i is the draft that token i continues, -1 where it continues the cached text.
-    Returns (visible int32 [T, ceil(T / 32)], depth int32 [T]): every token sees its ancestors and itself."""
+    Returns (visible int32 [T, ceil(T / 32)], depth int32 [T]): every token sees its ancestors and itself.
+    window, sinks: of the cache that the tree enters, at position pos (a number; needed beside sinks).  A token then sees the
+    ancestors that it would see as a single token: the last `window` positions of its path and those below `sinks`."""
     T = len(parents)
     if not T: raise ValueError("a draft tree has at least one token")
     if T > MAX_TREE: raise ValueError(f"a draft tree has at most {MAX_TREE} tokens, not {T}")
+    if window < 0 or sinks < 0 or sinks and not window: raise ValueError("window and sinks are not negative, and sinks need a window")
+    if sinks and pos is None: raise ValueError("beside sinks, pos says which drafts are among them")
     masks, depth = [], []
     for i, p in enumerate(parents):
         p = int(p)
         if not -1 <= p < i: raise ValueError(f"draft {i} hangs below draft {p}: a parent comes before its children (-1 = none)")
         masks.append((masks[p] if p >= 0 else 0) | 1 << i)
         depth.append(depth[p] + 1 if p >= 0 else 0)
+        if window and depth[i] >= window:                             # the ancestor that its parent saw last
+            left = i
+            for _ in range(window): left = int(parents[left])
+            if not (sinks and pos + depth[left] < sinks): masks[i] &= ~(1 << left)
     words = [[(m >> 32 * w) & 0xFFFFFFFF for w in range((T + 31) // 32)] for m in masks]
     signed = [[w - (1 << 32) if w >> 31 else w for w in row] for row in words]
     return torch.tensor(signed, dtype=torch.int32, device=device), torch.tensor(depth, dtype=torch.int32, device=device)
@@ -131,7 +140,7 @@ class KVCache:
 
     def attend(self, q, pos, visible=None, depth=None, layer=0, scale=None):
         """Attention of T stored tokens at positions pos .. pos + T - 1 (q [T, n_q, head_dim], bf16) over what each of them
-        sees; with the masks of draft_tree the tokens are drafts (at most 1024).  Returns bf16 [T, n_q * head_dim]; a token that
+        sees; with the masks of draft_tree (made with this cache's window and sinks) the tokens are drafts (at most 1024).  Returns bf16 [T, n_q * head_dim]; a token that
         sees nothing gets zeros.  scale: of the scores, 1 / sqrt(head_dim) by default."""
         T, n_q, hd = self._tokens(q, 3, "q")
         if hd != self.head_dim or n_q % self.n_kv or q.stride(1) != hd: raise ValueError(f"q is [T, n_q, {self.head_dim}] with n_q a multiple of {self.n_kv} and a token's heads side by side")

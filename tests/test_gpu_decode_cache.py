@@ -120,6 +120,27 @@ def test_verified_drafts_continue_as_greedy_decoding_would(kv, window, sinks):
         assert int(row.argmax()) == got
 
 
+@pytest.mark.parametrize("kv,sinks", [("bf16", 0), ("bf16", 3), ("fp8", 0)])
+def test_a_path_longer_than_the_window_is_verified_as_single_tokens_would(kv, sinks):
+    """One layer, a window of 4, twelve right drafts in a chain: the logits behind each of them are those of the token decoded
+    alone.  Ten roundings to bf16 in both (2^-8 / sqrt(3) each, independent) are 0.7 % of the logits' root mean square, and with the
+    codes that a rounding flips to their neighbour (one of 32, by 2^-3) 1.2 %; the largest of 13 x 2048 such errors is 4.5 of them,
+    the largest logit some 3.5 root mean squares: 0.016, and 0.04 leaves room."""
+    eng = engine(layers=1, kv=kv, window=4, sinks=sinks, chunk=16, max_len=64)
+    eng.prefill(TOKENS[:20], chunked=True)
+    first = int(eng.cur)
+    truth = eng.generate(12).tolist()
+    eng.prefill(TOKENS[:20], chunked=True)
+    new = eng.verify(truth, list(range(-1, 11)))
+    rows = eng.logits_rows.float()
+    want = logits_after(engine(layers=1, kv=kv, window=4, sinks=sinks, chunk=16, max_len=64), TOKENS[:20] + [first] + truth)[-13:]
+    assert_close(rows, want, 0.04)
+    for got, right, row in zip(new, truth, rows):
+        if margin(row) <= 2.0 ** -5 * row.abs().max().item(): return
+        assert got == right
+    assert len(new) == 13 and int(eng.pos) == 33
+
+
 def test_drafts_that_are_all_wrong_leave_the_next_token():
     eng = engine(chunk=8)
     eng.prefill(TOKENS[:10], chunked=True)

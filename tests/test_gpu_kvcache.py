@@ -214,6 +214,20 @@ def test_attention_of_a_draft_tree(elem, n_q, n_kv, hd, T, pos, window, sinks):
 
 
 @pytest.mark.parametrize("elem", ["bf16", "fp8"])
+@pytest.mark.parametrize("T,pos,window,sinks", [(12, 300, 8, 0), (12, 1, 5, 4), (70, 2000, 33, 3), (6, 9000, 1, 2)])
+def test_a_chain_of_drafts_longer_than_the_window(elem, T, pos, window, sinks):
+    """As a chain, a chunk sees what it sees as a chunk."""
+    from nwc_b200 import draft_tree
+    n_q, n_kv, hd = 8, 2, 128
+    c, k, v = filled(n_kv, hd, sinks + window + T - 1, elem, window, sinks, seed=T)
+    q = queries(T, n_q, hd)
+    visible, depth = draft_tree([t - 1 for t in range(T)], window=window, sinks=sinks, pos=pos)
+    out = c.attend(q.cuda(), at(pos), visible=visible, depth=depth)
+    c.check()
+    assert_attention(out, *R.attend(q.double(), k[0], v[0], pos, window, sinks))
+
+
+@pytest.mark.parametrize("elem", ["bf16", "fp8"])
 @pytest.mark.parametrize("T,pos", [(5, 0), (70, 0), (5, 40), (70, 300)])
 def test_drafts_that_see_nothing_or_not_themselves(elem, T, pos):
     """Masks other than a tree's: empty rows give zeros where nothing is cached, bits beyond a token's own position count."""

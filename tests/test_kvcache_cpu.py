@@ -113,3 +113,32 @@ def test_reference_attention_in_a_case_done_by_hand():
 
 def test_the_wait_probe_refuses_no_status_word(L):
     assert L.lib.nwc_kv_wait_probe(None, None) == -1
+
+
+@pytest.mark.parametrize("window,sinks,pos", [(8, 0, None), (1, 0, 0), (3, 2, 0), (3, 4, 1), (8, 5, 90), (64, 0, None)])
+def test_draft_tree_masks_under_a_window(window, sinks, pos):
+    """A draft sees the ancestors that the same token sees when it stands alone behind its path."""
+    from nwc_b200 import draft_tree
+    parents = [-1, 0, 0, 2, -1] + [4 + i for i in range(40)] + [20, 45, 7]
+    visible, depth = draft_tree(parents, "cpu", window=window, sinks=sinks, pos=pos)
+    for t in range(len(parents)):
+        seen, at = set(), t
+        while at >= 0:
+            if depth[t] - depth[at] < window or (sinks and pos + depth[at] < sinks): seen.add(at)
+            at = parents[at]
+        assert {j for j in range(len(parents)) if (int(visible[t, j // 32]) >> (j % 32)) & 1} == seen
+    for bad in (dict(window=-1), dict(sinks=2), dict(window=4, sinks=-1), dict(window=4, sinks=1)):
+        with pytest.raises(ValueError): draft_tree([-1, 0], "cpu", **bad)
+
+
+@pytest.mark.parametrize("window,sinks,pos", [(8, 0, 30), (8, 3, 30), (4, 3, 1), (1, 0, 0)])
+def test_a_chain_longer_than_the_window_sees_what_single_tokens_see(window, sinks, pos):
+    from nwc_b200 import draft_tree
+    T, n_q, n_kv, hd = 12, 2, 1, 64
+    g = torch.Generator().manual_seed(window + pos)
+    k, v = torch.randn(2, n_kv, sinks + window + T, hd, generator=g, dtype=torch.float64)
+    q = torch.randn(T, n_q, hd, generator=g, dtype=torch.float64)
+    visible, depth = draft_tree([t - 1 for t in range(T)], "cpu", window=window, sinks=sinks, pos=pos)
+    tree, _ = R.attend(q, k, v, pos, window, sinks, visible, depth)
+    chunk, _ = R.attend(q, k, v, pos, window, sinks)
+    assert (tree - chunk).abs().max() < 1e-12
