@@ -429,8 +429,12 @@ class DecodeEngine:
 
     # ---- graph ----
     def capture(self, warmup=3):
-        """Capture one decode step as a CUDA graph (state is saved and restored around the warm-up runs)."""
-        saved = (self.cur.clone(), self.pos.clone(), self.step_no.clone())
+        """Capture one decode step as a CUDA graph (state is saved and restored around the warm-up runs, which stand at position 0:
+        its row of every layer's keys and values among it)."""
+        c = self.cache
+        planes = (self.k_cache, self.v_cache) if c is None else (c.k, c.v) if c.k_exp is None else (c.k, c.v, c.k_exp, c.v_exp)
+        state = (self.cur, self.pos, self.step_no, self.log, *(t[:, :, 0] for t in planes))       # position 0 lives in slot 0
+        saved = [t.clone() for t in state]
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):
@@ -441,8 +445,7 @@ class DecodeEngine:
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph):
             self.forward_token()
-        for t, s in zip((self.cur, self.pos, self.step_no), saved): t.copy_(s)
-        self.log.zero_()
+        for t, s in zip(state, saved): t.copy_(s)
         torch.cuda.synchronize()
 
     def reset(self):

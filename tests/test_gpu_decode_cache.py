@@ -141,6 +141,18 @@ def test_a_path_longer_than_the_window_is_verified_as_single_tokens_would(kv, si
     assert len(new) == 13 and int(eng.pos) == 33
 
 
+@pytest.mark.parametrize("kw", [dict(), dict(chunk=8), dict(kv="fp8", chunk=8), dict(kv="fp8", window=16, sinks=2, chunk=8)], ids=lambda k: "-".join(k) or "plain")
+def test_capture_leaves_a_live_session_as_it_was(kw):
+    """Captured between two tokens of a session: what it holds, what it has logged and how it goes on are those of one that was not."""
+    eager, eng = engine(**kw), engine(**kw)
+    for e in (eager, eng): e.prefill(TOKENS[:12], chunked=bool(kw)); e.generate(3)
+    held = lambda e: [e.cur, e.pos, e.step_no, e.log] + ([e.k_cache, e.v_cache] if e.cache is None else [t.view(torch.uint8) for t in (e.cache.k, e.cache.v, e.cache.k_exp, e.cache.v_exp) if t is not None])
+    eng.capture()
+    for a, b in zip(held(eng), held(eager)): assert torch.equal(a, b)
+    assert eng.generate(6).tolist() == eager.generate(6).tolist()
+    for a, b in zip(held(eng) + [eng.logits], held(eager) + [eager.logits]): assert torch.equal(a, b)
+
+
 def test_drafts_that_are_all_wrong_leave_the_next_token():
     eng = engine(chunk=8)
     eng.prefill(TOKENS[:10], chunked=True)
