@@ -17,8 +17,13 @@
  * bf16 caches take bf16 products.  e4m3 codes become f16 (exactly, one conversion for two codes; bf16 would take bit moves and a
  * multiplication, 640 instead of 230 instructions of the 1150 per tile of 32 keys, and the kernel is bound by its issue rate),
  * with a query row scaled by a power of two to fill f16's range; the unit 2^e of a K row multiplies its scores, that of a V
- * row, relative to the largest met so far, its weights.  Tiles with V rows more than 2^10 smaller than that take bf16 products
- * for them.  The weights are rounded for the second product to bf16 (2^-8) or f16 (2^-11); their sum, the running maximum and all accumulators are fp32.
+ * row, relative to the largest that was met and seen so far, its weights.
+ *
+ * The weights are rounded for the second product: to bf16 (by up to 2^-8 of each), or, times the V rows' units, to f16.  A
+ * weight is at most 2^8 and is scaled up by 2^7, so that f16 holds it to 2^-11 of itself down to 2^-21 (the running maximum's is 1), and to 2^-32
+ * below.  Those absolute errors of a warp's N keys are less than 2^-12 of the row's sum of weights times units as long as
+ * that is N 2^-20 or more; until it is (a sink with a value of zero, an outlier among the units), tiles take bf16 products.
+ * The sum of the weights, the running maximum and all accumulators are fp32.
  */
 #include "nwc_kv.h"
 #include "nwc_async.cuh"
@@ -52,6 +57,7 @@ __device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t &lo, uint32_t
 }
 /* codes (in the high bytes of both halves of w; the low bytes may hold anything) -> bf16 pair */
 __device__ __forceinline__ uint32_t codes_to_bf16(uint32_t w) { return kv_mul2(((w >> 4) & 0x07F007F0u) | (w & 0x80008000u), kTwoTo120); }
+constexpr int32_t kWeightBits = 7;                                   /* weights in f16 are held times 2^7 (they reach 2^8: 2^15 of f16's 2^16) */
 /* 2^e for -126 <= e <= 127 */
 __device__ __forceinline__ float power_of_two(int32_t e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
@@ -191,7 +197,9 @@ __global__ void __launch_bounds__(32 * Few<HD, ELEM, MT, SHORT>::kWarps, 1) kv_a
     own_max = __reduce_max_sync(0xffffffffu, own_max); own_min = __reduce_min_sync(0xffffffffu, own_min);
     const uint32_t open_end = a.visible ? (uint32_t)pos : own_min + 1u;                 /* positions below it are seen by every row, window apart */
     const uint32_t words = (a.T + 31u) / 32u;
-    float o[MT][HD / 8][4], m[2 * MT], l[2 * MT];
+    float o[MT][HD / 8][4], m[2 * MT], l[2 * MT], held[2 * MT];                         /* held (e4m3): weights times units, as scaled for f16, of this lane's keys */
+    bool settled = false;                                                               /* every row holds at least `enough` */
+    const float enough = (float)my_tiles * (float)F::kKeys * 0x1p-20f * (float)(1 << kWeightBits);
 #pragma unroll
     for (uint32_t i = 0; i < MT; i++)
 #pragma unroll
@@ -199,7 +207,7 @@ __global__ void __launch_bounds__(32 * Few<HD, ELEM, MT, SHORT>::kWarps, 1) kv_a
 #pragma unroll
             for (uint32_t e = 0; e < 4u; e++) o[i][j][e] = 0.f;
 #pragma unroll
-    for (uint32_t i = 0; i < 2u * MT; i++) { m[i] = -INFINITY; l[i] = 0.f; }
+    for (uint32_t i = 0; i < 2u * MT; i++) { m[i] = -INFINITY; l[i] = held[i] = 0.f; }
     for (uint32_t it = 0; it < my_tiles; it++) {
         const uint32_t s = it % F::kStages, key0 = (first_tile + warp + it * kWarps) * F::kKeys, n = min(F::kKeys, span.count - key0);
         const uint32_t kt = mine + s * F::kStageBytes, vt = kt + F::kKeys * F::kRowBytes;
@@ -258,7 +266,9 @@ __global__ void __launch_bounds__(32 * Few<HD, ELEM, MT, SHORT>::kWarps, 1) kv_a
                     x *= ELEM == kKvE4m3 ? f * row_scale[i] : row_scale[i];
                 }
             }
+        uint32_t seen = F::kKeys == 32u ? 0xFFFFFFFFu : 0xFFFFu;                        /* (e4m3) keys of the tile that some row sees */
         if (!open) {
+            seen = 0u;
 #pragma unroll
             for (uint32_t j = 0; j < kNT; j++)
 #pragma unroll
@@ -270,8 +280,10 @@ __global__ void __launch_bounds__(32 * Few<HD, ELEM, MT, SHORT>::kWarps, 1) kv_a
                         if (!a.visible) sees = sees && p <= own[i];
                         else if (p >= (uint32_t)pos && kk < n) { const uint32_t d = p - (uint32_t)pos; sees = (a.visible[(uint64_t)token[i] * words + (d >> 5)] >> (d & 31u)) & 1u; }
                         if (!sees) sc[i >> 1][j][b + 2u * (i & 1u)] = -INFINITY;
+                        else seen |= 1u << kk;
                     }
                 }
+            if (ELEM == kKvE4m3) seen = __reduce_or_sync(0xffffffffu, seen);
         }
         /* running maximum: raised (and the sums rescaled) only when some row's tile maximum passes it by more than 2^8, so
            weights stay below 2^8 and the rescaling is rare */
@@ -285,17 +297,19 @@ __global__ void __launch_bounds__(32 * Few<HD, ELEM, MT, SHORT>::kWarps, 1) kv_a
             t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1)); t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
             top[i] = t; raise = raise || t > m[i] + 8.f;
         }
-        /* the same for the largest unit of the V rows: weights are multiplied by 2^(v_byte - top_byte) <= 1 */
+        /* the same for the largest unit of the V rows that are seen: weights are multiplied by 2^(v_seen - top_byte) <= 1 */
+        const uint32_t v_seen = (seen >> lane) & 1u ? v_byte : 0u;
         uint32_t byte_up = top_byte;
-        if (ELEM == kKvE4m3) { byte_up = max(top_byte, __reduce_max_sync(0xffffffffu, v_byte)); raise = raise || byte_up != top_byte; }
+        if (ELEM == kKvE4m3) { byte_up = max(top_byte, __reduce_max_sync(0xffffffffu, v_seen)); raise = raise || byte_up != top_byte; }
         if (__any_sync(0xffffffffu, raise)) {
             const float v_down = ELEM == kKvE4m3 ? power_of_two(max((int32_t)(top_byte - byte_up), -126)) : 1.f;
-            top_byte = byte_up;
+            top_byte = byte_up; settled = false;
 #pragma unroll
             for (uint32_t i = 0; i < 2u * MT; i++) {
                 const float up = fmaxf(m[i], top[i]), f = up == -INFINITY ? 1.f : exp2_fast(m[i] - up);
                 m[i] = up; l[i] *= f;
                 const float fo = f * v_down;
+                held[i] *= fo;
 #pragma unroll
                 for (uint32_t j = 0; j < HD / 8u; j++) { o[i >> 1][j][2u * (i & 1u)] *= fo; o[i >> 1][j][2u * (i & 1u) + 1u] *= fo; }
             }
@@ -303,9 +317,7 @@ __global__ void __launch_bounds__(32 * Few<HD, ELEM, MT, SHORT>::kWarps, 1) kv_a
         float base[2 * MT];
 #pragma unroll
         for (uint32_t i = 0; i < 2u * MT; i++) base[i] = m[i] == -INFINITY ? 0.f : m[i];
-        const float v_unit = power_of_two(max((int32_t)(v_byte - top_byte), -126));
-        /* rows more than 2^10 smaller than the largest met: their weights would reach f16's subnormal numbers */
-        const bool wide = ELEM == kKvE4m3 && __any_sync(0xffffffffu, v_byte && v_byte + 10u < top_byte);
+        const float v_unit = power_of_two(max((int32_t)(v_seen - top_byte), -126) + kWeightBits);
 #pragma unroll
         for (uint32_t j = 0; j < kNT; j++)
 #pragma unroll
@@ -319,6 +331,20 @@ __global__ void __launch_bounds__(32 * Few<HD, ELEM, MT, SHORT>::kWarps, 1) kv_a
                     if (ELEM == kKvE4m3) x *= vu;
                 }
             }
+        /* bf16 products for a tile while some row holds too little for f16 (a row that holds nothing has no weights yet) */
+        bool wide = false;
+        if (ELEM == kKvE4m3 && !settled) {
+            bool all = true;
+#pragma unroll
+            for (uint32_t i = 0; i < 2u * MT; i++) {
+#pragma unroll
+                for (uint32_t j = 0; j < kNT; j++) held[i] += sc[i >> 1][j][2u * (i & 1u)] + sc[i >> 1][j][2u * (i & 1u) + 1u];
+                float sum = held[i] + __shfl_xor_sync(0xffffffffu, held[i], 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                all = all && sum >= enough; wide = wide || (sum != 0.f && !(sum >= enough));
+            }
+            settled = __all_sync(0xffffffffu, all); wide = __any_sync(0xffffffffu, wide);
+        }
         /* o += P V, 16 keys at a time; lane (g, c) holds keys 2c, 2c + 1, 2c + 8, 2c + 9 of the columns of piece g */
 #pragma unroll
         for (uint32_t h = 0; h < kNT / 2u; h++) {
@@ -383,7 +409,7 @@ __global__ void __launch_bounds__(32 * Few<HD, ELEM, MT, SHORT>::kWarps, 1) kv_a
     __syncthreads();                                                                    /* every warp has done with its ring: O goes there */
     float *part = reinterpret_cast<float *>(few_raw);                                   /* [kWarps][kRows][kPitch] */
     constexpr uint32_t kPieceDims = ELEM == kKvE4m3 ? (HD == 64 ? 8u : 16u) : 8u;
-    const float o_unit = ELEM == kKvE4m3 ? kv_unit(top_byte) : 1.f;
+    const float o_unit = ELEM == kKvE4m3 ? kv_unit(top_byte) * (1.f / (1 << kWeightBits)) : 1.f;
 #pragma unroll
     for (uint32_t i = 0; i < 2u * MT; i++) {
         const uint32_t r = (i >> 1) * 16u + (i & 1u) * 8u + g;

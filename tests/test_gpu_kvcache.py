@@ -321,6 +321,62 @@ def test_value_rows_of_very_different_size(T, hd):
     assert_attention(out, want, weight)
 
 
+def quantised_into(c, k, v):
+    """64-bit rows k, v [n_kv, positions, hd] into the first slots of an fp8 cache; what it then holds."""
+    held = []
+    for x, t, e in ((k, c.k, c.k_exp), (v, c.v, c.v_exp)):
+        u = R.unit_exponent(x)
+        codes = R.rounded_e4m3(x * torch.exp2(-u.double())[..., None])
+        n = x.shape[1]
+        t.view(torch.uint8)[0, :, :n] = codes.to(torch.float32).to(torch.float8_e4m3fn).view(torch.uint8).cuda()
+        e[0, :, :n] = (u + 127).to(torch.uint8).cuda()
+        held.append(codes * torch.exp2(u.double())[..., None])
+    return held
+
+
+@pytest.mark.parametrize("bits,ratio", [(12, 6), (12, 10), (16, 6), (16, 10), (20, 6), (20, 10), (28, 9), (40, 0)])
+@pytest.mark.parametrize("hd,T,positions,first", [(128, 1, 700, "zero"), (128, 1, 9000, "zero"), (64, 5, 9000, "zero"), (256, 1, 6000, "zero"), (128, 3, 5000, "small"), (256, 1, 30000, "like the others")])
+def test_a_first_token_that_takes_almost_all_the_weight(bits, ratio, hd, T, positions, first):
+    """A sink: every other key's weight is 2^-bits of the first one's, whose value is zero, small or large; values are 2^-ratio of
+    one outlier's.  What the small weights bring comes out to the usual precision (there is no other output where the first value is zero)."""
+    from nwc_b200 import KVCache
+    n_q, n_kv, pos = 8, 2, positions - T
+    g = torch.Generator().manual_seed(bits + hd)
+    c = KVCache(n_kv, hd, positions, "fp8")
+    k = 0.1 * torch.randn(n_kv, positions, hd, generator=g, dtype=torch.float64)
+    v = torch.randn(n_kv, positions, hd, generator=g, dtype=torch.float64) * 2.0 ** -ratio
+    k[:, :, 0] = 0.0; k[:, 0, 0] = 8.0
+    v[:, 37] *= 2.0 ** ratio
+    v[:, 0] *= {"zero": 0.0, "small": 1.0, "like the others": 2.0 ** ratio}[first]
+    held = quantised_into(c, k, v)
+    q = torch.randn(T, n_q, hd, generator=g) * 0.1
+    q[:, :, 0] = bits * 0.6931 * hd ** 0.5 / 8.0
+    q = q.to(torch.bfloat16)
+    out = c.attend(q.cuda(), at(pos))
+    c.check()
+    assert_attention(out, *R.attend(q.double(), *held, pos))
+
+
+@pytest.mark.parametrize("hd,T,n_q,larger", [(256, 6, 16, 135), (128, 2, 8, 100), (64, 2, 8, 100)])
+def test_values_that_a_row_does_not_see_do_not_cost_it_precision(hd, T, n_q, larger):
+    """The last token's value is 2^100 of the others' (2^135 where its rows are computed apart from theirs): the tokens in front
+    of it are as precise as ever.  Compared times 2^60."""
+    from nwc_b200 import KVCache
+    n_kv, pos = 1, 500
+    g = torch.Generator().manual_seed(hd)
+    c = KVCache(n_kv, hd, 5000, "fp8")
+    k = 0.3 * torch.randn(n_kv, pos + T, hd, generator=g, dtype=torch.float64)
+    v = torch.randn(n_kv, pos + T, hd, generator=g, dtype=torch.float64) * 2.0 ** -60
+    v[:, -1] *= 2.0 ** larger
+    held = quantised_into(c, k, v)
+    q = queries(T, n_q, hd)
+    out = c.attend(q.cuda(), at(pos)).view(T, n_q, hd)
+    c.check()
+    want, weight = R.attend(q.double(), *held, pos)
+    assert_attention(out[:-1].double() * 2.0 ** 60, want[:-1] * 2.0 ** 60, weight[:-1] * 2.0 ** 60)
+    assert_attention(out[-1:], want[-1:], weight[-1:])
+
+
 def test_query_rows_may_be_slices():
     n_q, n_kv, hd, pos, T = 8, 2, 128, 90, 20
     c, k, v = filled(n_kv, hd, pos + T, "fp8")
