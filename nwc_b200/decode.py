@@ -497,7 +497,8 @@ class DecodeEngine:
 
     def extend(self, token_ids):
         """Feed tokens at the current position, `chunk` at a time; returns the greedy next token after each (int64, on the
-        device).  The last one becomes the current token."""
+        device).  The last one becomes the current token.  Waits for the device: a pass that met a position, a key or value or
+        a wait that is not right raises (the session then holds what it stored, reset() forgets it)."""
         tokens = torch.as_tensor(token_ids, dtype=torch.int64, device=self.device).reshape(-1)
         pos = int(self.pos.item())
         if not tokens.numel(): raise ValueError("no tokens")
@@ -508,6 +509,7 @@ class DecodeEngine:
         for part in tokens.split(max(self.chunk, 1)):
             out.append(self._rows(part)); self.pos += part.numel()
         out = torch.cat(out)
+        self._check_status()
         self.cur.copy_(out[-1:])
         return out
 
@@ -547,8 +549,6 @@ class DecodeEngine:
         self.reset()
         if chunked:
             self.extend(prompt_ids)
-            torch.cuda.synchronize()
-            self._check_status()
             return self.cur
         prompt = torch.as_tensor(prompt_ids, dtype=torch.int64, device=self.device).reshape(-1)
         if prompt.numel() > self.max_len: raise ValueError(f"prompt of {prompt.numel()} tokens does not fit the KV cache ({self.max_len})")

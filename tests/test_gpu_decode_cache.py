@@ -207,6 +207,16 @@ def test_the_engine_reports_a_wait_that_ran_out_once():
     eng._check_status()
 
 
+@pytest.mark.parametrize("call", [lambda e: e.extend(TOKENS[:6]), lambda e: e.prefill(TOKENS[:6], chunked=True), lambda e: e.verify(TOKENS[:2], [-1, 0])], ids=["extend", "prefill", "verify"])
+def test_keys_that_are_not_finite_are_reported_by_the_call_that_made_them(call):
+    eng = engine(chunk=4, max_len=32)
+    eng.w.layers[1]["k_norm"][3] = float("nan")
+    with pytest.raises(RuntimeError, match="finite"): call(eng)
+    eng.w.layers[1]["k_norm"][3] = 1.0
+    eng.reset()
+    assert int(eng.prefill(TOKENS[:6], chunked=True)) == int(eng.cur) and int(eng.pos) == 6
+
+
 @pytest.mark.parametrize("H,rows", [(256, 1), (1000, 3), (8192, 70)])
 def test_row_kernels_equal_the_single_row_ones(H, rows):
     from nwc_b200 import _lib as L
