@@ -197,6 +197,20 @@ def rope_tables(cfg, max_len, device):
     return emb.cos().to(torch.bfloat16).to(device).contiguous(), emb.sin().to(torch.bfloat16).to(device).contiguous()
 
 
+def accepted_path(drafts, parents, greedy):
+    """Rows (0 = the current token, i + 1 = draft i) of the longest path whose drafts are what greedy decoding chose behind their
+    parents, greedy[row] being its choice; of equal ones the one with the lowest last row.  (A token may be drafted twice
+    behind one parent: either may lead on.)"""
+    above, depth, last = [-1], [1], 0                                   # depth 0: not accepted
+    for i, (t, p) in enumerate(zip(drafts, parents)):
+        p = int(p) + 1
+        above.append(p); depth.append(depth[p] + 1 if depth[p] and greedy[p] == t else 0)
+        if depth[-1] > depth[last]: last = i + 1
+    path = []
+    while last >= 0: path.insert(0, last); last = above[last]
+    return path
+
+
 class DecodeEngine:
     def __init__(self, weights: DecoderWeights, max_len=1024, device="cuda", dependent_launch=False, tp_group=None, tp_reduce="push", side_tables=False, prefetch_next=True,
                  kv="bf16", window=0, sinks=0, chunk=0):
@@ -529,11 +543,8 @@ class DecodeEngine:
         tokens = torch.cat([self.cur, torch.tensor(drafts, dtype=torch.int64, device=self.device)])
         best = self._rows(tokens, visible, depth)
         greedy = best.tolist()                                          # (waits for the device)
-        path, new = [0], [greedy[0]]
-        while True:
-            child = next((i + 1 for i, p in enumerate(parents) if int(p) + 1 == path[-1] and drafts[i] == new[-1]), None)
-            if child is None: break
-            path.append(child); new.append(greedy[child])
+        path = accepted_path(drafts, parents, greedy)
+        new = [greedy[i] for i in path]
         n = torch.tensor([len(path)], dtype=torch.int32, device=self.device)
         self.cache.commit(self.pos, torch.tensor(path, dtype=torch.int32, device=self.device), n, tokens=tokens.numel())
         self.pos += n

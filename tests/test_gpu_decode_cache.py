@@ -153,6 +153,18 @@ def test_capture_leaves_a_live_session_as_it_was(kw):
     for a, b in zip(held(eng) + [eng.logits], held(eager) + [eager.logits]): assert torch.equal(a, b)
 
 
+def test_a_token_drafted_twice_is_followed_where_it_leads_on():
+    eng = engine(chunk=8)
+    eng.prefill(TOKENS[:10], chunked=True)
+    truth = eng.generate(3).tolist()
+    eng.prefill(TOKENS[:10], chunked=True)
+    new = eng.verify([truth[0], (truth[1] + 1) % 2048, truth[0], truth[1]], [-1, 0, -1, 2])
+    for got, right, row in zip(new, truth, eng.logits_rows.float()[[0, 3, 4]]):
+        if margin(row) <= 2.0 ** -5 * row.abs().max().item(): return
+        assert got == right
+    assert len(new) == 3 and int(eng.pos) == 13
+
+
 def test_drafts_that_are_all_wrong_leave_the_next_token():
     eng = engine(chunk=8)
     eng.prefill(TOKENS[:10], chunked=True)

@@ -142,3 +142,12 @@ def test_a_chain_longer_than_the_window_sees_what_single_tokens_see(window, sink
     tree, _ = R.attend(q, k, v, pos, window, sinks, visible, depth)
     chunk, _ = R.attend(q, k, v, pos, window, sinks)
     assert (tree - chunk).abs().max() < 1e-12
+
+
+def test_the_longest_accepted_path_of_a_draft_tree():
+    from nwc_b200.decode import accepted_path as path
+    assert path([], [], [7]) == [0] and path([5, 6], [-1, 0], [7, 1, 1]) == [0]
+    assert path([7, 8, 9], [-1, 0, 1], [7, 8, 1, 1]) == [0, 1, 2]                            # the third draft is wrong
+    assert path([7, 7, 8], [-1, -1, 1], [7, 8, 8, 4]) == [0, 2, 3]                           # drafted twice, the second leads on
+    assert path([7, 8, 7, 8], [-1, 0, -1, 2], [7, 8, 4, 8, 4]) == [0, 1, 2]                  # both do: the first
+    assert path([7, 3, 9, 9], [-1, 0, 1, 0], [7, 4, 9, 1, 1]) == [0, 1]                      # a child of a wrong draft counts for nothing
