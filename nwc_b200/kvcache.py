@@ -23,7 +23,7 @@ try:                                                                  # an alloc
 except ImportError:
     def empty_strided(shape, strides, dtype): return torch.empty(shape, dtype=dtype, device="cuda")
 current_device, raw_stream = getattr(torch._C, "_cuda_getDevice", None), getattr(torch._C, "_cuda_getCurrentRawStream", None)     # (absent without CUDA)
-MAX_TREE = 1024
+MAX_TREE, MAX_POSITIONS = 1024, 0x7FFFFFFF
 ELEMS = {"bf16": (0, torch.bfloat16), "fp8": (1, torch.float8_e4m3fn)}
 STATUS_TEXT = ((1, "a position outside the cache or the rotary tables"), (2, "a key or value that is not finite"), (4, "an accepted path that is not one"),
                (8, "a bounded wait inside the attention gave up, its outputs are not valid"))
@@ -166,6 +166,7 @@ class KVCache:
         first, count = int(first), int(count)
         if first < 0 or count < 1: raise ValueError("positions from 0 on, at least one")
         if not self.window and first + count > self.capacity: raise ValueError(f"positions {first} .. {first + count - 1} are outside a cache of {self.capacity}")
+        if first + count > MAX_POSITIONS: raise ValueError(f"a session has at most {MAX_POSITIONS} positions")
         if self.window and first + count - max(first, self.sinks) > self.capacity - self.sinks: raise ValueError(f"{count} positions do not lie in a ring of {self.capacity - self.sinks} at the same time")
         if not 0 <= layer < self.layers: self._layer(layer)
         hd = self.head_dim
@@ -181,6 +182,7 @@ class KVCache:
         if path.dim() != 1: raise ValueError("path is a vector of draft numbers")
         self._int32(path, path.numel(), "path"); self._int32(count, 1, "count"); self._int32(pos, 1, "pos")
         if tokens is None: tokens = min(MAX_TREE, self.capacity - self.sinks - self.window + 1 if self.window else self.capacity)
+        if not 1 <= tokens <= MAX_TREE: raise ValueError(f"a draft tree has 1 to {MAX_TREE} tokens, not {tokens}")
         self._call("nwc_kv_commit", L.lib.nwc_kv_commit, self._ref, tokens, pos.data_ptr(), path.data_ptr(), count.data_ptr(), min(path.numel(), tokens), self._status)
 
     def check(self):

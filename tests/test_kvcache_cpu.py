@@ -151,3 +151,32 @@ def test_the_longest_accepted_path_of_a_draft_tree():
     assert path([7, 7, 8], [-1, -1, 1], [7, 8, 8, 4]) == [0, 2, 3]                           # drafted twice, the second leads on
     assert path([7, 8, 7, 8], [-1, 0, -1, 2], [7, 8, 4, 8, 4]) == [0, 1, 2]                  # both do: the first
     assert path([7, 3, 9, 9], [-1, 0, 1, 0], [7, 4, 9, 1, 1]) == [0, 1]                      # a child of a wrong draft counts for nothing
+
+
+def fake_cache(L, **kw):
+    """A KVCache whose tensors nobody looks at: what its calls refuse before they reach the device."""
+    from nwc_b200 import KVCache
+    c = KVCache.__new__(KVCache)
+    f = dict(layers=1, n_kv=2, capacity=64, head_dim=128, window=20, sinks=4, elem="bf16", _at=0, device=torch.device("cuda:0"), status=None, _status=A, _need={})
+    f.update(kw)
+    for name, value in f.items(): setattr(c, name, value)
+    c._ref = cache(L, window=c.window, sinks=c.sinks)
+    return c
+
+
+def test_numbers_that_do_not_fit_the_calls_are_refused_not_cut(L):
+    """2^32 + 5 would arrive as 5."""
+    ring = fake_cache(L)
+    for first, count in ((2 ** 32 + 5, 1), (2 ** 31 - 1, 1), (5, 2 ** 32), (2 ** 63, 2)):
+        with pytest.raises(ValueError, match="positions"): ring.read(first, count)
+
+    class Int32:                                                        # a path, a count and a position on the device
+        dtype = torch.int32
+        def __init__(self, n): self.n = n
+        def dim(self): return 1
+        def numel(self): return self.n
+        def get_device(self): return 0
+        def is_contiguous(self): return True
+        def data_ptr(self): return A
+    for tokens in (0, -1, 1025, 2 ** 32 + 4):
+        with pytest.raises(ValueError, match="1 to 1024"): ring.commit(Int32(1), Int32(3), Int32(1), tokens=tokens)
