@@ -330,7 +330,7 @@ int nwc_kv_read(void *stream, const nwc_kv_cache *cache, uint32_t layer, uint32_
                 uint16_t *v_out);
 
 /* T tokens at positions *pos .. *pos + T - 1, already stored, attend: out[t] = sum_p softmax_p(scale q[t] . k_p) v_p (bf16
-   [T][n_q * head_dim]) over the positions that token t sees; a token that sees none gets zeros.  q rows are ldq apart (a multiple
+   [T][n_q * head_dim]) over the positions that token t sees; a token that sees none gets zeros.  scale is positive and at most 2e38.  q rows are ldq apart (a multiple
    of 8).  visible != NULL: the tokens are drafts of a tree (T <= NWC_KV_MAX_TREE); token t stands at position *pos + depth[t],
    sees what is cached below *pos as above, and of the drafts those whose bit is set: bit j of word visible[t][j / 32]
    ([T][(T + 31) / 32]), its own included or not.  The window is not applied to the drafts: masks of paths longer than it leave

@@ -417,7 +417,7 @@ NWC_EXPORT int nwc_kv_attention(void *stream, const nwc_kv_cache *cache, uint32_
     if (!cache_ok(cache, layer, T) || !T || T > NWC_KV_MAX_TOKENS || !n_q || n_q % cache->n_kv || n_q > 65535u) return -1;
     if (!q || !pos || !out || !status || !aligned16(q) || !aligned16(out) || !aligned16(workspace) || ldq < (uint64_t)n_q * cache->head_dim || ldq % 8u) return -1;
     if (visible ? T > NWC_KV_MAX_TREE || !depth : depth != nullptr) return -1;
-    if (!(scale > 0.f) || scale > 3e38f) return -1;
+    if (!(scale > 0.f) || scale > 2e38f) return -1;                  /* (times log2(e) it is a number too) */
     const int sms = nwc_setup();
     if (sms <= 0) return (int)cudaErrorNoDevice;
     const KvPlan plan = kv_attention_plan(cache->elem, cache->head_dim, cache->n_kv, cache->capacity, cache->window, cache->sinks, T, n_q, sms);

@@ -141,7 +141,7 @@ class KVCache:
     def attend(self, q, pos, visible=None, depth=None, layer=0, scale=None):
         """Attention of T stored tokens at positions pos .. pos + T - 1 (q [T, n_q, head_dim], bf16) over what each of them
         sees; with the masks of draft_tree (made with this cache's window and sinks) the tokens are drafts (at most 1024).  Returns bf16 [T, n_q * head_dim]; a token that
-        sees nothing gets zeros.  scale: of the scores, 1 / sqrt(head_dim) by default."""
+        sees nothing gets zeros.  scale: of the scores, positive, 1 / sqrt(head_dim) by default."""
         T, n_q, hd = self._tokens(q, 3, "q")
         if hd != self.head_dim or n_q % self.n_kv or q.stride(1) != hd: raise ValueError(f"q is [T, n_q, {self.head_dim}] with n_q a multiple of {self.n_kv} and a token's heads side by side")
         if (visible is None) != (depth is None): raise ValueError("visible and depth come together (draft_tree makes them)")
@@ -150,6 +150,8 @@ class KVCache:
             self._int32(visible, T * ((T + 31) // 32), "visible"); self._int32(depth, T, "depth")
         self._int32(pos, 1, "pos")
         if not 0 <= layer < self.layers: self._layer(layer)
+        if scale is None: scale = 1.0 / math.sqrt(hd)
+        elif not 0.0 < scale <= 2e38: raise ValueError(f"scale is a positive number up to 2e38, not {scale}")
         out = self._empty((T, n_q * hd), (n_q * hd, 1))
         need = self._need.get((T, n_q))
         if need is None:
@@ -157,7 +159,7 @@ class KVCache:
         # a workspace of the call's own: the allocator keeps it from calls on other streams, a graph keeps it in its pool
         work = self._empty((need // 2,), (1,)) if need else None
         self._call("nwc_kv_attention", L.lib.nwc_kv_attention, self._ref, layer, q.data_ptr(), q.stride(0), T, n_q, pos.data_ptr(), None if visible is None else visible.data_ptr(),
-                   None if depth is None else depth.data_ptr(), 1.0 / math.sqrt(hd) if scale is None else float(scale), out.data_ptr(), None if work is None else work.data_ptr(), need, self._status)
+                   None if depth is None else depth.data_ptr(), float(scale), out.data_ptr(), None if work is None else work.data_ptr(), need, self._status)
         return out
 
     def read(self, first, count, layer=0):

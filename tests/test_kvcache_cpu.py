@@ -180,3 +180,9 @@ def test_numbers_that_do_not_fit_the_calls_are_refused_not_cut(L):
         def data_ptr(self): return A
     for tokens in (0, -1, 1025, 2 ** 32 + 4):
         with pytest.raises(ValueError, match="1 to 1024"): ring.commit(Int32(1), Int32(3), Int32(1), tokens=tokens)
+
+
+def test_scales_that_leave_the_numbers_are_refused(L):
+    """The kernels work with scale x log2(e): 2.9e38 would become infinite."""
+    for scale in (2.9e38, 2.4e38, 0.0, -0.5):
+        assert L.lib.nwc_kv_attention(None, cache(L), 0, A, 512, 3, 4, A, None, None, scale, A, None, 0, A) == -1
