@@ -134,7 +134,7 @@ class KVCache:
         self._int32(pos, 1, "pos")
         if not 0 <= layer < self.layers: self._layer(layer)
         out = self._empty((T, n_q, hd), (n_q * hd, hd, 1))
-        self._call("nwc_kv_append", L.lib.nwc_kv_append, self._ref, layer, qkv.data_ptr(), qkv.stride(0), T, n_q, qn, kn, cos.data_ptr(), sin.data_ptr(), rows,
+        self._call("nwc_kv_append", L.lib.nwc_kv_append, self._ref, layer, qkv.data_ptr(), qkv.stride(0) if T > 1 else width, T, n_q, qn, kn, cos.data_ptr(), sin.data_ptr(), rows,
                    pos.data_ptr(), dp, eps, out.data_ptr(), self._status)
         return out
 
@@ -143,7 +143,7 @@ class KVCache:
         sees; with the masks of draft_tree (made with this cache's window and sinks) the tokens are drafts (at most 1024).  Returns bf16 [T, n_q * head_dim]; a token that
         sees nothing gets zeros.  scale: of the scores, positive, 1 / sqrt(head_dim) by default."""
         T, n_q, hd = self._tokens(q, 3, "q")
-        if hd != self.head_dim or n_q % self.n_kv or q.stride(1) != hd: raise ValueError(f"q is [T, n_q, {self.head_dim}] with n_q a multiple of {self.n_kv} and a token's heads side by side")
+        if hd != self.head_dim or n_q % self.n_kv or n_q > 1 and q.stride(1) != hd: raise ValueError(f"q is [T, n_q, {self.head_dim}] with n_q a multiple of {self.n_kv} and a token's heads side by side")
         if (visible is None) != (depth is None): raise ValueError("visible and depth come together (draft_tree makes them)")
         if visible is not None:
             if T > MAX_TREE: raise ValueError(f"a draft tree has at most {MAX_TREE} tokens, not {T}")
@@ -158,7 +158,7 @@ class KVCache:
             with torch.cuda.device(self.device): need = self._need[T, n_q] = L.lib.nwc_kv_attention_workspace(self._ref, T, n_q)
         # a workspace of the call's own: the allocator keeps it from calls on other streams, a graph keeps it in its pool
         work = self._empty((need // 2,), (1,)) if need else None
-        self._call("nwc_kv_attention", L.lib.nwc_kv_attention, self._ref, layer, q.data_ptr(), q.stride(0), T, n_q, pos.data_ptr(), None if visible is None else visible.data_ptr(),
+        self._call("nwc_kv_attention", L.lib.nwc_kv_attention, self._ref, layer, q.data_ptr(), q.stride(0) if T > 1 else n_q * hd, T, n_q, pos.data_ptr(), None if visible is None else visible.data_ptr(),
                    None if depth is None else depth.data_ptr(), float(scale), out.data_ptr(), None if work is None else work.data_ptr(), need, self._status)
         return out
 
@@ -196,9 +196,9 @@ class KVCache:
 
     # ---- helpers (a call of one token takes microseconds on the device: what every call checks is kept to plain comparisons) ----
     def _tokens(self, t, dims, name):
-        if t.dim() != dims or t.dtype is not BF16 or t.get_device() != self._at or t.stride(-1) != 1 or t.stride(0) % 8 or t.data_ptr() % 16:
-            raise ValueError(f"{name} is a {dims}-dimensional bf16 tensor on {self.device}, rows contiguous and 16-byte aligned")
         shape = t.shape
+        if t.dim() != dims or t.dtype is not BF16 or t.get_device() != self._at or t.stride(-1) != 1 or t.stride(0) % 8 and shape[0] > 1 or t.data_ptr() % 16:
+            raise ValueError(f"{name} is a {dims}-dimensional bf16 tensor on {self.device}, rows contiguous and 16-byte aligned")
         if not 0 < shape[0] <= 65535: raise ValueError(f"a call takes 1 to 65535 tokens, not {shape[0]}")
         return shape
 

@@ -387,6 +387,21 @@ def test_query_rows_may_be_slices():
     assert_attention(out, *R.attend(q.cpu().double(), k[0], v[0], pos))
 
 
+def test_strides_of_single_rows_and_heads_do_not_matter():
+    """Torch gives a dimension of one any stride."""
+    hd, pos = 128, 40
+    c, k, v = filled(1, hd, 64, "bf16")
+    qkv = queries(1, 3, hd).reshape(1, 3 * hd).cuda()
+    cos, sin = (t.cuda() for t in tables(64, hd))
+    want = c.append(qkv, at(pos), cos, sin)
+    for stride in (1, 4):
+        assert torch.equal(c.append(qkv.as_strided((1, 3 * hd), (stride, 1)), at(pos), cos, sin), want)
+        assert torch.equal(c.attend(want.as_strided((1, 1, hd), (stride, stride, 1)), at(pos)), c.attend(want, at(pos)))
+    q = queries(5, 1, hd).cuda()
+    assert torch.equal(c.attend(q.as_strided((5, 1, hd), (hd, 1, 1)), at(pos)), c.attend(q, at(pos)))
+    c.check()
+
+
 @pytest.mark.parametrize("elem", ["bf16", "fp8"])
 def test_offsets_beyond_32_bits(elem):
     """Layers whose bytes lie beyond 2^32 of the cache's first."""

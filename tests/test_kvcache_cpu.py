@@ -186,3 +186,11 @@ def test_scales_that_leave_the_numbers_are_refused(L):
     """The kernels work with scale x log2(e): 2.9e38 would become infinite."""
     for scale in (2.9e38, 2.4e38, 0.0, -0.5):
         assert L.lib.nwc_kv_attention(None, cache(L), 0, A, 512, 3, 4, A, None, None, scale, A, None, 0, A) == -1
+
+
+def test_the_stride_of_a_single_row_does_not_matter(L):
+    c = fake_cache(L, _at=-1)
+    row = torch.zeros(1024, dtype=torch.bfloat16)
+    for stride in (1024, 1, 0, 12):
+        assert c._tokens(row.as_strided((1, 1024), (stride, 1)), 2, "qkv") == (1, 1024)
+    with pytest.raises(ValueError): c._tokens(row.as_strided((2, 64), (12, 1)), 2, "qkv")
