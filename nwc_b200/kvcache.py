@@ -61,6 +61,8 @@ class KVCache:
     window > 0: a token sees the last `window` positions (its own among them) and the first `sinks`; slots beyond the sinks are
     taken in turn, so positions run on without end.  T tokens at once need capacity - sinks >= window + T - 1.
 
+    The calls have no backward pass: with gradients enabled they refuse tensors that require them.
+
     Position tensors are int32 [1] on the cache's device.  Values that are not finite are stored as 0 and reported by check(),
     as are positions outside the cache."""
 
@@ -127,6 +129,7 @@ class KVCache:
         qn = kn = dp = None
         if q_norm is not None and k_norm is not None:
             for t in (q_norm, k_norm):
+                if t.requires_grad: self._no_grad("q_norm and k_norm")
                 if t.dtype is not BF16 or t.get_device() != at or t.shape != (hd,) or not t.is_contiguous(): raise ValueError(f"q_norm and k_norm are contiguous bf16 [{hd}] on {self.device}")
             qn, kn = q_norm.data_ptr(), k_norm.data_ptr()
         elif q_norm is not None or k_norm is not None: raise ValueError("q_norm and k_norm come together")
@@ -199,6 +202,7 @@ class KVCache:
         shape = t.shape
         if t.dim() != dims or t.dtype is not BF16 or t.get_device() != self._at or t.stride(-1) != 1 or t.stride(0) % 8 and shape[0] > 1 or t.data_ptr() % 16:
             raise ValueError(f"{name} is a {dims}-dimensional bf16 tensor on {self.device}, rows contiguous and 16-byte aligned")
+        if t.requires_grad: self._no_grad(name)
         if not 0 < shape[0] <= 65535: raise ValueError(f"a call takes 1 to 65535 tokens, not {shape[0]}")
         return shape
 
@@ -208,6 +212,9 @@ class KVCache:
     def _empty(self, shape, strides):
         """bf16 on the cache's device."""
         return empty_strided(shape, strides, BF16) if current_device() == self._at else torch.empty(shape, dtype=BF16, device=self.device)
+
+    def _no_grad(self, name):
+        if torch.is_grad_enabled(): raise ValueError(f"{name}: the cache's calls have no backward pass; call them under torch.no_grad()")
 
     def _layer(self, layer):
         raise IndexError(f"layer {layer} of a cache of {self.layers}")

@@ -650,3 +650,14 @@ def test_a_wait_that_ran_out_is_reported_by_the_cache_and_by_the_library():
     with pytest.raises(RuntimeError, match="gave up"): c.check()
     c.check()                                                            # reported once
     assert L.lib.nwc_kernel_status(0) == 2 and L.lib.nwc_kernel_status(1) == 2 and L.lib.nwc_kernel_status(1) == 0
+
+
+def test_gradients_are_not_lost_silently():
+    c, _, _ = filled(2, 64, 32, "bf16")
+    qkv, t, w = queries(3, 8, 64).reshape(3, 512).cuda(), torch.ones(40, 64, dtype=torch.bfloat16, device="cuda"), torch.ones(64, dtype=torch.bfloat16, device="cuda")
+    q = c.append(qkv, at(0), t, t, w, w)
+    wants = lambda x: x.clone().requires_grad_()
+    for call in (lambda: c.append(wants(qkv), at(0), t, t, w, w), lambda: c.append(qkv, at(0), t, t, wants(w), w), lambda: c.append(qkv, at(0), t, t, w, wants(w)), lambda: c.attend(wants(q), at(0))):
+        with pytest.raises(ValueError, match="no_grad"): call()
+    with torch.no_grad(): assert torch.equal(c.append(wants(qkv), at(0), t, t, wants(w), w), q) and torch.equal(c.attend(wants(q), at(0)), c.attend(q, at(0)))
+    c.check()

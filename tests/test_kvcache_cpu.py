@@ -194,3 +194,11 @@ def test_the_stride_of_a_single_row_does_not_matter(L):
     for stride in (1024, 1, 0, 12):
         assert c._tokens(row.as_strided((1, 1024), (stride, 1)), 2, "qkv") == (1, 1024)
     with pytest.raises(ValueError): c._tokens(row.as_strided((2, 64), (12, 1)), 2, "qkv")
+
+
+def test_tensors_that_want_gradients_are_refused_while_gradients_are_on(L):
+    c = fake_cache(L, _at=-1)
+    x = torch.zeros(2, 1024, dtype=torch.bfloat16, requires_grad=True)
+    with pytest.raises(ValueError, match="no_grad"): c._tokens(x, 2, "qkv")
+    with torch.no_grad(): assert c._tokens(x, 2, "qkv") == (2, 1024)
+    assert c._tokens(x.detach(), 2, "qkv") == (2, 1024)
