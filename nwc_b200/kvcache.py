@@ -11,6 +11,7 @@ A draft tree is verified with the same two calls and the masks of `draft_tree` (
 moves the accepted path together.
 """
 import ctypes
+import functools
 import math
 
 import torch
@@ -18,15 +19,27 @@ import torch
 from . import _lib as L
 
 BF16, INT32 = torch.bfloat16, torch.int32
-try:                                                                  # an allocation without the dispatcher's way: 0.8 us instead of 1.9
-    from torch._C._dynamo.guards import _empty_strided_cuda as empty_strided
-except ImportError:
-    def empty_strided(shape, strides, dtype): return torch.empty(shape, dtype=dtype, device="cuda")
 current_device, raw_stream = getattr(torch._C, "_cuda_getDevice", None), getattr(torch._C, "_cuda_getCurrentRawStream", None)     # (absent without CUDA)
 MAX_TREE, MAX_POSITIONS = 1024, 0x7FFFFFFF
 ELEMS = {"bf16": (0, torch.bfloat16), "fp8": (1, torch.float8_e4m3fn)}
 STATUS_TEXT = ((1, "a position outside the cache or the rotary tables"), (2, "a key or value that is not finite"), (4, "an accepted path that is not one"),
                (8, "a bounded wait inside the attention gave up, its outputs are not valid"))
+
+
+def _plain_empty(shape, strides, dtype):
+    return torch.empty(shape, dtype=dtype, device="cuda")
+
+
+@functools.cache
+def _allocation():
+    """An allocation on the current device that does not go through the dispatcher (0.8 us instead of 1.9).  It is no public name
+    of torch: taken once it has answered as torch.empty does."""
+    try:
+        from torch._C._dynamo.guards import _empty_strided_cuda as direct
+        t = direct((2, 3), (3, 1), BF16)
+        if t.shape == (2, 3) and t.stride() == (3, 1) and t.dtype is BF16 and t.is_cuda and t.get_device() == torch.cuda.current_device(): return direct
+    except Exception: pass
+    return _plain_empty
 
 
 def draft_tree(parents, device="cuda", window=0, sinks=0, pos=None):
@@ -107,7 +120,7 @@ class KVCache:
         at = lambda t: None if t is None else t.data_ptr()
         self._c = L.KvCache(at(k), at(v), at(k_exp), at(v_exp), self.layers, self.n_kv, self.head_dim, self.capacity, window, sinks, 1 if quantised else 0)
         self._at = k.get_device()
-        with torch.cuda.device(self._at): L.lib.nwc_setup()           # not in the first call, which may be one that is captured
+        with torch.cuda.device(self._at): L.lib.nwc_setup(); self._strided = _allocation()           # not in the first call, which may be one that is captured
         self._need = {}                                               # workspace bytes per (tokens, query heads)
         self._ref, self._status = ctypes.byref(self._c), self.status.data_ptr()
 
@@ -211,7 +224,7 @@ class KVCache:
 
     def _empty(self, shape, strides):
         """bf16 on the cache's device."""
-        return empty_strided(shape, strides, BF16) if current_device() == self._at else torch.empty(shape, dtype=BF16, device=self.device)
+        return self._strided(shape, strides, BF16) if current_device() == self._at else torch.empty(shape, dtype=BF16, device=self.device)
 
     def _no_grad(self, name):
         if torch.is_grad_enabled(): raise ValueError(f"{name}: the cache's calls have no backward pass; call them under torch.no_grad()")

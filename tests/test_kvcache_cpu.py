@@ -202,3 +202,15 @@ def test_tensors_that_want_gradients_are_refused_while_gradients_are_on(L):
     with pytest.raises(ValueError, match="no_grad"): c._tokens(x, 2, "qkv")
     with torch.no_grad(): assert c._tokens(x, 2, "qkv") == (2, 1024)
     assert c._tokens(x.detach(), 2, "qkv") == (2, 1024)
+
+
+@pytest.mark.parametrize("answer", [None, lambda shape, dtype: None, lambda shape, strides, dtype: torch.empty(shape, dtype=dtype), lambda shape, strides, dtype: torch.empty(shape)],
+                         ids=["gone", "other arguments", "other device", "other type"])
+def test_torchs_own_allocation_is_used_only_where_it_answers_as_the_public_one(monkeypatch, answer):
+    from nwc_b200 import kvcache
+    guards = torch._C._dynamo.guards
+    if answer is None: monkeypatch.delattr(guards, "_empty_strided_cuda", raising=False)
+    else: monkeypatch.setattr(guards, "_empty_strided_cuda", answer, raising=False)
+    kvcache._allocation.cache_clear()
+    try: assert kvcache._allocation() is kvcache._plain_empty
+    finally: kvcache._allocation.cache_clear()
