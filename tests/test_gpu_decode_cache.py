@@ -71,6 +71,16 @@ def test_a_session_longer_than_its_cache_in_a_graph():
     assert eager == replay and int(eng.pos.item()) == 140
 
 
+@pytest.mark.parametrize("layout", [0, 2])
+@pytest.mark.parametrize("kw", [dict(chunk=8), dict(kv="fp8"), dict(kv="fp8", window=16, sinks=2, chunk=8)], ids=lambda k: "-".join(k))
+def test_dependent_launches_change_nothing(kw, layout):
+    """Kernels that start before the ones in front of them have ended, eager and captured: the same bits."""
+    a, b = engine(layout, **kw), engine(layout, dependent_launch=True, **kw)
+    assert torch.equal(logits_after(a, TOKENS), logits_after(b, TOKENS))
+    a.prefill(TOKENS); b.prefill(TOKENS); b.capture()
+    assert a.generate(30).tolist() == b.generate(30).tolist() and torch.equal(a.logits, b.logits)
+
+
 @pytest.mark.parametrize("kv,window,sinks", [("bf16", 0, 0), ("fp8", 0, 0), ("fp8", 24, 3)])
 @pytest.mark.parametrize("layout", [0, 2])
 def test_chunks_agree_with_single_tokens(kv, window, sinks, layout):
