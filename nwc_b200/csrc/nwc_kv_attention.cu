@@ -21,8 +21,10 @@
  *
  * The weights are rounded for the second product: to bf16 (by up to 2^-8 of each), or, times the V rows' units, to f16.  A
  * weight is at most 2^8 and is scaled up by 2^7, so that f16 holds it to 2^-11 of itself down to 2^-21 (the running maximum's is 1), and to 2^-32
- * below.  Those absolute errors of a warp's N keys are less than 2^-12 of the row's sum of weights times units as long as
- * that is N 2^-20 or more; until it is (a sink with a value of zero, an outlier among the units), tiles take bf16 products.
+ * below.  Those absolute errors of a warp's N keys stay below 2^-12 of the row's sum of weights times units (N 2^-28 of it for N up
+ * to 2^16) as long as that is 2^-4 and N 2^-20 or more; until it is (a sink with a value of zero, an outlier among the units),
+ * tiles take bf16 products.  What f16 costs then is small beside the row as a whole, and not beside a dimension in which every
+ * value of weight is a zero.
  * The sum of the weights, the running maximum and all accumulators are fp32.
  */
 #include "nwc_kv.h"
@@ -199,7 +201,7 @@ __global__ void __launch_bounds__(32 * Few<HD, ELEM, MT, SHORT>::kWarps, 1) kv_a
     const uint32_t words = (a.T + 31u) / 32u;
     float o[MT][HD / 8][4], m[2 * MT], l[2 * MT], held[2 * MT];                         /* held (e4m3): weights times units, as scaled for f16, of this lane's keys */
     bool settled = false;                                                               /* every row holds at least `enough` */
-    const float enough = (float)my_tiles * (float)F::kKeys * 0x1p-20f * (float)(1 << kWeightBits);
+    const float enough = fmaxf(0x1p-4f, (float)my_tiles * (float)F::kKeys * 0x1p-20f) * (float)(1 << kWeightBits);
 #pragma unroll
     for (uint32_t i = 0; i < MT; i++)
 #pragma unroll

@@ -357,6 +357,28 @@ def test_a_first_token_that_takes_almost_all_the_weight(bits, ratio, hd, T, posi
     assert_attention(out, *R.attend(q.double(), *held, pos))
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("positions,capacity", [(3, 3), (700, 700), (700, 6000)])
+def test_a_large_value_of_little_weight_beside_small_values(hd, positions, capacity):
+    """One value 2^28 of the others', with a weight of 2^-12 and zeros in half of its dimensions: in those, what the others bring
+    comes out to the usual precision."""
+    from nwc_b200 import KVCache
+    n_q, n_kv, pos = 8, 2, positions - 1
+    g = torch.Generator().manual_seed(hd + positions)
+    c = KVCache(n_kv, hd, capacity, "fp8")
+    k = 0.1 * torch.randn(n_kv, positions, hd, generator=g, dtype=torch.float64)
+    k[:, :, 0] = 8.0; k[:, 1, 0] = 0.0
+    v = torch.randn(n_kv, positions, hd, generator=g, dtype=torch.float64) * 2.0 ** -28
+    v[:, 1] *= 2.0 ** 28; v[:, 1, ::2] = 0.0
+    held = quantised_into(c, k, v)
+    q = torch.randn(1, n_q, hd, generator=g) * 0.1
+    q[:, :, 0] = 12 * 0.6931 * hd ** 0.5 / 8.0
+    q = q.to(torch.bfloat16)
+    out = c.attend(q.cuda(), at(pos))
+    c.check()
+    assert_attention(out, *R.attend(q.double(), *held, pos))
+
+
 @pytest.mark.parametrize("hd,T,n_q,larger", [(256, 6, 16, 135), (128, 2, 8, 100), (64, 2, 8, 100)])
 def test_values_that_a_row_does_not_see_do_not_cost_it_precision(hd, T, n_q, larger):
     """The last token's value is 2^100 of the others' (2^135 where its rows are computed apart from theirs): the tokens in front
