@@ -203,7 +203,7 @@ def accepted_path(drafts, parents, greedy):
     behind one parent: either may lead on.)"""
     above, depth, last = [-1], [1], 0                                   # depth 0: not accepted
     for i, (t, p) in enumerate(zip(drafts, parents)):
-        p = int(p) + 1
+        p += 1
         above.append(p); depth.append(depth[p] + 1 if depth[p] and greedy[p] == t else 0)
         if depth[-1] > depth[last]: last = i + 1
     path = []
@@ -532,12 +532,12 @@ class DecodeEngine:
         the current token.  The current token and all drafts run at once (at most `chunk` together), each seeing what
         it would see as a single token behind its ancestors; the longest path of drafts that greedy decoding would have chosen is kept in the cache.  Returns the new
         tokens: the accepted drafts and the one that follows them (at least one), which becomes the current token."""
-        drafts = [int(t) for t in drafts]
+        drafts, parents = [int(t) for t in drafts], [int(p) for p in parents]
         if len(drafts) != len(parents): raise ValueError("every draft has a parent")
         if any(not 0 <= t < self.cfg.vocab for t in drafts): raise ValueError(f"draft token ids are not all below {self.cfg.vocab}")
         start, pos = int(self.step_no.item()), int(self.pos.item())
         window, sinks = (self.cache.window, self.cache.sinks) if self.cache is not None else (0, 0)
-        visible, depth = draft_tree([-1] + [int(p) + 1 for p in parents], self.device, window, sinks, pos)
+        visible, depth = draft_tree([-1] + [p + 1 for p in parents], self.device, window, sinks, pos)
         deepest = int(depth.max())
         if pos + len(drafts) + 1 > self.max_len or start + deepest + 1 > self.log.numel(): raise ValueError(f"{len(drafts)} drafts from position {pos} do not fit {self.max_len}")
         tokens = torch.cat([self.cur, torch.tensor(drafts, dtype=torch.int64, device=self.device)])

@@ -52,15 +52,14 @@ def draft_tree(parents, device="cuda", window=0, sinks=0, pos=None):
     if T > MAX_TREE: raise ValueError(f"a draft tree has at most {MAX_TREE} tokens, not {T}")
     if window < 0 or sinks < 0 or sinks and not window: raise ValueError("window and sinks are not negative, and sinks need a window")
     if sinks and pos is None: raise ValueError("beside sinks, pos says which drafts are among them")
-    masks, depth = [], []
+    parents, masks, depth = [int(p) for p in parents], [], []
     for i, p in enumerate(parents):
-        p = int(p)
         if not -1 <= p < i: raise ValueError(f"draft {i} hangs below draft {p}: a parent comes before its children (-1 = none)")
         masks.append((masks[p] if p >= 0 else 0) | 1 << i)
         depth.append(depth[p] + 1 if p >= 0 else 0)
         if window and depth[i] >= window:                             # the ancestor that its parent saw last
             left = i
-            for _ in range(window): left = int(parents[left])
+            for _ in range(window): left = parents[left]
             if not (sinks and pos + depth[left] < sinks): masks[i] &= ~(1 << left)
     words = [[(m >> 32 * w) & 0xFFFFFFFF for w in range((T + 31) // 32)] for m in masks]
     signed = [[w - (1 << 32) if w >> 31 else w for w in row] for row in words]

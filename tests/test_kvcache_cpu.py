@@ -214,3 +214,16 @@ def test_torchs_own_allocation_is_used_only_where_it_answers_as_the_public_one(m
     kvcache._allocation.cache_clear()
     try: assert kvcache._allocation() is kvcache._plain_empty
     finally: kvcache._allocation.cache_clear()
+
+
+def test_a_draft_tree_reads_its_parents_once():
+    """They may lie on a device, where every number read is a wait."""
+    from nwc_b200 import draft_tree
+    class Parents(list):
+        read = 0
+        def __iter__(self):
+            for p in list.__iter__(self): self.read += 1; yield p
+        def __getitem__(self, i): self.read += 1; return list.__getitem__(self, i)
+    parents = Parents(range(-1, 63))
+    draft_tree(parents, "cpu", window=20)
+    assert parents.read == 64
