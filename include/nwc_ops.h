@@ -297,7 +297,8 @@ int nwc_argmax_rows(void *stream, const uint16_t *logits, uint32_t V, uint32_t r
 
    Per layer and key/value head `capacity` slots of head_dim numbers (64, 128 or 256) for K and for V: bf16, or e4m3 codes
    with one byte b per row: value = code * 2^(b - 127), the smallest exponent that keeps the row's largest magnitude within
-   448 * 2^(b - 127).
+   448 * 2^(b - 127).  The NaN codes 0x7F and 0xFF are never written here, and in a cache that was filled elsewhere a token must
+   not see them: read-back gives NaN, the attention NaN or what 480 in their place would give, by the call's size.
    window == 0: position p lives in slot p and a token sees every position up to its own; sessions end at `capacity`.
    window > 0: a token sees the last `window` positions, its own among them, and the first `sinks` positions of the session.
    Positions below `sinks` keep their slots, the others take the remaining capacity - sinks slots in turn, so a session may

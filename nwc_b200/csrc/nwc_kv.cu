@@ -172,10 +172,11 @@ __device__ __forceinline__ void store_row(const StoreArgs &a, uint8_t *plane, ui
 constexpr uint32_t kStoreQ = 4, kStoreK = 1, kStoreV = 2;             /* passes of a warp */
 template <int HD> __host__ __device__ constexpr uint32_t store_groups(uint32_t n, uint32_t passes) { return (n + passes * (256u / HD) - 1u) / (passes * (256u / HD)); }
 
-/* Bound: integer work (unpacking, packing) and the dependent start of a warp (position, cos / sin, rows), 4096 tokens of 64 +
-   16 heads without norms: 34 us for 160 MB, 0.73 of measured bandwidth.  So the warps that fit count: without the norm weights the
-   kernel is held to 64 registers (four CTAs per SM; with 80 and three it takes 39), with them it would spill (one token 2.8 -> 3.3
-   us, 517 tokens 5.9 -> 7.1, 4096 tokens no faster). */
+/* Bound: latency.  A warp's life is short and its loads depend on one another (rows, position, cos / sin); 4096 tokens of 64 +
+   16 heads without norms take 34 us for 160 MB, 0.73 of measured bandwidth, with 2.7 instructions of 4 per clock, the ALU at 55 % and waiting
+   for memory the largest stall.  So the warps that fit count: without the norm weights the kernel is held to 64 registers (four
+   CTAs per SM; with 80 and three it takes 39; two bf16 forms spill 8 bytes for it), with them it would spill more than it gains
+   (one token 2.8 -> 3.3 us, 517 tokens 5.9 -> 7.1, 4096 tokens no faster). */
 template <int HD, int ELEM, bool NORM>
 __global__ void __launch_bounds__(256, NORM ? 3 : 4) kv_store_kernel(const StoreArgs a) {
     using R = Row<HD>;

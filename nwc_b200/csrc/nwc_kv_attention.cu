@@ -15,8 +15,7 @@
  * dimension that lane group n's piece holds at that place.  Neither K nor V is ever transposed or re-stored.
  *
  * bf16 caches take bf16 products.  e4m3 codes become f16 (exactly, one conversion for two codes; bf16 would take bit moves and a
- * multiplication, 640 instead of 230 instructions of the 1150 per tile of 32 keys, and the kernel is bound by its issue rate),
- * with a query row scaled by a power of two to fill f16's range; the unit 2^e of a K row multiplies its scores, that of a V
+ * multiplication, 640 instead of 230 of a tile's instructions, which now are 735 for 32 keys), with a query row scaled by a power of two to fill f16's range; the unit 2^e of a K row multiplies its scores, that of a V
  * row, relative to the largest that was met and seen so far, its weights.
  *
  * The weights are rounded for the second product: to bf16 (by up to 2^-8 of each), or, times the V rows' units, to f16.  A
@@ -26,6 +25,10 @@
  * tiles take bf16 products.  What f16 costs then is small beside the row as a whole, and not beside a dimension in which every
  * value of weight is a zero.
  * The sum of the weights, the running maximum and all accumulators are fp32.
+ *
+ * One token over 131071 e4m3 positions (64 + 8 heads of 128): 51.4 us, 5.3 TB/s, 0.82 of measured bandwidth.  What is left is
+ * latency: three warps per scheduler (168 registers, rings that fill the shared memory) issue 2.0 instructions of 4 per clock,
+ * and no pipe is above 46 %.
  */
 #include "nwc_kv.h"
 #include "nwc_async.cuh"
@@ -583,13 +586,21 @@ template <int HD> void configure_few() {
 
 }  // namespace
 
-/* Which kernel and how many CTAs (times in us on B200, head_dim 128, eight key/value heads, calls of one kind in a graph):
-     rows per key/value head   keys     e4m3: few / many      bf16: few / many
-     32                        32768    31 / 44               41 / 34
-     32                        131072   93 / 143              104 / 92
-     32                        4096     23 / 17               22 / 15
+/* Which kernel and how many CTAs.  Times in us on B200, eight key/value heads, calls of one kind in a graph:
+     rows per key/value head   keys     head_dim 128:  e4m3 few / many   bf16 few / many     64:  e4m3 few / many   bf16 few / many
+     16                        1024                    11.0 / 15.7       9.0 / 12.2               8.7 / 11.1        7.6 / 10.5
+     16                        32768                   23 / 46           33 / 34                  17 / 30           16 / 25
+     32                        1024                    18 / 14           18 / 14                  9.3 / 11.2        8.3 / 10.8
+     32                        4096                    25 / 17           24 / 17                  12.3 / 13.6       10.7 / 12.8
+     32                        32768                   31 / 44           42 / 35                  23 / 30           27 / 25
+     32                        131072                  80 / 145          107 / 91                 59 / 111          68 / 61
+     48                        32768                   45 / 44           59 / 36                  33 / 31           38 / 26
    The many-rows kernel multiplies 128 rows whatever there are, on tensor cores that make nothing of it, but it takes a while to
-   fill and widens e4m3 rows at a rate of its own: the few-rows kernel takes up to 16 rows, and up to 32 of a long e4m3 cache. */
+   fill and widens e4m3 rows at a rate of its own: the few-rows kernel takes up to 16 rows, and up to 32 of a long e4m3 cache.
+   (Heads of 64 would gain 1 to 3 us over short caches with a border of 32.)
+   head_dim 256 has no many-rows kernel: its outputs and scores for two streams pass the tensor memory.  Its chunks and trees go
+   through the few-rows kernel, 16 rows and the keys of the whole call per CTA: 2048 tokens of 8 + 2 heads over 8192 positions 802 us (bf16; 77 with head_dim 128),
+   4096 tokens under a window of 64 1026 us. */
 KvPlan kv_attention_plan(int elem, uint32_t head_dim, uint32_t n_kv, uint32_t capacity, uint32_t window, uint32_t sinks, uint32_t T, uint32_t n_q, int sms) {
     const uint32_t rows = T * (n_q / n_kv);
     const uint64_t keys = window ? (uint64_t)sinks + window + T - 1u : capacity;
@@ -608,7 +619,10 @@ KvPlan kv_attention_plan(int elem, uint32_t head_dim, uint32_t n_kv, uint32_t ca
     if (ctas >= (uint64_t)sms * 2u) return p;
     if (!longer) {
         /* Clusters of 2^k CTAs, a tile of 16 keys for each of their four warps, as long as the GPU has room for them side by
-           side (sixteen clusters of sixteen one after the other: 34 us where eight are 13). */
+           side: up to 5/4 CTAs per SM (bf16, 4096 keys; 1, 5/4 and 2 per SM: ten heads 9.9, 9.4, 9.3 us, 40 heads 24.7, 18.4,
+           18.4, 16 heads 11.8, 11.8, 17.5, where a second round of clusters begins).  Against two launches (bf16, 32 + 8 heads of 128): 6.5 / 8.8 us at
+           1024 keys, 7.8 / 9.9 at 2048, 9.5 / 9.7 at 4096, 12.9 / 12.3 at 8192, 19.1 / 15.4 at 16384; e4m3 7.5 / 8.9, 8.6 / 9.7, 10.7 / 9.5, 14.8 / 12.2.
+           head_dim 256 would do better without: 12.8 / 11.3, 15.2 / 12.2, 19.3 / 12.4. */
         p.in_clusters = true;
         while (p.splits < 16u && (uint64_t)p.splits * 64u < keys && ctas * p.splits * 2u <= (uint64_t)sms * 5u / 4u) p.splits *= 2u;
         return p;

@@ -21,7 +21,8 @@
  * of the list of keys may begin, end and wrap anywhere in the ring; a row that is no key of the call is written as zeros
  * (whatever its slot holds, weight 0 times it must be 0).  Whole bf16 tiles are tensor-map copies; e4m3 rows become bf16 on
  * the way, exactly: code and unit have fewer bits than a bf16 number.  All waits are
- * bounded; a role that gives up records the status word and stops, the others run out, tensor memory is freed.
+ * bounded; a role that gives up says so in both status words and stops, the others run out, copies and products in flight are
+ * awaited, tensor memory is freed.
  *
  * O is rescaled in tensor memory only when a row's maximum passes the one it is scaled by by more than 2^8 (weights stay below
  * 2^8, sums are fp32): after the first tiles hardly ever.  P is rounded to bf16 (2^-8 relative), the sum of the weights is not.
@@ -45,7 +46,8 @@ template <int HD, int ELEM> struct Many {
     static constexpr uint32_t kSlots = HD == 64 ? 8u : 5u;
     /* Registers: the 16 warps start with 65536 / 512 = 128 each; those that hold a row of scores take what the others give back:
        8 x 184 + 4 x 72 + 4 x 72 = 16 x 128 (bf16: the producers only start copies), 8 x 168 + 4 x 112 + 4 x 64 = 16 x 128 (e4m3:
-       they hold two sets of codes; at 176 / 96 / 64 the tree of 64 over 32768 takes 107 us instead of 90). */
+       they hold two sets of codes; at 176 / 96 / 64 the tree of 64 over 32768 takes 107 us instead of 90; these forms spill 66 to 78
+       bytes). */
     static constexpr uint32_t kProducers = 128u, kMmaWarp = 8u + kProducers / 32u, kThreads = 256u + kProducers + 128u;
     static constexpr int kRegsWeights = ELEM == kKvE4m3 ? 168 : 184, kRegsProduce = ELEM == kKvE4m3 ? 112 : 72, kRegsMma = ELEM == kKvE4m3 ? 64 : 72;
     static constexpr uint32_t kQ = 0u, kRing = 2u * kTile, kBars = kRing + kSlots * kTile;
