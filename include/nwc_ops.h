@@ -303,11 +303,11 @@ int nwc_argmax_rows(void *stream, const uint16_t *logits, uint32_t V, uint32_t r
    window > 0: a token sees the last `window` positions, its own among them, and the first `sinks` positions of the session.
    Positions below `sinks` keep their slots, the others take the remaining capacity - sinks slots in turn, so a session may
    run to 2^31 - 1 positions; a call of T tokens needs capacity - sinks >= window + T - 1.
-   k, v, qkv, q and out are 16-byte aligned; every call is asynchronous on its stream, allocates nothing and can be captured.
-   *pos (device) is the position of a call's first token.  *status (device) collects bits, 0 = fine: 1 a position outside the
-   cache or the rotary tables (the call, or with `depth` that token, wrote nothing), 2 a key or value that was not finite (0
-   was stored in its place), 4 a path that is not one (nothing was moved), 8 a bounded wait inside the attention gave up (its outputs are
-   not valid; nwc_kernel_status() reports it as well). */
+   k, v, qkv, q and out are 16-byte aligned; every call is asynchronous on its stream, allocates nothing and can be
+   captured. *pos (device) is the position of a call's first token. *status (device) collects bits, 0 = fine: 1 a position
+   outside the cache or the rotary tables (the call, or with `depth` that token, wrote nothing), 2 a key or value that was not
+   finite (0 was stored in its place), 4 a path that is not one (nothing was moved), 8 a bounded wait inside the attention
+   gave up (its outputs are not valid; nwc_kernel_status() reports it as well). */
 #define NWC_KV_MAX_TOKENS 65535
 #define NWC_KV_MAX_TREE 1024
 typedef struct {
@@ -331,20 +331,21 @@ int nwc_kv_read(void *stream, const nwc_kv_cache *cache, uint32_t layer, uint32_
                 uint16_t *v_out);
 
 /* T tokens at positions *pos .. *pos + T - 1, already stored, attend: out[t] = sum_p softmax_p(scale q[t] . k_p) v_p (bf16
-   [T][n_q * head_dim]) over the positions that token t sees; a token that sees none gets zeros.  scale is positive and at most 2e38.  q rows are ldq apart (a multiple
-   of 8).  visible != NULL: the tokens are drafts of a tree (T <= NWC_KV_MAX_TREE); token t stands at position *pos + depth[t],
-   sees what is cached below *pos as above, and of the drafts those whose bit is set: bit j of word visible[t][j / 32]
-   ([T][(T + 31) / 32]), its own included or not.  The window is not applied to the drafts: masks of paths longer than it leave
-   out the ancestors that it no longer reaches (depth[t] - depth[j] >= window and *pos + depth[j] >= sinks).  workspace: nwc_kv_attention_workspace() bytes of device memory (16-byte
-   aligned; none for 0) that belong to this call until it is done: calls that may overlap use different ones. */
+   [T][n_q * head_dim]) over the positions that token t sees; a token that sees none gets zeros. scale is positive and at most
+   2e38. q rows are ldq apart (a multiple of 8). visible != NULL: the tokens are drafts of a tree (T <= NWC_KV_MAX_TREE);
+   token t stands at position *pos + depth[t], sees what is cached below *pos as above, and of the drafts those whose bit is
+   set: bit j of word visible[t][j / 32] ([T][(T + 31) / 32]), its own included or not. The window is not applied to the
+   drafts: masks of paths longer than it leave out the ancestors that it no longer reaches (depth[t] - depth[j] >= window and
+   *pos + depth[j] >= sinks). workspace: nwc_kv_attention_workspace() bytes of device memory (16-byte aligned; none for 0)
+   that belong to this call until it is done: calls that may overlap use different ones. */
 uint64_t nwc_kv_attention_workspace(const nwc_kv_cache *cache, uint32_t T, uint32_t n_q);
 int nwc_kv_attention(void *stream, const nwc_kv_cache *cache, uint32_t layer, const uint16_t *q, uint64_t ldq, uint32_t T,
                      uint32_t n_q, const int32_t *pos, const uint32_t *visible, const int32_t *depth, float scale,
                      uint16_t *out, void *workspace, uint64_t workspace_size, int *status);
 
-/* The accepted path of a draft tree of T tokens at *pos: row path[i] of the drafts becomes row i for i < *count (<= most <= T),
-   in all layers; path (device, `most` entries) rises strictly and stays below T and the cache's end.  The caller then advances *pos by *count; the drafts behind
-   the path count as never stored. */
+/* The accepted path of a draft tree of T tokens at *pos: row path[i] of the drafts becomes row i for i < *count (<= most <=
+   T), in all layers; path (device, `most` entries) rises strictly and stays below T and the cache's end. The caller then
+   advances *pos by *count; the drafts behind the path count as never stored. */
 int nwc_kv_commit(void *stream, const nwc_kv_cache *cache, uint32_t T, const int32_t *pos, const int32_t *path,
                   const int32_t *count, uint32_t most, int *status);
 

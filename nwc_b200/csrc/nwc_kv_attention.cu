@@ -598,9 +598,9 @@ template <int HD> void configure_few() {
    The many-rows kernel multiplies 128 rows whatever there are, on tensor cores that make nothing of it, but it takes a while to
    fill and widens e4m3 rows at a rate of its own: the few-rows kernel takes up to 16 rows, and up to 32 of a long e4m3 cache.
    (Heads of 64 would gain 1 to 3 us over short caches with a border of 32.)
-   head_dim 256 has no many-rows kernel: its outputs and scores for two streams pass the tensor memory.  Its chunks and trees go
-   through the few-rows kernel, 16 rows and the keys of the whole call per CTA: 2048 tokens of 8 + 2 heads over 8192 positions 802 us (bf16; 77 with head_dim 128),
-   4096 tokens under a window of 64 1026 us. */
+   head_dim 256 has no many-rows kernel: scores and outputs of two streams pass the tensor memory.  Its chunks and trees go
+   through the few-rows kernel, 16 rows and the keys of the whole call per CTA: 2048 tokens of 8 + 2 heads over 8192 positions
+   take 802 us (bf16; 77 with head_dim 128), 4096 tokens under a window of 64 1026 us. */
 KvPlan kv_attention_plan(int elem, uint32_t head_dim, uint32_t n_kv, uint32_t capacity, uint32_t window, uint32_t sinks, uint32_t T, uint32_t n_q, int sms) {
     const uint32_t rows = T * (n_q / n_kv);
     const uint64_t keys = window ? (uint64_t)sinks + window + T - 1u : capacity;
@@ -619,10 +619,11 @@ KvPlan kv_attention_plan(int elem, uint32_t head_dim, uint32_t n_kv, uint32_t ca
     if (ctas >= (uint64_t)sms * 2u) return p;
     if (!longer) {
         /* Clusters of 2^k CTAs, a tile of 16 keys for each of their four warps, as long as the GPU has room for them side by
-           side: up to 5/4 CTAs per SM (bf16, 4096 keys; 1, 5/4 and 2 per SM: ten heads 9.9, 9.4, 9.3 us, 40 heads 24.7, 18.4,
-           18.4, 16 heads 11.8, 11.8, 17.5, where a second round of clusters begins).  Against two launches (bf16, 32 + 8 heads of 128): 6.5 / 8.8 us at
-           1024 keys, 7.8 / 9.9 at 2048, 9.5 / 9.7 at 4096, 12.9 / 12.3 at 8192, 19.1 / 15.4 at 16384; e4m3 7.5 / 8.9, 8.6 / 9.7, 10.7 / 9.5, 14.8 / 12.2.
-           head_dim 256 would do better without: 12.8 / 11.3, 15.2 / 12.2, 19.3 / 12.4. */
+           side: up to 5/4 CTAs per SM (bf16, 4096 keys, up to 1, 5/4 and 2: ten key/value heads 9.9, 9.4, 9.3 us, forty 24.7,
+           18.4, 18.4, sixteen 11.8, 11.8, 17.5, where a second round of clusters begins).  Against two launches, 32 + 8 heads of
+           128, at 1024, 2048, 4096, 8192 and 16384 keys: bf16 6.5 / 8.8, 7.8 / 9.9, 9.5 / 9.7, 12.9 / 12.3, 19.1 / 15.4 us; e4m3
+           7.5 / 8.9, 8.6 / 9.7, 10.7 / 9.5, 14.8 / 12.2, 22.8 / 15.3.  (Heads of 256 would do better without: bf16 12.8 / 11.3,
+           15.2 / 12.2, 19.3 / 12.4.) */
         p.in_clusters = true;
         while (p.splits < 16u && (uint64_t)p.splits * 64u < keys && ctas * p.splits * 2u <= (uint64_t)sms * 5u / 4u) p.splits *= 2u;
         return p;

@@ -683,3 +683,54 @@ def test_gradients_are_not_lost_silently():
         with pytest.raises(ValueError, match="no_grad"): call()
     with torch.no_grad(): assert torch.equal(c.append(wants(qkv), at(0), t, t, wants(w), w), q) and torch.equal(c.attend(wants(q), at(0)), c.attend(q, at(0)))
     c.check()
+
+
+@pytest.mark.parametrize("elem,window,sinks", [("bf16", 0, 0), ("fp8", 40, 4)])
+def test_a_captured_verification_follows_position_path_and_count(elem, window, sinks):
+    """Store, attention and commit of a draft tree in one graph, replayed with other positions, paths and counts on the device."""
+    from nwc_b200 import draft_tree
+    n_q, n_kv, hd, T = 8, 2, 128, 9
+    capacity = sinks + window + T - 1 if window else 300
+    made = [filled(n_kv, hd, capacity, elem, window, sinks, seed=5, layers=2)[0] for _ in range(2)]
+    cos, sin = (t.cuda() for t in tables(700, hd))
+    x = torch.randn(T, (n_q + 2 * n_kv) * hd, generator=torch.Generator().manual_seed(6)).to(torch.bfloat16).cuda()
+    visible, depth = draft_tree([-1, 0, 0, 1, 2, 2, 4, 4, 7], window=window, sinks=sinks, pos=100)
+    p, path, count = at(100), torch.zeros(T, dtype=torch.int32, device="cuda"), at(0)
+    def step(c):
+        q = c.append(x, p, cos, sin, depth=depth, layer=1)
+        out = c.attend(q, p, visible=visible, depth=depth, layer=1)
+        c.commit(p, path, count, tokens=T)
+        return out
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side): step(made[0]); step(made[1])
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g): out = step(made[0])
+    bits = lambda c: [t.view(torch.uint8) for t in (c.k, c.v, c.k_exp, c.v_exp) if t is not None]
+    for pos, way in ((100, [0, 2, 5]), (103, [0, 1, 3]), (250, [0, 2, 4, 7, 8]), (251, [0])):
+        p.fill_(pos); path[:len(way)] = torch.tensor(way, dtype=torch.int32, device="cuda"); count.fill_(len(way))
+        g.replay()
+        want = step(made[1])
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        for a, b in zip(bits(made[0]), bits(made[1])): assert torch.equal(a, b)
+    for c in made: c.check()
+
+
+@pytest.mark.parametrize("elem", ["bf16", "fp8"])
+def test_the_most_tokens_stored_at_once(elem):
+    from nwc_b200 import KVCache
+    T, n_q, n_kv, hd = 65535, 3, 1, 64
+    c = KVCache(n_kv, hd, T + 5, elem)
+    x = torch.randn(T, (n_q + 2 * n_kv) * hd, device="cuda", generator=torch.Generator("cuda").manual_seed(2)).to(torch.bfloat16)
+    one, zero = torch.ones(T + 5, hd, dtype=torch.bfloat16, device="cuda"), torch.zeros(T + 5, hd, dtype=torch.bfloat16, device="cuda")
+    q = c.append(x, at(5), one, zero)
+    k, v = c.read(5, T)
+    c.check()
+    assert torch.equal(q.view(T, -1), x[:, :n_q * hd])
+    for got, want, byte in ((k[0], x[:, n_q * hd:(n_q + 1) * hd], c.k_exp), (v[0], x[:, (n_q + 1) * hd:], c.v_exp)):
+        if elem == "bf16": assert torch.equal(got, want); continue
+        u = R.unit_exponent(want.cpu())                                  # (what is stored is a bf16 number: its code is exact)
+        assert torch.equal(byte[0, 0, 5:].cpu().int(), (u + 127).int())
+        assert torch.equal(got.cpu().double(), R.rounded_e4m3(want.cpu().double() * torch.exp2(-u.double())[:, None]) * torch.exp2(u.double())[:, None])

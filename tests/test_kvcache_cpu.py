@@ -227,3 +227,13 @@ def test_a_draft_tree_reads_its_parents_once():
     parents = Parents(range(-1, 63))
     draft_tree(parents, "cpu", window=20)
     assert parents.read == 64
+
+
+def test_row_kernel_refusals(L):
+    for bad in (dict(h=None), dict(out=None), dict(w=None), dict(H=0), dict(rows=0), dict(xn=None)):
+        a = {**dict(h=A, delta=None, out=A, w=A, eps=1e-6, H=256, rows=3, xn=A), **bad}
+        assert L.lib.nwc_add_rmsnorm_rows(None, *a.values()) == -1, bad
+    for bad in (dict(gu=None), dict(I=0), dict(rows=0), dict(rows=65536), dict(a=None)):
+        assert L.lib.nwc_swiglu_rows(None, *{**dict(gu=A, I=256, rows=3, a=A), **bad}.values()) == -1, bad
+    for bad in (dict(logits=None), dict(V=0), dict(rows=0), dict(best=None)):
+        assert L.lib.nwc_argmax_rows(None, *{**dict(logits=A, V=256, rows=3, best=A), **bad}.values()) == -1, bad
